@@ -113,6 +113,7 @@ extern "C" {
 typedef struct nx_ctx nx_ctx;
 typedef struct nx_experts nx_experts;
 typedef struct nx_matrix nx_matrix;
+typedef struct nx_kv nx_kv;
 
 /* ---------------------------------------------------------------- runtime */
 const char *nx_last_error(void);
@@ -237,6 +238,96 @@ int nx_matvec(nx_ctx *ctx, const nx_matrix *m, const float *x, size_t x_len, int
               float *y);
 int nx_matvec_dev(nx_ctx *ctx, const nx_matrix *m, const float *d_x, size_t x_len,
                   int num_tokens, float *d_y);
+
+/* ---------------------------------------------------------------- key/value cache */
+/* formats of a cache's values */
+#define NX_KV_F16 0  /* IEEE half, rounded to nearest even */
+#define NX_KV_INT8 1 /* 8-bit codes with one f32 scale per token and head (keys and values
+                        apart): scale = max |x| / 127 in f32, code = x / scale (the exact
+                        quotient) rounded to nearest, ties to even, within +-127; read back as the f32
+                        product scale * code.  A row of zeros has scale 0; a row with an
+                        infinity or NaN is read back as NaNs */
+
+/* A device-resident cache of one layer's keys and values in num_pages pages of
+ * page_tokens tokens (32, 64, ... 1024), each token holding kv_heads rows of
+ * head_dim (64, 96, 128 or 256) for the keys and as many for the values.  A
+ * sequence's token p lies in its page p / page_tokens, wherever the batch's
+ * table puts that page; sequences may share pages that they only read.  The
+ * layout inside a page is the library's own (nx_kv_read gives the values).
+ * No counterpart in the reference, whose KvCache holds one sequence in f32
+ * (src/engine/mod.rs:410-426) on the host. */
+int nx_kv_create(nx_ctx *ctx, int fmt, int num_pages, int page_tokens, int kv_heads,
+                 int head_dim, nx_kv **out);
+int nx_kv_info(const nx_kv *kv, int *fmt, int *num_pages, int *page_tokens, int *kv_heads,
+               int *head_dim, size_t *device_bytes);
+/* Frees the cache's pages (after the device's work in flight); it may be
+ * destroyed before or after its context. */
+int nx_kv_destroy(nx_kv *kv);
+
+/* The sequences that a call works on, one descriptor for all calls of a step.
+ * Sequence s owns rows row_start[s] .. row_start[s + 1] - 1 of the call's
+ * buffers: with n of them, they are its last n tokens, kv_len[s] - n ..
+ * kv_len[s] - 1, so kv_len counts the step's own tokens.  n = 0 leaves a
+ * sequence out.  Rows from row_start[num_seqs] on are padding that no call
+ * touches.  Page p of sequence s is pages[s * max_pages + p].
+ * The struct itself is host memory, read during the call; its arrays are device
+ * memory for *_dev calls (read when the kernels run, so a captured graph
+ * follows lengths and tables that change between replays) and host memory for
+ * the others.  *_dev calls cannot refuse what the arrays hold: there, tokens
+ * before the first one, behind max_pages pages or on a page that the cache does
+ * not have are not written, not attended to and read as zeros, and row ranges are
+ * cut to num_tokens.  Sequences that share rows, or that write one token's
+ * place, get the values of either. */
+typedef struct nx_kv_batch {
+  int num_seqs;
+  int num_tokens;           /* rows of the call's buffers */
+  int max_pages;            /* entries of a sequence's table */
+  const int32_t *row_start; /* [num_seqs + 1], non-decreasing, at most num_tokens */
+  const int32_t *kv_len;    /* [num_seqs] */
+  const int32_t *pages;     /* [num_seqs x max_pages] */
+} nx_kv_batch;
+
+/* Writes the batch's tokens into their pages, quantized to the cache's format:
+ * row r's keys are the kv_heads * head_dim floats at k + r * stride, its values
+ * those at v + r * stride (stride in floats, so k and v may be columns of one
+ * fused projection's rows).  KvCache::add (src/engine/mod.rs:410-426) for a
+ * batch.  Host calls also refuse rows, lengths, pages that are not there
+ * and two sequences that write one token's place. */
+int nx_kv_write(nx_ctx *ctx, nx_kv *kv, const nx_kv_batch *batch, const float *k, const float *v,
+                size_t stride);
+int nx_kv_write_dev(nx_ctx *ctx, nx_kv *kv, const nx_kv_batch *batch, const float *d_k,
+                    const float *d_v, size_t stride);
+/* Reads the batch's tokens back as f32, rows as in nx_kv_write (kv_len = n reads
+ * a sequence whole). */
+int nx_kv_read(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float *k, float *v,
+               size_t stride);
+int nx_kv_read_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float *d_k, float *d_v,
+                   size_t stride);
+
+/* Causal attention of the batch's tokens over their sequences in the cache, the
+ * tokens themselves included (write them first): with p the row's token,
+ *   out[r][h] = sum_j softmax_j(scale q[r][h] . k_j) v_j
+ * over the tokens j <= p that it sees, h = 0 .. heads - 1 reading key/value head
+ * h / (heads / kv_heads).  window = 0: all of them; window > 0: its last
+ * `window` tokens (itself included) and the sequence's first `sinks` tokens.  A
+ * row that sees no token is zeros.  q rows are heads * head_dim floats, q_stride
+ * floats apart, out rows likewise; neither needs an alignment.  f32 in and
+ * out: scores, softmax and sums are held in f32, and the f32 factors of the
+ * f16 matrix products are split into two halves (relative error about 1e-6
+ * against the same cache in 64 bits).  A row's last bits depend on the batch
+ * that it is in (the order of the sums does), not on the run.
+ * attention_decode (src/engine/mod.rs:452-500) and
+ * kernel::grouped_query_attention (src/kernel/mod.rs:40-99) for a batch.
+ * The workspace is the context's, allocated with the first cache or call on it
+ * and never moved, so a captured call may be replayed while the context lives;
+ * calls on one context must not overlap in time (two graphs captured from it
+ * neither). */
+int nx_attention(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *q,
+                 size_t q_stride, int heads, float scale, int window, int sinks, float *out,
+                 size_t out_stride);
+int nx_attention_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *d_q,
+                     size_t q_stride, int heads, float scale, int window, int sinks, float *d_out,
+                     size_t out_stride);
 
 /* ---------------------------------------------------------------- GGUF */
 typedef struct nx_gguf nx_gguf;

@@ -30,6 +30,7 @@ SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 PATH_AUTO, PATH_GEMV, PATH_MFMA_F16, PATH_MFMA_BF16, PATH_MFMA_SPLIT = 0, 1, 2, 3, 4
 ROLE_GATE, ROLE_UP, ROLE_DOWN = 0, 1, 2
 EXPERT_SHARED = -1
+KV_F16, KV_INT8 = 0, 1
 FORMAT_NAMES = {F32: "F32", Q4_0: "Q4_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q2_K: "Q2_K", F16: "F16",
                 BF16: "BF16"}
 BLOCK = {Q4_0: (32, 18), Q8_0: (32, 34), Q4_K: (256, 144), Q2_K: (256, 84), F32: (1, 4),
@@ -50,6 +51,8 @@ EXPORTS = [
     "nx_rms_norm_dev", "nx_moe_block", "nx_moe_block_dev", "nx_matrix_create",
     "nx_matrix_load", "nx_matrix_info", "nx_matrix_destroy", "nx_matvec", "nx_matvec_dev",
     "nx_matrix_load_gguf", "nx_moe_last_routes", "nx_moe_forward_noalloc",
+    "nx_kv_create", "nx_kv_info", "nx_kv_destroy", "nx_kv_write", "nx_kv_write_dev",
+    "nx_kv_read", "nx_kv_read_dev", "nx_attention", "nx_attention_dev",
 ]
 
 _lib = None
@@ -57,6 +60,11 @@ _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)
 _i32p = C.POINTER(C.c_int32)
 _ip = C.POINTER(C.c_int)
+
+
+class _KvBatch(C.Structure):
+    _fields_ = [("num_seqs", C.c_int), ("num_tokens", C.c_int), ("max_pages", C.c_int),
+                ("row_start", _vp), ("kv_len", _vp), ("pages", _vp)]
 
 
 class NexusError(RuntimeError):
@@ -151,6 +159,19 @@ def lib():
         "nx_moe_last_routes": ([_vp, C.c_int, C.c_int, _i32p, _fp, _i32p], C.c_int),
         "nx_moe_forward_noalloc": ([_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
                                     _vp], C.c_int),
+    })
+    _kvb = C.POINTER(_KvBatch)
+    rows = [_vp, _vp, _kvb, _vp, _vp, C.c_size_t]
+    attention = [_vp, _vp, _kvb, _vp, C.c_size_t, C.c_int, C.c_float, C.c_int, C.c_int, _vp,
+                 C.c_size_t]
+    sig.update({
+        "nx_kv_create": ([_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(_vp)],
+                         C.c_int),
+        "nx_kv_info": ([_vp, _ip, _ip, _ip, _ip, _ip, _szp], C.c_int),
+        "nx_kv_destroy": ([_vp], C.c_int),
+        "nx_kv_write": (rows, C.c_int), "nx_kv_write_dev": (rows, C.c_int),
+        "nx_kv_read": (rows, C.c_int), "nx_kv_read_dev": (rows, C.c_int),
+        "nx_attention": (attention, C.c_int), "nx_attention_dev": (attention, C.c_int),
     })
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -479,6 +500,109 @@ class Matrix:
     def close(self):
         if self.h:
             lib().nx_matrix_destroy(self.h)
+            self.h = None
+
+    def __del__(self, _finalizing=sys.is_finalizing):
+        # bound at definition: module globals may already be None at exit
+        if _finalizing():  # the process is ending: leave it to the OS
+            return
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KvBatch:
+    """The sequences of a step (nx_kv_batch) by the addresses of int32 arrays on the
+    device: rows [seqs + 1], lengths [seqs] with the step's own tokens, and page
+    tables [seqs x max_pages].  The arrays must outlive the descriptor's use."""
+
+    def __init__(self, num_seqs: int, num_tokens: int, max_pages: int, row_start_ptr: int,
+                 kv_len_ptr: int, pages_ptr: int):
+        self.c = _KvBatch(num_seqs, num_tokens, max_pages, row_start_ptr, kv_len_ptr, pages_ptr)
+        self.ref = C.byref(self.c)
+
+
+class KvCache:
+    """A device-resident paged cache of one layer's keys and values."""
+
+    def __init__(self, ctx: Context, fmt: int, num_pages: int, page_tokens: int, kv_heads: int,
+                 head_dim: int):
+        self.h = None
+        h = _vp()
+        check(lib().nx_kv_create(ctx.h, fmt, num_pages, page_tokens, kv_heads, head_dim,
+                                 C.byref(h)))
+        self.h, self.ctx, self.fmt = h, ctx, fmt
+        self.num_pages, self.page_tokens = num_pages, page_tokens
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+
+    def device_bytes(self) -> int:
+        b = C.c_size_t(0)
+        check(lib().nx_kv_info(self.h, None, None, None, None, None, C.byref(b)))
+        return b.value
+
+    # ---- device memory (asynchronous on the context's stream)
+    def write_dev(self, batch: KvBatch, k_ptr: int, v_ptr: int, stride: int) -> None:
+        check(lib().nx_kv_write_dev(self.ctx.h, self.h, batch.ref, k_ptr, v_ptr, stride))
+
+    def read_dev(self, batch: KvBatch, k_ptr: int, v_ptr: int, stride: int) -> None:
+        check(lib().nx_kv_read_dev(self.ctx.h, self.h, batch.ref, k_ptr, v_ptr, stride))
+
+    def attention_dev(self, batch: KvBatch, q_ptr: int, q_stride: int, heads: int, out_ptr: int,
+                      out_stride: int, scale: float, window: int = 0, sinks: int = 0) -> None:
+        check(lib().nx_attention_dev(self.ctx.h, self.h, batch.ref, q_ptr, q_stride, heads, scale,
+                                     window, sinks, out_ptr, out_stride))
+
+    # ---- host arrays
+    def _host_batch(self, row_start, kv_len, pages, rows: int):
+        rs = np.ascontiguousarray(row_start, np.int32)
+        ln = np.ascontiguousarray(kv_len, np.int32)
+        pg = np.ascontiguousarray(pages, np.int32)
+        pg = pg.reshape(ln.size, -1)
+        if rs.size != ln.size + 1:
+            raise ValueError(f"{rs.size} row starts for {ln.size} sequences")
+        return KvBatch(ln.size, rows, pg.shape[1], rs.ctypes.data, ln.ctypes.data,
+                       pg.ctypes.data), (rs, ln, pg)
+
+    def _rows(self, x, width: int) -> np.ndarray:
+        x = _f32(x)
+        if x.size % width:
+            raise ValueError(f"{x.size} values are no rows of {width}")
+        return x.reshape(-1, width)
+
+    def write(self, row_start, kv_len, pages, k, v) -> None:
+        """Rows of k and v [rows x kv_heads * head_dim] into their sequences' pages."""
+        width = self.kv_heads * self.head_dim
+        k, v = self._rows(k, width), self._rows(v, width)
+        if k.shape != v.shape:
+            raise ValueError(f"{len(k)} rows of keys and {len(v)} of values")
+        b, _keep = self._host_batch(row_start, kv_len, pages, len(k))
+        check(lib().nx_kv_write(self.ctx.h, self.h, b.ref, k.ctypes.data, v.ctypes.data, width))
+
+    def read(self, row_start, kv_len, pages, rows: int | None = None):
+        """The keys and values [rows x kv_heads x head_dim] of the sequences' last tokens."""
+        n = int(np.asarray(row_start).ravel()[-1]) if rows is None else rows
+        k = np.zeros((n, self.kv_heads, self.head_dim), np.float32)
+        v = np.zeros_like(k)
+        b, _keep = self._host_batch(row_start, kv_len, pages, n)
+        check(lib().nx_kv_read(self.ctx.h, self.h, b.ref, k.ctypes.data, v.ctypes.data,
+                               self.kv_heads * self.head_dim))
+        return k, v
+
+    def attention(self, row_start, kv_len, pages, q, heads: int, scale: float | None = None,
+                  window: int = 0, sinks: int = 0) -> np.ndarray:
+        """out [rows x heads x head_dim] of q's rows; scale: 1 / sqrt(head_dim) by default."""
+        q = self._rows(q, heads * self.head_dim)
+        out = np.zeros((len(q), heads, self.head_dim), np.float32)
+        b, _keep = self._host_batch(row_start, kv_len, pages, len(q))
+        check(lib().nx_attention(self.ctx.h, self.h, b.ref, q.ctypes.data, q.shape[1], heads,
+                                 self.head_dim ** -0.5 if scale is None else scale, window, sinks,
+                                 out.ctypes.data, q.shape[1]))
+        return out
+
+    def close(self):
+        if self.h:
+            lib().nx_kv_destroy(self.h)
             self.h = None
 
     def __del__(self, _finalizing=sys.is_finalizing):

@@ -168,6 +168,8 @@ enum WsSlot {
   WS_MFV_PART, // partial sums and records of the split-activation MFMA path
   WS_TILES_DOWN, // grouped-GEMM tile list of the down pass
   WS_PERM_CHUNK, // per-chunk expert counts of the many-workgroup permutation
+  WS_KV_BATCH,   // device copy of a batch's arrays for blocking calls
+  WS_ATTN,       // partial results of the attention (one size, never moved)
   WS_COUNT
 };
 static_assert(WS_COUNT <= 32, "workspace slots of a context");

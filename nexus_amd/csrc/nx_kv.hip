@@ -1,0 +1,382 @@
+// nx_kv.hip — the paged key/value cache: its pages, writing tokens into them
+// (quantised to the cache's format) and reading them back.
+//
+// Both kernels move each value once: they are bound by memory, and a workgroup
+// takes one head's group of 32 tokens (nx_kv_plan.hpp), turning rows of f32 into
+// the group's operand order, or back, through LDS, so that both sides are whole
+// 16-byte runs.
+#include <hip/hip_runtime.h>
+
+#include "nx_kv_dev.hpp"
+
+namespace nx {
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+// x / s rounded to nearest, ties to even, from the exact quotient: n = rint of
+// the rounded quotient is off by one at most, and x - n s is exact (both are
+// multiples of a last place of x or s and |x - n s| < s), so comparing it with
+// s / 2 decides as the quotient would.
+__device__ __forceinline__ int code_of(float x, float s, float inv) {
+  float n = rintf(x * inv);
+  const float r = fmaf(-n, s, x), h = 0.5f * s;
+  const bool odd = ((int)n & 1) != 0;
+  if (r > h || (r == h && odd)) n += 1.f;
+  if (r < -h || (r == -h && odd)) n -= 1.f;
+  return (int)n;
+}
+
+// 8 threads of a token: float4 `4 (sub + 8 j)` of its row in v[j]
+template <int D>
+__device__ __forceinline__ void load_row(const float *row, int sub, bool wide, float4 (&v)[D / 32]) {
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    const float *p = row + 4 * (sub + 8 * j);
+    v[j] = wide ? *reinterpret_cast<const float4 *>(p) : float4{p[0], p[1], p[2], p[3]};
+  }
+}
+
+// The row's values in the cache's format into `tile` (a group in its layout).
+// Returns the row's scale (INT8).
+template <int FMT, int D, bool KEYS>
+__device__ __forceinline__ float stage_row(const float4 (&v)[D / 32], int t, int sub,
+                                           kv_elem<FMT> *tile) {
+  float scale = 0.f, inv = 0.f;
+  bool fine = true;
+  if constexpr (FMT == NX_KV_INT8) {
+    // NaN would be lost in a maximum: x - x is 0 for finite x only
+    float mx = 0.f, odd = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      mx = fmaxf(fmaxf(mx, fmaxf(fabsf(v[j].x), fabsf(v[j].y))), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
+      odd += (v[j].x - v[j].x) + (v[j].y - v[j].y) + (v[j].z - v[j].z) + (v[j].w - v[j].w);
+    }
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) {
+      mx = fmaxf(mx, __shfl_xor(mx, d, 8));
+      odd += __shfl_xor(odd, d, 8);
+    }
+    fine = odd == 0.f;
+    scale = fine ? mx / 127.0f : NAN;
+    inv = 1.0f / scale;
+    // a scale so small that its inverse may not be finite, or that is itself
+    // rounded far down, divides in 64 bits below
+  }
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+    const int d0 = 4 * (sub + 8 * j);
+    kv_elem<FMT> q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (FMT == NX_KV_INT8) {
+        if (!fine || scale == 0.f)
+          q[i] = 0;
+        else if (scale < 0x1p-120f)
+          q[i] = (int8_t)fmin(fmax(rint((double)e[i] / (double)scale), -127.0), 127.0);
+        else
+          q[i] = (int8_t)code_of(e[i], scale, inv);
+      } else {
+        q[i] = (_Float16)e[i];
+      }
+    }
+    if constexpr (KEYS) {  // four neighbouring elements of one chunk
+      kv_elem<FMT> *o = tile + kv_key_at(FMT, t, d0);
+      if constexpr (FMT == NX_KV_INT8)
+        *reinterpret_cast<char4 *>(o) = make_char4(q[0], q[1], q[2], q[3]);
+      else
+        *reinterpret_cast<f16x4 *>(o) = f16x4{q[0], q[1], q[2], q[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tile[kv_value_at(D, t, d0 + i)] = q[i];
+    }
+  }
+  return scale;
+}
+
+// item of a batch: group `at` of sequence s's touched groups
+__device__ __forceinline__ long touched(const KvSeq &q) {
+  const int lo = max(q.first, 0);
+  return q.n > 0 && q.len > lo ? (q.len - 1) / kKvGroup - lo / kKvGroup + 1 : 0;
+}
+
+template <int FMT, int D>
+__global__ __launch_bounds__(256) void k_kv_write(KvView kv, nx_kv_batch b, const float *k,
+                                                  const float *v, size_t stride, bool wide) {
+  using E = kv_elem<FMT>;
+  using Chunk = std::conditional_t<FMT == NX_KV_INT8, uint2, uint4>;  // 8 elements
+  __shared__ __align__(16) E tile[2][kKvGroup * D];
+  __shared__ long sums[4];
+  __shared__ Place place;
+  const int head = blockIdx.x % kv.heads;
+  const Place at = find_item(
+      b.num_seqs, blockIdx.x / kv.heads, [&](int s) { return touched(kv_seq(b, s, kv.page_log2)); },
+      sums, &place);
+  if (at.s < 0) return;
+  const KvSeq q = kv_seq(b, at.s, kv.page_log2);
+  const int g0 = (max(q.first, 0) / kKvGroup + (int)at.at) * kKvGroup;  // the group's first token
+  const long group = kv_group(kv, b, at.s, head, g0);
+  if (group < 0) return;
+  // its tokens that the batch has: [lo, hi)
+  const int lo = max(q.first - g0, 0), hi = min(q.len - g0, kKvGroup);
+
+  const int t = threadIdx.x >> 3, sub = threadIdx.x & 7;
+  if (t >= lo && t < hi) {
+    const size_t row = (size_t)(q.row + (g0 + t - q.first)) * stride + (size_t)head * D;
+    float4 r[D / 32];
+    load_row<D>(k + row, sub, wide, r);
+    const float s = stage_row<FMT, D, true>(r, t, sub, tile[0]);
+    if (FMT == NX_KV_INT8 && sub == 0) kv.ks[group * kKvGroup + t] = s;
+    load_row<D>(v + row, sub, wide, r);
+    const float sv = stage_row<FMT, D, false>(r, t, sub, tile[1]);
+    if (FMT == NX_KV_INT8 && sub == 0) kv.vs[group * kKvGroup + t] = sv;
+  }
+  __syncthreads();
+  E *gk = reinterpret_cast<E *>(kv.k) + group * (kKvGroup * D);
+  E *gv = reinterpret_cast<E *>(kv.v) + group * (kKvGroup * D);
+  for (int c = threadIdx.x; c < kKvGroup * D / 8; c += 256) {
+    const int token = kv_token(FMT, c & (kKvGroup - 1));
+    if (token >= lo && token < hi)
+      reinterpret_cast<Chunk *>(gk)[c] = reinterpret_cast<const Chunk *>(tile[0])[c];
+    // a value chunk: tokens t0 .. t0 + 7 of one element; other tokens of it may
+    // be in the cache already
+    const int t0 = c / D * 8;
+    if (t0 >= lo && t0 + 8 <= hi) {
+      reinterpret_cast<Chunk *>(gv)[c] = reinterpret_cast<const Chunk *>(tile[1])[c];
+    } else {
+      for (int i = max(lo - t0, 0); i < min(hi - t0, 8); ++i) gv[8 * c + i] = tile[1][8 * c + i];
+    }
+  }
+}
+
+template <int FMT, int D>
+__global__ __launch_bounds__(256) void k_kv_read(KvView kv, nx_kv_batch b, float *k, float *v,
+                                                 size_t stride, bool wide) {
+  using E = kv_elem<FMT>;
+  using Chunk = std::conditional_t<FMT == NX_KV_INT8, uint2, uint4>;
+  __shared__ __align__(16) E tile[2][kKvGroup * D];
+  __shared__ long sums[4];
+  __shared__ Place place;
+  const int head = blockIdx.x % kv.heads;
+  // rows without a token (before the first, behind the table) are read as zeros:
+  // items cover the rows, in the groups that their tokens would have
+  const Place at = find_item(
+      b.num_seqs, blockIdx.x / kv.heads,
+      [&](int s) {
+        const KvSeq q = kv_seq(b, s, kv.page_log2);
+        return q.n > 0 ? (long)((q.first + q.n - 1) >> 5) - (q.first >> 5) + 1 : 0;
+      },
+      sums, &place);
+  if (at.s < 0) return;
+  const KvSeq q = kv_seq(b, at.s, kv.page_log2);
+  const int g0 = ((q.first >> 5) + (int)at.at) * kKvGroup;
+  const bool there = g0 >= 0 && g0 < (b.max_pages << kv.page_log2);
+  const long group = there ? kv_group(kv, b, at.s, head, g0) : -1;
+  const int lo = max(q.first - g0, 0), hi = min(q.first + q.n - g0, kKvGroup);
+  if (group >= 0) {
+    const Chunk *gk = reinterpret_cast<const Chunk *>(kv.k) + group * (kKvGroup * D / 8);
+    const Chunk *gv = reinterpret_cast<const Chunk *>(kv.v) + group * (kKvGroup * D / 8);
+    for (int c = threadIdx.x; c < kKvGroup * D / 8; c += 256) {
+      const int token = kv_token(FMT, c & (kKvGroup - 1)), t0 = c / D * 8;
+      if (token >= lo && token < hi) reinterpret_cast<Chunk *>(tile[0])[c] = gk[c];
+      if (t0 + 8 > lo && t0 < hi) reinterpret_cast<Chunk *>(tile[1])[c] = gv[c];
+    }
+  }
+  __syncthreads();
+  const int t = threadIdx.x >> 3, sub = threadIdx.x & 7;
+  if (t < lo || t >= hi) return;
+  const size_t row = (size_t)(q.row + (g0 + t - q.first)) * stride + (size_t)head * D;
+  const float sk = FMT == NX_KV_INT8 && group >= 0 ? kv.ks[group * kKvGroup + t] : 1.f;
+  const float sv = FMT == NX_KV_INT8 && group >= 0 ? kv.vs[group * kKvGroup + t] : 1.f;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    const int d0 = 4 * (sub + 8 * j);
+    float ek[4], ev[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ek[i] = group >= 0 ? (float)tile[0][kv_key_at(FMT, t, d0 + i)] * sk : 0.f;
+      ev[i] = group >= 0 ? (float)tile[1][kv_value_at(D, t, d0 + i)] * sv : 0.f;
+    }
+    if (wide) {
+      *reinterpret_cast<float4 *>(k + row + d0) = float4{ek[0], ek[1], ek[2], ek[3]};
+      *reinterpret_cast<float4 *>(v + row + d0) = float4{ev[0], ev[1], ev[2], ev[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        k[row + d0 + i] = ek[i];
+        v[row + d0 + i] = ev[i];
+      }
+    }
+  }
+}
+
+static bool wide_rows(const void *a, const void *b, size_t stride) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0 && stride % 4 == 0;
+}
+
+static int kv_move_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, const float *rk,
+                       const float *rv, float *wk, float *wv, size_t stride, bool write) {
+  const long groups = kv_touched_groups(b.num_seqs, b.num_tokens);
+  if (groups * kv->heads > INT32_MAX)
+    return fail(NX_ERR_UNSUPPORTED, "a batch of more than 2^31 groups of tokens");
+  const dim3 grid((uint32_t)(groups * kv->heads));
+  const KvView view = view_of(kv);
+  return launch(c, write ? "kv_write" : "kv_read", [&] {
+    with_kernel(kv, [&](auto fmt, auto D) {
+      if (write)
+        go(c, k_kv_write<fmt(), D()>, grid, dim3(256), 0, view, b, rk, rv, stride,
+           wide_rows(rk, rv, stride));
+      else
+        go(c, k_kv_read<fmt(), D()>, grid, dim3(256), 0, view, b, wk, wv, stride,
+           wide_rows(wk, wv, stride));
+    });
+  });
+}
+
+int kv_check_call(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b) {
+  if (!c) return fail(NX_ERR_INVALID_ARG, "null context");
+  NX_HIP(hipSetDevice(c->device));
+  if (!kv) return fail(NX_ERR_INVALID_ARG, "null cache");
+  if (kv->device != c->device)
+    return fail(NX_ERR_INVALID_ARG, "the cache lives on device " + std::to_string(kv->device) +
+                                        ", the context on " + std::to_string(c->device));
+  return refuse(kv_check_batch(b, kv->page_tokens));
+}
+
+int kv_upload_batch(nx_ctx *c, const nx_kv_batch &b, nx_kv_batch *dev) {
+  const size_t S = b.num_seqs, table = S * b.max_pages;
+  void *p = nullptr;
+  NX_TRY(ws_get(c, WS_KV_BATCH, (2 * S + 1 + table) * 4, &p));
+  int32_t *d = static_cast<int32_t *>(p);
+  NX_HIP(hipMemcpyAsync(d, b.row_start, (S + 1) * 4, hipMemcpyHostToDevice, c->stream));
+  NX_HIP(hipMemcpyAsync(d + S + 1, b.kv_len, S * 4, hipMemcpyHostToDevice, c->stream));
+  NX_HIP(hipMemcpyAsync(d + 2 * S + 1, b.pages, table * 4, hipMemcpyHostToDevice, c->stream));
+  *dev = b;
+  dev->row_start = d;
+  dev->kv_len = d + S + 1;
+  dev->pages = d + 2 * S + 1;
+  return NX_OK;
+}
+
+static int kv_move(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const float *rk,
+                   const float *rv, float *wk, float *wv, size_t stride, bool write, bool host) {
+  NX_TRY(kv_check_call(c, kv, b));
+  const long width = (long)kv->heads * kv->D;
+  if (b->num_seqs == 0 || b->num_tokens == 0) return NX_OK;
+  if (write ? !rk || !rv : !wk || !wv) return fail(NX_ERR_INVALID_ARG, "null buffer");
+  if (stride > (size_t)1 << 40) return fail(NX_ERR_UNSUPPORTED, "row stride above 2^40");
+  NX_TRY(refuse(kv_check_rows("key and value", (long)stride, width)));
+  if (!host) return kv_move_dev(c, kv, *b, rk, rv, wk, wv, stride, write);
+  NX_TRY(refuse(kv_check_tables(*b, kv->pages, kv->page_tokens, false, write)));
+  // rows are packed on the device; padding rows do not travel
+  const size_t rows = b->row_start[b->num_seqs];
+  if (rows == 0) return NX_OK;
+  nx_kv_batch dev;
+  NX_TRY(kv_upload_batch(c, *b, &dev));
+  void *dk, *dv;
+  NX_TRY(ws_get(c, WS_XIN, rows * width * 4, &dk));
+  NX_TRY(ws_get(c, WS_OUT, rows * width * 4, &dv));
+  float *fk = static_cast<float *>(dk), *fv = static_cast<float *>(dv);
+  const size_t line = (size_t)width * 4, pitch = stride * 4;
+  if (write) {
+    NX_HIP(hipMemcpy2DAsync(fk, line, rk, pitch, line, rows, hipMemcpyHostToDevice, c->stream));
+    NX_HIP(hipMemcpy2DAsync(fv, line, rv, pitch, line, rows, hipMemcpyHostToDevice, c->stream));
+  }
+  NX_TRY(kv_move_dev(c, kv, dev, fk, fv, fk, fv, width, write));
+  if (!write) {
+    // rows that no sequence owns (below row_start[0]) keep what the caller had
+    const size_t r0 = b->row_start[0];
+    NX_HIP(hipMemcpy2DAsync(wk + r0 * stride, pitch, fk + r0 * width, line, line, rows - r0,
+                            hipMemcpyDeviceToHost, c->stream));
+    NX_HIP(hipMemcpy2DAsync(wv + r0 * stride, pitch, fv + r0 * width, line, line, rows - r0,
+                            hipMemcpyDeviceToHost, c->stream));
+  }
+  NX_HIP(hipStreamSynchronize(c->stream));
+  return NX_OK;
+}
+
+}  // namespace nx
+
+using namespace nx;
+
+extern "C" {
+
+int nx_kv_create(nx_ctx *c, int fmt, int pages, int page_tokens, int heads, int D, nx_kv **out) {
+  if (out) *out = nullptr;
+  if (!c) return fail(NX_ERR_INVALID_ARG, "null context");
+  if (!out) return fail(NX_ERR_INVALID_ARG, "null output pointer");
+  NX_TRY(refuse(kv_check_geometry(fmt, pages, page_tokens, heads, D)));
+  NX_HIP(hipSetDevice(c->device));
+  NX_TRY(attn_workspace(c, nullptr));
+  const size_t plane = kv_plane_bytes(fmt, pages, page_tokens, heads, D);
+  const size_t scales = kv_scale_bytes(fmt, pages, page_tokens, heads);
+  nx_kv *kv = new nx_kv();
+  kv->ctx = c;
+  kv->device = c->device;
+  kv->fmt = fmt;
+  kv->pages = pages;
+  kv->page_tokens = page_tokens;
+  kv->heads = heads;
+  kv->D = D;
+  // cleared once: what lies behind a sequence's last token enters products with
+  // probability 0 and has to be finite for that to be 0
+  auto alloc = [&](size_t bytes, void **p) {
+    if (!bytes) return (int)NX_OK;
+    if (hipMalloc(p, bytes) != hipSuccess) {
+      (void)hipGetLastError();
+      *p = nullptr;
+      return fail(NX_ERR_OOM, "device allocation of " + std::to_string(bytes) + " bytes failed");
+    }
+    kv->device_bytes += bytes;
+    NX_HIP(hipMemsetAsync(*p, 0, bytes, c->stream));
+    return (int)NX_OK;
+  };
+  int rc = alloc(plane, reinterpret_cast<void **>(&kv->k));
+  if (!rc) rc = alloc(plane, reinterpret_cast<void **>(&kv->v));
+  if (!rc) rc = alloc(scales, reinterpret_cast<void **>(&kv->ks));
+  if (!rc) rc = alloc(scales, reinterpret_cast<void **>(&kv->vs));
+  if (!rc && hipStreamSynchronize(c->stream) != hipSuccess) rc = fail(NX_ERR_DEVICE, "clearing the cache failed");
+  if (rc) {
+    const std::string why = nx_last_error();
+    nx_kv_destroy(kv);
+    return fail(rc, why);
+  }
+  *out = kv;
+  return NX_OK;
+}
+
+int nx_kv_info(const nx_kv *kv, int *fmt, int *pages, int *page_tokens, int *heads, int *D, size_t *bytes) {
+  if (!kv) return fail(NX_ERR_INVALID_ARG, "null cache");
+  if (fmt) *fmt = kv->fmt;
+  if (pages) *pages = kv->pages;
+  if (page_tokens) *page_tokens = kv->page_tokens;
+  if (heads) *heads = kv->heads;
+  if (D) *D = kv->D;
+  if (bytes) *bytes = kv->device_bytes;
+  return NX_OK;
+}
+
+int nx_kv_destroy(nx_kv *kv) {
+  if (!kv) return NX_OK;
+  (void)hipSetDevice(kv->device);
+  for (void *p : {(void *)kv->k, (void *)kv->v, (void *)kv->ks, (void *)kv->vs})
+    if (p) (void)hipFree(p);
+  delete kv;
+  return NX_OK;
+}
+
+int nx_kv_write(nx_ctx *c, nx_kv *kv, const nx_kv_batch *b, const float *k, const float *v, size_t stride) {
+  return kv_move(c, kv, b, k, v, nullptr, nullptr, stride, true, true);
+}
+int nx_kv_write_dev(nx_ctx *c, nx_kv *kv, const nx_kv_batch *b, const float *k, const float *v,
+                    size_t stride) {
+  return kv_move(c, kv, b, k, v, nullptr, nullptr, stride, true, false);
+}
+int nx_kv_read(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, float *k, float *v, size_t stride) {
+  return kv_move(c, kv, b, nullptr, nullptr, k, v, stride, false, true);
+}
+int nx_kv_read_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, float *k, float *v, size_t stride) {
+  return kv_move(c, kv, b, nullptr, nullptr, k, v, stride, false, false);
+}
+
+}  // extern "C"

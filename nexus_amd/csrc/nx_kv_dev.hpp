@@ -1,0 +1,134 @@
+// nx_kv_dev.hpp — what the kernels of the paged cache (nx_kv.hip) and of the
+// attention that reads it (nx_attn.hip) share: the device view of a cache and
+// of a batch, and finding a workgroup's work in a batch whose lengths only the
+// device knows.
+#pragma once
+
+#include <type_traits>
+
+#include "nx_device.hpp"
+#include "nx_internal.hpp"
+#include "nx_kv_plan.hpp"
+
+struct nx_kv {
+  nx_ctx *ctx = nullptr;  // compared, never followed, once the cache exists
+  int device = 0;
+  int fmt = 0, pages = 0, page_tokens = 0, heads = 0, D = 0;
+  uint8_t *k = nullptr, *v = nullptr;
+  float *ks = nullptr, *vs = nullptr;  // INT8: scales [pages][heads][page_tokens]
+  size_t device_bytes = 0;
+};
+
+namespace nx {
+
+// the attention's workspace on a context: allocated once, never moved
+int attn_workspace(nx_ctx *c, void **out);
+int kv_check_call(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b);
+// copies a host batch's arrays to the device; *dev describes them there
+int kv_upload_batch(nx_ctx *c, const nx_kv_batch &b, nx_kv_batch *dev);
+
+struct KvView {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int pages, page_log2, heads;
+};
+inline KvView view_of(const nx_kv *kv) {
+  return {kv->k, kv->v, kv->ks, kv->vs, kv->pages, __builtin_ctz(kv->page_tokens), kv->heads};
+}
+
+// One sequence of a batch, cut to what is there.
+struct KvSeq {
+  int row, n;  // first row, rows
+  int first;   // token of row `row` (below 0 where the batch says so)
+  int len;     // tokens that can be read: kv_len, at most the table's
+};
+
+__device__ __forceinline__ KvSeq kv_seq(const nx_kv_batch &b, int s, int page_log2) {
+  const int r0 = min(max(b.row_start[s], 0), b.num_tokens);
+  const int r1 = min(max(b.row_start[s + 1], r0), b.num_tokens);
+  const int len = max(b.kv_len[s], 0);
+  return {r0, r1 - r0, len - (r1 - r0), min(len, b.max_pages << page_log2)};
+}
+
+// The group of 32 tokens that holds token `first` of sequence s, as an index of
+// groups over the whole pool ([pages][heads][groups of a page]); -1 if the cache has no such page.
+__device__ __forceinline__ long kv_group(const KvView &kv, const nx_kv_batch &b, int s, int head,
+                                         int first) {
+  const int page = b.pages[(long)s * b.max_pages + (first >> kv.page_log2)];
+  if (page < 0 || page >= kv.pages) return -1;
+  const int in_page = (first & ((1 << kv.page_log2) - 1)) / kKvGroup;
+  return (((long)page * kv.heads + head) << (kv.page_log2 - 5)) + in_page;
+}
+
+// Inclusive sum over the workgroup's first 256 threads (blockDim.x == 256).
+__device__ __forceinline__ long scan256(long v, long *lds4) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const long o = __shfl_up(v, d, 64);
+    if (lane >= d) v += o;
+  }
+  __syncthreads();  // the last call's reads of lds4
+  if (lane == 63) lds4[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v += lds4[w];
+  return v;
+}
+
+// Which sequence holds item `item` when sequence s has count(s) of them, and
+// which of its items that is; *s = -1 past the last one.  All 256 threads.
+struct Place {
+  int s;
+  long at;
+};
+template <typename Count>
+__device__ __forceinline__ Place find_item(int seqs, long item, Count count, long *lds4, Place *lds) {
+  if (threadIdx.x == 0) *lds = {-1, 0};
+  long before = 0;
+  for (int s0 = 0; s0 < seqs; s0 += 256) {
+    const int s = s0 + (int)threadIdx.x;
+    const long c = s < seqs ? count(s) : 0;
+    const long end = before + scan256(c, lds4);
+    if (c > 0 && item >= end - c && item < end) *lds = {s, item - (end - c)};
+    before += lds4[0] + lds4[1] + lds4[2] + lds4[3];
+    if (item < before) break;  // uniform: every thread has the same sums
+  }
+  __syncthreads();
+  return *lds;
+}
+
+// The sequence that owns row `row`; -1 for padding.  All 256 threads.
+__device__ __forceinline__ int find_row(const nx_kv_batch &b, int row, int page_log2, int *lds) {
+  if (threadIdx.x == 0) *lds = -1;
+  __syncthreads();
+  for (int s = threadIdx.x; s < b.num_seqs; s += 256) {
+    const KvSeq q = kv_seq(b, s, page_log2);
+    if (row >= q.row && row < q.row + q.n) *lds = s;
+  }
+  __syncthreads();
+  return *lds;
+}
+
+// f(format, head_dim) as constants
+template <typename F>
+void with_kernel(const nx_kv *kv, F f) {
+  auto dims = [&](auto fmt) {
+    switch (kv->D) {
+    case 64: f(fmt, std::integral_constant<int, 64>()); break;
+    case 96: f(fmt, std::integral_constant<int, 96>()); break;
+    case 128: f(fmt, std::integral_constant<int, 128>()); break;
+    default: f(fmt, std::integral_constant<int, 256>()); break;
+    }
+  };
+  if (kv->fmt == NX_KV_INT8)
+    dims(std::integral_constant<int, NX_KV_INT8>());
+  else
+    dims(std::integral_constant<int, NX_KV_F16>());
+}
+
+template <int FMT>
+using kv_elem = std::conditional_t<FMT == NX_KV_INT8, int8_t, _Float16>;
+
+inline int refuse(const Refusal &r) { return r ? fail(r.code, r.why) : NX_OK; }
+
+}  // namespace nx
