@@ -44,19 +44,18 @@ __device__ __forceinline__ float stage_row(const float4 (&v)[D / 32], int t, int
   float scale = 0.f, inv = 0.f;
   bool fine = true;
   if constexpr (FMT == NX_KV_INT8) {
-    // NaN would be lost in a maximum: x - x is 0 for finite x only
-    float mx = 0.f, odd = 0.f;
+    float mx = 0.f;  // (a maximum loses NaNs)
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       mx = fmaxf(fmaxf(mx, fmaxf(fabsf(v[j].x), fabsf(v[j].y))), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
-      odd += (v[j].x - v[j].x) + (v[j].y - v[j].y) + (v[j].z - v[j].z) + (v[j].w - v[j].w);
+      fine = fine && __builtin_isfinite(v[j].x) && __builtin_isfinite(v[j].y) &&
+             __builtin_isfinite(v[j].z) && __builtin_isfinite(v[j].w);
     }
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) {
       mx = fmaxf(mx, __shfl_xor(mx, d, 8));
-      odd += __shfl_xor(odd, d, 8);
+      fine &= __shfl_xor((int)fine, d, 8) != 0;
     }
-    fine = odd == 0.f;
     scale = fine ? mx / 127.0f : NAN;
     inv = 1.0f / scale;
     // a scale so small that its inverse may not be finite, or that is itself

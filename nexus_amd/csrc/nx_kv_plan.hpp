@@ -151,6 +151,28 @@ inline Refusal kv_check_tables(const nx_kv_batch &b, int num_pages, int page_tok
   return {};
 }
 
+// The groups of 32 tokens that some of the tokens pmin .. pmax of a sequence of
+// len tokens see: [0, sinks) and [from, to).
+struct KeySpan {
+  int sinks, from, to;
+  constexpr int count() const { return sinks + to - from; }
+  // group number i of them
+  constexpr int group(int i) const { return i < sinks ? i : from + (i - sinks); }
+};
+constexpr KeySpan key_span(int pmin, int pmax, int len, int window, int sinks) {
+  const int last = pmax < len - 1 ? pmax : len - 1;
+  const int to = last < 0 ? 0 : last / kKvGroup + 1;
+  int from = 0, first = 0;
+  if (window > 0) {
+    const int lo = pmin - window + 1;  // (pmin >= -2^24, so no overflow)
+    from = lo > 0 ? lo / kKvGroup : 0;
+    if (from > to) from = to;
+    first = sinks / kKvGroup + (sinks % kKvGroup != 0);
+    if (first > from) first = from;
+  }
+  return {first, from, to};
+}
+
 // Groups of 32 tokens that a batch's rows touch, at most: a sequence of n rows
 // touches at most n, and at most n / 32 + 2.
 inline long kv_touched_groups(long seqs, long rows) { return std::min(rows, rows / kKvGroup + 2 * seqs); }
