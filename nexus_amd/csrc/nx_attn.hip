@@ -21,7 +21,15 @@ struct AttnCall {
   float scale;
   int window, sinks;
   bool wide_q, wide_out;  // rows of whole float4 runs
+  uint32_t magic;         // ceil(2^(31 + shift) / group), shift = ceil(log2 group)
+  int shift;
 };
+
+// row / a.group for 0 <= row < 2^31: magic group - 2^(31 + shift) < 2^shift, so the
+// quotient's excess row (magic group - 2^(31 + shift)) / 2^(31 + shift) is below 1 / group's step
+__device__ __forceinline__ int by_group(const AttnCall &a, int row) {
+  return (int)(__umulhi(2u * (uint32_t)row, a.magic) >> a.shift);
+}
 
 // whether token p sees token j <= p
 __device__ __forceinline__ bool sees(const AttnCall &a, int p, int j) {
@@ -150,17 +158,13 @@ struct Tile {
   int seq, head, r0, nr;
 };
 __device__ __forceinline__ KeySpan tile_span(const KvSeq &s, const AttnCall &a, int r0, int nr) {
-  return key_span(s.first + r0 / a.group, s.first + (r0 + nr - 1) / a.group, s.len, a.window, a.sinks);
+  return key_span(s.first + by_group(a, r0), s.first + by_group(a, r0 + nr - 1), s.len, a.window,
+                  a.sinks);
 }
 // units of a tile: at least one, so that rows which see nothing are written
 __device__ __forceinline__ int tile_units(const KvSeq &s, const AttnCall &a, int r0, int tile) {
   const int nr = min(tile, s.n * a.group - r0);
   return max(tile_span(s, a, r0, nr).count(), 1);
-}
-__device__ __forceinline__ long head_units(const KvSeq &s, const AttnCall &a, int tile) {
-  long u = 0;
-  for (int r0 = 0; r0 < s.n * a.group; r0 += tile) u += tile_units(s, a, r0, tile);
-  return u;
 }
 
 // Partial results of tiles that were split: per workgroup, those of the tile that
@@ -170,8 +174,136 @@ __device__ __forceinline__ long head_units(const KvSeq &s, const AttnCall &a, in
 struct AttnWork {
   int4 *desc;
   float *part;
-  int wgs, min_share;
+  int wgs_log2, min_share;
+  int rows_above, rows_upto;  // the kernel's sequences: those of so many rows
 };
+
+// A workgroup's run of units: [begin, end) of all, which starts `off` units into
+// the tile at (seq, head, r0).
+struct Run {
+  long begin, end, share;
+  int seq, head, r0, off;
+};
+struct RunLds {
+  long sums[4];
+  long at, in_head;
+  int seq, bigs, big[256], r0, off;
+};
+
+// what every lane has alike, as a scalar: addresses, bounds and branches on it
+// then cost no vector registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long uniform(long v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  return (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | lo);
+}
+
+// Finds run `wg`.  A sequence's units are summed over its tiles by one thread, or
+// by the workgroup where there are many; sequences are summed by a scan.
+template <int TILE>
+__device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
+                                         const AttnWork &w, int wg, RunLds &lds, Run &r) {
+  constexpr int kFew = 8;
+  const int tid = threadIdx.x;
+  auto rows_of = [&](const KvSeq &q) {
+    const int rows = q.n * a.group;
+    return rows > w.rows_above && rows <= w.rows_upto ? rows : 0;
+  };
+  // per-head units of sequence s0 + tid
+  auto count = [&](int s0) {
+    const KvSeq q = s0 + tid < b.num_seqs ? kv_seq(b, s0 + tid, kv.page_log2) : KvSeq{0, 0, 0, 0};
+    const int rows = rows_of(q);
+    long c = 0;
+    if (tid == 0) lds.bigs = 0;
+    __syncthreads();
+    if (rows <= kFew * TILE)
+      for (int r0 = 0; r0 < rows; r0 += TILE) c += tile_units(q, a, r0, TILE);
+    else
+      lds.big[atomicAdd(&lds.bigs, 1)] = tid;
+    __syncthreads();
+    const int bigs = lds.bigs;
+    for (int i = 0; i < bigs; ++i) {
+      const int t = lds.big[i];
+      const KvSeq o = kv_seq(b, s0 + t, kv.page_log2);
+      long part = 0;
+      for (long r0 = (long)tid * TILE; r0 < o.n * a.group; r0 += 256 * TILE)
+        part += tile_units(o, a, (int)r0, TILE);
+      scan256(part, lds.sums);
+      if (tid == t) c = lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
+    }
+    return c;
+  };
+  long total = 0, c = 0, upto = 0;
+  for (int s0 = 0; s0 < b.num_seqs; s0 += 256) {
+    c = count(s0);
+    upto = total + scan256(c * kv.heads, lds.sums);
+    total += lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
+  }
+  total = uniform(total);
+  r.share = max((total + (1 << w.wgs_log2) - 1) >> w.wgs_log2, (long)w.min_share);
+  r.begin = wg * r.share;
+  r.end = min(r.begin + r.share, total);
+  if (r.begin >= r.end) return false;
+  long before = 0;
+  for (int s0 = 0; s0 < b.num_seqs; s0 += 256) {
+    if (b.num_seqs > 256) {
+      c = count(s0);
+      upto = before + scan256(c * kv.heads, lds.sums);
+      before += lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
+    }
+    if (r.begin >= upto - c * kv.heads && r.begin < upto) {
+      lds.seq = s0 + tid;
+      lds.at = r.begin - (upto - c * kv.heads);
+      lds.in_head = c;
+    }
+    if (r.begin < before) break;  // uniform
+  }
+  __syncthreads();
+  r.seq = uniform(lds.seq);
+  const long at = uniform(lds.at), in_head = uniform(lds.in_head);
+  r.head = at < INT32_MAX && in_head < INT32_MAX ? (int)((uint32_t)at / (uint32_t)in_head) : (int)(at / in_head);
+  long rest = at - r.head * in_head;
+  const KvSeq s = kv_seq(b, r.seq, kv.page_log2);
+  const int rows = s.n * a.group;
+  if (rows <= kFew * TILE) {
+    int units;
+    r.r0 = 0;
+    while (units = tile_units(s, a, r.r0, TILE), rest >= units) rest -= units, r.r0 += TILE;
+    r.off = (int)rest;
+    return true;
+  }
+  long base = 0;
+  for (long r0 = 0; r0 < rows && base <= rest; r0 += 256 * TILE) {
+    const long mine = r0 + (long)tid * TILE;
+    const long u = mine < rows ? tile_units(s, a, (int)mine, TILE) : 0;
+    const long e = base + scan256(u, lds.sums);
+    if (rest >= e - u && rest < e) {
+      lds.r0 = (int)mine;
+      lds.off = (int)(rest - (e - u));
+    }
+    base += lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
+  }
+  __syncthreads();
+  r.r0 = uniform(lds.r0);
+  r.off = uniform(lds.off);
+  return true;
+}
+
+// the tile behind (seq, head, r0); the caller knows that there is one
+template <int TILE>
+__device__ __forceinline__ void next_tile(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
+                                          const AttnWork &w, Run &r, KvSeq &s) {
+  r.r0 += TILE;
+  if (r.r0 < s.n * a.group) return;
+  r.r0 = 0;
+  if (++r.head < kv.heads) return;
+  r.head = 0;
+  int rows;
+  do {
+    s = kv_seq(b, ++r.seq, kv.page_log2);
+    rows = s.n * a.group;
+  } while (rows <= w.rows_above || rows > w.rows_upto);
+}
 
 // four values of a finished row; *bad is set where they are not finite: a weight 0
 // times a value that is not finite, or a row whose result is not finite by the
@@ -181,8 +313,9 @@ __device__ __forceinline__ void store_out(const AttnCall &a, const KvSeq &s, int
                                           f32x4 o, float l, int *bad) {
   const float inv = 1.f / l;
   o *= inv;
-  float *out = a.out + (size_t)(s.row + row / a.group) * a.out_stride +
-               (size_t)(head * a.group + row % a.group) * D + d;
+  const int tok = by_group(a, row);
+  float *out = a.out + (size_t)(s.row + tok) * a.out_stride +
+               (size_t)(head * a.group + row - tok * a.group) * D + d;
   const bool fine = __builtin_isfinite(o.x) && __builtin_isfinite(o.y) && __builtin_isfinite(o.z) &&
                     __builtin_isfinite(o.w);
   if (!fine || !(l > 0.f)) *bad = 1;
@@ -208,7 +341,7 @@ __device__ __forceinline__ void finish_rows(const KvView &kv, const nx_kv_batch 
                                             const KvSeq &s, const Tile &t, const int *bad) {
   for (int r = threadIdx.x >> 6; r < t.nr; r += 4) {
     if (!bad[r]) continue;
-    const int row = t.r0 + r, h = t.head * a.group + row % a.group, i = row / a.group;
+    const int row = t.r0 + r, i = by_group(a, row), h = t.head * a.group + row - i * a.group;
     attn_row<FMT, D>(kv, b, a, s, t.seq, t.head, s.first + i,
                      a.q + (size_t)(s.row + i) * a.q_stride + (size_t)h * D,
                      a.out + (size_t)(s.row + i) * a.out_stride + (size_t)h * D);
@@ -222,54 +355,36 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
   constexpr bool I8 = FMT == NX_KV_INT8;
   constexpr int KS = D / 32, DT = D / 16;     // steps of a score, 16-element tiles of the output
   constexpr int KL = I8 ? KS : 2 * KS, VL = I8 ? DT / 2 : DT;  // 16-byte loads of a lane and group
-  __shared__ DecodeLds<FMT, D> lds;
-  __shared__ long sums[4];
-  __shared__ Place place;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  __shared__ union {
+    RunLds run;
+    DecodeLds<FMT, D> rows;
+  } shared;
+  DecodeLds<FMT, D> &lds = shared.rows;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   // neighbouring runs on one XCD: tiles of one head share its keys in that L2
-  const int wg = (blockIdx.x & 7) * (w.wgs >> 3) + (blockIdx.x >> 3);
-
-  auto seq_units = [&](int s) {
-    const KvSeq q = kv_seq(b, s, kv.page_log2);
-    return q.n > 0 ? (long)kv.heads * head_units(q, a, kTile) : 0;
-  };
-  // all units, then the run of this workgroup
-  long total = 0;
-  for (int s0 = 0; s0 < b.num_seqs; s0 += 256) {
-    const int s = s0 + (int)threadIdx.x;
-    scan256(s < b.num_seqs ? seq_units(s) : 0, sums);
-    total += sums[0] + sums[1] + sums[2] + sums[3];
-  }
-  const long share = max((total + w.wgs - 1) / w.wgs, (long)w.min_share);
-  const long begin = wg * share, end = min(begin + share, total);
+  const int wg = (blockIdx.x & 7) << (w.wgs_log2 - 3) | blockIdx.x >> 3;
   if (threadIdx.x == 0) w.desc[wg] = int4{0, 0, 0, 0};
-  if (begin >= end) return;
-  const Place at = find_item(b.num_seqs, begin, seq_units, sums, &place);
-  int seq = at.s;
-  KvSeq s = kv_seq(b, seq, kv.page_log2);
-  long in_head = head_units(s, a, kTile);
-  int head = (int)(at.at / in_head), r0 = 0;
-  int off = 0, units;
-  {
-    long rest = at.at - head * in_head;
-    while (units = tile_units(s, a, r0, kTile), rest >= units) rest -= units, r0 += kTile;
-    off = (int)rest;
-  }
+  Run run;
+  if (!find_run<kTile>(kv, b, a, w, wg, shared.run, run)) return;
+  __syncthreads();  // shared is free for the rows
+  KvSeq s = kv_seq(b, run.seq, kv.page_log2);
 
-  for (long u = begin; u < end;) {
+  for (long u = run.begin; u < run.end;) {
+    const int seq = run.seq, head = run.head, r0 = run.r0, off = run.off;
+    const int units = tile_units(s, a, r0, kTile);
     const Tile t{seq, head, r0, min(kTile, s.n * a.group - r0)};
     const KeySpan span = tile_span(s, a, r0, t.nr);
-    const int stop = (int)min((long)units, off + (end - u));  // units [off, stop) of the tile
+    const int stop = (int)min((long)units, off + (run.end - u));  // units [off, stop) of the tile
     const bool whole = off == 0 && stop == units;
 
     // ---- this lane's query
-    const int row = r0 + min(n, t.nr - 1), tok = row / a.group;
+    const int row = r0 + min(n, t.nr - 1), tok = by_group(a, row);
     const int p = s.first + tok;  // its token
     f16x8 qh[KS], ql[KS];
     float c;
     {
       const float *q = a.q + (size_t)(s.row + tok) * a.q_stride +
-                       (size_t)(head * a.group + row % a.group) * D + 8 * g;
+                       (size_t)(head * a.group + row - tok * a.group) * D + 8 * g;
       float x[KS][8], mx = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -370,7 +485,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
       load_k(gr1);  // the next group's keys, while this one's weights are made
 
       // which of them the lane's row sees: all, for groups inside every row's range
-      const int pmin = s.first + r0 / a.group, pmax = s.first + (r0 + t.nr - 1) / a.group;
+      const int pmin = s.first + by_group(a, r0), pmax = s.first + by_group(a, r0 + t.nr - 1);
       const bool all = there && first + kKvGroup - 1 <= pmin && first + kKvGroup <= s.len &&
                        (a.window == 0 || pmax - first < a.window || first + kKvGroup <= a.sinks);
       int vis = 0xff;
@@ -423,14 +538,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
         }
         if (__any(grew || ldexp1(wt, we) > 32768.f)) {
           wt = max_groups(wt);
-          if ((grew || ldexp1(wt, we) > 32768.f) && wt < INFINITY) {
-            wm = fmaxf(wm, wt);
-            const int e1 = wm > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(wm), 126) : 0;
-            const float f = ldexp1(1.f, min(e1 - we, 126));
+          const bool anew = (grew || ldexp1(wt, we) > 32768.f) && wt < INFINITY;
+          wm = anew ? fmaxf(wm, wt) : wm;
+          const int e1 = wm > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(wm), 126) : 0;
+          const float f = anew ? ldexp1(1.f, min(e1 - we, 126)) : 1.f;
+          we = anew ? e1 : we;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) acc[d] *= f;
-            we = e1;
-          }
+          for (int d = 0; d < DT; ++d) acc[d] *= f;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) pr[j] = ldexp1(pr[j], we);
@@ -496,45 +610,320 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
       finish_rows<FMT, D>(kv, b, a, s, t, lds.bad);
     } else if (off == 0 && threadIdx.x == 0) {
       // how many workgroups hold the tile's units
-      const long last = (u + units - 1) / share;
-      w.desc[wg] = int4{seq, head, r0, (int)(last - wg) + 1};
+      w.desc[wg] = int4{seq, head, r0, (int)((u + units - 1) / run.share - wg) + 1};
     }
     __syncthreads();  // lds is free
-
-    // ---- the next tile
     u += stop - off;
-    off = 0;
-    if (u >= end) break;
-    r0 += kTile;
-    if (r0 >= s.n * a.group) {
-      r0 = 0;
-      if (++head == kv.heads) {
-        head = 0;
-        do s = kv_seq(b, ++seq, kv.page_log2);
-        while (s.n <= 0);  // (units are left, so a sequence is)
-      }
-    }
-    units = tile_units(s, a, r0, kTile);
+    run.off = 0;
+    if (u < run.end) next_tile<kTile>(kv, b, a, w, run, s);
   }
 }
 
-// Joins the tiles whose units several workgroups had: rows y, y + 4, ... of the
-// tile that workgroup x begins.
+// ------------------------------------------------------------ prompts: k_attn_tile
+//
+// Chunks of many rows: 128 rows of a key/value head against the groups of 32 tokens,
+// which all four waves take from LDS, each for 32 rows of its own.  The same transposed
+// products on 32 x 32 x 16 tiles: a group is one 32-row tile of scores, a lane holds
+// tokens 16 s + 8 h .. + 7 of its query, the operand of value chunk 2 s + h.  The
+// next group is on its way to registers while one is worked on and one lies in LDS;
+// int8 codes become f16 on their way to LDS, once for the four waves.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kRows = 128;
+
+// the other half of the wave's value
+template <typename Op>
+__device__ __forceinline__ float across_halves(float v, Op op) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, AttnCall a, AttnWork w) {
+struct TileLds {
+  // keys [D / 8][32 rows][8], then values [4][D][8], of two groups
+  _Float16 kv[2][2 * kKvGroup * D];
+  float dk[2][kKvGroup], dv[2][kKvGroup];  // INT8 scales, in token order
+};
+
+template <int FMT, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, nx_kv_batch b,
+                                                                    AttnCall a, AttnWork w) {
+  using E = kv_elem<FMT>;
+  constexpr bool I8 = FMT == NX_KV_INT8;
+  constexpr int KS = D / 16, DT = D / 32;
+  constexpr int C = kKvGroup * D * (int)sizeof(E) / 16;  // 16-byte chunks of a group's keys
+  constexpr int L = (C + 255) / 256;                     // of which a thread moves
+  __shared__ union {
+    RunLds run;
+    TileLds<FMT, D> tile;
+  } shared;
+  __shared__ int bad[kRows];
+  TileLds<FMT, D> &lds = shared.tile;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+  const int wg = (blockIdx.x & 7) << (w.wgs_log2 - 3) | blockIdx.x >> 3;
+  if (threadIdx.x == 0) w.desc[wg] = int4{0, 0, 0, 0};
+  Run run;
+  if (!find_run<kRows>(kv, b, a, w, wg, shared.run, run)) return;
+  KvSeq s = kv_seq(b, run.seq, kv.page_log2);
+
+  for (long u = run.begin; u < run.end;) {
+    const int seq = run.seq, head = run.head, r0 = run.r0, off = run.off;
+    const int units = tile_units(s, a, r0, kRows);
+    const int nr = min(kRows, s.n * a.group - r0);
+    const KeySpan span = tile_span(s, a, r0, nr);
+    const int stop = (int)min((long)units, off + (run.end - u));
+    const bool whole = off == 0 && stop == units;
+
+    // ---- this lane's query (rows behind the tile's last repeat it)
+    const int row = r0 + min(32 * wave + n, nr - 1), tok = by_group(a, row);
+    const int p = s.first + tok;
+    // the wave's first and last token
+    const int pmin = uniform(s.first + by_group(a, r0 + min(32 * wave, nr - 1)));
+    const int pmax = uniform(s.first + by_group(a, r0 + min(32 * wave + 31, nr - 1)));
+    f16x8 qh[KS], ql[KS];
+    float c;
+    {
+      const float *q = a.q + (size_t)(s.row + tok) * a.q_stride +
+                       (size_t)(head * a.group + row - tok * a.group) * D + 8 * h;
+      float mx = 0.f;
+      // twice through the row (the second time from cache): once for its maximum
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(q[16 * ks + i]));
+      mx = across_halves(mx, [](float x, float y) { return fmaxf(x, y); });
+      const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
+      const float up = ldexp1(1.f, 14 - X);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = q[16 * ks + i] * up;
+        split2(x, qh[ks], ql[ks]);
+      }
+      c = ldexp1(a.scale * kLog2e, X - 14 + (I8 ? 9 : 0));
+    }
+    float m = kUnset, l = 0.f, wm = 0.f;
+    int we = 0;
+    f32x16 acc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
+
+    // ---- groups on their way: registers, then LDS
+    uint4 rk[L], rv[L];
+    float rs = 0.f;
+    auto fetch = [&](int i) {  // unit i of the tile
+      const long at = span.count() > 0 ? kv_group(kv, b, seq, head, span.group(i) * kKvGroup) : -1;
+      const long gr = max(at, 0L);  // (a group that is not there is masked)
+      const uint4 *gk = reinterpret_cast<const uint4 *>(kv.k) + gr * C;
+      const uint4 *gv = reinterpret_cast<const uint4 *>(kv.v) + gr * C;
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const int e = threadIdx.x + 256 * j;
+        if (C % 256 == 0 || e < C) {
+          rk[j] = gk[e];
+          rv[j] = gv[e];
+        }
+      }
+      if (I8 && threadIdx.x < 2 * kKvGroup)
+        rs = (threadIdx.x < kKvGroup ? kv.ks : kv.vs)[gr * kKvGroup + (threadIdx.x & (kKvGroup - 1))];
+      return at >= 0;
+    };
+    auto stage = [&](int buf) {
+      f16x8 *k8 = reinterpret_cast<f16x8 *>(lds.kv[buf]), *v8 = k8 + kKvGroup * D / 8;
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const int e = threadIdx.x + 256 * j;
+        if (C % 256 != 0 && e >= C) break;
+        if constexpr (I8) {
+          // rows 2 x, 2 x + 1 of a key chunk: tokens t and t + 4
+          const int d8 = e >> 4, t = kv_token(NX_KV_INT8, (e & 15) * 2);
+          k8[d8 * kKvGroup + kv_row(NX_KV_F16, t)] = from_codes(rk[j].x, rk[j].y);
+          k8[d8 * kKvGroup + kv_row(NX_KV_F16, t + 4)] = from_codes(rk[j].z, rk[j].w);
+          v8[2 * e] = from_codes(rv[j].x, rv[j].y);
+          v8[2 * e + 1] = from_codes(rv[j].z, rv[j].w);
+        } else {
+          k8[e] = __builtin_bit_cast(f16x8, rk[j]);
+          v8[e] = __builtin_bit_cast(f16x8, rv[j]);
+        }
+      }
+      if (I8 && threadIdx.x < 2 * kKvGroup)
+        (threadIdx.x < kKvGroup ? lds.dk : lds.dv)[buf][threadIdx.x & (kKvGroup - 1)] = rs;
+    };
+
+    __syncthreads();  // the last tile's (or the run's) use of shared
+    bool there = fetch(off), there1 = false;
+    stage(off & 1);
+    if (off + 1 < stop) there1 = fetch(off + 1);
+    for (int i = off; i < stop; ++i) {
+      const int buf = i & 1;
+      __syncthreads();  // group i is in LDS, and no wave reads group i - 1 any more
+      const bool here = there;
+      there = there1;
+      if (i + 1 < stop) {
+        stage(buf ^ 1);
+        if (i + 2 < stop) there1 = fetch(i + 2);
+      }
+      const int first = span.group(i) * kKvGroup;
+      // groups that none of the wave's rows see
+      if (!here || first > pmax ||
+          (a.window && first >= a.sinks && pmin - (first + kKvGroup - 1) >= a.window))
+        continue;
+      const f16x8 *k8 = reinterpret_cast<const f16x8 *>(lds.kv[buf]) + h * kKvGroup + n;
+      const f16x8 *v8 = reinterpret_cast<const f16x8 *>(lds.kv[buf]) + kKvGroup * D / 8 + h * D + n;
+      f32x16 sc;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc[j] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const f16x8 kx = k8[2 * ks * kKvGroup];
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, qh[ks], sc, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, ql[ks], sc, 0, 0, 0);
+      }
+      // sc[8 s + j]: token first + 16 s + 8 h + j
+      if constexpr (I8) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[j] *= lds.dk[buf][16 * (j >> 3) + 8 * h + (j & 7)];
+      }
+      const bool all = first + kKvGroup - 1 <= pmin && first + kKvGroup <= s.len &&
+                       (a.window == 0 || pmax - first < a.window || first + kKvGroup <= a.sinks);
+      int vis = 0xffff;
+      if (!all) {
+        vis = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int key = first + 16 * (j >> 3) + 8 * h + (j & 7);
+          if (key < s.len && sees(a, p, key)) vis |= 1 << j;
+        }
+      }
+      float y[16], top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        y[j] = (vis >> j) & 1 ? fmaf(sc[j], c, -m) : -INFINITY;
+        top = fmaxf(top, y[j]);
+      }
+      bool grew = false;
+      if (__any(top > kGrow)) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if ((vis >> j) & 1) x = fmaxf(x, sc[j] * c);
+        x = across_halves(x, [](float x, float y) { return fmaxf(x, y); });
+        grew = x > m + kGrow;
+        const float m1 = grew ? x - kHead : m, keep = exp2f(m - m1);
+        m = m1;
+        wm *= keep;
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] *= keep;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = (vis >> j) & 1 ? fmaf(sc[j], c, -m) : -INFINITY;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        y[j] = __builtin_amdgcn_exp2f(y[j]);
+        sum += y[j];
+      }
+      l += sum;
+      if constexpr (I8) {  // as in k_attn_split
+        float wt = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float dv = lds.dv[buf][16 * (j >> 3) + 8 * h + (j & 7)];
+          y[j] = (vis >> j) & 1 ? y[j] * dv : 0.f;
+          wt = fmaxf(wt, y[j]);
+        }
+        if (__any(grew || ldexp1(wt, we) > 32768.f)) {
+          wt = across_halves(wt, [](float x, float y) { return fmaxf(x, y); });
+          const bool anew = (grew || ldexp1(wt, we) > 32768.f) && wt < INFINITY;
+          wm = anew ? fmaxf(wm, wt) : wm;
+          const int e1 = wm > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(wm), 126) : 0;
+          const float f = anew ? ldexp1(1.f, min(e1 - we, 126)) : 1.f;
+          we = anew ? e1 : we;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[d] *= f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = ldexp1(y[j], we);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float pr[8];
+        f16x8 ph, pl;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pr[j] = y[8 * t + j];
+        split2(pr, ph, pl);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const f16x8 vx = v8[2 * t * D + 32 * d];
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx, ph, acc[d], 0, 0, 0);
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx, pl, acc[d], 0, 0, 0);
+        }
+      }
+    }
+
+    // ---- results: acc[d][4 x + j] is element 32 d + 8 x + 4 h + j of the lane's row
+    l = across_halves(l, [](float x, float y) { return x + y; });
+    const float un = I8 ? ldexp1(1.f, 9 - we) : 1.f;
+    const int r = 32 * wave + n;
+    if (threadIdx.x < kRows) bad[threadIdx.x] = 0;
+    __syncthreads();
+    float *part = w.part + ((size_t)wg * 2 + (off == 0)) * (kRows * (D + 2));
+    if (r < nr) {
+      if (!whole && h == 0) {
+        part[r] = m;
+        part[kRows + r] = l;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const f32x4 o = f32x4{acc[d][4 * x], acc[d][4 * x + 1], acc[d][4 * x + 2], acc[d][4 * x + 3]} * un;
+          const int d0 = 32 * d + 8 * x + 4 * h;
+          if (whole)
+            store_out<D>(a, s, head, row, d0, o, l, &bad[r]);
+          else
+            *reinterpret_cast<f32x4 *>(part + 2 * kRows + r * D + d0) = o;
+        }
+    }
+    if (whole) {
+      __syncthreads();
+      finish_rows<FMT, D>(kv, b, a, s, Tile{seq, head, r0, nr}, bad);
+    } else if (off == 0 && threadIdx.x == 0) {
+      w.desc[wg] = int4{seq, head, r0, (int)((u + units - 1) / run.share - wg) + 1};
+    }
+    u += stop - off;
+    run.off = 0;
+    if (u < run.end) next_tile<kRows>(kv, b, a, w, run, s);
+  }
+}
+
+// ------------------------------------------------------------ k_attn_join
+//
+// Joins the tiles whose units several workgroups had: rows y, y + gridDim.y, ... of
+// the tile that workgroup x of k_attn_split begins, or, from its workgroups on, of
+// k_attn_tile.
+template <int FMT, int D>
+__global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, AttnCall a, AttnWork w0,
+                                                   AttnWork w1, int wgs0) {
   constexpr int Q = 256 / (D / 4) >= 8 ? 8 : 256 / (D / 4);  // partial sums side by side
   __shared__ f32x4 lds[Q][D / 4];
   __shared__ float sum_l[Q];
   __shared__ int bad[1];
-  const int4 t = w.desc[blockIdx.x];
+  const bool wide = (int)blockIdx.x >= wgs0;
+  const int wg = wide ? blockIdx.x - wgs0 : blockIdx.x;
+  const int4 t = (wide ? w1 : w0).desc[wg];
   const int parts = t.w;
   if (parts == 0) return;
+  const int tile = wide ? kRows : kTile;
+  const float *first = (wide ? w1 : w0).part;
   const KvSeq s = kv_seq(b, t.x, kv.page_log2);
-  auto at = [&](int i) {
-    return w.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0)) * (kTile * (D + 2));
-  };
+  auto at = [&](int i) { return first + ((size_t)(wg + i) * 2 + (i == 0)) * (tile * (D + 2)); };
   const int lane = threadIdx.x & 63, q = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
-  for (int r = blockIdx.y; r < kTile && t.z + r < s.n * a.group; r += 4) {
+  for (int r = blockIdx.y; r < tile && t.z + r < s.n * a.group; r += gridDim.y) {
     float m = kUnset;
     for (int i = lane; i < parts; i += 64) m = fmaxf(m, at(i)[r]);
 #pragma unroll
@@ -545,8 +934,8 @@ __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, Att
       for (int i = q; i < parts; i += Q) {
         const float *p = at(i);
         const float f = exp2f(p[r] - m);
-        l += p[kTile + r] * f;
-        o += *reinterpret_cast<const f32x4 *>(p + 2 * kTile + r * D + 4 * d) * f;
+        l += p[tile + r] * f;
+        o += *reinterpret_cast<const f32x4 *>(p + 2 * tile + r * D + 4 * d) * f;
       }
       lds[q][d] = o;
       if (d == 0) sum_l[q] = l;
@@ -567,16 +956,21 @@ __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, Att
   }
 }
 
-// Workgroups of a call, and the workspace of their parts: of one size for every
-// cache, so that it is allocated once.
+// Workgroups of a call (a power of two, so that whole XCDs get equal shares), and
+// the workspace of their parts: of one size for every cache, so that it is
+// allocated once.
 constexpr int kAttnWgsPerCu = 2;
-static int attn_wgs(const nx_ctx *c) { return c->num_cu * kAttnWgsPerCu / 8 * 8; }  // whole XCDs
-static size_t attn_bytes(const nx_ctx *c) {
-  return (size_t)attn_wgs(c) * (sizeof(int4) + 2 * kTile * (256 + 2) * 4);
-}
+// rows of a sequence from which k_attn_tile takes it
+constexpr int kTileFrom = 64;
+
+static int attn_wgs_log2(const nx_ctx *c) { return std::max(3, 31 - __builtin_clz(c->num_cu * kAttnWgsPerCu)); }
+static size_t part_floats(int tile, int D) { return (size_t)2 * tile * (D + 2); }
 int attn_workspace(nx_ctx *c, void **out) {
+  const size_t wgs = (size_t)1 << attn_wgs_log2(c);
+  // (k_attn_tile runs half as many workgroups on heads of 256)
+  const size_t wide = std::max(part_floats(kRows, 128), part_floats(kRows, 256) / 2);
   void *p;
-  NX_TRY(ws_get(c, WS_ATTN, attn_bytes(c), &p));
+  NX_TRY(ws_get(c, WS_ATTN, wgs * (2 * sizeof(int4) + 4 * (part_floats(kTile, 256) + wide)), &p));
   if (out) *out = p;
   return NX_OK;
 }
@@ -584,19 +978,36 @@ int attn_workspace(nx_ctx *c, void **out) {
 static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnCall a) {
   a.wide_q = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride % 4 == 0;
   a.wide_out = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.out_stride % 4 == 0;
+  a.shift = a.group > 1 ? 32 - __builtin_clz(a.group - 1) : 0;
+  a.magic = (uint32_t)((((uint64_t)1 << (31 + a.shift)) + a.group - 1) / a.group);
   void *p;
   NX_TRY(attn_workspace(c, &p));
-  const int wgs = attn_wgs(c);
-  AttnWork w{static_cast<int4 *>(p), reinterpret_cast<float *>(static_cast<int4 *>(p) + wgs), wgs, 4};
+  // Which kernels the batch may need: only the device knows its sequences' rows.
+  const bool wide = (long)b.num_tokens * a.group > kTileFrom;
+  const bool narrow = !wide || b.num_seqs > 1;
+  const int log2 = attn_wgs_log2(c), wgs = 1 << log2;
+  int4 *desc = static_cast<int4 *>(p);
+  float *part = reinterpret_cast<float *>(desc + 2 * wgs);
+  const AttnWork w0{desc, part, log2, 4, 0, wide ? kTileFrom : INT32_MAX};
+  const AttnWork w1{desc + wgs, part + wgs * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2, 4,
+                    narrow ? kTileFrom : 0, INT32_MAX};
+  const int wgs0 = narrow ? wgs : 0, wgs1 = wide ? 1 << w1.wgs_log2 : 0;
   const KvView view = view_of(kv);
-  NX_TRY(launch(c, "attn_split", [&] {
-    with_kernel(kv, [&](auto fmt, auto D) {
-      go(c, k_attn_split<fmt(), D()>, dim3(wgs), dim3(256), 0, view, b, a, w);
-    });
-  }));
+  if (wide)
+    NX_TRY(launch(c, "attn_tile", [&] {
+      with_kernel(kv, [&](auto fmt, auto D) {
+        go(c, k_attn_tile<fmt(), D()>, dim3(wgs1), dim3(256), 0, view, b, a, w1);
+      });
+    }));
+  if (narrow)
+    NX_TRY(launch(c, "attn_split", [&] {
+      with_kernel(kv, [&](auto fmt, auto D) {
+        go(c, k_attn_split<fmt(), D()>, dim3(wgs0), dim3(256), 0, view, b, a, w0);
+      });
+    }));
   return launch(c, "attn_join", [&] {
     with_kernel(kv, [&](auto fmt, auto D) {
-      go(c, k_attn_join<fmt(), D()>, dim3(wgs, 4), dim3(256), 0, view, b, a, w);
+      go(c, k_attn_join<fmt(), D()>, dim3(wgs0 + wgs1, wide ? 16 : 4), dim3(256), 0, view, b, a, w0, w1, wgs0);
     });
   });
 }
@@ -615,7 +1026,7 @@ static int attention(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const flo
     return fail(NX_ERR_UNSUPPORTED, "row stride above 2^40");
   NX_TRY(refuse(kv_check_rows("query", (long)q_stride, (long)width)));
   NX_TRY(refuse(kv_check_rows("output", (long)out_stride, (long)width)));
-  AttnCall a{q, out, q_stride, out_stride, heads, heads / kv->heads, scale, window, sinks, false, false};
+  AttnCall a{q, out, q_stride, out_stride, heads, heads / kv->heads, scale, window, sinks, false, false, 0, 0};
   if (!host) return attention_dev(c, kv, *b, a);
   NX_TRY(refuse(kv_check_tables(*b, kv->pages, kv->page_tokens, true, false)));
   const size_t r0 = b->row_start[0], rows = b->row_start[b->num_seqs];
