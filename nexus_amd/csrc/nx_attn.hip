@@ -121,21 +121,48 @@ __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b,
 // value's on the weight.
 constexpr int kTile = 16;
 constexpr float kLog2e = 1.4426950408889634f;
-// weights reach 2^6 at the maximum that they are relative to, and 2^14 when the
-// maximum has grown by 2^8 since: only then are the sums scaled anew
-constexpr float kHead = 6.f, kGrow = 14.f, kUnset = -1e30f;
+// The largest weight of a row (p, or p times the value's scale) is 2^8 or more when the
+// reference m is set; m is set anew, and the sums scaled, when one passes 2^15.  So
+// halves stay in range, and weights down to 2^-18 of the largest keep all their bits.
+constexpr float kHead = 9.f, kGrow = 15.f, kUnset = -1e30f;
 
 // int8 code -> f16 q 2^-9, exact: 0x80 ^ code as the low bits of a subnormal half
 __device__ __forceinline__ f16x8 from_codes(uint32_t lo, uint32_t hi) { return operand8(lo, hi); }
 
 __device__ __forceinline__ float ldexp1(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 
-__device__ __forceinline__ void split2(const float (&x)[8], f16x8 &h, f16x8 &l) {
+// 8 values as two halves each, x = hi + lo to 22 bits.  `one` is 1 that the compiler
+// does not know: x one - hi is then one instruction that reads the packed half.
+__device__ __forceinline__ void split2(const float (&x)[8], float one, f16x8 &h, f16x8 &l) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  f16x2 hi[4], lo[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    h[i] = (_Float16)x[i];
-    l[i] = (_Float16)(x[i] - (float)h[i]);
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), f16x2);
+    asm("" : "+v"(hi[i]));  // converted once, packed
+    lo[i] = __builtin_convertvector(
+        (f32x2{fmaf(x[2 * i], one, -(float)hi[i][0]), fmaf(x[2 * i + 1], one, -(float)hi[i][1])}), f16x2);
   }
+  h = f16x8{hi[0][0], hi[0][1], hi[1][0], hi[1][1], hi[2][0], hi[2][1], hi[3][0], hi[3][1]};
+  l = f16x8{lo[0][0], lo[0][1], lo[1][0], lo[1][1], lo[2][0], lo[2][1], lo[3][0], lo[3][1]};
+}
+__device__ __forceinline__ void load8(const float *p, bool wide, float (&x)[8]) {
+  if (wide) {
+    const f32x4 lo = *reinterpret_cast<const f32x4 *>(p), hi = *reinterpret_cast<const f32x4 *>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = lo[i];
+      x[4 + i] = hi[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
+  }
+}
+__device__ __forceinline__ float opaque_one() {
+  float one = 1.f;
+  asm("" : "+s"(one));
+  return one;
 }
 
 // the largest (sum) over the four lane groups, in all of them
@@ -153,6 +180,68 @@ __device__ __forceinline__ float sum_groups(float v) {
   return across_groups(v, [](float a, float b) { return a + b; });
 }
 
+// A row's running reference: m, and whether none is set yet (m is 0 then).
+struct Ref {
+  float m = 0.f;
+  bool fresh = true;
+  __device__ __forceinline__ float value() const { return fresh ? kUnset : m; }
+};
+
+// A value scale's exponent: above log2 of it by at most 1, from -90 on, so that no
+// weight without its scale passes 2^(90 + kGrow) either (they are summed too).
+__device__ __forceinline__ float scale_exponent(float s) {
+  return fmaxf(s > 0.f ? (float)__builtin_amdgcn_frexp_expf(s) : -90.f, -90.f);
+}
+
+// Scores to weights, in place: w = 2^(s c - m) (INT8: times the values' scales dv(j),
+// of exponents de(j)), added to l; where a weight has outgrown the reference of its
+// row, m is set anew and l and acc are scaled.  vis: the scores that the row sees,
+// unless `all` of the wave's rows see all of them; `top` makes a maximum that of the
+// row's lanes.
+template <bool I8, int N, typename Scale, typename Exp, typename Acc, int DT, typename Top>
+__device__ __forceinline__ void weigh(float (&w)[N], Scale dv, Exp de, float c, bool all, int vis, Ref &ref,
+                                      float &l, Acc (&acc)[DT], Top top) {
+  float sum = 0.f, most = -INFINITY;
+  if (all) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = fmaf(w[j], c, -ref.m);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = (vis >> j) & 1 ? fmaf(w[j], c, -ref.m) : -INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) most = fmaxf(most, I8 ? w[j] + de(j) : w[j]);
+  if (__any(most > (ref.fresh ? -INFINITY : kGrow))) {
+    most = top(most);
+    const bool anew = most > (ref.fresh ? -INFINITY : kGrow);
+    const float m1 = anew ? ref.m + (most - kHead) : ref.m;
+    const float keep = ref.fresh ? 0.f : exp2f(ref.m - m1);
+    l *= keep;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] *= keep;
+    // (rounded in the last places of scores of this size, as they are themselves)
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] += ref.m - m1;
+    ref.m = m1;
+    ref.fresh = ref.fresh && !anew;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    w[j] = __builtin_amdgcn_exp2f(w[j]);
+    sum += w[j];
+  }
+  l += sum;
+  if constexpr (I8) {
+    if (all) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) w[j] *= dv(j);
+    } else {  // (a scale that is not seen may be NaN)
+#pragma unroll
+      for (int j = 0; j < N; ++j) w[j] = (vis >> j) & 1 ? w[j] * dv(j) : 0.f;
+    }
+  }
+}
+
 // A tile of a sequence: rows r0 .. r0 + nr - 1 of its n * group (token, head) rows
 struct Tile {
   int seq, head, r0, nr;
@@ -161,12 +250,6 @@ __device__ __forceinline__ KeySpan tile_span(const KvSeq &s, const AttnCall &a, 
   return key_span(s.first + by_group(a, r0), s.first + by_group(a, r0 + nr - 1), s.len, a.window,
                   a.sinks);
 }
-// units of a tile: at least one, so that rows which see nothing are written
-__device__ __forceinline__ int tile_units(const KvSeq &s, const AttnCall &a, int r0, int tile) {
-  const int nr = min(tile, s.n * a.group - r0);
-  return max(tile_span(s, a, r0, nr).count(), 1);
-}
-
 // Partial results of tiles that were split: per workgroup, those of the tile that
 // it ends (or passes through) and of the tile that it begins.
 //   desc [workgroups] {seq, head, r0, workgroups of the tile that begins here or 0}
@@ -175,8 +258,17 @@ struct AttnWork {
   int4 *desc;
   float *part;
   int wgs_log2, min_share;
+  int tile_cost;              // what a tile takes besides its groups, in units
   int rows_above, rows_upto;  // the kernel's sequences: those of so many rows
 };
+
+// Units of a tile: its cost, then one per group (at least one, so that rows which
+// see nothing are written).
+__device__ __forceinline__ int tile_units(const KvSeq &s, const AttnCall &a, const AttnWork &w, int r0,
+                                          int tile) {
+  const int nr = min(tile, s.n * a.group - r0);
+  return w.tile_cost + max(tile_span(s, a, r0, nr).count(), 1);
+}
 
 // A workgroup's run of units: [begin, end) of all, which starts `off` units into
 // the tile at (seq, head, r0).
@@ -217,7 +309,7 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
     if (tid == 0) lds.bigs = 0;
     __syncthreads();
     if (rows <= kFew * TILE)
-      for (int r0 = 0; r0 < rows; r0 += TILE) c += tile_units(q, a, r0, TILE);
+      for (int r0 = 0; r0 < rows; r0 += TILE) c += tile_units(q, a, w, r0, TILE);
     else
       lds.big[atomicAdd(&lds.bigs, 1)] = tid;
     __syncthreads();
@@ -227,7 +319,7 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
       const KvSeq o = kv_seq(b, s0 + t, kv.page_log2);
       long part = 0;
       for (long r0 = (long)tid * TILE; r0 < o.n * a.group; r0 += 256 * TILE)
-        part += tile_units(o, a, (int)r0, TILE);
+        part += tile_units(o, a, w, (int)r0, TILE);
       scan256(part, lds.sums);
       if (tid == t) c = lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
     }
@@ -268,14 +360,14 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
   if (rows <= kFew * TILE) {
     int units;
     r.r0 = 0;
-    while (units = tile_units(s, a, r.r0, TILE), rest >= units) rest -= units, r.r0 += TILE;
+    while (units = tile_units(s, a, w, r.r0, TILE), rest >= units) rest -= units, r.r0 += TILE;
     r.off = (int)rest;
     return true;
   }
   long base = 0;
   for (long r0 = 0; r0 < rows && base <= rest; r0 += 256 * TILE) {
     const long mine = r0 + (long)tid * TILE;
-    const long u = mine < rows ? tile_units(s, a, (int)mine, TILE) : 0;
+    const long u = mine < rows ? tile_units(s, a, w, (int)mine, TILE) : 0;
     const long e = base + scan256(u, lds.sums);
     if (rest >= e - u && rest < e) {
       lds.r0 = (int)mine;
@@ -318,7 +410,7 @@ __device__ __forceinline__ void store_out(const AttnCall &a, const KvSeq &s, int
                (size_t)(head * a.group + row - tok * a.group) * D + d;
   const bool fine = __builtin_isfinite(o.x) && __builtin_isfinite(o.y) && __builtin_isfinite(o.z) &&
                     __builtin_isfinite(o.w);
-  if (!fine || !(l > 0.f)) *bad = 1;
+  if (!fine || !(l > 0.f && l < INFINITY)) *bad = 1;
   if (a.wide_out) {
     *reinterpret_cast<f32x4 *>(out) = o;
   } else {
@@ -368,14 +460,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
   if (!find_run<kTile>(kv, b, a, w, wg, shared.run, run)) return;
   __syncthreads();  // shared is free for the rows
   KvSeq s = kv_seq(b, run.seq, kv.page_log2);
+  const float one = opaque_one();
 
   for (long u = run.begin; u < run.end;) {
-    const int seq = run.seq, head = run.head, r0 = run.r0, off = run.off;
-    const int units = tile_units(s, a, r0, kTile);
+    const int seq = run.seq, head = run.head, r0 = run.r0;
+    // groups [off, stop) of the tile's; units past its cost
+    const int units = tile_units(s, a, w, r0, kTile);
+    const int till = (int)min((long)units, run.off + (run.end - u));
+    const int off = max(run.off - w.tile_cost, 0), stop = till - w.tile_cost;
+    const bool whole = off == 0 && till == units;
+    const long next = u - run.off + units;  // the batch's units up to the next tile
+    u += till - run.off;
+    run.off = 0;
+    if (stop <= off) {  // its cost alone: the next workgroup has it
+      break;
+    }
     const Tile t{seq, head, r0, min(kTile, s.n * a.group - r0)};
     const KeySpan span = tile_span(s, a, r0, t.nr);
-    const int stop = (int)min((long)units, off + (run.end - u));  // units [off, stop) of the tile
-    const bool whole = off == 0 && stop == units;
 
     // ---- this lane's query
     const int row = r0 + min(n, t.nr - 1), tok = by_group(a, row);
@@ -388,13 +489,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
       float x[KS][8], mx = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if (a.wide_q) {
-          *reinterpret_cast<f32x4 *>(&x[ks][0]) = *reinterpret_cast<const f32x4 *>(q + 32 * ks);
-          *reinterpret_cast<f32x4 *>(&x[ks][4]) = *reinterpret_cast<const f32x4 *>(q + 32 * ks + 4);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[ks][i] = q[32 * ks + i];
-        }
+        load8(q + 32 * ks, a.wide_q, x[ks]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
       }
@@ -406,14 +501,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
       for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[ks][i] *= up;
-        split2(x[ks], qh[ks], ql[ks]);
+        split2(x[ks], one, qh[ks], ql[ks]);
       }
       c = ldexp1(a.scale * kLog2e, E - 14 + (I8 ? 9 : 0));
     }
 
-    float m = kUnset, l = 0.f;
-    float wm = 0.f;  // INT8: the row's largest weight p scale when last looked at,
-    int we = 0;      // and the power of two that keeps weights in half's range
+    Ref ref;
+    float l = 0.f;
     f32x4 acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -497,60 +591,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
           if (there && key < s.len && sees(a, p, key)) vis |= 1 << j;
         }
       }
-      float y[8], top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[j] = (vis >> j) & 1 ? fmaf(sc[j >> 2][j & 3], c, -m) : -INFINITY;
-        top = fmaxf(top, y[j]);
-      }
-      bool grew = false;
-      if (__any(top > kGrow)) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if ((vis >> j) & 1) x = fmaxf(x, sc[j >> 2][j & 3] * c);
-        x = max_groups(x);
-        grew = x > m + kGrow;
-        const float m1 = grew ? x - kHead : m, keep = exp2f(m - m1);
-        m = m1;
-        wm *= keep;
-        l *= keep;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] *= keep;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = (vis >> j) & 1 ? fmaf(sc[j >> 2][j & 3], c, -m) : -INFINITY;
-      }
-      float pr[8], sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        pr[j] = __builtin_amdgcn_exp2f(y[j]);
-        sum += pr[j];
-      }
-      l += sum;
-      if constexpr (I8) {
-        // weights p scale: the row's largest is kept near 2^12 (below 2^15), so that
-        // the halves of those down to 2^-24 of it keep their bits
-        float wt = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          pr[j] = (vis >> j) & 1 ? pr[j] * dv[j] : 0.f;
-          wt = fmaxf(wt, pr[j]);
-        }
-        if (__any(grew || ldexp1(wt, we) > 32768.f)) {
-          wt = max_groups(wt);
-          const bool anew = (grew || ldexp1(wt, we) > 32768.f) && wt < INFINITY;
-          wm = anew ? fmaxf(wm, wt) : wm;
-          const int e1 = wm > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(wm), 126) : 0;
-          const float f = anew ? ldexp1(1.f, min(e1 - we, 126)) : 1.f;
-          we = anew ? e1 : we;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) acc[d] *= f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pr[j] = ldexp1(pr[j], we);
-      }
+      float pr[8] = {sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]};
+      weigh<I8>(pr, [&](int j) { return dv[j]; }, [&](int j) { return scale_exponent(dv[j]); }, c, all, vis,
+                ref, l, acc, max_groups);
       f16x8 ph, pl;
-      split2(pr, ph, pl);
+      split2(pr, one, ph, pl);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         f16x8 vx;
@@ -569,9 +614,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
 
     // ---- join the waves
     l = sum_groups(l);
-    const float un = I8 ? ldexp1(1.f, 9 - we) : 1.f;
+    const float un = I8 ? 512.f : 1.f;
     if (g == 0) {
-      lds.m[wave][n] = m;
+      lds.m[wave][n] = ref.value();
       lds.l[wave][n] = l;
     }
 #pragma unroll
@@ -609,12 +654,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
     if (whole) {
       finish_rows<FMT, D>(kv, b, a, s, t, lds.bad);
     } else if (off == 0 && threadIdx.x == 0) {
-      // how many workgroups hold the tile's units
-      w.desc[wg] = int4{seq, head, r0, (int)((u + units - 1) / run.share - wg) + 1};
+      // how many workgroups hold the tile's groups
+      w.desc[wg] = int4{seq, head, r0, (int)((next - 1) / run.share - wg) + 1};
     }
     __syncthreads();  // lds is free
-    u += stop - off;
-    run.off = 0;
     if (u < run.end) next_tile<kTile>(kv, b, a, w, run, s);
   }
 }
@@ -638,11 +681,18 @@ __device__ __forceinline__ float across_halves(float v, Op op) {
   return op(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
+__device__ __forceinline__ float max_halves(float v) {
+  return across_halves(v, [](float x, float y) { return fmaxf(x, y); });
+}
+
 template <int FMT, int D>
 struct TileLds {
   // keys [D / 8][32 rows][8], then values [4][D][8], of two groups
   _Float16 kv[2][2 * kKvGroup * D];
-  float dk[2][kKvGroup], dv[2][kKvGroup];  // INT8 scales, in token order
+  // INT8: scales of keys and values, and the latter's exponents, in token order
+  float dk[2][kKvGroup], dv[2][kKvGroup], de[2][kKvGroup];
+  // heads of 256: q's lower halves, each lane's its own, which registers do not hold
+  f16x8 ql[D == 256 ? D / 16 : 1][D == 256 ? 256 : 1];
 };
 
 template <int FMT, int D>
@@ -665,14 +715,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
   Run run;
   if (!find_run<kRows>(kv, b, a, w, wg, shared.run, run)) return;
   KvSeq s = kv_seq(b, run.seq, kv.page_log2);
+  const float one = opaque_one();
 
   for (long u = run.begin; u < run.end;) {
-    const int seq = run.seq, head = run.head, r0 = run.r0, off = run.off;
-    const int units = tile_units(s, a, r0, kRows);
+    const int seq = run.seq, head = run.head, r0 = run.r0;
+    // groups [off, stop) of the tile's; units past its cost
+    const int units = tile_units(s, a, w, r0, kRows);
+    const int till = (int)min((long)units, run.off + (run.end - u));
+    const int off = max(run.off - w.tile_cost, 0), stop = till - w.tile_cost;
+    const bool whole = off == 0 && till == units;
+    const long next = u - run.off + units;  // the batch's units up to the next tile
+    u += till - run.off;
+    run.off = 0;
+    if (stop <= off) {  // its cost alone: the next workgroup has it
+      break;
+    }
     const int nr = min(kRows, s.n * a.group - r0);
     const KeySpan span = tile_span(s, a, r0, nr);
-    const int stop = (int)min((long)units, off + (run.end - u));
-    const bool whole = off == 0 && stop == units;
 
     // ---- this lane's query (rows behind the tile's last repeat it)
     const int row = r0 + min(32 * wave + n, nr - 1), tok = by_group(a, row);
@@ -680,31 +739,35 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
     // the wave's first and last token
     const int pmin = uniform(s.first + by_group(a, r0 + min(32 * wave, nr - 1)));
     const int pmax = uniform(s.first + by_group(a, r0 + min(32 * wave + 31, nr - 1)));
-    f16x8 qh[KS], ql[KS];
+    f16x8 qh[KS], ql[D == 256 ? 1 : KS];
     float c;
+    __syncthreads();  // the last tile's (or the run's) use of shared
     {
       const float *q = a.q + (size_t)(s.row + tok) * a.q_stride +
                        (size_t)(head * a.group + row - tok * a.group) * D + 8 * h;
-      float mx = 0.f;
-      // twice through the row (the second time from cache): once for its maximum
+      float x[KS][8], mx = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks) {
+        load8(q + 16 * ks, a.wide_q, x[ks]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(q[16 * ks + i]));
-      mx = across_halves(mx, [](float x, float y) { return fmaxf(x, y); });
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
+      }
+      mx = max_halves(mx);
       const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
       const float up = ldexp1(1.f, 14 - X);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = q[16 * ks + i] * up;
-        split2(x, qh[ks], ql[ks]);
+        for (int i = 0; i < 8; ++i) x[ks][i] *= up;
+        if constexpr (D == 256)
+          split2(x[ks], one, qh[ks], lds.ql[ks][threadIdx.x]);
+        else
+          split2(x[ks], one, qh[ks], ql[ks]);
       }
       c = ldexp1(a.scale * kLog2e, X - 14 + (I8 ? 9 : 0));
     }
-    float m = kUnset, l = 0.f, wm = 0.f;
-    int we = 0;
+    Ref ref;
+    float l = 0.f;
     f32x16 acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -749,11 +812,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
           v8[e] = __builtin_bit_cast(f16x8, rv[j]);
         }
       }
-      if (I8 && threadIdx.x < 2 * kKvGroup)
+      if (I8 && threadIdx.x < 2 * kKvGroup) {
         (threadIdx.x < kKvGroup ? lds.dk : lds.dv)[buf][threadIdx.x & (kKvGroup - 1)] = rs;
+        if (threadIdx.x >= kKvGroup) lds.de[buf][threadIdx.x - kKvGroup] = scale_exponent(rs);
+      }
     };
 
-    __syncthreads();  // the last tile's (or the run's) use of shared
     bool there = fetch(off), there1 = false;
     stage(off & 1);
     if (off + 1 < stop) there1 = fetch(off + 1);
@@ -773,6 +837,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
         continue;
       const f16x8 *k8 = reinterpret_cast<const f16x8 *>(lds.kv[buf]) + h * kKvGroup + n;
       const f16x8 *v8 = reinterpret_cast<const f16x8 *>(lds.kv[buf]) + kKvGroup * D / 8 + h * D + n;
+      auto low = [&](int ks) {
+        if constexpr (D == 256)
+          return lds.ql[ks][threadIdx.x];
+        else
+          return ql[ks];
+      };
       f32x16 sc;
 #pragma unroll
       for (int j = 0; j < 16; ++j) sc[j] = 0.f;
@@ -780,7 +850,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
       for (int ks = 0; ks < KS; ++ks) {
         const f16x8 kx = k8[2 * ks * kKvGroup];
         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, qh[ks], sc, 0, 0, 0);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, ql[ks], sc, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, low(ks), sc, 0, 0, 0);
       }
       // sc[8 s + j]: token first + 16 s + 8 h + j
       if constexpr (I8) {
@@ -798,64 +868,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
           if (key < s.len && sees(a, p, key)) vis |= 1 << j;
         }
       }
-      float y[16], top = -INFINITY;
+      float y[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        y[j] = (vis >> j) & 1 ? fmaf(sc[j], c, -m) : -INFINITY;
-        top = fmaxf(top, y[j]);
-      }
-      bool grew = false;
-      if (__any(top > kGrow)) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if ((vis >> j) & 1) x = fmaxf(x, sc[j] * c);
-        x = across_halves(x, [](float x, float y) { return fmaxf(x, y); });
-        grew = x > m + kGrow;
-        const float m1 = grew ? x - kHead : m, keep = exp2f(m - m1);
-        m = m1;
-        wm *= keep;
-        l *= keep;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] *= keep;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) y[j] = (vis >> j) & 1 ? fmaf(sc[j], c, -m) : -INFINITY;
-      }
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        y[j] = __builtin_amdgcn_exp2f(y[j]);
-        sum += y[j];
-      }
-      l += sum;
-      if constexpr (I8) {  // as in k_attn_split
-        float wt = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float dv = lds.dv[buf][16 * (j >> 3) + 8 * h + (j & 7)];
-          y[j] = (vis >> j) & 1 ? y[j] * dv : 0.f;
-          wt = fmaxf(wt, y[j]);
-        }
-        if (__any(grew || ldexp1(wt, we) > 32768.f)) {
-          wt = across_halves(wt, [](float x, float y) { return fmaxf(x, y); });
-          const bool anew = (grew || ldexp1(wt, we) > 32768.f) && wt < INFINITY;
-          wm = anew ? fmaxf(wm, wt) : wm;
-          const int e1 = wm > 0.f ? min(12 - __builtin_amdgcn_frexp_expf(wm), 126) : 0;
-          const float f = anew ? ldexp1(1.f, min(e1 - we, 126)) : 1.f;
-          we = anew ? e1 : we;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) acc[d] *= f;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) y[j] = ldexp1(y[j], we);
-      }
+      for (int j = 0; j < 16; ++j) y[j] = sc[j];
+      const int at = 8 * h;  // score j's token is at + j + 8 (j >> 3)
+      weigh<I8>(y, [&](int j) { return lds.dv[buf][at + j + (j & 8)]; },
+                [&](int j) { return lds.de[buf][at + j + (j & 8)]; }, c, all, vis, ref, l, acc, max_halves);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         float pr[8];
         f16x8 ph, pl;
 #pragma unroll
         for (int j = 0; j < 8; ++j) pr[j] = y[8 * t + j];
-        split2(pr, ph, pl);
+        split2(pr, one, ph, pl);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const f16x8 vx = v8[2 * t * D + 32 * d];
@@ -867,14 +892,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
 
     // ---- results: acc[d][4 x + j] is element 32 d + 8 x + 4 h + j of the lane's row
     l = across_halves(l, [](float x, float y) { return x + y; });
-    const float un = I8 ? ldexp1(1.f, 9 - we) : 1.f;
+    const float un = I8 ? 512.f : 1.f;
     const int r = 32 * wave + n;
     if (threadIdx.x < kRows) bad[threadIdx.x] = 0;
     __syncthreads();
     float *part = w.part + ((size_t)wg * 2 + (off == 0)) * (kRows * (D + 2));
     if (r < nr) {
       if (!whole && h == 0) {
-        part[r] = m;
+        part[r] = ref.value();
         part[kRows + r] = l;
       }
 #pragma unroll
@@ -893,10 +918,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
       __syncthreads();
       finish_rows<FMT, D>(kv, b, a, s, Tile{seq, head, r0, nr}, bad);
     } else if (off == 0 && threadIdx.x == 0) {
-      w.desc[wg] = int4{seq, head, r0, (int)((u + units - 1) / run.share - wg) + 1};
+      w.desc[wg] = int4{seq, head, r0, (int)((next - 1) / run.share - wg) + 1};
     }
-    u += stop - off;
-    run.off = 0;
     if (u < run.end) next_tile<kRows>(kv, b, a, w, run, s);
   }
 }
@@ -960,6 +983,11 @@ __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, Att
 // the workspace of their parts: of one size for every cache, so that it is
 // allocated once.
 constexpr int kAttnWgsPerCu = 2;
+// What a tile costs besides its groups (its query, its results), in groups, of each
+// kernel: without it runs of many short tiles end last.  A prompt of 4093 tokens took 418 us
+// at 0, 357 at 4, 353 at 8 and 362 at 16, a batch of 17 sequences and one chunk 93, 84, 86 and
+// 101; decode steps differ by less than 1 us up to 8.
+constexpr int kTileCost = 6, kRowsCost = 6;
 // rows of a sequence from which k_attn_tile takes it
 constexpr int kTileFrom = 64;
 
@@ -988,9 +1016,9 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   const int log2 = attn_wgs_log2(c), wgs = 1 << log2;
   int4 *desc = static_cast<int4 *>(p);
   float *part = reinterpret_cast<float *>(desc + 2 * wgs);
-  const AttnWork w0{desc, part, log2, 4, 0, wide ? kTileFrom : INT32_MAX};
-  const AttnWork w1{desc + wgs, part + wgs * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2, 4,
-                    narrow ? kTileFrom : 0, INT32_MAX};
+  const AttnWork w0{desc, part, log2, 4 + kTileCost, kTileCost, 0, wide ? kTileFrom : INT32_MAX};
+  const AttnWork w1{desc + wgs, part + wgs * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2, 4 + kRowsCost,
+                    kRowsCost, narrow ? kTileFrom : 0, INT32_MAX};
   const int wgs0 = narrow ? wgs : 0, wgs1 = wide ? 1 << w1.wgs_log2 : 0;
   const KvView view = view_of(kv);
   if (wide)

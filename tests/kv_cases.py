@@ -70,9 +70,10 @@ def attention(batch, k, v, q, heads, scale, window=0, sinks=0):
     magnitudes; exp adds 2^-21 of its own.  So a weight is off by
     e = 2 ((2^-21 + D 2^-24) sum |scale q k| + 2^-21) relative to itself, against the
     other weights, and the sums over N keys by at most (N + 64) 2^-24: in all
-    (2 e + 2 (N + 64) 2^-24 + 2^-21) sum p |v| / sum p.  Weights p scale_j whose two
-    halves end 37 bits below the row's largest are off by 2^-38 of that one each:
-    N 2^-37 max_j p_j max |v_j| / sum p besides.  (Non-finite keys and values are
+    (2 e + 2 (N + 64) 2^-24 + 2^-21) sum p |v| / sum p.  The largest weight
+    p_j scale_j of a row is held at 2^8 or more, in halves whose places end at 2^-24:
+    every weight may be off by 2^-25 for that, 2^-33 of the largest, and a value is up
+    to max |v_j|: N 2^-33 max_j p_j max |v_j| / sum p besides.  (Non-finite keys and values are
     left out of the bound: where the result is finite their weight is 0, or they
     are other elements.)"""
     G, D = k.shape[1:]
@@ -100,7 +101,7 @@ def attention(batch, k, v, q, heads, scale, window=0, sinks=0):
                     part = 2 * e + 2 * (len(j) + 64) * 2.0 ** -24 + 2.0 ** -21
                     bound[row, hs] = part * (p @ va[j, g]) / total
                     top = (p * va[j, g].max(1)).max(1, keepdims=True)
-                    bound[row, hs] += len(j) * 2.0 ** -37 * top / total
+                    bound[row, hs] += len(j) * 2.0 ** -33 * top / total
         at += length
     return out, bound
 
