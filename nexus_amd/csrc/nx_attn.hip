@@ -926,57 +926,101 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
 
 // ------------------------------------------------------------ k_attn_join
 //
-// Joins the tiles whose units several workgroups had: rows y, y + gridDim.y, ... of
-// the tile that workgroup x of k_attn_split begins, or, from its workgroups on, of
-// k_attn_tile.
+// Joins the tiles whose units several workgroups had: a share of the rows of the tile
+// that workgroup x of k_attn_split begins, or, from its workgroups on, of k_attn_tile.
+// A row takes D / 4 threads.  Few parts (a run's end and the next one's begin): several
+// rows side by side, each thread adding its row's parts; many (a long context): one
+// row, the threads taking the parts in turn.
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, AttnCall a, AttnWork w0,
                                                    AttnWork w1, int wgs0) {
-  constexpr int Q = 256 / (D / 4) >= 8 ? 8 : 256 / (D / 4);  // partial sums side by side
-  __shared__ f32x4 lds[Q][D / 4];
-  __shared__ float sum_l[Q];
-  __shared__ int bad[1];
+  constexpr int kSlots = 256 / (D / 4);
+  __shared__ f32x4 lds[kSlots][D / 4];
+  __shared__ float sum_l[kSlots];
+  __shared__ int bad[kRows];
   const bool wide = (int)blockIdx.x >= wgs0;
   const int wg = wide ? blockIdx.x - wgs0 : blockIdx.x;
   const int4 t = (wide ? w1 : w0).desc[wg];
-  const int parts = t.w;
+  const int parts = uniform(t.w);
   if (parts == 0) return;
-  const int tile = wide ? kRows : kTile;
+  const int tile = wide ? kRows : kTile, seq = uniform(t.x), head = uniform(t.y), r0 = uniform(t.z);
+  const KvSeq s = kv_seq(b, seq, kv.page_log2);
+  const int nr = min(tile, s.n * a.group - r0);
   const float *first = (wide ? w1 : w0).part;
-  const KvSeq s = kv_seq(b, t.x, kv.page_log2);
   auto at = [&](int i) { return first + ((size_t)(wg + i) * 2 + (i == 0)) * (tile * (D + 2)); };
-  const int lane = threadIdx.x & 63, q = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
-  for (int r = blockIdx.y; r < tile && t.z + r < s.n * a.group; r += gridDim.y) {
-    float m = kUnset;
-    for (int i = lane; i < parts; i += 64) m = fmaxf(m, at(i)[r]);
+  const int slot = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
+  if (threadIdx.x < kRows) bad[threadIdx.x] = 0;
+  __syncthreads();
+  // rows y, y + gridDim.y, ...
+  const int y = blockIdx.y, dy = gridDim.y;
+  // two rows of up to P parts at once, every load ahead of its use
+  auto rows = [&](auto P, int r) {
+    float m[2], l[2] = {}, mp[2][P()], lp[2][P()];
+    f32x4 o[2] = {}, op[2][P()];
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    if (q < Q) {
-      for (int i = q; i < parts; i += Q) {
-        const float *p = at(i);
-        const float f = exp2f(p[r] - m);
-        l += p[tile + r] * f;
-        o += *reinterpret_cast<const f32x4 *>(p + 2 * tile + r * D + 4 * d) * f;
-      }
-      lds[q][d] = o;
-      if (d == 0) sum_l[q] = l;
-    }
-    if (threadIdx.x == 0) bad[0] = 0;
-    __syncthreads();
-    if (q == 0) {
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int i = 1; i < Q; ++i) {
-        o += lds[i][d];
-        l += sum_l[i];
+      for (int i = 0; i < P(); ++i) {
+        const float *p = at(min(i, parts - 1));
+        const int rx = min(r + x * kSlots * dy, nr - 1);
+        mp[x][i] = p[rx];
+        lp[x][i] = p[tile + rx];
+        op[x][i] = *reinterpret_cast<const f32x4 *>(p + 2 * tile + rx * D + 4 * d);
       }
-      store_out<D>(a, s, t.y, t.z + r, 4 * d, o, l, bad);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      m[x] = kUnset;
+#pragma unroll
+      for (int i = 0; i < P(); ++i) m[x] = fmaxf(m[x], mp[x][i]);
+#pragma unroll
+      for (int i = 0; i < P(); ++i) {
+        const float f = i < parts ? exp2f(mp[x][i] - m[x]) : 0.f;
+        l[x] += i < parts ? lp[x][i] * f : 0.f;
+        o[x] += op[x][i] * f;
+      }
+      const int rx = r + x * kSlots * dy;
+      if (rx < nr) store_out<D>(a, s, head, r0 + rx, 4 * d, o[x], l[x], &bad[rx]);
     }
-    __syncthreads();
-    if (threadIdx.x < 64) finish_rows<FMT, D>(kv, b, a, s, Tile{t.x, t.y, t.z + r, 1}, bad);
-    __syncthreads();  // lds and bad are free
+  };
+  if (parts <= 4) {
+    if (slot < kSlots)
+      for (int r = y + slot * dy; r < nr; r += 2 * kSlots * dy) {
+        if (parts <= 2)
+          rows(std::integral_constant<int, 2>(), r);
+        else
+          rows(std::integral_constant<int, 4>(), r);
+      }
+  } else {
+    auto add = [&](const float *p, int r, float m, float &l, f32x4 &o) {
+      const float f = exp2f(p[r] - m);
+      l += p[tile + r] * f;
+      o += *reinterpret_cast<const f32x4 *>(p + 2 * tile + r * D + 4 * d) * f;
+    };
+    for (int r = y; r < nr; r += dy) {
+      float m = kUnset, l = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int i = threadIdx.x & 63; i < parts; i += 64) m = fmaxf(m, at(i)[r]);
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+      if (slot < kSlots) {
+        for (int i = slot; i < parts; i += kSlots) add(at(i), r, m, l, o);
+        lds[slot][d] = o;
+        if (d == 0) sum_l[slot] = l;
+      }
+      __syncthreads();
+      if (slot == 0) {
+#pragma unroll
+        for (int i = 1; i < kSlots; ++i) {
+          o += lds[i][d];
+          l += sum_l[i];
+        }
+        store_out<D>(a, s, head, r0 + r, 4 * d, o, l, &bad[r]);
+      }
+      __syncthreads();  // lds is free
+    }
   }
+  __syncthreads();
+  finish_rows<FMT, D>(kv, b, a, s, Tile{seq, head, r0, nr}, bad);
 }
 
 // Workgroups of a call (a power of two, so that whole XCDs get equal shares), and
@@ -1010,8 +1054,10 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   a.magic = (uint32_t)((((uint64_t)1 << (31 + a.shift)) + a.group - 1) / a.group);
   void *p;
   NX_TRY(attn_workspace(c, &p));
-  // Which kernels the batch may need: only the device knows its sequences' rows.
-  const bool wide = (long)b.num_tokens * a.group > kTileFrom;
+  // Which kernels the batch may need: only the device knows its sequences' rows.  With a row
+  // or more in each, one has at most num_tokens - num_seqs + 1; a batch that leaves
+  // sequences out for a long one is right on k_attn_split too, if slower.
+  const bool wide = ((long)b.num_tokens - b.num_seqs + 1) * a.group > kTileFrom;
   const bool narrow = !wide || b.num_seqs > 1;
   const int log2 = attn_wgs_log2(c), wgs = 1 << log2;
   int4 *desc = static_cast<int4 *>(p);
@@ -1035,7 +1081,7 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
     }));
   return launch(c, "attn_join", [&] {
     with_kernel(kv, [&](auto fmt, auto D) {
-      go(c, k_attn_join<fmt(), D()>, dim3(wgs0 + wgs1, wide ? 16 : 4), dim3(256), 0, view, b, a, w0, w1, wgs0);
+      go(c, k_attn_join<fmt(), D()>, dim3(wgs0 + wgs1, wide ? 8 : 4), dim3(256), 0, view, b, a, w0, w1, wgs0);
     });
   });
 }
