@@ -187,14 +187,18 @@ struct Ref {
   __device__ __forceinline__ float value() const { return fresh ? kUnset : m; }
 };
 
-// A value scale's exponent: above log2 of it by at most 1, from -90 on, so that no
-// weight without its scale passes 2^(90 + kGrow) either (they are summed too).
-__device__ __forceinline__ float scale_exponent(float s) {
-  return fmaxf(s > 0.f ? (float)__builtin_amdgcn_frexp_expf(s) : -90.f, -90.f);
+// A value scale's exponent field: 126 and its log2 rounded up, at least 36, so that no
+// weight without its scale passes 2^(90 + kGrow) either (they are summed too).  A NaN
+// (a token that is not finite) outgrows everything, and counts as a scale of 0: rows that
+// see it end without a sum, and attn_row gives what the formula does.
+constexpr float kExpBias = 126.f, kExpNan = 1e9f;
+__device__ __forceinline__ float scale_field(float s) {
+  return fmaxf((float)(__float_as_uint(s) >> 23), 36.f);
 }
+__device__ __forceinline__ float finite_scale(float s) { return fmaxf(s, 0.f); }
 
 // Scores to weights, in place: w = 2^(s c - m) (INT8: times the values' scales dv(j),
-// of exponents de(j)), added to l; where a weight has outgrown the reference of its
+// of exponent fields de(j)), added to l; where a weight has outgrown the reference of its
 // row, m is set anew and l and acc are scaled.  vis: the scores that the row sees,
 // unless `all` of the wave's rows see all of them; `top` makes a maximum that of the
 // row's lanes.
@@ -211,8 +215,9 @@ __device__ __forceinline__ void weigh(float (&w)[N], Scale dv, Exp de, float c, 
   }
 #pragma unroll
   for (int j = 0; j < N; ++j) most = fmaxf(most, I8 ? w[j] + de(j) : w[j]);
-  if (__any(most > (ref.fresh ? -INFINITY : kGrow))) {
-    most = top(most);
+  constexpr float bias = I8 ? kExpBias : 0.f;
+  if (__any(most > (ref.fresh ? -INFINITY : kGrow + bias))) {
+    most = top(most) - bias;
     const bool anew = most > (ref.fresh ? -INFINITY : kGrow);
     const float m1 = anew ? ref.m + (most - kHead) : ref.m;
     const float keep = ref.fresh ? 0.f : exp2f(ref.m - m1);
@@ -232,13 +237,8 @@ __device__ __forceinline__ void weigh(float (&w)[N], Scale dv, Exp de, float c, 
   }
   l += sum;
   if constexpr (I8) {
-    if (all) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) w[j] *= dv(j);
-    } else {  // (a scale that is not seen may be NaN)
-#pragma unroll
-      for (int j = 0; j < N; ++j) w[j] = (vis >> j) & 1 ? w[j] * dv(j) : 0.f;
-    }
+    for (int j = 0; j < N; ++j) w[j] *= dv(j);
   }
 }
 
@@ -591,9 +591,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
           if (there && key < s.len && sees(a, p, key)) vis |= 1 << j;
         }
       }
+      float de[8], most_de = 0.f;
+      if constexpr (I8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          de[j] = scale_field(dv[j]);
+          most_de = fmaxf(most_de, de[j]);
+        }
+        if (__any(most_de >= 255.f))
+#pragma unroll
+          for (int j = 0; j < 8; ++j) de[j] = dv[j] == dv[j] ? de[j] : kExpNan;
+      }
       float pr[8] = {sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]};
-      weigh<I8>(pr, [&](int j) { return dv[j]; }, [&](int j) { return scale_exponent(dv[j]); }, c, all, vis,
-                ref, l, acc, max_groups);
+      weigh<I8>(pr, [&](int j) { return finite_scale(dv[j]); }, [&](int j) { return de[j]; }, c, all, vis, ref,
+                l, acc, max_groups);
       f16x8 ph, pl;
       split2(pr, one, ph, pl);
 #pragma unroll
@@ -777,9 +788,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
     // ---- groups on their way: registers, then LDS
     uint4 rk[L], rv[L];
     float rs = 0.f;
-    auto fetch = [&](int i) {  // unit i of the tile
-      const long at = span.count() > 0 ? kv_group(kv, b, seq, head, span.group(i) * kKvGroup) : -1;
-      const long gr = max(at, 0L);  // (a group that is not there is masked)
+    auto page_of = [&](int i) {  // of group i (of the last one behind it)
+      const int first = span.group(min(i, stop - 1)) * kKvGroup;
+      return span.count() > 0 ? b.pages[(long)seq * b.max_pages + (first >> kv.page_log2)] : -1;
+    };
+    int page = page_of(off);  // of the group to fetch next, looked up a group ahead
+    auto fetch = [&](int i) {
+      const bool found = page >= 0 && page < kv.pages;
+      const int in_page = (span.group(i) * kKvGroup & ((1 << kv.page_log2) - 1)) / kKvGroup;
+      // (pool group 0, masked, for one that is not there)
+      const long gr = found ? (((long)page * kv.heads + head) << (kv.page_log2 - 5)) + in_page : 0;
+      page = page_of(i + 1);
       const uint4 *gk = reinterpret_cast<const uint4 *>(kv.k) + gr * C;
       const uint4 *gv = reinterpret_cast<const uint4 *>(kv.v) + gr * C;
 #pragma unroll
@@ -792,7 +811,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
       }
       if (I8 && threadIdx.x < 2 * kKvGroup)
         rs = (threadIdx.x < kKvGroup ? kv.ks : kv.vs)[gr * kKvGroup + (threadIdx.x & (kKvGroup - 1))];
-      return at >= 0;
+      return found;
     };
     auto stage = [&](int buf) {
       f16x8 *k8 = reinterpret_cast<f16x8 *>(lds.kv[buf]), *v8 = k8 + kKvGroup * D / 8;
@@ -813,8 +832,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
         }
       }
       if (I8 && threadIdx.x < 2 * kKvGroup) {
-        (threadIdx.x < kKvGroup ? lds.dk : lds.dv)[buf][threadIdx.x & (kKvGroup - 1)] = rs;
-        if (threadIdx.x >= kKvGroup) lds.de[buf][threadIdx.x - kKvGroup] = scale_exponent(rs);
+        (threadIdx.x < kKvGroup ? lds.dk : lds.dv)[buf][threadIdx.x & (kKvGroup - 1)] =
+            threadIdx.x < kKvGroup ? rs : finite_scale(rs);
+        if (threadIdx.x >= kKvGroup) lds.de[buf][threadIdx.x - kKvGroup] = rs == rs ? scale_field(rs) : kExpNan;
       }
     };
 
@@ -953,12 +973,12 @@ __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, Att
   __syncthreads();
   // rows y, y + gridDim.y, ...
   const int y = blockIdx.y, dy = gridDim.y;
-  // two rows of up to P parts at once, every load ahead of its use
-  auto rows = [&](auto P, int r) {
-    float m[2], l[2] = {}, mp[2][P()], lp[2][P()];
-    f32x4 o[2] = {}, op[2][P()];
+  // X rows of up to P parts at once, every load ahead of its use
+  auto rows = [&](auto X, auto P, int r) {
+    float m[X()], l[X()] = {}, mp[X()][P()], lp[X()][P()];
+    f32x4 o[X()] = {}, op[X()][P()];
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < X(); ++x)
 #pragma unroll
       for (int i = 0; i < P(); ++i) {
         const float *p = at(min(i, parts - 1));
@@ -968,7 +988,7 @@ __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, Att
         op[x][i] = *reinterpret_cast<const f32x4 *>(p + 2 * tile + rx * D + 4 * d);
       }
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < X(); ++x) {
       m[x] = kUnset;
 #pragma unroll
       for (int i = 0; i < P(); ++i) m[x] = fmaxf(m[x], mp[x][i]);
@@ -982,13 +1002,17 @@ __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, Att
       if (rx < nr) store_out<D>(a, s, head, r0 + rx, 4 * d, o[x], l[x], &bad[rx]);
     }
   };
-  if (parts <= 4) {
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  if (parts <= 8) {
     if (slot < kSlots)
-      for (int r = y + slot * dy; r < nr; r += 2 * kSlots * dy) {
+      for (int r = y + slot * dy; r < nr; r += (parts <= 4 ? 2 : 1) * kSlots * dy) {
         if (parts <= 2)
-          rows(std::integral_constant<int, 2>(), r);
+          rows(two, two, r);
+        else if (parts <= 4)
+          rows(two, std::integral_constant<int, 4>(), r);
         else
-          rows(std::integral_constant<int, 4>(), r);
+          rows(one, std::integral_constant<int, 8>(), r);
       }
   } else {
     auto add = [&](const float *p, int r, float m, float &l, f32x4 &o) {
