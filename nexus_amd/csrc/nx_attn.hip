@@ -119,7 +119,6 @@ __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b,
 // are f32 split into two f16 halves (hi + lo: 22 bits), K and V enter as they are
 // stored; int8 codes as exact f16 values, with the key's scale on the score and the
 // value's on the weight.
-constexpr int kTile = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 // The largest weight of a row (p, or p times the value's scale) is 2^8 or more when the
 // reference m is set; m is set anew, and the sums scaled, when one passes 2^15.  So
@@ -252,10 +251,13 @@ __device__ __forceinline__ KeySpan tile_span(const KvSeq &s, const AttnCall &a, 
 }
 // Partial results of tiles that were split: per workgroup, those of the tile that
 // it ends (or passes through) and of the tile that it begins.
-//   desc [workgroups] {seq, head, r0, workgroups of the tile that begins here or 0}
 //   part [workgroups][2] {m[tile], l[tile], o[tile][D]}
+// The tile that a workgroup begins, where others go on with it:
+//   k_attn_split: done [workgroups] parts that are written, 0 between calls
+//   k_attn_tile: desc [workgroups] {seq, head, r0, its workgroups, or 0}
 struct AttnWork {
   int4 *desc;
+  int *done;
   float *part;
   int wgs_log2, min_share;
   int tile_cost;              // what a tile takes besides its groups, in units
@@ -288,6 +290,10 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ long uniform(long v) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
   return (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | lo);
+}
+
+__device__ __forceinline__ int quotient(long x, long y) {
+  return x <= UINT32_MAX && y <= UINT32_MAX ? (int)((uint32_t)x / (uint32_t)y) : (int)(x / y);
 }
 
 // Finds run `wg`.  A sequence's units are summed over its tiles by one thread, or
@@ -353,7 +359,7 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
   __syncthreads();
   r.seq = uniform(lds.seq);
   const long at = uniform(lds.at), in_head = uniform(lds.in_head);
-  r.head = at < INT32_MAX && in_head < INT32_MAX ? (int)((uint32_t)at / (uint32_t)in_head) : (int)(at / in_head);
+  r.head = quotient(at, in_head);
   long rest = at - r.head * in_head;
   const KvSeq s = kv_seq(b, r.seq, kv.page_log2);
   const int rows = s.n * a.group;
@@ -422,13 +428,6 @@ __device__ __forceinline__ void store_out(const AttnCall &a, const KvSeq &s, int
 }
 
 template <int FMT, int D>
-struct DecodeLds {
-  float m[4][kTile], l[4][kTile];
-  float o[4][kTile][D + 4];
-  int bad[kTile];
-};
-
-template <int FMT, int D>
 __device__ __forceinline__ void finish_rows(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                             const KvSeq &s, const Tile &t, const int *bad) {
   for (int r = threadIdx.x >> 6; r < t.nr; r += 4) {
@@ -440,6 +439,130 @@ __device__ __forceinline__ void finish_rows(const KvView &kv, const nx_kv_batch 
   }
 }
 
+// Memory that workgroups of one kernel pass on, on any XCD: each has an L2 of its own,
+// so these stores write through it and these loads go past it (device-scope atomics,
+// relaxed).  A device-wide fence instead writes back everything that the L2 holds:
+// with one per workgroup a decode batch took 442 us, not 233.
+template <typename T>
+__device__ __forceinline__ void store_through(T *p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void store_through(float *p, f32x4 v) {
+  const auto w = __builtin_bit_cast(ulong2, v);
+  store_through(reinterpret_cast<unsigned long *>(p), w.x);
+  store_through(reinterpret_cast<unsigned long *>(p) + 1, w.y);
+}
+template <bool THROUGH>
+__device__ __forceinline__ float load1(const float *p) {
+  return THROUGH ? __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *p;
+}
+template <bool THROUGH>
+__device__ __forceinline__ f32x4 load4(const float *p) {
+  if constexpr (!THROUGH) return *reinterpret_cast<const f32x4 *>(p);
+  const unsigned long *q = reinterpret_cast<const unsigned long *>(p);
+  const ulong2 w = {__hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                    __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)};
+  return __builtin_bit_cast(f32x4, w);
+}
+// waits until this wave's stores are where they go
+__device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+constexpr int kTile = 16, kRows = 128;  // rows of a tile of k_attn_split, k_attn_tile
+
+template <int D>
+struct JoinLds {
+  static constexpr int kSlots = 256 / (D / 4);
+  f32x4 o[kSlots][D / 4];
+  float m[kSlots], l[kSlots];
+  int bad[kRows];
+};
+
+// Joins rows y, y + dy, ... of a tile from its `parts` parts: the first one at `first`
+// in slot 1 of its workgroup, the others in slot 0 of the workgroups behind.  A row
+// takes D / 4 threads, or 2, 4, ... times as many that share its parts where rows are few.
+// THROUGH: this kernel wrote them.
+template <int FMT, int D, bool THROUGH>
+__device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
+                                          const KvSeq &s, const Tile &t, const float *first, int tile,
+                                          int parts, int y, int dy, JoinLds<D> &lds) {
+  constexpr int kSlots = JoinLds<D>::kSlots;
+  const int slot = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4), size = tile * (D + 2);
+  const int mine = (t.nr - y + dy - 1) / dy;
+  int share = 1;
+  while (2 * share * mine <= kSlots && share < parts) share *= 2;
+  const int sub = slot & (share - 1), at_once = kSlots / share;
+  if (threadIdx.x < kRows) lds.bad[threadIdx.x] = 0;
+  for (int k0 = 0; k0 < mine; k0 += at_once) {
+    const int k = k0 + slot / share, r = y + min(k, mine - 1) * dy;
+    float m = kUnset, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    auto take = [&](auto U, int i0) {  // U of the thread's parts, loaded ahead of their use
+      float mp[U()], lp[U()];
+      f32x4 op[U()];
+#pragma unroll
+      for (int x = 0; x < U(); ++x) {
+        const int i = min(i0 + x * share, parts - 1);
+        const float *p = first + (i == 0 ? 0 : (ptrdiff_t)(2 * i - 1) * size);
+        mp[x] = load1<THROUGH>(p + r);
+        lp[x] = load1<THROUGH>(p + tile + r);
+        op[x] = load4<THROUGH>(p + 2 * tile + r * D + 4 * d);
+      }
+      float m1 = m;
+#pragma unroll
+      for (int x = 0; x < U(); ++x) m1 = fmaxf(m1, mp[x]);
+      const float keep = exp2f(m - m1);
+      m = m1;
+      l *= keep;
+      o *= keep;
+#pragma unroll
+      for (int x = 0; x < U(); ++x) {
+        const bool is = i0 + x * share < parts;
+        const float f = is ? exp2f(mp[x] - m) : 0.f;
+        l += is ? lp[x] * f : 0.f;
+        o += (is ? op[x] : f32x4{0.f, 0.f, 0.f, 0.f}) * f;
+      }
+    };
+    if (parts <= 2 * share)
+      take(std::integral_constant<int, 2>(), sub);
+    else
+      for (int i = sub; i < parts; i += 4 * share) take(std::integral_constant<int, 4>(), i);
+    __syncthreads();  // bad is clear, and the last rows' sums are read
+    if (share > 1) {
+      if (slot < kSlots) {
+        lds.o[slot][d] = o;
+        if (d == 0) {
+          lds.m[slot] = m;
+          lds.l[slot] = l;
+        }
+      }
+      __syncthreads();
+      if (sub == 0 && slot < kSlots) {
+        float m1 = m;
+        for (int x = 1; x < share; ++x) m1 = fmaxf(m1, lds.m[slot + x]);
+        float f = exp2f(m - m1);
+        l *= f;
+        o *= f;
+        for (int x = 1; x < share; ++x) {
+          f = exp2f(lds.m[slot + x] - m1);
+          l += lds.l[slot + x] * f;
+          o += lds.o[slot + x][d] * f;
+        }
+      }
+    }
+    if (sub == 0 && slot < at_once * share && k < mine)
+      store_out<D>(a, s, t.head, t.r0 + r, 4 * d, o, l, &lds.bad[r]);
+  }
+  __syncthreads();
+  finish_rows<FMT, D>(kv, b, a, s, t, lds.bad);
+}
+
+template <int FMT, int D>
+struct DecodeLds {
+  float m[4][kTile], l[4][kTile];
+  float o[4][kTile][D + 4];
+  int bad[kTile];
+};
+
 template <int FMT, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv, nx_kv_batch b,
                                                                      AttnCall a, AttnWork w) {
@@ -450,12 +573,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
   __shared__ union {
     RunLds run;
     DecodeLds<FMT, D> rows;
+    JoinLds<D> join;
   } shared;
+  __shared__ int lead, parts;  // the first workgroup of a split tile, and how many have it
   DecodeLds<FMT, D> &lds = shared.rows;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   // neighbouring runs on one XCD: tiles of one head share its keys in that L2
   const int wg = (blockIdx.x & 7) << (w.wgs_log2 - 3) | blockIdx.x >> 3;
-  if (threadIdx.x == 0) w.desc[wg] = int4{0, 0, 0, 0};
   Run run;
   if (!find_run<kTile>(kv, b, a, w, wg, shared.run, run)) return;
   __syncthreads();  // shared is free for the rows
@@ -652,21 +776,36 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
       }
       if (!whole) {
         if (d == 0) {
-          part[r] = m1;
-          part[kTile + r] = lt;
+          store_through(part + r, m1);
+          store_through(part + kTile + r, lt);
         }
-        *reinterpret_cast<f32x4 *>(part + 2 * kTile + r * D + d) = o;
+        store_through(part + 2 * kTile + r * D + d, o);
       } else {
         const int rr = r0 + r;
         store_out<D>(a, s, head, rr, d, o, lt, &lds.bad[r]);
       }
     }
-    __syncthreads();
     if (whole) {
+      __syncthreads();
       finish_rows<FMT, D>(kv, b, a, s, t, lds.bad);
-    } else if (off == 0 && threadIdx.x == 0) {
-      // how many workgroups hold the tile's groups
-      w.desc[wg] = int4{seq, head, r0, (int)((next - 1) / run.share - wg) + 1};
+    } else {
+      // The last workgroup to write its part joins them all, in their order.
+      stores_done();  // this part, before the count says so
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const long begin = next - units + w.tile_cost;  // its first group
+        const int by = off == 0 ? wg : quotient(begin, run.share);
+        const int of = quotient(next - 1, run.share) - by + 1;
+        const bool last = atomicAdd(&w.done[by], 1) == of - 1;
+        if (last) w.done[by] = 0;  // for the next call
+        lead = by;
+        parts = last ? of : 0;
+      }
+      __syncthreads();
+      if (parts > 0) {
+        join_tile<FMT, D, true>(kv, b, a, s, t, w.part + ((size_t)lead * 2 + 1) * (kTile * (D + 2)), kTile, parts,
+                          0, 1, shared.join);
+      }
     }
     __syncthreads();  // lds is free
     if (u < run.end) next_tile<kTile>(kv, b, a, w, run, s);
@@ -682,8 +821,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
 // next group is on its way to registers while one is worked on and one lies in LDS;
 // int8 codes become f16 on their way to LDS, once for the four waves.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-constexpr int kRows = 128;
 
 // the other half of the wave's value
 template <typename Op>
@@ -938,113 +1075,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
       __syncthreads();
       finish_rows<FMT, D>(kv, b, a, s, Tile{seq, head, r0, nr}, bad);
     } else if (off == 0 && threadIdx.x == 0) {
-      w.desc[wg] = int4{seq, head, r0, (int)((next - 1) / run.share - wg) + 1};
+      w.desc[wg] = int4{seq, head, r0, quotient(next - 1, run.share) - wg + 1};
     }
     if (u < run.end) next_tile<kRows>(kv, b, a, w, run, s);
   }
 }
 
-// ------------------------------------------------------------ k_attn_join
-//
-// Joins the tiles whose units several workgroups had: a share of the rows of the tile
-// that workgroup x of k_attn_split begins, or, from its workgroups on, of k_attn_tile.
-// A row takes D / 4 threads.  Few parts (a run's end and the next one's begin): several
-// rows side by side, each thread adding its row's parts; many (a long context): one
-// row, the threads taking the parts in turn.
+// Joins the tiles of k_attn_tile whose units several workgroups had: a share of the
+// rows of the tile that workgroup x begins.  (A kernel of its own: 128 rows of many parts
+// are much for the one workgroup that ends last.)
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, AttnCall a, AttnWork w0,
-                                                   AttnWork w1, int wgs0) {
-  constexpr int kSlots = 256 / (D / 4);
-  __shared__ f32x4 lds[kSlots][D / 4];
-  __shared__ float sum_l[kSlots];
-  __shared__ int bad[kRows];
-  const bool wide = (int)blockIdx.x >= wgs0;
-  const int wg = wide ? blockIdx.x - wgs0 : blockIdx.x;
-  const int4 t = (wide ? w1 : w0).desc[wg];
-  const int parts = uniform(t.w);
-  if (parts == 0) return;
-  const int tile = wide ? kRows : kTile, seq = uniform(t.x), head = uniform(t.y), r0 = uniform(t.z);
+__global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, AttnCall a, AttnWork w) {
+  __shared__ JoinLds<D> lds;
+  const int4 t = w.desc[blockIdx.x];
+  if (t.w == 0) return;
+  const int seq = uniform(t.x), r0 = uniform(t.z);
   const KvSeq s = kv_seq(b, seq, kv.page_log2);
-  const int nr = min(tile, s.n * a.group - r0);
-  const float *first = (wide ? w1 : w0).part;
-  auto at = [&](int i) { return first + ((size_t)(wg + i) * 2 + (i == 0)) * (tile * (D + 2)); };
-  const int slot = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
-  if (threadIdx.x < kRows) bad[threadIdx.x] = 0;
-  __syncthreads();
-  // rows y, y + gridDim.y, ...
-  const int y = blockIdx.y, dy = gridDim.y;
-  // X rows of up to P parts at once, every load ahead of its use
-  auto rows = [&](auto X, auto P, int r) {
-    float m[X()], l[X()] = {}, mp[X()][P()], lp[X()][P()];
-    f32x4 o[X()] = {}, op[X()][P()];
-#pragma unroll
-    for (int x = 0; x < X(); ++x)
-#pragma unroll
-      for (int i = 0; i < P(); ++i) {
-        const float *p = at(min(i, parts - 1));
-        const int rx = min(r + x * kSlots * dy, nr - 1);
-        mp[x][i] = p[rx];
-        lp[x][i] = p[tile + rx];
-        op[x][i] = *reinterpret_cast<const f32x4 *>(p + 2 * tile + rx * D + 4 * d);
-      }
-#pragma unroll
-    for (int x = 0; x < X(); ++x) {
-      m[x] = kUnset;
-#pragma unroll
-      for (int i = 0; i < P(); ++i) m[x] = fmaxf(m[x], mp[x][i]);
-#pragma unroll
-      for (int i = 0; i < P(); ++i) {
-        const float f = i < parts ? exp2f(mp[x][i] - m[x]) : 0.f;
-        l[x] += i < parts ? lp[x][i] * f : 0.f;
-        o[x] += op[x][i] * f;
-      }
-      const int rx = r + x * kSlots * dy;
-      if (rx < nr) store_out<D>(a, s, head, r0 + rx, 4 * d, o[x], l[x], &bad[rx]);
-    }
-  };
-  constexpr std::integral_constant<int, 1> one{};
-  constexpr std::integral_constant<int, 2> two{};
-  if (parts <= 8) {
-    if (slot < kSlots)
-      for (int r = y + slot * dy; r < nr; r += (parts <= 4 ? 2 : 1) * kSlots * dy) {
-        if (parts <= 2)
-          rows(two, two, r);
-        else if (parts <= 4)
-          rows(two, std::integral_constant<int, 4>(), r);
-        else
-          rows(one, std::integral_constant<int, 8>(), r);
-      }
-  } else {
-    auto add = [&](const float *p, int r, float m, float &l, f32x4 &o) {
-      const float f = exp2f(p[r] - m);
-      l += p[tile + r] * f;
-      o += *reinterpret_cast<const f32x4 *>(p + 2 * tile + r * D + 4 * d) * f;
-    };
-    for (int r = y; r < nr; r += dy) {
-      float m = kUnset, l = 0.f;
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
-      for (int i = threadIdx.x & 63; i < parts; i += 64) m = fmaxf(m, at(i)[r]);
-#pragma unroll
-      for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-      if (slot < kSlots) {
-        for (int i = slot; i < parts; i += kSlots) add(at(i), r, m, l, o);
-        lds[slot][d] = o;
-        if (d == 0) sum_l[slot] = l;
-      }
-      __syncthreads();
-      if (slot == 0) {
-#pragma unroll
-        for (int i = 1; i < kSlots; ++i) {
-          o += lds[i][d];
-          l += sum_l[i];
-        }
-        store_out<D>(a, s, head, r0 + r, 4 * d, o, l, &bad[r]);
-      }
-      __syncthreads();  // lds is free
-    }
-  }
-  __syncthreads();
-  finish_rows<FMT, D>(kv, b, a, s, Tile{seq, head, r0, nr}, bad);
+  const int nr = min(kRows, s.n * a.group - r0);
+  if ((int)blockIdx.y >= nr) return;
+  join_tile<FMT, D, false>(kv, b, a, s, Tile{seq, uniform(t.y), r0, nr},
+                    w.part + ((size_t)blockIdx.x * 2 + 1) * (kRows * (D + 2)), kRows, uniform(t.w), blockIdx.y,
+                    gridDim.y, lds);
 }
 
 // Workgroups of a call (a power of two, so that whole XCDs get equal shares), and
@@ -1065,8 +1116,13 @@ int attn_workspace(nx_ctx *c, void **out) {
   const size_t wgs = (size_t)1 << attn_wgs_log2(c);
   // (k_attn_tile runs half as many workgroups on heads of 256)
   const size_t wide = std::max(part_floats(kRows, 128), part_floats(kRows, 256) / 2);
+  // (and a descriptor and a count of each)
+  const size_t bytes = wgs * (sizeof(int4) + sizeof(int) + 4 * (part_floats(kTile, 256) + wide));
+  const bool there = c->ws[WS_ATTN].cap >= bytes;
   void *p;
-  NX_TRY(ws_get(c, WS_ATTN, wgs * (2 * sizeof(int4) + 4 * (part_floats(kTile, 256) + wide)), &p));
+  NX_TRY(ws_get(c, WS_ATTN, bytes, &p));
+  if (!there)  // counts begin at 0
+    NX_HIP(hipMemsetAsync(static_cast<int4 *>(p) + wgs, 0, wgs * sizeof(int), c->stream));
   if (out) *out = p;
   return NX_OK;
 }
@@ -1085,11 +1141,12 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   const bool narrow = !wide || b.num_seqs > 1;
   const int log2 = attn_wgs_log2(c), wgs = 1 << log2;
   int4 *desc = static_cast<int4 *>(p);
-  float *part = reinterpret_cast<float *>(desc + 2 * wgs);
-  const AttnWork w0{desc, part, log2, 4 + kTileCost, kTileCost, 0, wide ? kTileFrom : INT32_MAX};
-  const AttnWork w1{desc + wgs, part + wgs * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2, 4 + kRowsCost,
-                    kRowsCost, narrow ? kTileFrom : 0, INT32_MAX};
-  const int wgs0 = narrow ? wgs : 0, wgs1 = wide ? 1 << w1.wgs_log2 : 0;
+  int *done = reinterpret_cast<int *>(desc + wgs);
+  float *part = reinterpret_cast<float *>(done + wgs);
+  const AttnWork w0{nullptr, done, part, log2, 4 + kTileCost, kTileCost, 0, wide ? kTileFrom : INT32_MAX};
+  const AttnWork w1{desc, nullptr, part + wgs * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2,
+                    4 + kRowsCost, kRowsCost, narrow ? kTileFrom : 0, INT32_MAX};
+  const int wgs1 = 1 << w1.wgs_log2;
   const KvView view = view_of(kv);
   if (wide)
     NX_TRY(launch(c, "attn_tile", [&] {
@@ -1100,12 +1157,13 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   if (narrow)
     NX_TRY(launch(c, "attn_split", [&] {
       with_kernel(kv, [&](auto fmt, auto D) {
-        go(c, k_attn_split<fmt(), D()>, dim3(wgs0), dim3(256), 0, view, b, a, w0);
+        go(c, k_attn_split<fmt(), D()>, dim3(wgs), dim3(256), 0, view, b, a, w0);
       });
     }));
+  if (!wide) return NX_OK;
   return launch(c, "attn_join", [&] {
     with_kernel(kv, [&](auto fmt, auto D) {
-      go(c, k_attn_join<fmt(), D()>, dim3(wgs0 + wgs1, wide ? 8 : 4), dim3(256), 0, view, b, a, w0, w1, wgs0);
+      go(c, k_attn_join<fmt(), D()>, dim3(wgs1, 8), dim3(256), 0, view, b, a, w1);
     });
   });
 }
