@@ -277,6 +277,7 @@ __device__ __forceinline__ int tile_units(const KvSeq &s, const AttnCall &a, con
 struct Run {
   long begin, end, share;
   int seq, head, r0, off;
+  KvSeq s;  // the sequence
 };
 struct RunLds {
   long sums[4];
@@ -296,11 +297,72 @@ __device__ __forceinline__ int quotient(long x, long y) {
   return x <= UINT32_MAX && y <= UINT32_MAX ? (int)((uint32_t)x / (uint32_t)y) : (int)(x / y);
 }
 
-// Finds run `wg`.  A sequence's units are summed over its tiles by one thread, or
-// by the workgroup where there are many; sequences are summed by a scan.
+// inclusive sum over the wave's lanes
+__device__ __forceinline__ uint32_t scan64(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// find_run for up to 64 sequences of few tiles and units, the usual decode step:
+// every wave by itself, a lane per sequence, without a barrier.  false: not such a batch.
+template <int TILE>
+__device__ __forceinline__ bool find_run_wave(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
+                                              const AttnWork &w, int wg, Run &r, bool &some) {
+  constexpr int kFew = 4;
+  const int lane = threadIdx.x & 63;
+  const KvSeq q = lane < b.num_seqs ? kv_seq(b, lane, kv.page_log2) : KvSeq{0, 0, 0, 0};
+  int rows = q.n * a.group;
+  if (rows <= w.rows_above || rows > w.rows_upto) rows = 0;
+  int u[kFew];
+  uint32_t c = 0;
+#pragma unroll
+  for (int i = 0; i < kFew; ++i) {
+    u[i] = i * TILE < rows ? tile_units(q, a, w, i * TILE, TILE) : 0;
+    c += u[i];
+  }
+  if (__any(rows > kFew * TILE || (long)c * kv.heads > (1 << 24))) return false;
+  const uint32_t mine = c * kv.heads, upto = scan64(mine);
+  const uint32_t total = __builtin_amdgcn_readlane(upto, 63);
+  const uint32_t share = max((total + (1u << w.wgs_log2) - 1) >> w.wgs_log2, (uint32_t)w.min_share);
+  const uint32_t begin = wg * share;
+  r.share = share;
+  r.begin = begin;
+  r.end = min(begin + share, total);
+  some = begin < total;
+  if (!some) return true;
+  const int s = __builtin_ctzll(__ballot(upto > begin));  // (its own units begin at or before)
+  auto of = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
+  const uint32_t at = begin - (of(upto) - of(mine)), in_head = of(c);
+  r.seq = s;
+  r.s = {of(q.row), of(q.n), of(q.first), of(q.len)};
+  r.head = at / in_head;
+  int rest = at - r.head * in_head, i = 0;
+#pragma unroll
+  for (int k = 0; k < kFew - 1; ++k) {
+    const int uk = of(u[k]);
+    const bool past = i == k && rest >= uk;
+    rest -= past ? uk : 0;
+    i += past;
+  }
+  r.r0 = i * TILE;
+  r.off = rest;
+  return true;
+}
+
+// Finds run `wg` in any batch.  A sequence's units are summed over its tiles by one
+// thread, or by the workgroup where there are many; sequences are summed by a scan.
 template <int TILE>
 __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                          const AttnWork &w, int wg, RunLds &lds, Run &r) {
+  if (b.num_seqs <= 64) {
+    bool some;
+    if (find_run_wave<TILE>(kv, b, a, w, wg, r, some)) return some;
+  }
   constexpr int kFew = 8;
   const int tid = threadIdx.x;
   auto rows_of = [&](const KvSeq &q) {
@@ -361,7 +423,7 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
   const long at = uniform(lds.at), in_head = uniform(lds.in_head);
   r.head = quotient(at, in_head);
   long rest = at - r.head * in_head;
-  const KvSeq s = kv_seq(b, r.seq, kv.page_log2);
+  const KvSeq s = r.s = kv_seq(b, r.seq, kv.page_log2);
   const int rows = s.n * a.group;
   if (rows <= kFew * TILE) {
     int units;
@@ -583,7 +645,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
   Run run;
   if (!find_run<kTile>(kv, b, a, w, wg, shared.run, run)) return;
   __syncthreads();  // shared is free for the rows
-  KvSeq s = kv_seq(b, run.seq, kv.page_log2);
+  KvSeq s = run.s;
   const float one = opaque_one();
 
   for (long u = run.begin; u < run.end;) {
@@ -862,7 +924,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
   if (threadIdx.x == 0) w.desc[wg] = int4{0, 0, 0, 0};
   Run run;
   if (!find_run<kRows>(kv, b, a, w, wg, shared.run, run)) return;
-  KvSeq s = kv_seq(b, run.seq, kv.page_log2);
+  KvSeq s = run.s;
   const float one = opaque_one();
 
   for (long u = run.begin; u < run.end;) {
