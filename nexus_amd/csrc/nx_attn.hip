@@ -260,16 +260,15 @@ struct AttnWork {
   int *done;
   float *part;
   int wgs_log2, min_share;
-  int tile_cost;              // what a tile takes besides its groups, in units
+  int tile_cost, join_cost;   // what a tile, and one in parts, takes besides its groups, in units
   int rows_above, rows_upto;  // the kernel's sequences: those of so many rows
 };
 
 // Units of a tile: its cost, then one per group (at least one, so that rows which
 // see nothing are written).
-__device__ __forceinline__ int tile_units(const KvSeq &s, const AttnCall &a, const AttnWork &w, int r0,
-                                          int tile) {
+__device__ __forceinline__ int tile_units(const KvSeq &s, const AttnCall &a, int cost, int r0, int tile) {
   const int nr = min(tile, s.n * a.group - r0);
-  return w.tile_cost + max(tile_span(s, a, r0, nr).count(), 1);
+  return cost + max(tile_span(s, a, r0, nr).count(), 1);
 }
 
 // A workgroup's run of units: [begin, end) of all, which starts `off` units into
@@ -277,7 +276,8 @@ __device__ __forceinline__ int tile_units(const KvSeq &s, const AttnCall &a, con
 struct Run {
   long begin, end, share;
   int seq, head, r0, off;
-  KvSeq s;  // the sequence
+  int cost;  // what a tile takes besides its groups, in units
+  KvSeq s;   // the sequence
 };
 struct RunLds {
   long sums[4];
@@ -310,6 +310,11 @@ __device__ __forceinline__ uint32_t scan64(uint32_t v) {
 
 // find_run for up to 64 sequences of few tiles and units, the usual decode step:
 // every wave by itself, a lane per sequence, without a barrier.  false: not such a batch.
+//
+// Here the tiles may also get the same number of workgroups each, and each workgroup one
+// tile: runs of `share` units that begin anew with every tile.  That is for steps whose
+// time is latency: a run that crosses into another tile waits for its query and its keys
+// again, and a tile that is split waits for its parts (join_cost).
 template <int TILE>
 __device__ __forceinline__ bool find_run_wave(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                               const AttnWork &w, int wg, Run &r, bool &some) {
@@ -318,39 +323,71 @@ __device__ __forceinline__ bool find_run_wave(const KvView &kv, const nx_kv_batc
   const KvSeq q = lane < b.num_seqs ? kv_seq(b, lane, kv.page_log2) : KvSeq{0, 0, 0, 0};
   int rows = q.n * a.group;
   if (rows <= w.rows_above || rows > w.rows_upto) rows = 0;
-  int u[kFew];
+  int u[kFew], tiles = 0, longest = 0;
   uint32_t c = 0;
 #pragma unroll
   for (int i = 0; i < kFew; ++i) {
-    u[i] = i * TILE < rows ? tile_units(q, a, w, i * TILE, TILE) : 0;
+    u[i] = i * TILE < rows ? tile_units(q, a, 0, i * TILE, TILE) : 0;
+    tiles += u[i] > 0;
+    longest = max(longest, u[i]);
     c += u[i];
   }
-  if (__any(rows > kFew * TILE || (long)c * kv.heads > (1 << 24))) return false;
-  const uint32_t mine = c * kv.heads, upto = scan64(mine);
-  const uint32_t total = __builtin_amdgcn_readlane(upto, 63);
-  const uint32_t share = max((total + (1u << w.wgs_log2) - 1) >> w.wgs_log2, (uint32_t)w.min_share);
-  const uint32_t begin = wg * share;
-  r.share = share;
-  r.begin = begin;
-  r.end = min(begin + share, total);
-  some = begin < total;
+  if (__any(rows > kFew * TILE || (long)(c + tiles * w.tile_cost) * kv.heads > (1 << 24))) return false;
+  const uint32_t total = __builtin_amdgcn_readlane(scan64(c * kv.heads), 63);
+  const uint32_t all_tiles = __builtin_amdgcn_readlane(scan64(tiles * kv.heads), 63);
+  if (all_tiles == 0) {
+    some = false;
+    return true;
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) longest = max(longest, __shfl_xor(longest, x, 64));
+  const uint32_t wgs = 1u << w.wgs_log2, most = uniform(longest);
+  // equal runs of all units, or the tiles apart, in one part or in as many as there are workgroups for
+  const uint32_t equal = ((total + all_tiles * w.tile_cost + wgs - 1) >> w.wgs_log2) + w.tile_cost + w.join_cost;
+  uint32_t share = equal, apart = 0;
+  if (all_tiles <= wgs) {
+    const uint32_t split = max((most + wgs / all_tiles - 1) / (wgs / all_tiles), (uint32_t)w.min_share);
+    const bool one = most <= split + w.join_cost;
+    const uint32_t cost = one ? most : split + w.join_cost;
+    if (cost <= equal) apart = one ? most : split;
+  }
+  if (apart > 0) {
+    r.cost = 0;
+    share = apart;
+    c = 0;
+#pragma unroll
+    for (int i = 0; i < kFew; ++i) c += ((uint32_t)u[i] + share - 1) / share * share;  // whole runs
+  } else {
+    r.cost = w.tile_cost;
+    c += tiles * w.tile_cost;
+#pragma unroll
+    for (int i = 0; i < kFew; ++i) u[i] += u[i] > 0 ? w.tile_cost : 0;
+    share = max((total + all_tiles * w.tile_cost + wgs - 1) >> w.wgs_log2, (uint32_t)w.min_share);
+  }
+  const uint32_t mine = c * kv.heads, upto = scan64(mine), begin = wg * share;
+  some = begin < (uint32_t)__builtin_amdgcn_readlane(upto, 63);
   if (!some) return true;
   const int s = __builtin_ctzll(__ballot(upto > begin));  // (its own units begin at or before)
   auto of = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
   const uint32_t at = begin - (of(upto) - of(mine)), in_head = of(c);
+  r.share = share;
+  r.begin = begin;
+  r.end = min(begin + share, (uint32_t)__builtin_amdgcn_readlane(upto, 63));
   r.seq = s;
   r.s = {of(q.row), of(q.n), of(q.first), of(q.len)};
   r.head = at / in_head;
   int rest = at - r.head * in_head, i = 0;
 #pragma unroll
   for (int k = 0; k < kFew - 1; ++k) {
-    const int uk = of(u[k]);
-    const bool past = i == k && rest >= uk;
-    rest -= past ? uk : 0;
+    const uint32_t uk = of(u[k]);
+    const int size = apart > 0 ? (uk + share - 1) / share * share : uk;
+    const bool past = i == k && rest >= size;
+    rest -= past ? size : 0;
     i += past;
   }
   r.r0 = i * TILE;
   r.off = rest;
+  if (apart > 0) r.end = begin + min((int)share, of(i == 0 ? u[0] : i == 1 ? u[1] : i == 2 ? u[2] : u[3]) - rest);
   return true;
 }
 
@@ -365,6 +402,7 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
   }
   constexpr int kFew = 8;
   const int tid = threadIdx.x;
+  r.cost = w.tile_cost;
   auto rows_of = [&](const KvSeq &q) {
     const int rows = q.n * a.group;
     return rows > w.rows_above && rows <= w.rows_upto ? rows : 0;
@@ -377,7 +415,7 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
     if (tid == 0) lds.bigs = 0;
     __syncthreads();
     if (rows <= kFew * TILE)
-      for (int r0 = 0; r0 < rows; r0 += TILE) c += tile_units(q, a, w, r0, TILE);
+      for (int r0 = 0; r0 < rows; r0 += TILE) c += tile_units(q, a, r.cost, r0, TILE);
     else
       lds.big[atomicAdd(&lds.bigs, 1)] = tid;
     __syncthreads();
@@ -387,7 +425,7 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
       const KvSeq o = kv_seq(b, s0 + t, kv.page_log2);
       long part = 0;
       for (long r0 = (long)tid * TILE; r0 < o.n * a.group; r0 += 256 * TILE)
-        part += tile_units(o, a, w, (int)r0, TILE);
+        part += tile_units(o, a, r.cost, (int)r0, TILE);
       scan256(part, lds.sums);
       if (tid == t) c = lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
     }
@@ -428,14 +466,14 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
   if (rows <= kFew * TILE) {
     int units;
     r.r0 = 0;
-    while (units = tile_units(s, a, w, r.r0, TILE), rest >= units) rest -= units, r.r0 += TILE;
+    while (units = tile_units(s, a, r.cost, r.r0, TILE), rest >= units) rest -= units, r.r0 += TILE;
     r.off = (int)rest;
     return true;
   }
   long base = 0;
   for (long r0 = 0; r0 < rows && base <= rest; r0 += 256 * TILE) {
     const long mine = r0 + (long)tid * TILE;
-    const long u = mine < rows ? tile_units(s, a, w, (int)mine, TILE) : 0;
+    const long u = mine < rows ? tile_units(s, a, r.cost, (int)mine, TILE) : 0;
     const long e = base + scan256(u, lds.sums);
     if (rest >= e - u && rest < e) {
       lds.r0 = (int)mine;
@@ -651,9 +689,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
   for (long u = run.begin; u < run.end;) {
     const int seq = run.seq, head = run.head, r0 = run.r0;
     // groups [off, stop) of the tile's; units past its cost
-    const int units = tile_units(s, a, w, r0, kTile);
+    const int units = tile_units(s, a, run.cost, r0, kTile);
     const int till = (int)min((long)units, run.off + (run.end - u));
-    const int off = max(run.off - w.tile_cost, 0), stop = till - w.tile_cost;
+    const int off = max(run.off - run.cost, 0), stop = till - run.cost;
     const bool whole = off == 0 && till == units;
     const long next = u - run.off + units;  // the batch's units up to the next tile
     u += till - run.off;
@@ -855,7 +893,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
       stores_done();  // this part, before the count says so
       __syncthreads();
       if (threadIdx.x == 0) {
-        const long begin = next - units + w.tile_cost;  // its first group
+        const long begin = next - units + run.cost;  // its first group
         const int by = off == 0 ? wg : quotient(begin, run.share);
         const int of = quotient(next - 1, run.share) - by + 1;
         const bool last = atomicAdd(&w.done[by], 1) == of - 1;
@@ -930,9 +968,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
   for (long u = run.begin; u < run.end;) {
     const int seq = run.seq, head = run.head, r0 = run.r0;
     // groups [off, stop) of the tile's; units past its cost
-    const int units = tile_units(s, a, w, r0, kRows);
+    const int units = tile_units(s, a, run.cost, r0, kRows);
     const int till = (int)min((long)units, run.off + (run.end - u));
-    const int off = max(run.off - w.tile_cost, 0), stop = till - w.tile_cost;
+    const int off = max(run.off - run.cost, 0), stop = till - run.cost;
     const bool whole = off == 0 && till == units;
     const long next = u - run.off + units;  // the batch's units up to the next tile
     u += till - run.off;
@@ -1169,6 +1207,19 @@ constexpr int kAttnWgsPerCu = 2;
 // at 0, 357 at 4, 353 at 8 and 362 at 16, a batch of 17 sequences and one chunk 93, 84, 86 and
 // 101; decode steps differ by less than 1 us up to 8.
 constexpr int kTileCost = 6, kRowsCost = 6;
+#ifndef NX_MS
+#define NX_MS 4
+#endif
+#ifndef NX_MR
+#define NX_MR 10
+#endif
+#ifndef NX_JC
+#define NX_JC 20
+#endif
+#ifndef NX_JR
+#define NX_JR 4
+#endif
+constexpr int kMinShare = NX_MS, kMinRows = NX_MR, kJoinCost = NX_JC, kJoinRows = NX_JR;
 // rows of a sequence from which k_attn_tile takes it
 constexpr int kTileFrom = 64;
 
@@ -1205,9 +1256,9 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   int4 *desc = static_cast<int4 *>(p);
   int *done = reinterpret_cast<int *>(desc + wgs);
   float *part = reinterpret_cast<float *>(done + wgs);
-  const AttnWork w0{nullptr, done, part, log2, 4 + kTileCost, kTileCost, 0, wide ? kTileFrom : INT32_MAX};
+  const AttnWork w0{nullptr, done, part, log2, kMinShare, kTileCost, kJoinCost, 0, wide ? kTileFrom : INT32_MAX};
   const AttnWork w1{desc, nullptr, part + wgs * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2,
-                    4 + kRowsCost, kRowsCost, narrow ? kTileFrom : 0, INT32_MAX};
+                    kMinRows, kRowsCost, kJoinRows, narrow ? kTileFrom : 0, INT32_MAX};
   const int wgs1 = 1 << w1.wgs_log2;
   const KvView view = view_of(kv);
   if (wide)
