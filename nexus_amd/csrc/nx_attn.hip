@@ -280,9 +280,9 @@ struct Run {
   KvSeq s;   // the sequence
 };
 struct RunLds {
-  long sums[4];
+  long sums[8];
   long at, in_head;
-  int seq, bigs, big[256], r0, off;
+  int seq, bigs, big[512], r0, off;
 };
 
 // what every lane has alike, as a scalar: addresses, bounds and branches on it
@@ -295,6 +295,27 @@ __device__ __forceinline__ long uniform(long v) {
 
 __device__ __forceinline__ int quotient(long x, long y) {
   return x <= UINT32_MAX && y <= UINT32_MAX ? (int)((uint32_t)x / (uint32_t)y) : (int)(x / y);
+}
+
+// inclusive sum over the workgroup's NW waves, and the whole sum
+template <int NW>
+__device__ __forceinline__ long scan_wg(long v, long *sums, long &total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const long o = __shfl_up(v, d, 64);
+    if (lane >= d) v += o;
+  }
+  __syncthreads();  // the last call's reads of sums
+  if (lane == 63) sums[wave] = v;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    v += w < wave ? sums[w] : 0;
+    total += sums[w];
+  }
+  return v;
 }
 
 // inclusive sum over the wave's lanes
@@ -393,14 +414,14 @@ __device__ __forceinline__ bool find_run_wave(const KvView &kv, const nx_kv_batc
 
 // Finds run `wg` in any batch.  A sequence's units are summed over its tiles by one
 // thread, or by the workgroup where there are many; sequences are summed by a scan.
-template <int TILE>
+template <int TILE, int NW>
 __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                          const AttnWork &w, int wg, RunLds &lds, Run &r) {
   if (b.num_seqs <= 64) {
     bool some;
     if (find_run_wave<TILE>(kv, b, a, w, wg, r, some)) return some;
   }
-  constexpr int kFew = 8;
+  constexpr int kFew = 8, kThreads = 64 * NW;
   const int tid = threadIdx.x;
   r.cost = w.tile_cost;
   auto rows_of = [&](const KvSeq &q) {
@@ -424,18 +445,19 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
       const int t = lds.big[i];
       const KvSeq o = kv_seq(b, s0 + t, kv.page_log2);
       long part = 0;
-      for (long r0 = (long)tid * TILE; r0 < o.n * a.group; r0 += 256 * TILE)
+      for (long r0 = (long)tid * TILE; r0 < o.n * a.group; r0 += kThreads * TILE)
         part += tile_units(o, a, r.cost, (int)r0, TILE);
-      scan256(part, lds.sums);
-      if (tid == t) c = lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
+      long whole;
+      scan_wg<NW>(part, lds.sums, whole);
+      if (tid == t) c = whole;
     }
     return c;
   };
-  long total = 0, c = 0, upto = 0;
-  for (int s0 = 0; s0 < b.num_seqs; s0 += 256) {
+  long total = 0, c = 0, upto = 0, chunk;
+  for (int s0 = 0; s0 < b.num_seqs; s0 += kThreads) {
     c = count(s0);
-    upto = total + scan256(c * kv.heads, lds.sums);
-    total += lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
+    upto = total + scan_wg<NW>(c * kv.heads, lds.sums, chunk);
+    total += chunk;
   }
   total = uniform(total);
   r.share = max((total + (1 << w.wgs_log2) - 1) >> w.wgs_log2, (long)w.min_share);
@@ -443,11 +465,11 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
   r.end = min(r.begin + r.share, total);
   if (r.begin >= r.end) return false;
   long before = 0;
-  for (int s0 = 0; s0 < b.num_seqs; s0 += 256) {
-    if (b.num_seqs > 256) {
+  for (int s0 = 0; s0 < b.num_seqs; s0 += kThreads) {
+    if (b.num_seqs > kThreads) {
       c = count(s0);
-      upto = before + scan256(c * kv.heads, lds.sums);
-      before += lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
+      upto = before + scan_wg<NW>(c * kv.heads, lds.sums, chunk);
+      before += chunk;
     }
     if (r.begin >= upto - c * kv.heads && r.begin < upto) {
       lds.seq = s0 + tid;
@@ -471,15 +493,15 @@ __device__ __forceinline__ bool find_run(const KvView &kv, const nx_kv_batch &b,
     return true;
   }
   long base = 0;
-  for (long r0 = 0; r0 < rows && base <= rest; r0 += 256 * TILE) {
+  for (long r0 = 0; r0 < rows && base <= rest; r0 += kThreads * TILE) {
     const long mine = r0 + (long)tid * TILE;
     const long u = mine < rows ? tile_units(s, a, r.cost, (int)mine, TILE) : 0;
-    const long e = base + scan256(u, lds.sums);
+    const long e = base + scan_wg<NW>(u, lds.sums, chunk);
     if (rest >= e - u && rest < e) {
       lds.r0 = (int)mine;
       lds.off = (int)(rest - (e - u));
     }
-    base += lds.sums[0] + lds.sums[1] + lds.sums[2] + lds.sums[3];
+    base += chunk;
   }
   __syncthreads();
   r.r0 = uniform(lds.r0);
@@ -527,10 +549,10 @@ __device__ __forceinline__ void store_out(const AttnCall &a, const KvSeq &s, int
   }
 }
 
-template <int FMT, int D>
+template <int FMT, int D, int NW>
 __device__ __forceinline__ void finish_rows(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                             const KvSeq &s, const Tile &t, const int *bad) {
-  for (int r = threadIdx.x >> 6; r < t.nr; r += 4) {
+  for (int r = threadIdx.x >> 6; r < t.nr; r += NW) {
     if (!bad[r]) continue;
     const int row = t.r0 + r, i = by_group(a, row), h = t.head * a.group + row - i * a.group;
     attn_row<FMT, D>(kv, b, a, s, t.seq, t.head, s.first + i,
@@ -569,9 +591,9 @@ __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)
 
 constexpr int kTile = 16, kRows = 128;  // rows of a tile of k_attn_split, k_attn_tile
 
-template <int D>
+template <int D, int NW>
 struct JoinLds {
-  static constexpr int kSlots = 256 / (D / 4);
+  static constexpr int kSlots = 64 * NW / (D / 4);
   f32x4 o[kSlots][D / 4];
   float m[kSlots], l[kSlots];
   int bad[kRows];
@@ -581,11 +603,11 @@ struct JoinLds {
 // in slot 1 of its workgroup, the others in slot 0 of the workgroups behind.  A row
 // takes D / 4 threads, or 2, 4, ... times as many that share its parts where rows are few.
 // THROUGH: this kernel wrote them.
-template <int FMT, int D, bool THROUGH>
+template <int FMT, int D, int NW, bool THROUGH>
 __device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                           const KvSeq &s, const Tile &t, const float *first, int tile,
-                                          int parts, int y, int dy, JoinLds<D> &lds) {
-  constexpr int kSlots = JoinLds<D>::kSlots;
+                                          int parts, int y, int dy, JoinLds<D, NW> &lds) {
+  constexpr int kSlots = JoinLds<D, NW>::kSlots;
   const int slot = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4), size = tile * (D + 2);
   const int mine = (t.nr - y + dy - 1) / dy;
   int share = 1;
@@ -653,35 +675,40 @@ __device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b
       store_out<D>(a, s, t.head, t.r0 + r, 4 * d, o, l, &lds.bad[r]);
   }
   __syncthreads();
-  finish_rows<FMT, D>(kv, b, a, s, t, lds.bad);
+  finish_rows<FMT, D, NW>(kv, b, a, s, t, lds.bad);
 }
 
-template <int FMT, int D>
+// waves of a decode workgroup: two per SIMD, or one where heads of 256 need the registers
+template <int D>
+constexpr int kDecodeWaves = D == 256 ? 4 : 8;
+
+template <int D, int NW>
 struct DecodeLds {
-  float m[4][kTile], l[4][kTile];
-  float o[4][kTile][D + 4];
+  float m[NW][kTile], l[NW][kTile];
+  float o[NW][kTile][D + 4];
   int bad[kTile];
 };
 
 template <int FMT, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv, nx_kv_batch b,
-                                                                     AttnCall a, AttnWork w) {
+__global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn_split(KvView kv, nx_kv_batch b,
+                                                                                    AttnCall a, AttnWork w) {
   using E = kv_elem<FMT>;
+  constexpr int NW = kDecodeWaves<D>;
   constexpr bool I8 = FMT == NX_KV_INT8;
   constexpr int KS = D / 32, DT = D / 16;     // steps of a score, 16-element tiles of the output
   constexpr int KL = I8 ? KS : 2 * KS, VL = I8 ? DT / 2 : DT;  // 16-byte loads of a lane and group
   __shared__ union {
     RunLds run;
-    DecodeLds<FMT, D> rows;
-    JoinLds<D> join;
+    DecodeLds<D, NW> rows;
+    JoinLds<D, NW> join;
   } shared;
   __shared__ int lead, parts;  // the first workgroup of a split tile, and how many have it
-  DecodeLds<FMT, D> &lds = shared.rows;
+  DecodeLds<D, NW> &lds = shared.rows;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   // neighbouring runs on one XCD: tiles of one head share its keys in that L2
   const int wg = (blockIdx.x & 7) << (w.wgs_log2 - 3) | blockIdx.x >> 3;
   Run run;
-  if (!find_run<kTile>(kv, b, a, w, wg, shared.run, run)) return;
+  if (!find_run<kTile, NW>(kv, b, a, w, wg, shared.run, run)) return;
   __syncthreads();  // shared is free for the rows
   KvSeq s = run.s;
   const float one = opaque_one();
@@ -701,6 +728,54 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
     }
     const Tile t{seq, head, r0, min(kTile, s.n * a.group - r0)};
     const KeySpan span = tile_span(s, a, r0, t.nr);
+
+    // ---- groups on their way: the page number a group ahead, then keys and values
+    uint4 kf[KL], vf[VL];
+    f32x4 dk[2], dv[2];  // INT8: scales of the lane's tokens
+    auto page_of = [&](int i) {  // of group i (of the last one behind it)
+      const int first = span.group(min(i, stop - 1)) * kKvGroup;
+      return span.count() > 0 ? b.pages[(long)seq * b.max_pages + (first >> kv.page_log2)] : -1;
+    };
+    auto is_there = [&](int page) { return page >= 0 && page < kv.pages; };
+    auto group_of = [&](int i, int page) {  // (pool group 0, masked, for one that is not there)
+      const int in_page = (span.group(min(i, stop - 1)) * kKvGroup & ((1 << kv.page_log2) - 1)) / kKvGroup;
+      return is_there(page) ? (((long)page * kv.heads + head) << (kv.page_log2 - 5)) + in_page : 0;
+    };
+    auto load_k = [&](long gr) {
+      const E *base = reinterpret_cast<const E *>(kv.k) + gr * (kKvGroup * D);
+      if constexpr (I8) {
+        const f32x4 *s = reinterpret_cast<const f32x4 *>(kv.ks + gr * kKvGroup + 8 * g);
+        dk[0] = s[0];
+        dk[1] = s[1];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          kf[ks] = *reinterpret_cast<const uint4 *>(base + ((4 * ks + g) * kKvGroup + 2 * n) * 8);
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            kf[2 * ks + h] = *reinterpret_cast<const uint4 *>(
+                base + ((4 * ks + g) * kKvGroup + 16 * (n >> 3) + 8 * h + (n & 7)) * 8);
+      }
+    };
+    auto load_v = [&](long gr) {
+      const E *base = reinterpret_cast<const E *>(kv.v) + gr * (kKvGroup * D);
+      if constexpr (I8) {
+        const f32x4 *s = reinterpret_cast<const f32x4 *>(kv.vs + gr * kKvGroup + 8 * g);
+        dv[0] = s[0];
+        dv[1] = s[1];
+      }
+#pragma unroll
+      for (int i = 0; i < VL; ++i)
+        vf[i] = *reinterpret_cast<const uint4 *>(base + (g * D + (I8 ? 32 * i + 2 * n : 16 * i + n)) * 8);
+    };
+    int page = page_of(off + wave), page1 = page_of(off + wave + NW);
+    {
+      const long gr = group_of(off + wave, page);
+      load_k(gr);
+      load_v(gr);
+    }
 
     // ---- this lane's query
     const int row = r0 + min(n, t.nr - 1), tok = by_group(a, row);
@@ -736,45 +811,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    uint4 kf[KL], vf[VL];
-    auto locate = [&](int i, int &first, bool &there) {  // unit i's first token and pool group
-      first = span.group(i) * kKvGroup;
-      const long gr = span.count() > 0 ? kv_group(kv, b, seq, head, first) : -1;
-      there = gr >= 0;
-      return there ? gr : 0;
-    };
-    auto load_k = [&](long gr) {
-      const E *base = reinterpret_cast<const E *>(kv.k) + gr * (kKvGroup * D);
-      if constexpr (I8) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          kf[ks] = *reinterpret_cast<const uint4 *>(base + ((4 * ks + g) * kKvGroup + 2 * n) * 8);
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            kf[2 * ks + h] = *reinterpret_cast<const uint4 *>(
-                base + ((4 * ks + g) * kKvGroup + 16 * (n >> 3) + 8 * h + (n & 7)) * 8);
-      }
-    };
-    auto load_v = [&](long gr) {
-      const E *base = reinterpret_cast<const E *>(kv.v) + gr * (kKvGroup * D);
-#pragma unroll
-      for (int i = 0; i < VL; ++i)
-        vf[i] = *reinterpret_cast<const uint4 *>(base + (g * D + (I8 ? 32 * i + 2 * n : 16 * i + n)) * 8);
-    };
-
-    int first, first1;
-    bool there, there1;
-    long gr = 0, gr1;
-    if (off + wave < stop) {
-      gr = locate(off + wave, first, there);
-      load_k(gr);
-      load_v(gr);
-    }
-    for (int i = off + wave; i < stop; i += 4) {
-      gr1 = locate(min(i + 4, stop - 1), first1, there1);
+    for (int i = off + wave; i < stop; i += NW) {
+      const int first = span.group(i) * kKvGroup;
+      const bool there = is_there(page);
+      const long gr1 = group_of(i + NW, page1);
+      page = page1;
+      page1 = page_of(i + 2 * NW);
       // scores of tokens first + 8 g + 4 h + j
       f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -789,16 +831,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
           sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, qh[ks], sc[h], 0, 0, 0);
           sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, ql[ks], sc[h], 0, 0, 0);
         }
-      float dv[8];
       if constexpr (I8) {
-        const f32x4 *dk = reinterpret_cast<const f32x4 *>(kv.ks + gr * kKvGroup + 8 * g);
-        const f32x4 *d2 = reinterpret_cast<const f32x4 *>(kv.vs + gr * kKvGroup + 8 * g);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          sc[h] *= dk[h];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) dv[4 * h + j] = d2[h][j];
-        }
+        sc[0] *= dk[0];
+        sc[1] *= dk[1];
       }
       load_k(gr1);  // the next group's keys, while this one's weights are made
 
@@ -819,15 +854,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
       if constexpr (I8) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          de[j] = scale_field(dv[j]);
+          de[j] = scale_field(dv[j >> 2][j & 3]);
           most_de = fmaxf(most_de, de[j]);
         }
         if (__any(most_de >= 255.f))
 #pragma unroll
-          for (int j = 0; j < 8; ++j) de[j] = dv[j] == dv[j] ? de[j] : kExpNan;
+          for (int j = 0; j < 8; ++j) de[j] = dv[j >> 2][j & 3] == dv[j >> 2][j & 3] ? de[j] : kExpNan;
       }
       float pr[8] = {sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]};
-      weigh<I8>(pr, [&](int j) { return finite_scale(dv[j]); }, [&](int j) { return de[j]; }, c, all, vis, ref,
+      weigh<I8>(pr, [&](int j) { return finite_scale(dv[j >> 2][j & 3]); }, [&](int j) { return de[j]; }, c, all, vis, ref,
                 l, acc, max_groups);
       f16x8 ph, pl;
       split2(pr, one, ph, pl);
@@ -842,9 +877,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
         acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vx, pl, acc[d], 0, 0, 0);
       }
       load_v(gr1);
-      first = first1;
-      there = there1;
-      gr = gr1;
     }
 
     // ---- join the waves
@@ -863,13 +895,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
     __syncthreads();
     // a tile's first workgroup keeps its part in slot 1, the others in slot 0
     float *part = w.part + ((size_t)wg * 2 + (off == 0)) * (kTile * (D + 2));
-    for (int e = threadIdx.x; e < t.nr * (D / 4); e += 256) {
+    for (int e = threadIdx.x; e < t.nr * (D / 4); e += 64 * NW) {
       const int r = e / (D / 4), d = e % (D / 4) * 4;
-      const float m1 = fmaxf(fmaxf(lds.m[0][r], lds.m[1][r]), fmaxf(lds.m[2][r], lds.m[3][r]));
+      float m1 = lds.m[0][r];
+#pragma unroll
+      for (int v = 1; v < NW; ++v) m1 = fmaxf(m1, lds.m[v][r]);
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
       float lt = 0.f;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
+      for (int v = 0; v < NW; ++v) {
         const float f = exp2f(lds.m[v][r] - m1);
         lt += lds.l[v][r] * f;
         o += *reinterpret_cast<const f32x4 *>(&lds.o[v][r][d]) * f;
@@ -887,7 +921,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
     }
     if (whole) {
       __syncthreads();
-      finish_rows<FMT, D>(kv, b, a, s, t, lds.bad);
+      finish_rows<FMT, D, NW>(kv, b, a, s, t, lds.bad);
     } else {
       // The last workgroup to write its part joins them all, in their order.
       stores_done();  // this part, before the count says so
@@ -903,7 +937,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_split(KvView kv,
       }
       __syncthreads();
       if (parts > 0) {
-        join_tile<FMT, D, true>(kv, b, a, s, t, w.part + ((size_t)lead * 2 + 1) * (kTile * (D + 2)), kTile, parts,
+        join_tile<FMT, D, NW, true>(kv, b, a, s, t, w.part + ((size_t)lead * 2 + 1) * (kTile * (D + 2)), kTile, parts,
                           0, 1, shared.join);
       }
     }
@@ -961,7 +995,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
   const int wg = (blockIdx.x & 7) << (w.wgs_log2 - 3) | blockIdx.x >> 3;
   if (threadIdx.x == 0) w.desc[wg] = int4{0, 0, 0, 0};
   Run run;
-  if (!find_run<kRows>(kv, b, a, w, wg, shared.run, run)) return;
+  if (!find_run<kRows, 4>(kv, b, a, w, wg, shared.run, run)) return;
   KvSeq s = run.s;
   const float one = opaque_one();
 
@@ -1173,7 +1207,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
     }
     if (whole) {
       __syncthreads();
-      finish_rows<FMT, D>(kv, b, a, s, Tile{seq, head, r0, nr}, bad);
+      finish_rows<FMT, D, 4>(kv, b, a, s, Tile{seq, head, r0, nr}, bad);
     } else if (off == 0 && threadIdx.x == 0) {
       w.desc[wg] = int4{seq, head, r0, quotient(next - 1, run.share) - wg + 1};
     }
@@ -1186,14 +1220,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
 // are much for the one workgroup that ends last.)
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, AttnCall a, AttnWork w) {
-  __shared__ JoinLds<D> lds;
+  __shared__ JoinLds<D, 4> lds;
   const int4 t = w.desc[blockIdx.x];
   if (t.w == 0) return;
   const int seq = uniform(t.x), r0 = uniform(t.z);
   const KvSeq s = kv_seq(b, seq, kv.page_log2);
   const int nr = min(kRows, s.n * a.group - r0);
   if ((int)blockIdx.y >= nr) return;
-  join_tile<FMT, D, false>(kv, b, a, s, Tile{seq, uniform(t.y), r0, nr},
+  join_tile<FMT, D, 4, false>(kv, b, a, s, Tile{seq, uniform(t.y), r0, nr},
                     w.part + ((size_t)blockIdx.x * 2 + 1) * (kRows * (D + 2)), kRows, uniform(t.w), blockIdx.y,
                     gridDim.y, lds);
 }
@@ -1206,15 +1240,18 @@ constexpr int kAttnWgsPerCu = 2;
 // kernel: without it runs of many short tiles end last.  A prompt of 4093 tokens took 418 us
 // at 0, 357 at 4, 353 at 8 and 362 at 16, a batch of 17 sequences and one chunk 93, 84, 86 and
 // 101; decode steps differ by less than 1 us up to 8.
-constexpr int kTileCost = 6, kRowsCost = 6;
+#ifndef NX_C0
+#define NX_C0 12
+#endif
+constexpr int kTileCost = NX_C0, kRowsCost = 6;
 #ifndef NX_MS
-#define NX_MS 4
+#define NX_MS 8
 #endif
 #ifndef NX_MR
 #define NX_MR 10
 #endif
 #ifndef NX_JC
-#define NX_JC 20
+#define NX_JC 16
 #endif
 #ifndef NX_JR
 #define NX_JR 4
@@ -1223,14 +1260,14 @@ constexpr int kMinShare = NX_MS, kMinRows = NX_MR, kJoinCost = NX_JC, kJoinRows 
 // rows of a sequence from which k_attn_tile takes it
 constexpr int kTileFrom = 64;
 
-static int attn_wgs_log2(const nx_ctx *c) { return std::max(3, 31 - __builtin_clz(c->num_cu * kAttnWgsPerCu)); }
+static int attn_wgs_log2(const nx_ctx *c) { return std::max(4, 31 - __builtin_clz(c->num_cu * kAttnWgsPerCu)); }
 static size_t part_floats(int tile, int D) { return (size_t)2 * tile * (D + 2); }
 int attn_workspace(nx_ctx *c, void **out) {
   const size_t wgs = (size_t)1 << attn_wgs_log2(c);
   // (k_attn_tile runs half as many workgroups on heads of 256)
   const size_t wide = std::max(part_floats(kRows, 128), part_floats(kRows, 256) / 2);
   // (and a descriptor and a count of each)
-  const size_t bytes = wgs * (sizeof(int4) + sizeof(int) + 4 * (part_floats(kTile, 256) + wide));
+  const size_t bytes = wgs * (sizeof(int4) + sizeof(int) + 4 * (part_floats(kTile, 256) / 2 + wide));
   const bool there = c->ws[WS_ATTN].cap >= bytes;
   void *p;
   NX_TRY(ws_get(c, WS_ATTN, bytes, &p));
@@ -1256,8 +1293,9 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   int4 *desc = static_cast<int4 *>(p);
   int *done = reinterpret_cast<int *>(desc + wgs);
   float *part = reinterpret_cast<float *>(done + wgs);
-  const AttnWork w0{nullptr, done, part, log2, kMinShare, kTileCost, kJoinCost, 0, wide ? kTileFrom : INT32_MAX};
-  const AttnWork w1{desc, nullptr, part + wgs * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2,
+  // (k_attn_split: one workgroup per CU)
+  const AttnWork w0{nullptr, done, part, log2 - 1, kMinShare, kTileCost, kJoinCost, 0, wide ? kTileFrom : INT32_MAX};
+  const AttnWork w1{desc, nullptr, part + wgs / 2 * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2,
                     kMinRows, kRowsCost, kJoinRows, narrow ? kTileFrom : 0, INT32_MAX};
   const int wgs1 = 1 << w1.wgs_log2;
   const KvView view = view_of(kv);
@@ -1270,7 +1308,7 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   if (narrow)
     NX_TRY(launch(c, "attn_split", [&] {
       with_kernel(kv, [&](auto fmt, auto D) {
-        go(c, k_attn_split<fmt(), D()>, dim3(wgs), dim3(256), 0, view, b, a, w0);
+        go(c, k_attn_split<fmt(), D()>, dim3(wgs / 2), dim3(64 * kDecodeWaves<D()>), 0, view, b, a, w0);
       });
     }));
   if (!wide) return NX_OK;
