@@ -285,48 +285,8 @@ struct RunLds {
   int seq, bigs, big[512], r0, off;
 };
 
-// what every lane has alike, as a scalar: addresses, bounds and branches on it
-// then cost no vector registers
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ long uniform(long v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-  return (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | lo);
-}
-
 __device__ __forceinline__ int quotient(long x, long y) {
   return x <= UINT32_MAX && y <= UINT32_MAX ? (int)((uint32_t)x / (uint32_t)y) : (int)(x / y);
-}
-
-// inclusive sum over the workgroup's NW waves, and the whole sum
-template <int NW>
-__device__ __forceinline__ long scan_wg(long v, long *sums, long &total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const long o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
-  __syncthreads();  // the last call's reads of sums
-  if (lane == 63) sums[wave] = v;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    v += w < wave ? sums[w] : 0;
-    total += sums[w];
-  }
-  return v;
-}
-
-// inclusive sum over the wave's lanes
-__device__ __forceinline__ uint32_t scan64(uint32_t v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return v;
 }
 
 // find_run for up to 64 sequences of few tiles and units, the usual decode step:

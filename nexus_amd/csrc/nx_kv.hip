@@ -94,49 +94,52 @@ __device__ __forceinline__ float stage_row(const float4 (&v)[D / 32], int t, int
 }
 
 // item of a batch: group `at` of sequence s's touched groups
-__device__ __forceinline__ long touched(const KvSeq &q) {
+__device__ __forceinline__ int touched(const KvSeq &q) {
   const int lo = max(q.first, 0);
   return q.n > 0 && q.len > lo ? (q.len - 1) / kKvGroup - lo / kKvGroup + 1 : 0;
 }
 
+// Eight waves: four for the keys, four for the values.
+constexpr int kMoveWaves = 8;
+
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void k_kv_write(KvView kv, nx_kv_batch b, const float *k,
-                                                  const float *v, size_t stride, bool wide) {
+__global__ __launch_bounds__(64 * kMoveWaves) void k_kv_write(KvView kv, nx_kv_batch b, const float *k,
+                                                              const float *v, size_t stride, bool wide) {
   using E = kv_elem<FMT>;
   using Chunk = std::conditional_t<FMT == NX_KV_INT8, uint2, uint4>;  // 8 elements
   __shared__ __align__(16) E tile[2][kKvGroup * D];
-  __shared__ long sums[4];
+  __shared__ long sums[kMoveWaves];
   __shared__ Place place;
   const int head = blockIdx.x % kv.heads;
-  const Place at = find_item(
-      b.num_seqs, blockIdx.x / kv.heads, [&](int s) { return touched(kv_seq(b, s, kv.page_log2)); },
-      sums, &place);
+  const Place at = find_item<kMoveWaves>(kv, b, blockIdx.x / kv.heads, touched, sums, &place);
   if (at.s < 0) return;
-  const KvSeq q = kv_seq(b, at.s, kv.page_log2);
-  const int g0 = (max(q.first, 0) / kKvGroup + (int)at.at) * kKvGroup;  // the group's first token
+  const KvSeq q = at.seq;
+  const int g0 = (max(q.first, 0) / kKvGroup + at.at) * kKvGroup;  // the group's first token
   const long group = kv_group(kv, b, at.s, head, g0);
   if (group < 0) return;
   // its tokens that the batch has: [lo, hi)
   const int lo = max(q.first - g0, 0), hi = min(q.len - g0, kKvGroup);
 
-  const int t = threadIdx.x >> 3, sub = threadIdx.x & 7;
+  const bool keys = threadIdx.x < 256;
+  const int tid = threadIdx.x & 255, t = tid >> 3, sub = tid & 7;
   if (t >= lo && t < hi) {
     const size_t row = (size_t)(q.row + (g0 + t - q.first)) * stride + (size_t)head * D;
     float4 r[D / 32];
-    load_row<D>(k + row, sub, wide, r);
-    const float s = stage_row<FMT, D, true>(r, t, sub, tile[0]);
-    if (FMT == NX_KV_INT8 && sub == 0) kv.ks[group * kKvGroup + t] = s;
-    load_row<D>(v + row, sub, wide, r);
-    const float sv = stage_row<FMT, D, false>(r, t, sub, tile[1]);
-    if (FMT == NX_KV_INT8 && sub == 0) kv.vs[group * kKvGroup + t] = sv;
+    load_row<D>((keys ? k : v) + row, sub, wide, r);
+    const float s = keys ? stage_row<FMT, D, true>(r, t, sub, tile[0]) : stage_row<FMT, D, false>(r, t, sub, tile[1]);
+    if (FMT == NX_KV_INT8 && sub == 0) (keys ? kv.ks : kv.vs)[group * kKvGroup + t] = s;
   }
   __syncthreads();
-  E *gk = reinterpret_cast<E *>(kv.k) + group * (kKvGroup * D);
+  if (keys) {
+    Chunk *gk = reinterpret_cast<Chunk *>(kv.k) + group * (kKvGroup * D / 8);
+    for (int c = tid; c < kKvGroup * D / 8; c += 256) {
+      const int token = kv_token(FMT, c & (kKvGroup - 1));
+      if (token >= lo && token < hi) gk[c] = reinterpret_cast<const Chunk *>(tile[0])[c];
+    }
+    return;
+  }
   E *gv = reinterpret_cast<E *>(kv.v) + group * (kKvGroup * D);
-  for (int c = threadIdx.x; c < kKvGroup * D / 8; c += 256) {
-    const int token = kv_token(FMT, c & (kKvGroup - 1));
-    if (token >= lo && token < hi)
-      reinterpret_cast<Chunk *>(gk)[c] = reinterpret_cast<const Chunk *>(tile[0])[c];
+  for (int c = tid; c < kKvGroup * D / 8; c += 256) {
     // a value chunk: tokens t0 .. t0 + 7 of one element; other tokens of it may
     // be in the cache already
     const int t0 = c / D * 8;
@@ -149,62 +152,59 @@ __global__ __launch_bounds__(256) void k_kv_write(KvView kv, nx_kv_batch b, cons
 }
 
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void k_kv_read(KvView kv, nx_kv_batch b, float *k, float *v,
-                                                 size_t stride, bool wide) {
+__global__ __launch_bounds__(64 * kMoveWaves) void k_kv_read(KvView kv, nx_kv_batch b, float *k, float *v,
+                                                             size_t stride, bool wide) {
   using E = kv_elem<FMT>;
   using Chunk = std::conditional_t<FMT == NX_KV_INT8, uint2, uint4>;
   __shared__ __align__(16) E tile[2][kKvGroup * D];
-  __shared__ long sums[4];
+  __shared__ long sums[kMoveWaves];
   __shared__ Place place;
   const int head = blockIdx.x % kv.heads;
   // rows without a token (before the first, behind the table) are read as zeros:
   // items cover the rows, in the groups that their tokens would have
-  const Place at = find_item(
-      b.num_seqs, blockIdx.x / kv.heads,
-      [&](int s) {
-        const KvSeq q = kv_seq(b, s, kv.page_log2);
-        return q.n > 0 ? (long)((q.first + q.n - 1) >> 5) - (q.first >> 5) + 1 : 0;
-      },
-      sums, &place);
+  const Place at = find_item<kMoveWaves>(
+      kv, b, blockIdx.x / kv.heads,
+      [](const KvSeq &q) { return q.n > 0 ? ((q.first + q.n - 1) >> 5) - (q.first >> 5) + 1 : 0; }, sums, &place);
   if (at.s < 0) return;
-  const KvSeq q = kv_seq(b, at.s, kv.page_log2);
-  const int g0 = ((q.first >> 5) + (int)at.at) * kKvGroup;
+  const KvSeq q = at.seq;
+  const int g0 = ((q.first >> 5) + at.at) * kKvGroup;
   const bool there = g0 >= 0 && g0 < (b.max_pages << kv.page_log2);
   const long group = there ? kv_group(kv, b, at.s, head, g0) : -1;
   const int lo = max(q.first - g0, 0), hi = min(q.first + q.n - g0, kKvGroup);
+  const bool keys = threadIdx.x < 256;
+  const int tid = threadIdx.x & 255, t = tid >> 3, sub = tid & 7;
+  float scale = 1.f;
   if (group >= 0) {
-    const Chunk *gk = reinterpret_cast<const Chunk *>(kv.k) + group * (kKvGroup * D / 8);
-    const Chunk *gv = reinterpret_cast<const Chunk *>(kv.v) + group * (kKvGroup * D / 8);
-    for (int c = threadIdx.x; c < kKvGroup * D / 8; c += 256) {
-      const int token = kv_token(FMT, c & (kKvGroup - 1)), t0 = c / D * 8;
-      if (token >= lo && token < hi) reinterpret_cast<Chunk *>(tile[0])[c] = gk[c];
-      if (t0 + 8 > lo && t0 < hi) reinterpret_cast<Chunk *>(tile[1])[c] = gv[c];
+    if (FMT == NX_KV_INT8 && t >= lo && t < hi) scale = (keys ? kv.ks : kv.vs)[group * kKvGroup + t];
+    const Chunk *from = reinterpret_cast<const Chunk *>(keys ? kv.k : kv.v) + group * (kKvGroup * D / 8);
+    Chunk *to = reinterpret_cast<Chunk *>(tile[keys ? 0 : 1]);
+#pragma unroll
+    for (int j = 0; j < kKvGroup * D / 8 / 256; ++j) {
+      const int c = tid + 256 * j, token = kv_token(FMT, c & (kKvGroup - 1)), t0 = c / D * 8;
+      if (keys ? token >= lo && token < hi : t0 + 8 > lo && t0 < hi) to[c] = from[c];
+    }
+    if constexpr (kKvGroup * D / 8 % 256 != 0) {
+      const int c = tid + kKvGroup * D / 8 / 256 * 256, token = kv_token(FMT, c & (kKvGroup - 1)), t0 = c / D * 8;
+      if (c < kKvGroup * D / 8 && (keys ? token >= lo && token < hi : t0 + 8 > lo && t0 < hi)) to[c] = from[c];
     }
   }
   __syncthreads();
-  const int t = threadIdx.x >> 3, sub = threadIdx.x & 7;
   if (t < lo || t >= hi) return;
-  const size_t row = (size_t)(q.row + (g0 + t - q.first)) * stride + (size_t)head * D;
-  const float sk = FMT == NX_KV_INT8 && group >= 0 ? kv.ks[group * kKvGroup + t] : 1.f;
-  const float sv = FMT == NX_KV_INT8 && group >= 0 ? kv.vs[group * kKvGroup + t] : 1.f;
+  float *out = (keys ? k : v) + (size_t)(q.row + (g0 + t - q.first)) * stride + (size_t)head * D;
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
     const int d0 = 4 * (sub + 8 * j);
-    float ek[4], ev[4];
+    float e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      ek[i] = group >= 0 ? (float)tile[0][kv_key_at(FMT, t, d0 + i)] * sk : 0.f;
-      ev[i] = group >= 0 ? (float)tile[1][kv_value_at(D, t, d0 + i)] * sv : 0.f;
+      const E x = keys ? tile[0][kv_key_at(FMT, t, d0 + i)] : tile[1][kv_value_at(D, t, d0 + i)];
+      e[i] = group >= 0 ? (float)x * scale : 0.f;
     }
     if (wide) {
-      *reinterpret_cast<float4 *>(k + row + d0) = float4{ek[0], ek[1], ek[2], ek[3]};
-      *reinterpret_cast<float4 *>(v + row + d0) = float4{ev[0], ev[1], ev[2], ev[3]};
+      *reinterpret_cast<float4 *>(out + d0) = float4{e[0], e[1], e[2], e[3]};
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        k[row + d0 + i] = ek[i];
-        v[row + d0 + i] = ev[i];
-      }
+      for (int i = 0; i < 4; ++i) out[d0 + i] = e[i];
     }
   }
 }
@@ -223,10 +223,10 @@ static int kv_move_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, const f
   return launch(c, write ? "kv_write" : "kv_read", [&] {
     with_kernel(kv, [&](auto fmt, auto D) {
       if (write)
-        go(c, k_kv_write<fmt(), D()>, grid, dim3(256), 0, view, b, rk, rv, stride,
+        go(c, k_kv_write<fmt(), D()>, grid, dim3(64 * kMoveWaves), 0, view, b, rk, rv, stride,
            wide_rows(rk, rv, stride));
       else
-        go(c, k_kv_read<fmt(), D()>, grid, dim3(256), 0, view, b, wk, wv, stride,
+        go(c, k_kv_read<fmt(), D()>, grid, dim3(64 * kMoveWaves), 0, view, b, wk, wv, stride,
            wide_rows(wk, wv, stride));
     });
   });

@@ -60,50 +60,75 @@ __device__ __forceinline__ long kv_group(const KvView &kv, const nx_kv_batch &b,
   return (((long)page * kv.heads + head) << (kv.page_log2 - 5)) + in_page;
 }
 
-// Inclusive sum over the workgroup's first 256 threads (blockDim.x == 256).
-__device__ __forceinline__ long scan256(long v, long *lds4) {
+// what every lane has alike, as a scalar: addresses, bounds and branches on it
+// then cost no vector registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long uniform(long v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  return (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | lo);
+}
+
+// inclusive sum over the workgroup's NW waves, and the whole sum
+template <int NW>
+__device__ __forceinline__ long scan_wg(long v, long *sums, long &total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const long o = __shfl_up(v, d, 64);
     if (lane >= d) v += o;
   }
-  __syncthreads();  // the last call's reads of lds4
-  if (lane == 63) lds4[wave] = v;
+  __syncthreads();  // the last call's reads of sums
+  if (lane == 63) sums[wave] = v;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) v += lds4[w];
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    v += w < wave ? sums[w] : 0;
+    total += sums[w];
+  }
   return v;
 }
 
-// Which sequence holds item `item` when sequence s has count(s) of them, and
-// which of its items that is; *s = -1 past the last one.  All 256 threads.
-struct Place {
-  int s;
-  long at;
-};
-template <typename Count>
-__device__ __forceinline__ Place find_item(int seqs, long item, Count count, long *lds4, Place *lds) {
-  if (threadIdx.x == 0) *lds = {-1, 0};
-  long before = 0;
-  for (int s0 = 0; s0 < seqs; s0 += 256) {
-    const int s = s0 + (int)threadIdx.x;
-    const long c = s < seqs ? count(s) : 0;
-    const long end = before + scan256(c, lds4);
-    if (c > 0 && item >= end - c && item < end) *lds = {s, item - (end - c)};
-    before += lds4[0] + lds4[1] + lds4[2] + lds4[3];
-    if (item < before) break;  // uniform: every thread has the same sums
-  }
-  __syncthreads();
-  return *lds;
+// inclusive sum over the wave's lanes
+__device__ __forceinline__ uint32_t scan64(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
 }
 
-// The sequence that owns row `row`; -1 for padding.  All 256 threads.
-__device__ __forceinline__ int find_row(const nx_kv_batch &b, int row, int page_log2, int *lds) {
-  if (threadIdx.x == 0) *lds = -1;
-  __syncthreads();
-  for (int s = threadIdx.x; s < b.num_seqs; s += 256) {
-    const KvSeq q = kv_seq(b, s, page_log2);
-    if (row >= q.row && row < q.row + q.n) *lds = s;
+// Which sequence holds item `item` when sequence s has count(its KvSeq) of them, at
+// most 2^31 in all, and which of its items that is; s = -1 past the last one.  All threads
+// of a workgroup of NW waves; up to 64 sequences each wave finds it by itself.
+struct Place {
+  int s, at;
+  KvSeq seq;
+};
+template <int NW, typename Count>
+__device__ __forceinline__ Place find_item(const KvView &kv, const nx_kv_batch &b, int item, Count count,
+                                           long *sums, Place *lds) {
+  if (b.num_seqs <= 64) {
+    const int lane = threadIdx.x & 63;
+    const KvSeq q = lane < b.num_seqs ? kv_seq(b, lane, kv.page_log2) : KvSeq{0, 0, 0, 0};
+    const uint32_t c = count(q), upto = scan64(c);
+    const uint64_t past = __ballot(upto > (uint32_t)item);
+    if (!past) return {-1, 0, q};
+    const int s = __builtin_ctzll(past);
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
+    return {s, item - (of(upto) - of(c)), {of(q.row), of(q.n), of(q.first), of(q.len)}};
+  }
+  if (threadIdx.x == 0) lds->s = -1;
+  long before = 0, chunk;
+  for (int s0 = 0; s0 < b.num_seqs; s0 += 64 * NW) {
+    const int s = s0 + (int)threadIdx.x;
+    const KvSeq q = s < b.num_seqs ? kv_seq(b, s, kv.page_log2) : KvSeq{0, 0, 0, 0};
+    const long c = count(q), end = before + scan_wg<NW>(c, sums, chunk);
+    if (item >= end - c && item < end) *lds = {s, (int)(item - (end - c)), q};
+    before += chunk;
+    if (item < before) break;  // uniform: every thread has the same sums
   }
   __syncthreads();
   return *lds;
