@@ -120,6 +120,10 @@ def assert_close(got, ref, bound, scores=8.0):
     assert np.linalg.norm(got - ref) <= limit * norm, np.linalg.norm(got - ref) / norm
 
 
+def rel_l2(got, ref) -> float:
+    return float(np.linalg.norm(np.asarray(got, np.float64) - ref) / np.linalg.norm(ref))
+
+
 def random_kv(rng, tokens, G, D):
     """Keys with a few large channels, values: f32 [tokens x G x D]."""
     k = rng.standard_normal((tokens, G, D), dtype=np.float32)
