@@ -311,17 +311,17 @@ int nx_kv_read_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float
  * h / (heads / kv_heads).  window = 0: all of them; window > 0: its last
  * `window` tokens (itself included) and the sequence's first `sinks` tokens.  A
  * row that sees no token is zeros.  q rows are heads * head_dim floats, q_stride
- * floats apart, out rows likewise; neither needs an alignment.  f32 in and
- * out: scores, softmax and sums are held in f32, and the f32 factors of the
+ * floats apart, out rows likewise; neither needs an alignment, and out must not
+ * overlap q.  f32 in and out: scores, softmax and sums are held in f32, and the f32 factors of the
  * f16 matrix products are split into two halves (relative error about 1e-6
  * against the same cache in 64 bits).  A row's last bits depend on the batch
  * that it is in (the order of the sums does), not on the run.
  * attention_decode (src/engine/mod.rs:452-500) and
  * kernel::grouped_query_attention (src/kernel/mod.rs:40-99) for a batch.
- * The workspace is the context's, allocated with the first cache or call on it
- * and never moved, so a captured call may be replayed while the context lives;
- * calls on one context must not overlap in time (two graphs captured from it
- * neither). */
+ * The workspace (some 80 MB) is the context's, allocated with the first cache or
+ * call on it and never moved, so a captured call may be replayed while the context
+ * lives; calls on one context must not overlap in time (two graphs captured from
+ * it neither), and a context's first call or cache is not made under capture. */
 int nx_attention(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *q,
                  size_t q_stride, int heads, float scale, int window, int sinks, float *out,
                  size_t out_stride);

@@ -68,6 +68,10 @@ __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b,
     const uint64_t seen = __ballot(group >= 0);
     if (!seen) continue;
     any = true;
+    if (__any(x != x)) {  // a NaN score makes the row NaNs
+      l = NAN;
+      break;
+    }
     float top = x;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
@@ -1323,12 +1327,16 @@ extern "C" {
 
 int nx_attention(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const float *q, size_t q_stride,
                  int heads, float scale, int window, int sinks, float *out, size_t out_stride) {
-  return attention(c, kv, b, q, q_stride, heads, scale, window, sinks, out, out_stride, true);
+  return guarded([&] {
+    return attention(c, kv, b, q, q_stride, heads, scale, window, sinks, out, out_stride, true);
+  });
 }
 int nx_attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const float *q,
                      size_t q_stride, int heads, float scale, int window, int sinks, float *out,
                      size_t out_stride) {
-  return attention(c, kv, b, q, q_stride, heads, scale, window, sinks, out, out_stride, false);
+  return guarded([&] {
+    return attention(c, kv, b, q, q_stride, heads, scale, window, sinks, out, out_stride, false);
+  });
 }
 
 }  // extern "C"

@@ -294,13 +294,7 @@ static int kv_move(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const float
   return NX_OK;
 }
 
-}  // namespace nx
-
-using namespace nx;
-
-extern "C" {
-
-int nx_kv_create(nx_ctx *c, int fmt, int pages, int page_tokens, int heads, int D, nx_kv **out) {
+static int kv_create(nx_ctx *c, int fmt, int pages, int page_tokens, int heads, int D, nx_kv **out) {
   if (out) *out = nullptr;
   if (!c) return fail(NX_ERR_INVALID_ARG, "null context");
   if (!out) return fail(NX_ERR_INVALID_ARG, "null output pointer");
@@ -344,6 +338,16 @@ int nx_kv_create(nx_ctx *c, int fmt, int pages, int page_tokens, int heads, int 
   return NX_OK;
 }
 
+}  // namespace nx
+
+using namespace nx;
+
+extern "C" {
+
+int nx_kv_create(nx_ctx *c, int fmt, int pages, int page_tokens, int heads, int D, nx_kv **out) {
+  return guarded([&] { return kv_create(c, fmt, pages, page_tokens, heads, D, out); });
+}
+
 int nx_kv_info(const nx_kv *kv, int *fmt, int *pages, int *page_tokens, int *heads, int *D, size_t *bytes) {
   if (!kv) return fail(NX_ERR_INVALID_ARG, "null cache");
   if (fmt) *fmt = kv->fmt;
@@ -365,17 +369,17 @@ int nx_kv_destroy(nx_kv *kv) {
 }
 
 int nx_kv_write(nx_ctx *c, nx_kv *kv, const nx_kv_batch *b, const float *k, const float *v, size_t stride) {
-  return kv_move(c, kv, b, k, v, nullptr, nullptr, stride, true, true);
+  return guarded([&] { return kv_move(c, kv, b, k, v, nullptr, nullptr, stride, true, true); });
 }
 int nx_kv_write_dev(nx_ctx *c, nx_kv *kv, const nx_kv_batch *b, const float *k, const float *v,
                     size_t stride) {
-  return kv_move(c, kv, b, k, v, nullptr, nullptr, stride, true, false);
+  return guarded([&] { return kv_move(c, kv, b, k, v, nullptr, nullptr, stride, true, false); });
 }
 int nx_kv_read(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, float *k, float *v, size_t stride) {
-  return kv_move(c, kv, b, nullptr, nullptr, k, v, stride, false, true);
+  return guarded([&] { return kv_move(c, kv, b, nullptr, nullptr, k, v, stride, false, true); });
 }
 int nx_kv_read_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, float *k, float *v, size_t stride) {
-  return kv_move(c, kv, b, nullptr, nullptr, k, v, stride, false, false);
+  return guarded([&] { return kv_move(c, kv, b, nullptr, nullptr, k, v, stride, false, false); });
 }
 
 }  // extern "C"

@@ -164,7 +164,7 @@ constexpr KeySpan key_span(int pmin, int pmax, int len, int window, int sinks) {
   const int to = last < 0 ? 0 : last / kKvGroup + 1;
   int from = 0, first = 0;
   if (window > 0) {
-    const int lo = pmin - window + 1;  // (pmin >= -2^24, so no overflow)
+    const int lo = (pmin > 0 ? pmin : 0) - window + 1;  // (a row before token 0 sees nothing)
     from = lo > 0 ? lo / kKvGroup : 0;
     if (from > to) from = to;
     first = sinks / kKvGroup + (sinks % kKvGroup != 0);

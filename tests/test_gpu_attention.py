@@ -259,6 +259,27 @@ def test_rows_that_see_nothing(ctx, fmt):
         cache.close()
 
 
+@pytest.mark.parametrize("window", [1, 9, 2 ** 31 - 1])
+def test_rows_before_the_first_token_in_a_window(ctx, window):
+    """A tile whose first rows are before the first token: the others' windows count."""
+    rng = np.random.default_rng(20)
+    H, G, D, n, length = 4, 2, 64, 30, 12
+    b = Batch(rng, [n], [n], 32)
+    cache, k, v = filled(ctx, rng, b, F16, G, D)
+    b.kv_len[0] = length  # rows 0 .. 17 are tokens -18 .. -1
+    q = rng.standard_normal((n, H, D)).astype(np.float32)
+    dq, do = DeviceArray(q.size), DeviceArray(q.size, fill=7.0)
+    dq.upload(q)
+    cache.attention_dev(device_batch(b), dq.ptr, H * D, H, do.ptr, H * D, 0.125, window=window)
+    ctx.sync()
+    got = do.download().reshape(q.shape)
+    assert np.all(got[:n - length] == 0)
+    short = Batch(rng, [length], [length], 32)
+    ref, bound = attention(short, k[:length], v[:length], q[n - length:], H, np.float32(0.125), window)
+    assert_close(got[n - length:], ref, bound)
+    cache.close()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_missing_page_in_the_middle(ctx, fmt):
     """Tokens on a page that the cache does not have are not attended to."""

@@ -163,6 +163,37 @@ def test_attention_arguments(tmp_path):
 
 
 @needs_gxx
+def test_key_spans(tmp_path):
+    """The groups of a span hold every token that some row sees, in order, each
+    once; rows before a sequence's first token see nothing and cost none."""
+    run(tmp_path, r"""
+  auto sees = [](int p, int j, int window, int sinks) {
+    return j <= p && (window == 0 || (long)p - j < window || j < sinks);
+  };
+  for (int len : {0, 1, 31, 32, 33, 64, 100, 200})
+    for (int pmin = -40; pmin < 210; pmin += 7)
+      for (int width : {0, 1, 5, 33})
+        for (int window : {0, 1, 2, 31, 32, 33, 90, 1000, INT_MAX})
+          for (int sinks : {0, 1, 32, 33, 64, 500, INT_MAX}) {
+            const int pmax = pmin + width;
+            const KeySpan s = key_span(pmin, pmax, len, window, sinks);
+            is(s.sinks >= 0 && s.sinks <= s.from && s.from <= s.to && s.to <= (len + 31) / 32, "in order");
+            std::set<int> groups;
+            for (int i = 0; i < s.count(); ++i) groups.insert(s.group(i));
+            is((int)groups.size() == s.count(), "each once");
+            for (int p = pmin; p <= pmax; ++p)
+              for (int j = 0; j < len; ++j)
+                if (sees(p, j, window, sinks)) is(groups.count(j / 32) == 1, "a token that is seen");
+            if (pmax < 0) is(s.count() == 0, "rows before the first token");
+          }
+  // the longest sequences and windows
+  const KeySpan far = key_span(INT_MAX - 70000, INT_MAX - 69999, INT_MAX - 65536, INT_MAX, INT_MAX);
+  is(far.from == 0 && far.to == (INT_MAX - 69999) / 32 + 1, "far");
+  is(key_span(-(1 << 24), 5, 6, INT_MAX, 0).count() == 1, "before the first token, wide window");
+""")
+
+
+@needs_gxx
 def test_touched_groups_bound(tmp_path):
     run(tmp_path, r"""
   for (int first = 0; first < 64; ++first)
