@@ -293,13 +293,14 @@ __device__ __forceinline__ int quotient(long x, long y) {
   return x <= UINT32_MAX && y <= UINT32_MAX ? (int)((uint32_t)x / (uint32_t)y) : (int)(x / y);
 }
 
-// find_run for up to 64 sequences of few tiles and units, the usual decode step:
-// every wave by itself, a lane per sequence, without a barrier.  false: not such a batch.
+// find_run for up to 64 sequences, the usual step: every wave by itself, a lane per
+// sequence, without a barrier.  false: left to the workgroup (equal runs over many tiles).
 //
-// Here the tiles may also get the same number of workgroups each, and each workgroup one
-// tile: runs of `share` units that begin anew with every tile.  That is for steps whose
-// time is latency: a run that crosses into another tile waits for its query and its keys
-// again, and a tile that is split waits for its parts (join_cost).
+// Two ways to deal the units out.  Equal runs of all of them load every CU alike.  Or the
+// tiles apart: the same number of workgroups for each, and a workgroup has one tile.
+// That is for steps whose time is latency: a run that crosses into another tile waits for
+// its query and its keys again, and a tile in parts waits for them (join_cost), so
+// tiles are also taken whole where that ends sooner.
 template <int TILE>
 __device__ __forceinline__ bool find_run_wave(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                               const AttnWork &w, int wg, Run &r, bool &some) {
@@ -308,71 +309,85 @@ __device__ __forceinline__ bool find_run_wave(const KvView &kv, const nx_kv_batc
   const KvSeq q = lane < b.num_seqs ? kv_seq(b, lane, kv.page_log2) : KvSeq{0, 0, 0, 0};
   int rows = q.n * a.group;
   if (rows <= w.rows_above || rows > w.rows_upto) rows = 0;
-  int u[kFew], tiles = 0, longest = 0;
+  const int tiles = (rows + TILE - 1) / TILE;
+  if (__any(tiles > 1 << 12)) return false;
+  // first, last and longest tile (through a window: a bound of the longest), and all by their mean
+  const int begin_u = tiles > 0 ? tile_units(q, a, 0, 0, TILE) : 0;
+  const int end_u = tiles > 1 ? tile_units(q, a, 0, (tiles - 1) * TILE, TILE) : begin_u;
+  int longest = end_u;
+  if (a.window > 0 && tiles > 1) {
+    const long seen = min((long)a.sinks, (long)q.len) / kKvGroup + 1 +
+                      ((long)a.window + by_group(a, TILE) + 2) / kKvGroup + 2;
+    longest = (int)min(seen, (long)max(q.len, 1) / kKvGroup + 1);
+  }
+  const uint32_t guess = min((long)tiles * (begin_u + end_u) / 2 * kv.heads, 1L << 24);
+  const uint32_t tiles_upto = scan64(tiles * kv.heads);
+  const uint32_t all_tiles = __builtin_amdgcn_readlane(tiles_upto, 63);
+  some = all_tiles > 0;
+  if (!some) return true;
+  const uint32_t wgs = 1u << w.wgs_log2;
+  if (all_tiles <= wgs) {
+    const uint32_t total = __builtin_amdgcn_readlane(scan64(guess), 63);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) longest = max(longest, __shfl_xor(longest, x, 64));
+    const uint32_t most = uniform(longest), each = wgs / all_tiles;
+    const uint32_t split = max((most + each - 1) / each, (uint32_t)w.min_share);
+    const bool one = most <= split + w.join_cost;
+    const uint32_t share = one ? most : split, cost = one ? most : split + w.join_cost;
+    if (cost <= (total + all_tiles * w.tile_cost) / wgs + w.tile_cost + w.join_cost) {
+      const uint32_t parts = (most + share - 1) / share, tile = wg / parts, part = wg - tile * parts;
+      some = tile < all_tiles;
+      if (!some) return true;
+      const int s = __builtin_ctzll(__ballot(tiles_upto > tile));
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
+      const uint32_t in_head = of(tiles), at = tile - (of(tiles_upto) - in_head * kv.heads);
+      r.seq = s;
+      r.s = {of(q.row), of(q.n), of(q.first), of(q.len)};
+      r.head = at / in_head;
+      r.r0 = (int)(at - r.head * in_head) * TILE;
+      r.cost = 0;
+      r.share = share;
+      r.off = part * share;
+      const int units = tile_units(r.s, a, 0, r.r0, TILE);
+      some = r.off < units;
+      r.begin = (long)wg * share;
+      r.end = r.begin + min((int)share, units - r.off);
+      return true;
+    }
+  }
+  if (__any(rows > kFew * TILE)) return false;
+  r.cost = w.tile_cost;
+  int u[kFew];
   uint32_t c = 0;
 #pragma unroll
   for (int i = 0; i < kFew; ++i) {
-    u[i] = i * TILE < rows ? tile_units(q, a, 0, i * TILE, TILE) : 0;
-    tiles += u[i] > 0;
-    longest = max(longest, u[i]);
+    u[i] = i * TILE < rows ? tile_units(q, a, r.cost, i * TILE, TILE) : 0;
     c += u[i];
   }
-  if (__any(rows > kFew * TILE || (long)(c + tiles * w.tile_cost) * kv.heads > (1 << 24))) return false;
-  const uint32_t total = __builtin_amdgcn_readlane(scan64(c * kv.heads), 63);
-  const uint32_t all_tiles = __builtin_amdgcn_readlane(scan64(tiles * kv.heads), 63);
-  if (all_tiles == 0) {
-    some = false;
-    return true;
-  }
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) longest = max(longest, __shfl_xor(longest, x, 64));
-  const uint32_t wgs = 1u << w.wgs_log2, most = uniform(longest);
-  // equal runs of all units, or the tiles apart, in one part or in as many as there are workgroups for
-  const uint32_t equal = ((total + all_tiles * w.tile_cost + wgs - 1) >> w.wgs_log2) + w.tile_cost + w.join_cost;
-  uint32_t share = equal, apart = 0;
-  if (all_tiles <= wgs) {
-    const uint32_t split = max((most + wgs / all_tiles - 1) / (wgs / all_tiles), (uint32_t)w.min_share);
-    const bool one = most <= split + w.join_cost;
-    const uint32_t cost = one ? most : split + w.join_cost;
-    if (cost <= equal) apart = one ? most : split;
-  }
-  if (apart > 0) {
-    r.cost = 0;
-    share = apart;
-    c = 0;
-#pragma unroll
-    for (int i = 0; i < kFew; ++i) c += ((uint32_t)u[i] + share - 1) / share * share;  // whole runs
-  } else {
-    r.cost = w.tile_cost;
-    c += tiles * w.tile_cost;
-#pragma unroll
-    for (int i = 0; i < kFew; ++i) u[i] += u[i] > 0 ? w.tile_cost : 0;
-    share = max((total + all_tiles * w.tile_cost + wgs - 1) >> w.wgs_log2, (uint32_t)w.min_share);
-  }
-  const uint32_t mine = c * kv.heads, upto = scan64(mine), begin = wg * share;
-  some = begin < (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+  if (__any((long)c * kv.heads > (1 << 24))) return false;
+  const uint32_t mine = c * kv.heads, upto = scan64(mine), total = __builtin_amdgcn_readlane(upto, 63);
+  const uint32_t share = max((total + wgs - 1) >> w.wgs_log2, (uint32_t)w.min_share), begin = wg * share;
+  some = begin < total;
   if (!some) return true;
   const int s = __builtin_ctzll(__ballot(upto > begin));  // (its own units begin at or before)
   auto of = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
   const uint32_t at = begin - (of(upto) - of(mine)), in_head = of(c);
   r.share = share;
   r.begin = begin;
-  r.end = min(begin + share, (uint32_t)__builtin_amdgcn_readlane(upto, 63));
+  r.end = min(begin + share, total);
   r.seq = s;
   r.s = {of(q.row), of(q.n), of(q.first), of(q.len)};
   r.head = at / in_head;
   int rest = at - r.head * in_head, i = 0;
 #pragma unroll
   for (int k = 0; k < kFew - 1; ++k) {
-    const uint32_t uk = of(u[k]);
-    const int size = apart > 0 ? (uk + share - 1) / share * share : uk;
-    const bool past = i == k && rest >= size;
-    rest -= past ? size : 0;
+    const int uk = of(u[k]);
+    const bool past = i == k && rest >= uk;
+    rest -= past ? uk : 0;
     i += past;
   }
   r.r0 = i * TILE;
   r.off = rest;
-  if (apart > 0) r.end = begin + min((int)share, of(i == 0 ? u[0] : i == 1 ? u[1] : i == 2 ? u[2] : u[3]) - rest);
   return true;
 }
 
