@@ -256,9 +256,10 @@ __device__ __forceinline__ KeySpan tile_span(const KvSeq &s, const AttnCall &a, 
 // Partial results of tiles that were split: per workgroup, those of the tile that
 // it ends (or passes through) and of the tile that it begins.
 //   part [workgroups][2] {m[tile], l[tile], o[tile][D]}
-// The tile that a workgroup begins, where others go on with it:
-//   k_attn_split: done [workgroups] parts that are written, 0 between calls
-//   k_attn_tile: desc [workgroups] {seq, head, r0, its workgroups, or 0}
+// Of those tiles:
+//   k_attn_split: done [workgroups] parts that are written of the tile it begins, 0 between calls
+//   k_attn_tile: desc [workgroups][2], as part: {seq, head, r0, its parts 2^16 + which
+//   one this is, or 0}
 struct AttnWork {
   int4 *desc;
   int *done;
@@ -972,7 +973,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
   TileLds<FMT, D> &lds = shared.tile;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
   const int wg = (blockIdx.x & 7) << (w.wgs_log2 - 3) | blockIdx.x >> 3;
-  if (threadIdx.x == 0) w.desc[wg] = int4{0, 0, 0, 0};
+  if (threadIdx.x < 2) w.desc[2 * wg + threadIdx.x] = int4{0, 0, 0, 0};
   Run run;
   if (!find_run<kRows, 4>(kv, b, a, w, wg, shared.run, run)) return;
   KvSeq s = run.s;
@@ -1187,57 +1188,67 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
     if (whole) {
       __syncthreads();
       finish_rows<FMT, D, 4>(kv, b, a, s, Tile{seq, head, r0, nr}, bad);
-    } else if (off == 0 && threadIdx.x == 0) {
-      w.desc[wg] = int4{seq, head, r0, quotient(next - 1, run.share) - wg + 1};
+    } else if (threadIdx.x == 0) {
+      const int by = off == 0 ? wg : quotient(next - units + run.cost, run.share);  // its first group's
+      w.desc[2 * wg + (off == 0)] = int4{seq, head, r0, (quotient(next - 1, run.share) - by + 1) << 16 | (wg - by)};
     }
     if (u < run.end) next_tile<kRows>(kv, b, a, w, run, s);
   }
 }
 
-// Joins the tiles of k_attn_tile whose units several workgroups had: a share of the
-// rows of the tile that workgroup x begins.  (A kernel of its own: 128 rows of many parts
-// are much for the one workgroup that ends last.)
+// Joins the tiles of k_attn_tile whose units several workgroups had: one workgroup here for
+// each of theirs takes every (parts)th row, so all have as much to read, whatever the parts.
+// (With the rows of any tile over 8 workgroups, 16 tiles of 32 parts took 88 us, not 36;
+// with 4 or 2 times as many workgroups, 46 and 39.)
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, AttnCall a, AttnWork w) {
   __shared__ JoinLds<D, 4> lds;
   const int4 t = w.desc[blockIdx.x];
   if (t.w == 0) return;
-  const int seq = uniform(t.x), r0 = uniform(t.z);
+  const int seq = uniform(t.x), r0 = uniform(t.z), parts = uniform(t.w) >> 16, y = uniform(t.w) & 0xffff;
   const KvSeq s = kv_seq(b, seq, kv.page_log2);
   const int nr = min(kRows, s.n * a.group - r0);
-  if ((int)blockIdx.y >= nr) return;
+  if (y >= nr) return;
+  const int lead = (blockIdx.x >> 1) - y;
   join_tile<FMT, D, 4, false>(kv, b, a, s, Tile{seq, uniform(t.y), r0, nr},
-                    w.part + ((size_t)blockIdx.x * 2 + 1) * (kRows * (D + 2)), kRows, uniform(t.w), blockIdx.y,
-                    gridDim.y, lds);
+                              w.part + ((size_t)lead * 2 + 1) * (kRows * (D + 2)), kRows, parts, y, parts, lds);
 }
 
 // Workgroups of a call (a power of two, so that whole XCDs get equal shares), and
 // the workspace of their parts: of one size for every cache, so that it is
 // allocated once.
 constexpr int kAttnWgsPerCu = 2;
-// What a tile costs besides its groups (its query, its results), in groups, of each
-// kernel: without it runs of many short tiles end last.  A prompt of 4093 tokens took 418 us
-// at 0, 357 at 4, 353 at 8 and 362 at 16, a batch of 17 sequences and one chunk 93, 84, 86 and
-// 101; decode steps differ by less than 1 us up to 8.
-#ifndef NX_C0
-#define NX_C0 12
-#endif
-constexpr int kTileCost = NX_C0, kRowsCost = 6;
-#ifndef NX_MS
-#define NX_MS 8
-#endif
-#ifndef NX_MR
-#define NX_MR 10
-#endif
-#ifndef NX_JC
-#define NX_JC 16
-#endif
-#ifndef NX_JR
-#define NX_JR 4
-#endif
-constexpr int kMinShare = NX_MS, kMinRows = NX_MR, kJoinCost = NX_JC, kJoinRows = NX_JR;
-// rows of a sequence from which k_attn_tile takes it
-constexpr int kTileFrom = 64;
+// The costs are in groups of 32 tokens, and measured at 4 to 32 heads of 64 to 256:
+// what a tile costs besides its groups (its query, its results); without it runs of many
+// short tiles end last.  k_attn_split: 512 sequences' worth of long decode tiles
+//   120.1 us at 4, 118.4 at 12, 117.2 at 24; a batch of 64 sequences 226, 226 and 228.5
+// k_attn_tile: a prompt of 4093 tokens 333 us at 2, 310 at 6, 314 at 12
+constexpr int kTileCost = 12, kRowsCost = 6;
+// The fewest groups of a workgroup where a tile is split.  k_attn_split (two for each wave):
+// two sequences of 14304 tokens 25.0 us at 4, 23.7 at 8, 19.6 at 16, 22.2 at 32
+// k_attn_tile: three chunks of 37 tokens over 2592 41.5 us at 4 (and 2), 47.0 at 10, 63.6 at 20
+constexpr int kMinShare = 16, kMinRows = 4;
+// What a split tile's join costs.  k_attn_split: one sequence of 1049 tokens 11.6 us at 4, 10.0
+// at 16; 16 sequences and a chunk 70.5 us at 16, 78.0 at 48.  k_attn_tile: four chunks of 306
+// tokens 43.2 us at 0, 33.7 at 4; three of 564 tokens 37.5 us at 4, 40.4 at 16
+constexpr int kJoinCost = 16, kJoinRows = 4;
+// The kernel of a sequence.  A 16-row tile has a workgroup (or several) and a wave a group of
+// its own: least latency, but every tile reads the keys again; a 128-row tile reads them once
+// for all, at full cost whatever its rows.  So, in a step of many sequences, k_attn_tile
+// takes those beyond two 16-row tiles (F16), or three (INT8, half the bytes):
+//   rows of each, 64 sequences of 1024 tokens   24    40    56    72
+//   F16,  D 128: k_attn_split, k_attn_tile, us  47 47 66 49 84 52  -  54
+//   INT8, D 256: the same                       112 205 163 207 210 209  -  214
+constexpr int tile_from(int fmt) { return kTile * (fmt == NX_KV_INT8 ? 3 : 2); }
+// And all of a step goes to k_attn_split while its rows are a 16-row tile for each of half
+// the CUs, or for each CU where the keys are few (the page table's width bounds them): one
+// chunk over 4 heads of 128, F16,
+//   rows                        1024          2048          4096              8192
+//   tokens                    1024  16384   1024  16384   1024 4096 16384   1024 16384
+//   k_attn_split, us            14     34     14     53     14   30    90     32   181
+//   k_attn_tile, us             29     46     30     61     32   45    92     38   152
+// and 4096 rows over 65536 tokens 319 us and 307 (INT8 of 64: 309 and 231).
+constexpr double kFewScores = 4e7;  // rows times keys
 
 static int attn_wgs_log2(const nx_ctx *c) { return std::max(4, 31 - __builtin_clz(c->num_cu * kAttnWgsPerCu)); }
 static size_t part_floats(int tile, int D) { return (size_t)2 * tile * (D + 2); }
@@ -1246,12 +1257,12 @@ int attn_workspace(nx_ctx *c, void **out) {
   // (k_attn_tile runs half as many workgroups on heads of 256)
   const size_t wide = std::max(part_floats(kRows, 128), part_floats(kRows, 256) / 2);
   // (and a descriptor and a count of each)
-  const size_t bytes = wgs * (sizeof(int4) + sizeof(int) + 4 * (part_floats(kTile, 256) / 2 + wide));
+  const size_t bytes = wgs * (2 * sizeof(int4) + sizeof(int) + 4 * (part_floats(kTile, 256) / 2 + wide));
   const bool there = c->ws[WS_ATTN].cap >= bytes;
   void *p;
   NX_TRY(ws_get(c, WS_ATTN, bytes, &p));
   if (!there)  // counts begin at 0
-    NX_HIP(hipMemsetAsync(static_cast<int4 *>(p) + wgs, 0, wgs * sizeof(int), c->stream));
+    NX_HIP(hipMemsetAsync(static_cast<int4 *>(p) + 2 * wgs, 0, wgs * sizeof(int), c->stream));
   if (out) *out = p;
   return NX_OK;
 }
@@ -1266,16 +1277,19 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   // Which kernels the batch may need: only the device knows its sequences' rows.  With a row
   // or more in each, one has at most num_tokens - num_seqs + 1; a batch that leaves
   // sequences out for a long one is right on k_attn_split too, if slower.
-  const bool wide = ((long)b.num_tokens - b.num_seqs + 1) * a.group > kTileFrom;
+  const int log2 = attn_wgs_log2(c), wgs = 1 << log2, from = tile_from(kv->fmt);
+  const long rows = (long)b.num_tokens * a.heads, table = (long)b.max_pages * kv->page_tokens;
+  const long keys = a.window > 0 ? std::min(table, (long)a.window + a.sinks + b.num_tokens) : table;
+  const bool few = rows <= kTile * wgs / 4 || (rows <= kTile * wgs / 2 && (double)rows * keys <= kFewScores);
+  const bool wide = ((long)b.num_tokens - b.num_seqs + 1) * a.group > from && !few;
   const bool narrow = !wide || b.num_seqs > 1;
-  const int log2 = attn_wgs_log2(c), wgs = 1 << log2;
   int4 *desc = static_cast<int4 *>(p);
-  int *done = reinterpret_cast<int *>(desc + wgs);
+  int *done = reinterpret_cast<int *>(desc + 2 * wgs);
   float *part = reinterpret_cast<float *>(done + wgs);
   // (k_attn_split: one workgroup per CU)
-  const AttnWork w0{nullptr, done, part, log2 - 1, kMinShare, kTileCost, kJoinCost, 0, wide ? kTileFrom : INT32_MAX};
+  const AttnWork w0{nullptr, done, part, log2 - 1, kMinShare, kTileCost, kJoinCost, 0, wide ? from : INT32_MAX};
   const AttnWork w1{desc, nullptr, part + wgs / 2 * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2,
-                    kMinRows, kRowsCost, kJoinRows, narrow ? kTileFrom : 0, INT32_MAX};
+                    kMinRows, kRowsCost, kJoinRows, narrow ? from : 0, INT32_MAX};
   const int wgs1 = 1 << w1.wgs_log2;
   const KvView view = view_of(kv);
   if (wide)
@@ -1293,7 +1307,7 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   if (!wide) return NX_OK;
   return launch(c, "attn_join", [&] {
     with_kernel(kv, [&](auto fmt, auto D) {
-      go(c, k_attn_join<fmt(), D()>, dim3(wgs1, 8), dim3(256), 0, view, b, a, w1);
+      go(c, k_attn_join<fmt(), D()>, dim3(2 * wgs1), dim3(256), 0, view, b, a, w1);
     });
   });
 }

@@ -10,6 +10,8 @@ from test_gpu_kv import device_batch, ints
 
 pytestmark = pytest.mark.gpu
 FORMATS = [F16, INT8]
+# (token, head) rows of a step from which sequences of several are taken 128 rows at a time
+MANY = 4096
 
 
 @pytest.fixture(scope="module")
@@ -27,7 +29,11 @@ def filled(ctx, rng, b, fmt, G, D):
     return cache, stored(fmt, k), stored(fmt, v)
 
 
-def check(ctx, fmt, H, G, D, page, ns, lens, window=0, sinks=0, seed=0, factor=1.0):
+def check(ctx, fmt, H, G, D, page, ns, lens, window=0, sinks=0, seed=0, factor=1.0, beside=False):
+    """beside: with one sequence more, whose rows make the step one of many."""
+    if beside:
+        n = MANY // H + 1
+        ns, lens = [*ns, n], [*lens, n + 5]
     rng = np.random.default_rng([seed, D, page, len(ns), sum(lens)])
     b = Batch(rng, ns, lens, page)
     cache, k, v = filled(ctx, rng, b, fmt, G, D)
@@ -52,37 +58,41 @@ BATCHES = [
 ]
 
 
+@pytest.mark.parametrize("beside", [False, True], ids=["alone", "beside"])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("H,G,D", SHAPES)
 @pytest.mark.parametrize("ns,lens", BATCHES, ids=lambda v: "-".join(map(str, v))[:24])
-def test_parity(ctx, fmt, H, G, D, ns, lens):
+def test_parity(ctx, fmt, H, G, D, ns, lens, beside):
     print(f"attention fmt={fmt} H={H} G={G} D={D} ns={ns} lens={lens}", flush=True)
-    check(ctx, fmt, H, G, D, 64, ns, lens)
+    check(ctx, fmt, H, G, D, 64, ns, lens, beside=beside)
 
 
+@pytest.mark.parametrize("beside", [False, True], ids=["alone", "beside"])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("page", [32, 128, 1024])
-def test_pages(ctx, fmt, page):
-    check(ctx, fmt, 8, 2, 128, page, [1, 50, 2], [1500, 65, 320])
+def test_pages(ctx, fmt, page, beside):
+    check(ctx, fmt, 8, 2, 128, page, [1, 50, 2], [1500, 65, 320], beside=beside)
 
 
+@pytest.mark.parametrize("beside", [False, True], ids=["alone", "beside"])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 4), (7, 1), (32, 33), (100, 0), (128, 4), (300, 64),
                                           (4096, 4), (2 ** 31 - 1, 2 ** 31 - 1), (5, 2000)])
 @pytest.mark.parametrize("ns,lens", [([1, 1, 1], [5, 130, 1100]), ([200, 3], [900, 40]), ([65], [65])],
                          ids=["step", "chunk", "prompt"])
-def test_window(ctx, fmt, window, sinks, ns, lens):
+def test_window(ctx, fmt, window, sinks, ns, lens, beside):
     print(f"window fmt={fmt} window={window} sinks={sinks} ns={ns} lens={lens}", flush=True)
-    check(ctx, fmt, 8, 2, 64, 32, ns, lens, window, sinks)
+    check(ctx, fmt, 8, 2, 64, 32, ns, lens, window, sinks, beside=beside)
 
 
+@pytest.mark.parametrize("beside", [False, True], ids=["alone", "beside"])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("H,G,D", [(32, 8, 128), (8, 1, 64), (6, 6, 96), (4, 2, 256)])
-def test_chunks(ctx, fmt, H, G, D):
+def test_chunks(ctx, fmt, H, G, D, beside):
     """Chunks of several hundred tokens, behind a context and from the first token on."""
     print(f"chunk fmt={fmt} H={H} G={G} D={D}", flush=True)
-    check(ctx, fmt, H, G, D, 64, [517, 1, 130], [1203, 700, 130])
-    check(ctx, fmt, H, G, D, 32, [300], [2500], window=257, sinks=5)
+    check(ctx, fmt, H, G, D, 64, [517, 1, 130], [1203, 700, 130], beside=beside)
+    check(ctx, fmt, H, G, D, 32, [300], [2500], window=257, sinks=5, beside=beside)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -93,30 +103,32 @@ def test_long_context(ctx, fmt):
     check(ctx, fmt, 4, 2, 128, 128, [1], [20000], window=5000, sinks=70)
 
 
+@pytest.mark.parametrize("beside", [False, True], ids=["alone", "beside"])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("factor", [1e-30, 30.0, 1e-5])
-def test_score_ranges(ctx, fmt, factor):
+def test_score_ranges(ctx, fmt, factor, beside):
     """Scores of all but nothing, and a softmax that one token takes."""
-    check(ctx, fmt, 8, 2, 128, 64, [1, 40], [500, 300], factor=factor)
+    check(ctx, fmt, 8, 2, 128, 64, [1, 40], [500, 300], factor=factor, beside=beside)
 
 
 def test_value_scales_of_all_sizes(ctx):
     """INT8: neighbouring tokens' scales many powers of two apart."""
     rng = np.random.default_rng(3)
-    for n, length in ((1, 700), (150, 300)):
+    for n, length, H in ((1, 700, 4), (150, 300, 4), (150, 300, 28)):
         b = Batch(rng, [n], [length], 32)
         k, v = random_kv(rng, length, 2, 128)
         v *= (10.0 ** rng.integers(-20, 5, (length, 2, 1))).astype(np.float32)
         k *= (10.0 ** rng.integers(-3, 1, (length, 2, 1))).astype(np.float32)
         cache = nx.KvCache(ctx, INT8, b.num_pages, 32, 2, 128)
         cache.write(b.whole(), b.kv_len, b.pages, k, v)
-        q = rng.standard_normal((n, 4, 128)).astype(np.float32)
-        ref, bound = attention(b, stored(INT8, k), stored(INT8, v), q, 4, np.float32(128 ** -0.5))
-        assert_close(cache.attention(*b.args(), q, 4), ref, bound)
+        q = rng.standard_normal((n, H, 128)).astype(np.float32)
+        ref, bound = attention(b, stored(INT8, k), stored(INT8, v), q, H, np.float32(128 ** -0.5))
+        assert_close(cache.attention(*b.args(), q, H), ref, bound)
         cache.close()
 
 
-def test_zeros(ctx):
+@pytest.mark.parametrize("H", [4, 204])
+def test_zeros(ctx, H):
     """Zero queries average, zero keys and values give what the formula gives."""
     rng = np.random.default_rng(4)
     for fmt in FORMATS:
@@ -126,25 +138,26 @@ def test_zeros(ctx):
         v[10:40] = 0
         cache = nx.KvCache(ctx, fmt, b.num_pages, 32, 2, 64)
         cache.write(b.whole(), b.kv_len, b.pages, k, v)
-        q = rng.standard_normal((21, 4, 64)).astype(np.float32)
+        q = rng.standard_normal((21, H, 64)).astype(np.float32)
         q[0] = 0
         q[5] = -0.0
-        ref, bound = attention(b, stored(fmt, k), stored(fmt, v), q, 4, np.float32(0.125))
-        assert_close(cache.attention(*b.args(), q, 4), ref, bound)
+        ref, bound = attention(b, stored(fmt, k), stored(fmt, v), q, H, np.float32(0.125))
+        assert_close(cache.attention(*b.args(), q, H), ref, bound)
         cache.close()
 
 
+@pytest.mark.parametrize("H", [4, 80])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("n", [1, 60])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
-def test_non_finite_where_no_row_looks(ctx, fmt, n, bad):
+def test_non_finite_where_no_row_looks(ctx, fmt, n, bad, H):
     """Keys and values between the first tokens and the windows, and behind the
     last token of a sequence, change nothing."""
     rng = np.random.default_rng(11)
     G, D, page, length = 2, 128, 64, 400
     b = Batch(rng, [n], [length], page, max_pages=8)
     k, v = random_kv(rng, length, G, D)
-    q = rng.standard_normal((n, 4, D)).astype(np.float32)
+    q = rng.standard_normal((n, H, D)).astype(np.float32)
     window, sinks = 50, 3
     for where in ("between", "behind"):
         cache = nx.KvCache(ctx, fmt, b.num_pages, page, G, D)
@@ -157,14 +170,15 @@ def test_non_finite_where_no_row_looks(ctx, fmt, n, bad):
             old = 448 - length
             cache.write([0, old], [448], b.pages, np.full((old, G, D), bad), np.full((old, G, D), bad))
             cache.write(b.whole(), b.kv_len, b.pages, k, v)
-        ref, bound = attention(b, stored(fmt, k), stored(fmt, v), q, 4, np.float32(D ** -0.5), window, sinks)
-        assert_close(cache.attention(*b.args(), q, 4, window=window, sinks=sinks), ref, bound)
+        ref, bound = attention(b, stored(fmt, k), stored(fmt, v), q, H, np.float32(D ** -0.5), window, sinks)
+        assert_close(cache.attention(*b.args(), q, H, window=window, sinks=sinks), ref, bound)
         cache.close()
 
 
+@pytest.mark.parametrize("H", [4, 60])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
-def test_non_finite_future(ctx, fmt, bad):
+def test_non_finite_future(ctx, fmt, bad, H):
     """A chunk's later tokens hold infinities or NaNs: earlier rows are what they
     are without them, rows that see them what the formula gives."""
     rng = np.random.default_rng(12)
@@ -175,9 +189,9 @@ def test_non_finite_future(ctx, fmt, bad):
     v[185, 1, 9] = bad
     cache = nx.KvCache(ctx, fmt, b.num_pages, 32, G, D)
     cache.write(b.whole(), b.kv_len, b.pages, k, v)
-    q = rng.standard_normal((n, 4, D)).astype(np.float32)
-    got = cache.attention(*b.args(), q, 4)
-    ref, bound = attention(b, stored(fmt, k), stored(fmt, v), q, 4, np.float32(0.125))
+    q = rng.standard_normal((n, H, D)).astype(np.float32)
+    got = cache.attention(*b.args(), q, H)
+    ref, bound = attention(b, stored(fmt, k), stored(fmt, v), q, H, np.float32(0.125))
     fine = np.isfinite(ref)
     assert np.array_equal(np.isnan(got), np.isnan(ref))
     assert np.array_equal(got[~fine & ~np.isnan(ref)], ref[~fine & ~np.isnan(ref)])
@@ -186,30 +200,32 @@ def test_non_finite_future(ctx, fmt, bad):
     cache.close()
 
 
+@pytest.mark.parametrize("H", [8, 104])
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_non_finite_query(ctx, fmt):
+def test_non_finite_query(ctx, fmt, H):
     """A NaN or infinite query spoils its own head's row and no other."""
     rng = np.random.default_rng(13)
     for n, length in ((1, 100), (40, 140)):
         b = Batch(rng, [n], [length], 32)
         cache, k, v = filled(ctx, rng, b, fmt, 2, 64)
-        q = rng.standard_normal((n, 8, 64)).astype(np.float32)
-        clean = cache.attention(*b.args(), q, 8)
+        q = rng.standard_normal((n, H, 64)).astype(np.float32)
+        clean = cache.attention(*b.args(), q, H)
         q[n - 1, 3, 7] = np.nan
         q[0, 6, 0] = np.inf
-        got = cache.attention(*b.args(), q, 8)
-        spoiled = np.zeros((n, 8), bool)
+        got = cache.attention(*b.args(), q, H)
+        spoiled = np.zeros((n, H), bool)
         spoiled[n - 1, 3] = spoiled[0, 6] = True
         assert np.all(np.isnan(got[spoiled]))
         assert_same_bits(got[~spoiled], clean[~spoiled])
         cache.close()
 
 
+@pytest.mark.parametrize("H", [4, 46])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("shift,extra", [(0, 0), (0, 16), (1, 3)])
-def test_strided_and_unaligned_rows(ctx, fmt, shift, extra):
+def test_strided_and_unaligned_rows(ctx, fmt, shift, extra, H):
     rng = np.random.default_rng(14)
-    H, G, D = 4, 2, 128
+    G, D = 2, 128
     for ns in ([1, 1], [3, 90]):
         b = Batch(rng, ns, [77, 210], 64, first_row=1, padding=2)
         cache, k, v = filled(ctx, rng, b, fmt, G, D)
@@ -231,11 +247,12 @@ def test_strided_and_unaligned_rows(ctx, fmt, shift, extra):
         cache.close()
 
 
+@pytest.mark.parametrize("H", [4, 28])
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_rows_that_see_nothing(ctx, fmt):
+def test_rows_that_see_nothing(ctx, fmt, H):
     """Device batches whose lengths and tables leave rows without a token give zeros."""
     rng = np.random.default_rng(15)
-    H, G, D, page = 4, 2, 64, 32
+    G, D, page = 2, 64, 32
     for n in (2, 50):
         b = Batch(rng, [n, n, n], [n + 40, n + 40, n + 40], page, max_pages=3)
         cache, k, v = filled(ctx, rng, b, fmt, G, D)
@@ -259,11 +276,12 @@ def test_rows_that_see_nothing(ctx, fmt):
         cache.close()
 
 
+@pytest.mark.parametrize("H", [4, 138])
 @pytest.mark.parametrize("window", [1, 9, 2 ** 31 - 1])
-def test_rows_before_the_first_token_in_a_window(ctx, window):
+def test_rows_before_the_first_token_in_a_window(ctx, window, H):
     """A tile whose first rows are before the first token: the others' windows count."""
     rng = np.random.default_rng(20)
-    H, G, D, n, length = 4, 2, 64, 30, 12
+    G, D, n, length = 2, 64, 30, 12
     b = Batch(rng, [n], [n], 32)
     cache, k, v = filled(ctx, rng, b, F16, G, D)
     b.kv_len[0] = length  # rows 0 .. 17 are tokens -18 .. -1
@@ -280,11 +298,12 @@ def test_rows_before_the_first_token_in_a_window(ctx, window):
     cache.close()
 
 
+@pytest.mark.parametrize("H", [4, 70])
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_missing_page_in_the_middle(ctx, fmt):
+def test_missing_page_in_the_middle(ctx, fmt, H):
     """Tokens on a page that the cache does not have are not attended to."""
     rng = np.random.default_rng(16)
-    H, G, D = 4, 2, 64
+    G, D = 2, 64
     for n in (1, 60):
         b = Batch(rng, [n], [200], 32)
         cache, k, v = filled(ctx, rng, b, fmt, G, D)
@@ -327,14 +346,14 @@ def test_offsets_past_32_bits(ctx, fmt):
     pages = (1 << 32) // (page * G * D) + 3
     rng = np.random.default_rng(18)
     cache = nx.KvCache(ctx, fmt, pages, page, G, D)
-    for n in (1, 40):
+    for n, H in ((1, G), (40, G), (40, 7 * G)):
         b = Batch(rng, [n], [1100], page)
         b.pages = np.array([[pages - 1, pages - 2]], np.int32)
         k, v = random_kv(rng, 1100, G, D)
         cache.write(b.whole(), b.kv_len, b.pages, k, v)
-        q = rng.standard_normal((n, G, D)).astype(np.float32)
-        ref, bound = attention(b, stored(fmt, k), stored(fmt, v), q, G, np.float32(0.0625))
-        assert_close(cache.attention(*b.args(), q, G), ref, bound)
+        q = rng.standard_normal((n, H, D)).astype(np.float32)
+        ref, bound = attention(b, stored(fmt, k), stored(fmt, v), q, H, np.float32(0.0625))
+        assert_close(cache.attention(*b.args(), q, H), ref, bound)
     cache.close()
 
 

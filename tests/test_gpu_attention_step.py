@@ -174,14 +174,15 @@ class Step:
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("ns", [[1, 1, 1], [40, 1, 3]], ids=["decode", "mixed"])
-def test_captured_step_follows_the_lengths(fmt, ns):
+@pytest.mark.parametrize("ns,heads", [([1, 1, 1], 8), ([40, 1, 3], 8), ([150, 1, 3], 32)],
+                         ids=["decode", "mixed", "chunk"])
+def test_captured_step_follows_the_lengths(fmt, ns, heads):
     """A graph of a write and its attention, replayed while the sequences grow, with
     other work of the context (that enlarges its workspace) in between: every replay
     equals the eager calls bit for bit."""
     hip = Hip()
     rng = np.random.default_rng(31)
-    heads, G, D, page = 8, 2, 128, 32
+    G, D, page = 2, 128, 32
     with nx.Context(0) as ctx:
         stream = hip.stream()
         ctx.set_stream(stream.value)
@@ -229,7 +230,7 @@ def test_two_graphs_of_a_context_in_turn(ctx):
     stream = C.c_void_p()
     nx.check(nx.lib().nx_ctx_get_stream(ctx.h, C.byref(stream)))
     cases = []
-    for ns, lens in (([1, 1], [3000, 40]), ([1], [5000]), ([90], [400])):
+    for ns, lens in (([1, 1], [3000, 40]), ([1], [5000]), ([90], [400]), ([700, 1, 400], [900, 5000, 400])):
         b = Batch(rng, ns, lens, 64)
         cache, k, v = filled(ctx, rng, b, F16, G, D)
         s = Step(b, heads, G, D)
@@ -281,8 +282,9 @@ def test_contexts_on_streams_of_their_own():
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("ns,lens", [([1], [9000]), ([1] * 20, [700 + 37 * i for i in range(20)]),
-                                     ([200], [5000]), ([3, 80, 1], [2000, 300, 4000])],
-                         ids=["long", "batch", "chunk", "mixed"])
+                                     ([200], [5000]), ([3, 80, 1], [2000, 300, 4000]),
+                                     ([300], [5000]), ([3, 280, 1], [2000, 300, 4000])],
+                         ids=["long", "batch", "chunk", "mixed", "chunk-of-many", "mixed-of-many"])
 def test_many_runs_agree(ctx, fmt, ns, lens):
     """Split tiles are joined in the order of their parts, whoever ends last: 200
     calls in a row give the same bits."""
@@ -310,7 +312,7 @@ def test_many_runs_agree(ctx, fmt, ns, lens):
     cache.close()
 
 
-@pytest.mark.parametrize("long", [1, 150])
+@pytest.mark.parametrize("long", [1, 150, 1000])
 def test_very_many_sequences(ctx, long):
     """Several rounds of a workgroup's threads of sequences, a long one among them,
     in both kernels."""
@@ -335,7 +337,7 @@ def test_profile_and_lifetimes():
     b = Batch(rng, [1, 100], [50, 100], 32)
     cache, _, _ = filled(ctx, rng, b, F16, 1, 64)
     ctx.profile(True)
-    cache.attention(*b.args(), np.zeros((101, 64), np.float32), 1)
+    cache.attention(*b.args(), np.zeros((101, 41 * 64), np.float32), 41)
     names = ctx.profile_stats()
     assert {"attn_split", "attn_tile", "attn_join"} <= set(names)
     assert all(n == 1 and ms > 0 for n, ms in names.values())
