@@ -1218,27 +1218,32 @@ __global__ __launch_bounds__(256) void k_attn_join(KvView kv, nx_kv_batch b, Att
 // the workspace of their parts: of one size for every cache, so that it is
 // allocated once.
 constexpr int kAttnWgsPerCu = 2;
-// The costs are in groups of 32 tokens, and measured at 4 to 32 heads of 64 to 256:
-// what a tile costs besides its groups (its query, its results); without it runs of many
-// short tiles end last.  k_attn_split: 512 sequences' worth of long decode tiles
-//   120.1 us at 4, 118.4 at 12, 117.2 at 24; a batch of 64 sequences 226, 226 and 228.5
-// k_attn_tile: a prompt of 4093 tokens 333 us at 2, 310 at 6, 314 at 12
+// What a tile costs besides its groups (its query, its results), in groups; without it runs
+// of many short tiles end last.
+//   k_attn_split: three sequences of up to 131071 tokens (INT8) 120.1 us at 4, 118.4 at 12,
+//   117.2 at 24; 61 of up to 8191 (F16) 226 at 4 and 12, 228.5 at 24
+//   k_attn_tile: a prompt of 4093 tokens 333 us at 2, 310 at 6, 314 at 12
 constexpr int kTileCost = 12, kRowsCost = 6;
-// The fewest groups of a workgroup where a tile is split.  k_attn_split (two for each wave):
-// two sequences of 14304 tokens 25.0 us at 4, 23.7 at 8, 19.6 at 16, 22.2 at 32
-// k_attn_tile: three chunks of 37 tokens over 2592 41.5 us at 4 (and 2), 47.0 at 10, 63.6 at 20
+// The fewest groups of a workgroup where a tile is split.
+//   k_attn_split (two for each wave): two sequences of up to 14304 tokens 25.0 us at 4, 23.7 at
+//   8, 19.6 at 16, 22.2 at 32
+//   k_attn_tile: three chunks of 37 tokens, 32 heads over 4 of 128, at up to 2592 tokens 41.5 us
+//   at 2 and 4, 47.0 at 10, 63.6 at 20
 constexpr int kMinShare = 16, kMinRows = 4;
-// What a split tile's join costs.  k_attn_split: one sequence of 1049 tokens 11.6 us at 4, 10.0
-// at 16; 16 sequences and a chunk 70.5 us at 16, 78.0 at 48.  k_attn_tile: four chunks of 306
-// tokens 43.2 us at 0, 33.7 at 4; three of 564 tokens 37.5 us at 4, 40.4 at 16
-constexpr int kJoinCost = 16, kJoinRows = 4;
+// What the join of a split tile costs, in groups: a tile that ends no later is taken whole.
+//   k_attn_split: one token after 516 11.6 us at 4, 10.0 at 16; 16 tokens and a chunk of 257
+//   70.5 us at 16, 78.0 at 48
+//   k_attn_tile: 709 tokens through a window of 13, 8 heads of 256, 49.1 us at 0, 38.7 at 8;
+//   four prompts of 306 tokens 36.6 at 0, 33.3 at 8; three of 564 35.1 at 8, 40.4 at 16
+constexpr int kJoinCost = 16, kJoinRows = 8;
 // The kernel of a sequence.  A 16-row tile has a workgroup (or several) and a wave a group of
 // its own: least latency, but every tile reads the keys again; a 128-row tile reads them once
 // for all, at full cost whatever its rows.  So, in a step of many sequences, k_attn_tile
-// takes those beyond two 16-row tiles (F16), or three (INT8, half the bytes):
-//   rows of each, 64 sequences of 1024 tokens   24    40    56    72
-//   F16,  D 128: k_attn_split, k_attn_tile, us  47 47 66 49 84 52  -  54
-//   INT8, D 256: the same                       112 205 163 207 210 209  -  214
+// takes those beyond two 16-row tiles (F16), or three (INT8, half the bytes); us for 64
+// sequences of 1024 tokens, by k_attn_split and k_attn_tile:
+//   rows of each                    24          40          56
+//   F16,  8 heads over 1 of 128   47  47      66  49      84  52
+//   INT8, 2 heads over 1 of 256  112 205     163 207     212 210
 constexpr int tile_from(int fmt) { return kTile * (fmt == NX_KV_INT8 ? 3 : 2); }
 // And all of a step goes to k_attn_split while its rows are a 16-row tile for each of half
 // the CUs, or for each CU where the keys are few (the page table's width bounds them): one
