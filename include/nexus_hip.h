@@ -44,6 +44,14 @@
  *   nx_experts_load_gguf
  *       the tensor loop of InferenceEngine::new (src/engine/mod.rs:600-650)
  *       for a block's expert tensors, without the f32 step or the 10M cap
+ *   nx_kv_create / nx_kv_write / nx_kv_read
+ *       KvCache::add and the views of its rows that a layer attends to
+ *                                            src/engine/mod.rs:410-426
+ *       for the sequences of a step, on pages, in f16 or int8
+ *   nx_attention / nx_attention_dev
+ *       InferenceEngine::attention_decode    src/engine/mod.rs:452-500
+ *       kernel::grouped_query_attention      src/kernel/mod.rs:40-99
+ *       causal, for any new tokens of each sequence; with a window, too
  *   nx_device_count / nx_ctx_* / nx_sync / nx_mem_info
  *       Backend::{is_available, memory_info, synchronize}
  *                                            src/backend/mod.rs:74-96
@@ -315,7 +323,8 @@ int nx_kv_read_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float
  * overlap q.  f32 in and out: scores, softmax and sums are held in f32, and the f32 factors of the
  * f16 matrix products are split into two halves (relative error about 1e-6
  * against the same cache in 64 bits).  A row's last bits depend on the batch
- * that it is in (the order of the sums does), not on the run.
+ * that it is in, the width of its table among it (the order of the sums does), not on the
+ * run.
  * attention_decode (src/engine/mod.rs:452-500) and
  * kernel::grouped_query_attention (src/kernel/mod.rs:40-99) for a batch.
  * The workspace (some 80 MB) is the context's, allocated with the first cache or

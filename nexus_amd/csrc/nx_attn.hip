@@ -5,7 +5,13 @@
 //
 // over the tokens j that token i sees, in one pass over the cache: m_i is the
 // running maximum, and the sums taken so far are scaled by exp(m_old - m_new)
-// when it grows.
+// when it grows.  Scores, weights, maxima and sums are f32.
+//
+// Three kernels.  k_attn_split reads the keys for 16 rows at a time and splits them over
+// waves and workgroups: steps of few rows, bound by memory or, short ones, by latency.
+// k_attn_tile reads them for 128 rows at a time: prompts, bound by the matrix cores and
+// what feeds them.  k_attn_join puts the second one's split tiles together.  Which
+// sequences go where: tile_from and kFewScores below.
 #include <hip/hip_runtime.h>
 
 #include "nx_kv_dev.hpp"
@@ -37,7 +43,9 @@ __device__ __forceinline__ bool sees(const AttnCall &a, int p, int j) {
 }
 
 // One row by the formula alone, in f32: a wave, each lane a key's whole score,
-// then each lane some elements of the sum over the keys.
+// then each lane some elements of the sum over the keys.  For rows whose result on the
+// matrix cores is not finite or sums to nothing: infinities and NaNs in the row's own keys,
+// values or query, 0 times a masked one, or no token to see.  (Rare, and not made fast.)
 template <int FMT, int D>
 __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                          const KvSeq &s, int seq, int head, int p, const float *q,
@@ -114,8 +122,10 @@ __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b,
 // Rows of up to kTile (token, head) pairs that share a key/value head are one tile
 // of the matrix cores; a unit of work is one tile against one group of 32 tokens.
 // All units of the batch, in order of (sequence, head, tile, group), are dealt out
-// in equal runs, one per workgroup, so a ragged batch loads every CU alike. A tile
-// whose units end up in several workgroups is joined by k_attn_join.
+// in equal runs, one per workgroup, so a ragged batch loads every CU alike (or, in
+// short steps, tile by tile: find_run_wave).  The waves of a workgroup take groups in
+// turn and join in LDS; a tile that several workgroups have is joined by the last of them
+// to end, in the order of its parts, so the result does not depend on who that is.
 //
 // Transposed products: S^T = K Q^T puts a query in each lane column, the scores of
 // tokens 8 g .. 8 g + 7 in lane group g (kv_row), which is the operand layout of
@@ -123,6 +133,16 @@ __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b,
 // are f32 split into two f16 halves (hi + lo: 22 bits), K and V enter as they are
 // stored; int8 codes as exact f16 values, with the key's scale on the score and the
 // value's on the weight.
+//
+// One token of one sequence uses a part of a matrix instruction, and still the loads are what
+// it waits for: each lane's 16-byte loads of a group's keys are its operands as they lie in
+// the cache, the next group's are on their way while one is worked on, its page number a
+// group before that.  32 heads over 8 of 128: 61 sequences of up to 8191 tokens (F16, 1.29
+// GB) 224-226 us, 5.7 TB/s; three of up to 131071 (INT8, 623 MB) 118, 5.3 TB/s; a large
+// read reaches 6.5.  Eight waves, two on a SIMD, not four: 226 us against 233, and 29
+// sequences through a window of 1024 tokens 18 against 22.  One token after 516: 10.0 us, of
+// which an empty launch is 4.4 and the rest the round trips of the tables, a page number,
+// the keys, the parts and their count.
 constexpr float kLog2e = 1.4426950408889634f;
 // The largest weight of a row (p, or p times the value's scale) is 2^8 or more when the
 // reference m is set; m is set anew, and the sums scaled, when one passes 2^15.  So
@@ -934,6 +954,16 @@ __global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn
 // tokens 16 s + 8 h .. + 7 of its query, the operand of value chunk 2 s + h.  The
 // next group is on its way to registers while one is worked on and one lies in LDS;
 // int8 codes become f16 on their way to LDS, once for the four waves.
+//
+// Each product is two matrix instructions (q's and p's halves; one alone would leave 11 bits
+// of them).  Bound by the wave's own alternation: its scores, then maximum, exponentials and
+// halves (F16 134, INT8 220 vector instructions for 32 matrix ones of a group), then its
+// values; the CU's other workgroup fills the gaps, and the matrix cores are busy 43% of the
+// time at about 2 GHz.  32 heads over 8 of 128, F16: a prompt of 4093 tokens 300-310 us, 440-457
+// TFLOP/s with the halves counted once; 2039 tokens through a window of 4096 274 us, 500.
+// INT8, 32 heads over 4, two chunks of 509 tokens at up to 16127: 460-470 us, 455-465.  Scores
+// of the next group ahead of this one's weights, with q's lower halves in LDS to make room:
+// 346 us for the prompt, against 314.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // the other half of the wave's value
@@ -1198,6 +1228,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
 
 // Joins the tiles of k_attn_tile whose units several workgroups had: one workgroup here for
 // each of theirs takes every (parts)th row, so all have as much to read, whatever the parts.
+// Bound by the round trips of its few loads: 5 us for 2039 tokens through a window, 17-18 us
+// for a prompt of 4093 (512 tiles of two parts).  Four rows of a thread at once changed nothing.
 // (With the rows of any tile over 8 workgroups, 16 tiles of 32 parts took 88 us, not 36;
 // with 4 or 2 times as many workgroups, 46 and 39.)
 template <int FMT, int D>
