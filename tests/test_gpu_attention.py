@@ -111,6 +111,21 @@ def test_score_ranges(ctx, fmt, factor, beside):
     check(ctx, fmt, 8, 2, 128, 64, [1, 40], [500, 300], factor=factor, beside=beside)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("H", [8, 104])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 4.0])
+def test_scales_of_the_scores(ctx, fmt, H, scale):
+    """No scale (all tokens alike), a negative one, and the extremes of a softmax."""
+    rng = np.random.default_rng(22)
+    b = Batch(rng, [1, 40], [70, 300], 32)
+    cache, k, v = filled(ctx, rng, b, fmt, 2, 64)
+    q = rng.standard_normal((b.rows, H, 64)).astype(np.float32)
+    ref, bound = attention(b, k, v, q, H, np.float32(scale))
+    # q k: a standard deviation of sqrt(61 + 3 * 9) = 9.4, up to some four of them
+    assert_close(cache.attention(*b.args(), q, H, scale=scale), ref, bound, scores=40 * abs(scale))
+    cache.close()
+
+
 def test_value_scales_of_all_sizes(ctx):
     """INT8: neighbouring tokens' scales many powers of two apart."""
     rng = np.random.default_rng(3)
