@@ -287,7 +287,21 @@ struct AttnWork {
   int wgs_log2, min_share;
   int tile_cost, join_cost;   // what a tile, and one in parts, takes besides its groups, in units
   int rows_above, rows_upto;  // the kernel's sequences: those of so many rows
+  long few;                   // or, above 0: all are k_attn_split's for up to so many scores
 };
+
+// whether the step has w.few scores or fewer (up to 64 sequences; in integers, so that
+// both kernels find the same)
+__device__ __forceinline__ bool few_scores(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
+                                           const AttnWork &w) {
+  const int lane = threadIdx.x & 63;
+  const KvSeq q = lane < b.num_seqs ? kv_seq(b, lane, kv.page_log2) : KvSeq{0, 0, 0, 0};
+  const long keys = a.window > 0 ? min((long)q.len, (long)a.window + a.sinks + q.n) : q.len;
+  long scores = keys * q.n * a.heads;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) scores += __shfl_xor(scores, x, 64);
+  return uniform(scores) <= w.few;
+}
 
 // Units of a tile: its cost, then one per group (at least one, so that rows which
 // see nothing are written).
@@ -707,6 +721,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   // neighbouring runs on one XCD: tiles of one head share its keys in that L2
   const int wg = (blockIdx.x & 7) << (w.wgs_log2 - 3) | blockIdx.x >> 3;
+  if (w.few > 0 && few_scores(kv, b, a, w)) w.rows_upto = INT32_MAX;
   Run run;
   if (!find_run<kTile, NW>(kv, b, a, w, wg, shared.run, run)) return;
   __syncthreads();  // shared is free for the rows
@@ -1004,6 +1019,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
   const int wg = (blockIdx.x & 7) << (w.wgs_log2 - 3) | blockIdx.x >> 3;
   if (threadIdx.x < 2) w.desc[2 * wg + threadIdx.x] = int4{0, 0, 0, 0};
+  if (w.few > 0 && few_scores(kv, b, a, w)) return;
   Run run;
   if (!find_run<kRows, 4>(kv, b, a, w, wg, shared.run, run)) return;
   KvSeq s = run.s;
@@ -1277,15 +1293,20 @@ constexpr int kJoinCost = 16, kJoinRows = 8;
 //   F16,  8 heads over 1 of 128   47  47      66  49      84  52
 //   INT8, 2 heads over 1 of 256  112 205     163 207     212 210
 constexpr int tile_from(int fmt) { return kTile * (fmt == NX_KV_INT8 ? 3 : 2); }
-// And all of a step goes to k_attn_split while its rows are a 16-row tile for each of half
-// the CUs, or for each CU where the keys are few (the page table's width bounds them): one
-// chunk over 4 heads of 128, F16,
+// And all of a step goes to k_attn_split while it has a 16-row tile or less for each CU, and
+// few scores: us for one chunk over 4 heads of 128,
 //   rows                        1024          2048          4096              8192
 //   tokens                    1024  16384   1024  16384   1024 4096 16384   1024 16384
-//   k_attn_split, us            14     34     14     53     14   30    90     32   181
-//   k_attn_tile, us             29     46     30     61     32   45    92     38   152
-// and 4096 rows over 65536 tokens 319 us and 307 (INT8 of 64: 309 and 231).
-constexpr double kFewScores = 4e7;  // rows times keys
+//   F16,  k_attn_split          14     34     14     50     14   30    90     32   181
+//         k_attn_tile           29     47     30     62     32   45    92     38   152
+//   rows                        1024             2048             4096
+//   tokens                    65536 131072     65536 131072     65536
+//   INT8, k_attn_split          126    236       235    458       458
+//         k_attn_tile            94    160       159    293       292
+// Where the page table's width does not bound the scores so, both kernels are launched and
+// sum up the lengths (1024 rows over 1024 tokens 19 us, not 14; 4096 18, not 32), but for the
+// rows of an eighth of the CUs: 512 over 65536 tokens F16 62 and 126, INT8 73 and 128.
+constexpr long kFewScores = 40'000'000;  // rows times keys
 
 static int attn_wgs_log2(const nx_ctx *c) { return std::max(4, 31 - __builtin_clz(c->num_cu * kAttnWgsPerCu)); }
 static size_t part_floats(int tile, int D) { return (size_t)2 * tile * (D + 2); }
@@ -1317,16 +1338,18 @@ static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnC
   const int log2 = attn_wgs_log2(c), wgs = 1 << log2, from = tile_from(kv->fmt);
   const long rows = (long)b.num_tokens * a.heads, table = (long)b.max_pages * kv->page_tokens;
   const long keys = a.window > 0 ? std::min(table, (long)a.window + a.sinks + b.num_tokens) : table;
-  const bool few = rows <= kTile * wgs / 4 || (rows <= kTile * wgs / 2 && (double)rows * keys <= kFewScores);
+  const bool one_each = rows <= kTile * wgs / 2, few = one_each && (rows * keys <= kFewScores || rows <= kTile * wgs / 16);
   const bool wide = ((long)b.num_tokens - b.num_seqs + 1) * a.group > from && !few;
-  const bool narrow = !wide || b.num_seqs > 1;
+  const bool ask = wide && one_each && b.num_seqs <= 64;
+  const bool narrow = !wide || ask || b.num_seqs > 1;
   int4 *desc = static_cast<int4 *>(p);
   int *done = reinterpret_cast<int *>(desc + 2 * wgs);
   float *part = reinterpret_cast<float *>(done + wgs);
   // (k_attn_split: one workgroup per CU)
-  const AttnWork w0{nullptr, done, part, log2 - 1, kMinShare, kTileCost, kJoinCost, 0, wide ? from : INT32_MAX};
+  const AttnWork w0{nullptr, done, part, log2 - 1, kMinShare, kTileCost, kJoinCost, 0, wide ? from : INT32_MAX,
+                    ask ? kFewScores : 0};
   const AttnWork w1{desc, nullptr, part + wgs / 2 * part_floats(kTile, 256), kv->D == 256 ? log2 - 1 : log2,
-                    kMinRows, kRowsCost, kJoinRows, narrow ? from : 0, INT32_MAX};
+                    kMinRows, kRowsCost, kJoinRows, narrow ? from : 0, INT32_MAX, w0.few};
   const int wgs1 = 1 << w1.wgs_log2;
   const KvView view = view_of(kv);
   if (wide)

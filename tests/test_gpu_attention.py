@@ -96,6 +96,25 @@ def test_chunks(ctx, fmt, H, G, D, beside):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+def test_wide_tables(ctx, fmt, window, sinks):
+    """Tables far wider than the sequences: only the lengths say how much there is to do."""
+    rng = np.random.default_rng(23)
+    H, G, D, page = 16, 2, 64, 32
+    for ns, lens in (([200], [900]), ([90, 1, 40], [700, 50, 40]), ([120], [21000])):
+        b = Batch(rng, ns, lens, page)
+        cache, k, v = filled(ctx, rng, b, fmt, G, D)
+        q = rng.standard_normal((b.rows, H, D)).astype(np.float32)
+        got = cache.attention(*b.args(), q, H, window=window, sinks=sinks)
+        ref, bound = attention(b, k, v, q, H, np.float32(D ** -0.5), window, sinks)
+        assert_close(got, ref, bound)
+        pages = np.full((len(ns), 8000), -1, np.int32)
+        pages[:, :b.max_pages] = b.pages
+        assert_same_bits(cache.attention(b.row_start, b.kv_len, pages, q, H, window=window, sinks=sinks), got)
+        cache.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_long_context(ctx, fmt):
     """Few rows and many tokens: the axis that is split and joined."""
     check(ctx, fmt, 8, 1, 64, 256, [1], [40013])
