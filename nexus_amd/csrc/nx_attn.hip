@@ -1290,8 +1290,8 @@ constexpr int kJoinCost = 16, kJoinRows = 8;
 // takes those beyond two 16-row tiles (F16), or three (INT8, half the bytes); us for 64
 // sequences of 1024 tokens, by k_attn_split and k_attn_tile:
 //   rows of each                    24          40          56
-//   F16,  8 heads over 1 of 128   47  47      66  49      84  52
-//   INT8, 2 heads over 1 of 256  112 205     163 207     212 210
+//   F16,  32 heads over 4 of 128  47  47      66  49      84  52
+//   INT8, 16 heads over 8 of 256 112 205     163 207     212 210
 constexpr int tile_from(int fmt) { return kTile * (fmt == NX_KV_INT8 ? 3 : 2); }
 // And all of a step goes to k_attn_split while it has a 16-row tile or less for each CU, and
 // few scores: us for one chunk over 4 heads of 128,
@@ -1305,7 +1305,8 @@ constexpr int tile_from(int fmt) { return kTile * (fmt == NX_KV_INT8 ? 3 : 2); }
 //         k_attn_tile            94    160       159    293       292
 // Where the page table's width does not bound the scores so, both kernels are launched and
 // sum up the lengths (1024 rows over 1024 tokens 19 us, not 14; 4096 18, not 32), but for the
-// rows of an eighth of the CUs: 512 over 65536 tokens F16 62 and 126, INT8 73 and 128.
+// rows of an eighth of the CUs: 512 over 1024, 16384, 65536 and 131072 tokens take k_attn_split
+// 14, 25, 60 and 113 us (INT8 16, 29, 75, 132) and k_attn_tile 25, 37, 64 and 100 (26, 39, 65, 99).
 constexpr long kFewScores = 40'000'000;  // rows times keys
 
 static int attn_wgs_log2(const nx_ctx *c) { return std::max(4, 31 - __builtin_clz(c->num_cu * kAttnWgsPerCu)); }
