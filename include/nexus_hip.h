@@ -317,7 +317,8 @@ int nx_kv_read_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float
  *   out[r][h] = sum_j softmax_j(scale q[r][h] . k_j) v_j
  * over the tokens j <= p that it sees, h = 0 .. heads - 1 reading key/value head
  * h / (heads / kv_heads).  window = 0: all of them; window > 0: its last
- * `window` tokens (itself included) and the sequence's first `sinks` tokens.  A
+ * `window` tokens (itself included) and the sequence's first `sinks` tokens; pages
+ * that no row sees are not looked at, and their table entries may name none.  A
  * row that sees no token is zeros.  q rows are heads * head_dim floats, q_stride
  * floats apart, out rows likewise; neither needs an alignment, and out must not
  * overlap q.  f32 in and out: scores, softmax and sums are held in f32, and the f32 factors of the

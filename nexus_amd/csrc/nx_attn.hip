@@ -1389,7 +1389,7 @@ static int attention(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const flo
   NX_TRY(refuse(kv_check_rows("output", (long)out_stride, (long)width)));
   AttnCall a{q, out, q_stride, out_stride, heads, heads / kv->heads, scale, window, sinks, false, false, 0, 0};
   if (!host) return attention_dev(c, kv, *b, a);
-  NX_TRY(refuse(kv_check_tables(*b, kv->pages, kv->page_tokens, true, false)));
+  NX_TRY(refuse(kv_check_tables(*b, kv->pages, kv->page_tokens, true, false, window, sinks)));
   const size_t r0 = b->row_start[0], rows = b->row_start[b->num_seqs];
   if (rows == r0) return NX_OK;
   nx_kv_batch dev;

@@ -116,9 +116,10 @@ inline Refusal attn_check(int heads, int kv_heads, float scale, int window, int 
 // What the calls on host memory check besides: that every row, length and page
 // is one the cache has.  (Calls on device memory cannot look: their kernels
 // leave out what is not there.)  `whole`: the call reads the sequences from
-// their first token on (attention); else only the batch's rows.  `writes`: no
-// two sequences may write one token's place.
-inline Refusal kv_check_tables(const nx_kv_batch &b, int num_pages, int page_tokens, bool whole, bool writes) {
+// their first token on (attention; with a window, but for the pages that no row sees); else
+// only the batch's rows.  `writes`: no two sequences may write one token's place.
+inline Refusal kv_check_tables(const nx_kv_batch &b, int num_pages, int page_tokens, bool whole, bool writes,
+                               int window = 0, int sinks = 0) {
   struct Span {
     int page, lo, hi;
   };
@@ -135,6 +136,8 @@ inline Refusal kv_check_tables(const nx_kv_batch &b, int num_pages, int page_tok
       return {NX_ERR_SHAPE, "sequence " + std::to_string(s) + " is longer than its pages"};
     if (n == 0) continue;
     for (int p = whole ? 0 : (len - n) / page_tokens; p <= (len - 1) / page_tokens; ++p) {
+      const int64_t from = (int64_t)p * page_tokens;
+      if (window > 0 && from >= sinks && from + page_tokens <= (int64_t)len - n - window + 1) continue;
       const int page = b.pages[(size_t)s * b.max_pages + p];
       if (page < 0 || page >= num_pages)
         return {NX_ERR_INVALID_ARG, "page " + std::to_string(page) + " of sequence " + std::to_string(s) +

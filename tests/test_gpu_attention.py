@@ -355,6 +355,28 @@ def test_missing_page_in_the_middle(ctx, fmt, H):
         cache.close()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("H", [4, 46])
+def test_pages_behind_a_window(ctx, fmt, H):
+    """A window's caller may give back the pages that no row sees any more."""
+    rng = np.random.default_rng(24)
+    G, D, page = 2, 96, 64
+    for n in (1, 90):
+        b = Batch(rng, [n], [900], page)
+        cache, k, v = filled(ctx, rng, b, fmt, G, D)
+        q = rng.standard_normal((n, H, D)).astype(np.float32)
+        want = cache.attention(*b.args(), q, H, window=130, sinks=3)
+        first = (900 - n - 129) // page
+        other = [np.full((64, G, D), np.nan)] * 2
+        for p in range(1, first):  # the next owners write to them
+            cache.write([0, 64], [64], b.pages[:, p:p + 1], *other)
+        b.pages[0, 1:first] = -1
+        assert_same_bits(cache.attention(*b.args(), q, H, window=130, sinks=3), want)
+        with pytest.raises(nx.NexusError):
+            cache.attention(*b.args(), q, H, window=130 + page, sinks=3)
+        cache.close()
+
+
 def test_shared_pages(ctx):
     """Two sequences with one prefix in the same pages."""
     rng = np.random.default_rng(17)

@@ -148,6 +148,28 @@ def test_batches(tmp_path):
 
 
 @needs_gxx
+def test_tables_behind_a_window(tmp_path):
+    """Pages that no row sees need not be there; each that some row sees does."""
+    run(tmp_path, r"""
+  for (int n : {1, 40})
+    for (int window : {1, 64, 65, 200, INT_MAX})
+      for (int sinks : {0, 1, 64, 65, INT_MAX})
+        for (int missing = 0; missing < 6; ++missing) {
+          const int len = 350;
+          int rows[] = {0, n}, lens[] = {len}, pages[] = {0, 1, 2, 3, 4, 5};
+          pages[missing] = -1;
+          const nx_kv_batch b{1, n, 6, rows, lens, pages};
+          bool seen = false;
+          for (int p = len - n; p < len; ++p)
+            for (int j = 64 * missing; j < 64 * (missing + 1); ++j)
+              seen = seen || (j <= p && (p - j < window || j < sinks));
+          is((kv_check_tables(b, 6, 64, true, false, window, sinks).code != NX_OK) == seen, "seen");
+          is(kv_check_tables(b, 6, 64, true, false).code != NX_OK, "without a window");
+        }
+""")
+
+
+@needs_gxx
 def test_attention_arguments(tmp_path):
     run(tmp_path, r"""
   is(attn_check(8, 2, 0.1f, 0, 0).code == NX_OK && attn_check(2, 2, -3.f, 1, 0).code == NX_OK, "good");
