@@ -624,9 +624,8 @@ __device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b
   constexpr int kSlots = JoinLds<D, NW>::kSlots;
   const int slot = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4), size = tile * (D + 2);
   const int mine = (t.nr - y + dy - 1) / dy;
-  int share = 1;
-  while (2 * share * mine <= kSlots && share < parts) share *= 2;
-  const int sub = slot & (share - 1), at_once = kSlots / share;
+  const JoinSlots by = join_slots(kSlots, mine, parts);
+  const int share = by.share, sub = slot & (share - 1), at_once = by.rows();
   if (threadIdx.x < kRows) lds.bad[threadIdx.x] = 0;
   for (int k0 = 0; k0 < mine; k0 += at_once) {
     const int k = k0 + slot / share, r = y + min(k, mine - 1) * dy;
@@ -672,7 +671,7 @@ __device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b
         }
       }
       __syncthreads();
-      if (sub == 0 && slot < kSlots) {
+      if (by.leads(slot)) {
         float m1 = m;
         for (int x = 1; x < share; ++x) m1 = fmaxf(m1, lds.m[slot + x]);
         float f = exp2f(m - m1);
@@ -685,7 +684,7 @@ __device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b
         }
       }
     }
-    if (sub == 0 && slot < at_once * share && k < mine)
+    if (by.leads(slot) && k < mine)
       store_out<D>(a, s, t.head, t.r0 + r, 4 * d, o, l, &lds.bad[r]);
   }
   __syncthreads();

@@ -176,6 +176,21 @@ constexpr KeySpan key_span(int pmin, int pmax, int len, int window, int sinks) {
   return {first, from, to};
 }
 
+// Which of a join's slots (D / 4 threads each) take what: a row has `share` of them, a power
+// of two, which share its parts, and rows() rows are joined at once.  Slots behind the last
+// whole row (there are 10 or 21 for heads of 96) have no row.
+struct JoinSlots {
+  int slots, share;
+  constexpr int rows() const { return slots / share; }
+  // whether the slot adds up its row's, slot .. slot + share - 1
+  constexpr bool leads(int slot) const { return (slot & (share - 1)) == 0 && slot < rows() * share; }
+};
+constexpr JoinSlots join_slots(int slots, int rows, int parts) {
+  int share = 1;
+  while (2 * share * rows <= slots && share < parts) share *= 2;
+  return {slots, share};
+}
+
 // Groups of 32 tokens that a batch's rows touch, at most: a sequence of n rows
 // touches at most n, and at most n / 32 + 2.
 inline long kv_touched_groups(long seqs, long rows) { return std::min(rows, rows / kKvGroup + 2 * seqs); }

@@ -224,6 +224,31 @@ def test_touched_groups_bound(tmp_path):
 """)
 
 
+@needs_gxx
+def test_join_slots(tmp_path):
+    """A join's slots add up only slots that there are, every row has one that does, and
+    no slot is added twice; heads of 96 leave slots over."""
+    run(tmp_path, r"""
+  for (int D : {64, 96, 128, 256})
+    for (int waves : {4, 8}) {
+      const int slots = 64 * waves / (D / 4);
+      for (int rows = 1; rows <= 128; ++rows)
+        for (int parts : {2, 3, 4, 8, 9, 16, 17, 100, 512}) {
+          const JoinSlots j = join_slots(slots, rows, parts);
+          is(j.share >= 1 && (j.share & (j.share - 1)) == 0 && j.share <= slots && j.rows() >= 1, "share");
+          int leads = 0;
+          // (threads behind the last slot have numbers too)
+          for (int slot = 0; slot <= slots; ++slot)
+            if (j.leads(slot)) {
+              is(slot / j.share == leads++, "rows in order");
+              is(slot + j.share <= slots, "adds up slots that there are");
+            }
+          is(leads == j.rows(), "a leader each");
+        }
+    }
+""")
+
+
 def test_null_handles():
     """Refused without a device."""
     L = nx.lib()
