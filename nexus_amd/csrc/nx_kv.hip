@@ -106,18 +106,19 @@ __device__ __forceinline__ int touched(const KvSeq &q) {
 }
 
 // Eight waves: four for the keys, four for the values.
-constexpr int kMoveWaves = 8;
+constexpr int kMoveWaves = kMoveThreads / 64;
+static_assert(kMoveWaves == 8);
 
 template <int FMT, int D>
-__global__ __launch_bounds__(64 * kMoveWaves) void k_kv_write(KvView kv, nx_kv_batch b, const float *k,
-                                                              const float *v, size_t stride, bool wide) {
+__global__ __launch_bounds__(kMoveThreads) void k_kv_write(KvView kv, nx_kv_batch b, int first, const float *k,
+                                                          const float *v, size_t stride, bool wide) {
   using E = kv_elem<FMT>;
   using Chunk = std::conditional_t<FMT == NX_KV_INT8, uint2, uint4>;  // 8 elements
   __shared__ __align__(16) E tile[2][kKvGroup * D];
   __shared__ long sums[kMoveWaves];
   __shared__ Place place;
   const int head = blockIdx.x % kv.heads;
-  const Place at = find_item<kMoveWaves>(kv, b, blockIdx.x / kv.heads, touched, sums, &place);
+  const Place at = find_item<kMoveWaves>(kv, b, first + blockIdx.x / kv.heads, touched, sums, &place);
   if (at.s < 0) return;
   const KvSeq q = at.seq;
   const int g0 = (max(q.first, 0) / kKvGroup + at.at) * kKvGroup;  // the group's first token
@@ -158,8 +159,8 @@ __global__ __launch_bounds__(64 * kMoveWaves) void k_kv_write(KvView kv, nx_kv_b
 }
 
 template <int FMT, int D>
-__global__ __launch_bounds__(64 * kMoveWaves) void k_kv_read(KvView kv, nx_kv_batch b, float *k, float *v,
-                                                             size_t stride, bool wide) {
+__global__ __launch_bounds__(kMoveThreads) void k_kv_read(KvView kv, nx_kv_batch b, int first, float *k, float *v,
+                                                         size_t stride, bool wide) {
   using E = kv_elem<FMT>;
   using Chunk = std::conditional_t<FMT == NX_KV_INT8, uint2, uint4>;
   __shared__ __align__(16) E tile[2][kKvGroup * D];
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(64 * kMoveWaves) void k_kv_read(KvView kv, nx_kv_ba
   // rows without a token (before the first, behind the table) are read as zeros:
   // items cover the rows, in the groups that their tokens would have
   const Place at = find_item<kMoveWaves>(
-      kv, b, blockIdx.x / kv.heads,
+      kv, b, first + blockIdx.x / kv.heads,
       [](const KvSeq &q) { return q.n > 0 ? ((q.first + q.n - 1) >> 5) - (q.first >> 5) + 1 : 0; }, sums, &place);
   if (at.s < 0) return;
   const KvSeq q = at.seq;
@@ -221,21 +222,22 @@ static bool wide_rows(const void *a, const void *b, size_t stride) {
 
 static int kv_move_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, const float *rk,
                        const float *rv, float *wk, float *wv, size_t stride, bool write) {
-  const long groups = kv_touched_groups(b.num_seqs, b.num_tokens);
-  if (groups * kv->heads > INT32_MAX)
-    return fail(NX_ERR_UNSUPPORTED, "a batch of more than 2^31 groups of tokens");
-  const dim3 grid((uint32_t)(groups * kv->heads));
+  const long groups = kv_touched_groups(b.num_seqs, b.num_tokens), at_once = kv_groups_at_once(kv->heads);
   const KvView view = view_of(kv);
-  return launch(c, write ? "kv_write" : "kv_read", [&] {
-    with_kernel(kv, [&](auto fmt, auto D) {
-      if (write)
-        go(c, k_kv_write<fmt(), D()>, grid, dim3(64 * kMoveWaves), 0, view, b, rk, rv, stride,
-           wide_rows(rk, rv, stride));
-      else
-        go(c, k_kv_read<fmt(), D()>, grid, dim3(64 * kMoveWaves), 0, view, b, wk, wv, stride,
-           wide_rows(wk, wv, stride));
-    });
-  });
+  for (long first = 0; first < groups; first += at_once) {
+    const dim3 grid((uint32_t)(std::min(groups - first, at_once) * kv->heads)), block(kMoveThreads);
+    NX_TRY(launch(c, write ? "kv_write" : "kv_read", [&] {
+      with_kernel(kv, [&](auto fmt, auto D) {
+        if (write)
+          go(c, k_kv_write<fmt(), D()>, grid, block, 0, view, b, (int)first, rk, rv, stride,
+             wide_rows(rk, rv, stride));
+        else
+          go(c, k_kv_read<fmt(), D()>, grid, block, 0, view, b, (int)first, wk, wv, stride,
+             wide_rows(wk, wv, stride));
+      });
+    }));
+  }
+  return NX_OK;
 }
 
 int kv_check_call(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b) {

@@ -195,4 +195,9 @@ constexpr JoinSlots join_slots(int slots, int rows, int parts) {
 // touches at most n, and at most n / 32 + 2.
 inline long kv_touched_groups(long seqs, long rows) { return std::min(rows, rows / kKvGroup + 2 * seqs); }
 
+// Threads of a workgroup that moves a head's group of tokens into or out of the cache, and the
+// groups that one launch takes: it has fewer than 2^32 threads.  More go in several launches.
+constexpr int kMoveThreads = 512;
+constexpr long kv_groups_at_once(int heads) { return (long)(UINT32_MAX / kMoveThreads) / heads; }
+
 }  // namespace nx

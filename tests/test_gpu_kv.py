@@ -223,6 +223,27 @@ def test_many_sequences(ctx):
     cache.close()
 
 
+def test_more_tokens_than_one_launch_takes(ctx):
+    """2100 single tokens on 4096 heads: more than 2^32 threads.  Each page has 32 sequences'
+    tokens, and a row's values are the next row's keys."""
+    G, D, page, S = 4096, 64, 32, 2100
+    x = np.add.outer((np.arange(S + 1) % 1021).astype(np.float32), (np.arange(G * D) % 1024).astype(np.float32))
+    src, out = DeviceArray(x.size), DeviceArray(2 * S * G * D)
+    src.upload(x)
+    s = np.arange(S)
+    rs, ln, pg = ints(np.arange(S + 1)), ints(s % page + 1), ints(s // page)
+    d = nx.KvBatch(S, S, 1, rs.ptr, ln.ptr, pg.ptr)
+    cache = nx.KvCache(ctx, F16, -(-S // page), page, G, D)
+    print(f"kv S={S} G={G} D={D}", flush=True)
+    cache.write_dev(d, src.ptr, src.ptr + 4 * G * D, G * D)
+    cache.read_dev(d, out.ptr, out.ptr + 4 * G * D, 2 * G * D)
+    ctx.sync()
+    got = out.download().reshape(S, 2, G * D)
+    assert np.array_equal(got[:, 0], x[:-1])
+    assert np.array_equal(got[:, 1], x[1:])
+    cache.close()
+
+
 def test_refusals(ctx):
     def refused(code, f, *a, **kw):
         with pytest.raises(nx.NexusError) as e:

@@ -249,6 +249,19 @@ def test_join_slots(tmp_path):
 """)
 
 
+@needs_gxx
+def test_launches_of_the_largest_batches(tmp_path):
+    """A launch has fewer than 2^32 threads, whatever the batch; the groups' numbers fit an int."""
+    run(tmp_path, r"""
+  for (int heads : {1, 7, 8, 32, 4096}) {
+    const long at_once = kv_groups_at_once(heads);
+    is(at_once >= 1 && at_once * heads * kMoveThreads <= UINT32_MAX, "threads of a launch");
+    is((at_once + 1) * heads * kMoveThreads > UINT32_MAX, "as many as fit");
+  }
+  is(kv_touched_groups(1 << 20, 1 << 24) < INT32_MAX / 2, "the largest batch");
+""")
+
+
 def test_null_handles():
     """Refused without a device."""
     L = nx.lib()
