@@ -328,7 +328,7 @@ int nx_kv_read_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float
  * run.
  * attention_decode (src/engine/mod.rs:452-500) and
  * kernel::grouped_query_attention (src/kernel/mod.rs:40-99) for a batch.
- * The workspace (some 80 MB) is the context's, allocated with the first cache or
+ * The workspace (some 77 MB) is the context's, allocated with the first cache or
  * call on it and never moved, so a captured call may be replayed while the context
  * lives; calls on one context must not overlap in time (two graphs captured from
  * it neither), and a context's first call or cache is not made under capture. */

@@ -1316,12 +1316,18 @@ int attn_workspace(nx_ctx *c, void **out) {
   const size_t wide = std::max(part_floats(kRows, 128), part_floats(kRows, 256) / 2);
   // (and a descriptor and a count of each)
   const size_t bytes = wgs * (2 * sizeof(int4) + sizeof(int) + 4 * (part_floats(kTile, 256) / 2 + wide));
-  const bool there = c->ws[WS_ATTN].cap >= bytes;
-  void *p;
-  NX_TRY(ws_get(c, WS_ATTN, bytes, &p));
-  if (!there)  // counts begin at 0
+  DevBuf &ws = c->ws[WS_ATTN];
+  if (!ws.ptr) {  // of this size: it never grows
+    void *p = nullptr;
+    if (hipMalloc(&p, bytes) != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(NX_ERR_OOM, "device allocation of " + std::to_string(bytes) + " bytes failed");
+    }
+    ws = {p, bytes};
+    // counts begin at 0
     NX_HIP(hipMemsetAsync(static_cast<int4 *>(p) + 2 * wgs, 0, wgs * sizeof(int), c->stream));
-  if (out) *out = p;
+  }
+  if (out) *out = ws.ptr;
   return NX_OK;
 }
 

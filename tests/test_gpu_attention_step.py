@@ -330,6 +330,17 @@ def test_very_many_sequences(ctx, long):
     cache.close()
 
 
+def test_size_of_the_workspace():
+    """A context's attention takes the memory that the header states, and nothing for growth."""
+    with nx.Context(0) as ctx:
+        ctx.sync()
+        free, _ = ctx.mem_info()
+        cache = nx.KvCache(ctx, F16, 1, 32, 1, 64)
+        now, _ = ctx.mem_info()
+        assert free - now < 82 << 20  # 77 MB, the cache, and whole 2 MiB pages of either
+        cache.close()
+
+
 def test_profile_and_lifetimes():
     """The launches show in the context's profile; a cache may outlive its context."""
     rng = np.random.default_rng(36)
