@@ -331,7 +331,8 @@ int nx_kv_read_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float
  * The workspace (some 77 MB) is the context's, allocated with the first cache or
  * call on it and never moved, so a captured call may be replayed while the context
  * lives; calls on one context must not overlap in time (two graphs captured from
- * it neither), and a context's first call or cache is not made under capture. */
+ * it neither).  A context's first call, and any cache, is refused while its stream is
+ * captured (NX_ERR_UNSUPPORTED, the capture goes on). */
 int nx_attention(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *q,
                  size_t q_stride, int heads, float scale, int window, int sinks, float *out,
                  size_t out_stride);

@@ -1318,14 +1318,21 @@ int attn_workspace(nx_ctx *c, void **out) {
   const size_t bytes = wgs * (2 * sizeof(int4) + sizeof(int) + 4 * (part_floats(kTile, 256) / 2 + wide));
   DevBuf &ws = c->ws[WS_ATTN];
   if (!ws.ptr) {  // of this size: it never grows
+    NX_TRY(refuse_capture(c));
     void *p = nullptr;
     if (hipMalloc(&p, bytes) != hipSuccess) {
       (void)hipGetLastError();
       return fail(NX_ERR_OOM, "device allocation of " + std::to_string(bytes) + " bytes failed");
     }
+    // counts begin at 0, and the workspace is there once they are: a call that finds others
+    // would leave split tiles out
+    if (hipMemsetAsync(static_cast<int4 *>(p) + 2 * wgs, 0, wgs * sizeof(int), c->stream) != hipSuccess ||
+        hipStreamSynchronize(c->stream) != hipSuccess) {
+      (void)hipGetLastError();
+      (void)hipFree(p);
+      return fail(NX_ERR_DEVICE, "clearing the attention's workspace failed");
+    }
     ws = {p, bytes};
-    // counts begin at 0
-    NX_HIP(hipMemsetAsync(static_cast<int4 *>(p) + 2 * wgs, 0, wgs * sizeof(int), c->stream));
   }
   if (out) *out = ws.ptr;
   return NX_OK;

@@ -240,6 +240,15 @@ static int kv_move_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, const f
   return NX_OK;
 }
 
+int refuse_capture(nx_ctx *c) {
+  hipStreamCaptureStatus status;
+  if (hipStreamIsCapturing(c->stream, &status) == hipSuccess && status == hipStreamCaptureStatusNone)
+    return NX_OK;
+  (void)hipGetLastError();
+  return fail(NX_ERR_UNSUPPORTED, "a context's first cache or attention call, and every cache, is made "
+                                  "outside of stream capture");
+}
+
 int kv_check_call(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b) {
   if (!c) return fail(NX_ERR_INVALID_ARG, "null context");
   NX_HIP(hipSetDevice(c->device));
@@ -308,6 +317,7 @@ static int kv_create(nx_ctx *c, int fmt, int pages, int page_tokens, int heads, 
   if (!out) return fail(NX_ERR_INVALID_ARG, "null output pointer");
   NX_TRY(refuse(kv_check_geometry(fmt, pages, page_tokens, heads, D)));
   NX_HIP(hipSetDevice(c->device));
+  NX_TRY(refuse_capture(c));
   NX_TRY(attn_workspace(c, nullptr));
   const size_t plane = kv_plane_bytes(fmt, pages, page_tokens, heads, D);
   const size_t scales = kv_scale_bytes(fmt, pages, page_tokens, heads);

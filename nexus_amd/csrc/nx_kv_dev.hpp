@@ -24,6 +24,9 @@ namespace nx {
 
 // the attention's workspace on a context: allocated once, never moved
 int attn_workspace(nx_ctx *c, void **out);
+// refuses what allocates and clears memory while the context's stream is captured: the graph
+// would clear it again with every replay, and not before the first
+int refuse_capture(nx_ctx *c);
 int kv_check_call(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b);
 // copies a host batch's arrays to the device; *dev describes them there
 int kv_upload_batch(nx_ctx *c, const nx_kv_batch &b, nx_kv_batch *dev);

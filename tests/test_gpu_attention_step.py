@@ -330,6 +330,54 @@ def test_very_many_sequences(ctx, long):
     cache.close()
 
 
+def test_first_calls_under_capture_are_refused():
+    """What allocates and clears memory is refused while the context's stream is captured, and
+    leaves the capture whole; the same calls outside of it, and captured ones behind them, run."""
+    hip = Hip()
+    rng = np.random.default_rng(37)
+    heads, G, D = 8, 2, 64
+    with nx.Context(0) as one, nx.Context(0) as two:
+        b = Batch(rng, [1, 1], [4000, 77], 64)
+        cache, k, v = filled(one, rng, b, F16, G, D)
+        q = rng.standard_normal((b.rows, heads, D)).astype(np.float32)
+        ref, bound = attention(b, k, v, q, heads, np.float32(D ** -0.5))
+        s = Step(b, heads, G, D)
+        s.q.upload(q)
+        stream = hip.stream()
+        two.set_stream(stream.value)
+        cache.ctx = two
+        attend = lambda: cache.attention_dev(s.d, s.q.ptr, heads * D, heads, s.out.ptr,  # noqa: E731
+                                             heads * D, D ** -0.5)
+
+        def refused():
+            for f in (attend, lambda: nx.KvCache(two, F16, 1, 32, 1, 64)):
+                with pytest.raises(nx.NexusError) as e:
+                    f()
+                assert e.value.code == nx.NX_ERR_UNSUPPORTED and "capture" in str(e.value)
+
+        graphs = [hip.graph(stream, refused)]
+        attend()
+        two.sync()
+        assert_close(s.got(), ref, bound)
+        want = s.got()
+        graphs.append(hip.graph(stream, attend))
+        for _ in range(3):
+            s.out.upload(np.zeros(s.out.n, np.float32))
+            for _, x in graphs:
+                hip.hipGraphLaunch(x, stream)
+            two.sync()
+            assert_same_bits(s.got(), want)
+            attend()
+            two.sync()
+            assert_same_bits(s.got(), want)
+        for g, x in graphs:
+            hip.hipGraphExecDestroy(x)
+            hip.hipGraphDestroy(g)
+        cache.close()
+        two.set_stream(None)
+        hip.hipStreamDestroy(stream)
+
+
 def test_size_of_the_workspace():
     """A context's attention takes the memory that the header states, and nothing for growth."""
     with nx.Context(0) as ctx:
