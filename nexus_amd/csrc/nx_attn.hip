@@ -210,6 +210,25 @@ struct Ref {
   __device__ __forceinline__ float value() const { return fresh ? kUnset : m; }
 };
 
+// Takes sums of reference m to reference m1 >= m: by 2^(m - m1).  INT8: m follows the weights
+// times their values' scales, and may move by more than 2^-126 reaches while the plain sum of
+// the weights, of tokens whose scales are small, counts all the same.  So references are whole
+// there, and that sum moves by its exponent (exactly, too).
+template <bool I8>
+struct Shift {
+  float f;
+  int e;
+  __device__ __forceinline__ Shift(float m, float m1) {
+    if constexpr (I8) {
+      e = (int)fmaxf(m - m1, -1000.f);
+      f = ldexp1(1.f, e);
+    } else {
+      f = exp2f(m - m1);
+    }
+  }
+  __device__ __forceinline__ float weights(float l) const { return I8 ? ldexp1(l, e) : l * f; }
+};
+
 // A value scale's exponent field: 126 and its log2 rounded up, at least 36, so that no
 // weight without its scale passes 2^(90 + kGrow) either (they are summed too).  A NaN
 // (a token that is not finite) outgrows everything, and counts as a scale of 0: rows that
@@ -242,9 +261,10 @@ __device__ __forceinline__ void weigh(float (&w)[N], Scale dv, Exp de, float c, 
   if (__any(most > (ref.fresh ? -INFINITY : kGrow + bias))) {
     most = top(most) - bias;
     const bool anew = most > (ref.fresh ? -INFINITY : kGrow);
-    const float m1 = anew ? ref.m + (most - kHead) : ref.m;
-    const float keep = ref.fresh ? 0.f : exp2f(ref.m - m1);
-    l *= keep;
+    const float m1 = anew ? ref.m + (I8 ? floorf(most - kHead) : most - kHead) : ref.m;
+    const Shift<I8> to(ref.m, m1);
+    const float keep = ref.fresh ? 0.f : to.f;
+    l = I8 ? (ref.fresh ? 0.f : to.weights(l)) : l * keep;
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] *= keep;
     // (rounded in the last places of scores of this size, as they are themselves)
@@ -621,6 +641,7 @@ template <int FMT, int D, int NW, bool THROUGH>
 __device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                           const KvSeq &s, const Tile &t, const float *first, int tile,
                                           int parts, int y, int dy, JoinLds<D, NW> &lds) {
+  using To = Shift<FMT == NX_KV_INT8>;
   constexpr int kSlots = JoinLds<D, NW>::kSlots;
   const int slot = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4), size = tile * (D + 2);
   const int mine = (t.nr - y + dy - 1) / dy;
@@ -645,16 +666,17 @@ __device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b
       float m1 = m;
 #pragma unroll
       for (int x = 0; x < U(); ++x) m1 = fmaxf(m1, mp[x]);
-      const float keep = exp2f(m - m1);
+      const To keep(m, m1);
       m = m1;
-      l *= keep;
-      o *= keep;
+      l = keep.weights(l);
+      o *= keep.f;
 #pragma unroll
       for (int x = 0; x < U(); ++x) {
         const bool is = i0 + x * share < parts;
-        const float f = is ? exp2f(mp[x] - m) : 0.f;
-        l += is ? lp[x] * f : 0.f;
-        o += (is ? op[x] : f32x4{0.f, 0.f, 0.f, 0.f}) * f;
+        To to(mp[x], m);
+        to.f = is ? to.f : 0.f;
+        l += is ? to.weights(lp[x]) : 0.f;
+        o += (is ? op[x] : f32x4{0.f, 0.f, 0.f, 0.f}) * to.f;
       }
     };
     if (parts <= 2 * share)
@@ -674,13 +696,13 @@ __device__ __forceinline__ void join_tile(const KvView &kv, const nx_kv_batch &b
       if (by.leads(slot)) {
         float m1 = m;
         for (int x = 1; x < share; ++x) m1 = fmaxf(m1, lds.m[slot + x]);
-        float f = exp2f(m - m1);
-        l *= f;
-        o *= f;
+        const To own(m, m1);
+        l = own.weights(l);
+        o *= own.f;
         for (int x = 1; x < share; ++x) {
-          f = exp2f(lds.m[slot + x] - m1);
-          l += lds.l[slot + x] * f;
-          o += lds.o[slot + x][d] * f;
+          const To to(lds.m[slot + x], m1);
+          l += to.weights(lds.l[slot + x]);
+          o += lds.o[slot + x][d] * to.f;
         }
       }
     }
@@ -918,9 +940,9 @@ __global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn
       float lt = 0.f;
 #pragma unroll
       for (int v = 0; v < NW; ++v) {
-        const float f = exp2f(lds.m[v][r] - m1);
-        lt += lds.l[v][r] * f;
-        o += *reinterpret_cast<const f32x4 *>(&lds.o[v][r][d]) * f;
+        const Shift<I8> to(lds.m[v][r], m1);
+        lt += to.weights(lds.l[v][r]);
+        o += *reinterpret_cast<const f32x4 *>(&lds.o[v][r][d]) * to.f;
       }
       if (!whole) {
         if (d == 0) {

@@ -161,6 +161,48 @@ def test_value_scales_of_all_sizes(ctx):
         cache.close()
 
 
+def close_int8(ctx, k, v, q, n, scale):
+    """INT8 attention of the last n of the tokens k, v against its formula."""
+    length, G, D = k.shape
+    b = Batch(np.random.default_rng(25), [n], [length], 32)
+    cache = nx.KvCache(ctx, INT8, b.num_pages, 32, G, D)
+    cache.write(b.whole(), b.kv_len, b.pages, k, v)
+    H = q.shape[1]
+    ref, bound = attention(b, stored(INT8, k), stored(INT8, v), q, H, np.float32(scale))
+    assert_close(cache.attention(*b.args(), q, H, scale=scale), ref, bound)
+    cache.close()
+
+
+# one workgroup of 16-row tiles, several, and 128-row tiles whole and in parts
+INT8_STEPS = [(1, 4, 700), (2, 2, 9000), (150, 28, 300), (150, 28, 1500)]
+
+
+@pytest.mark.parametrize("n,H,length", INT8_STEPS)
+@pytest.mark.parametrize("small,large", [(0.0, 1e25), (1e-24, 1e29), (0.0, 1.0)])
+@pytest.mark.parametrize("order", ["first", "last", "groups", "tokens"])
+def test_value_scales_far_apart(ctx, n, H, length, small, large, order):
+    """INT8: tokens of next to no value count in the denominator, wherever the large ones are."""
+    rng = np.random.default_rng(26)
+    j = np.arange(length)
+    is_large = {"first": j < length // 2, "last": j >= length // 2, "groups": j // 32 % 2 == 1,
+                "tokens": rng.random(length) < 0.5}[order]
+    k, v = random_kv(rng, length, 2, 128)
+    v *= np.where(is_large, large, small).astype(np.float32)[:, None, None]
+    close_int8(ctx, k, v, rng.standard_normal((n, H, 128)).astype(np.float32), n, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("n,H,length", INT8_STEPS)
+@pytest.mark.parametrize("large", [1.0, 1e20, 1e30])
+def test_many_small_weights_beside_a_large_value(ctx, n, H, length, large):
+    """INT8: one token's value decides the reference, the others' weights the denominator."""
+    rng = np.random.default_rng(27)
+    u = rng.choice([-1.0, 1.0], 128)
+    k = np.repeat((-6.0 / 128 * u).astype(np.float32)[None, None], length, 0).repeat(2, 1)
+    _, v = random_kv(rng, length, 2, 128)
+    k[7], v[7] = 0, v[7] * np.float32(large)
+    close_int8(ctx, k, v, np.tile(u.astype(np.float32), (n, H, 1)), n, 1.0)
+
+
 @pytest.mark.parametrize("H", [4, 204])
 def test_zeros(ctx, H):
     """Zero queries average, zero keys and values give what the formula gives."""
