@@ -42,18 +42,31 @@ __device__ __forceinline__ bool sees(const AttnCall &a, int p, int j) {
   return j <= p && (a.window == 0 || p - j < a.window || j < a.sinks);
 }
 
-// One row by the formula alone, in f32: a wave, each lane a key's whole score,
-// then each lane some elements of the sum over the keys.  For rows whose result on the
-// matrix cores is not finite or sums to nothing: infinities and NaNs in the row's own keys,
-// values or query, 0 times a masked one, or no token to see.  (Rare, and not made fast.)
+// the largest (sum) over the wave's lanes, in all of them
+template <typename Op>
+__device__ __forceinline__ double across_wave(double v, Op op) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = op(v, __shfl_xor(v, d, 64));
+  return v;
+}
+
+// One row by the formula alone, on the values that the cache reads back and summed in 64 bits
+// (whose range holds any sum of f32 products): a wave, each lane a key's whole score, then each
+// lane some elements of the sum over the keys.  For rows whose result on the matrix cores is
+// not finite or sums to nothing: infinities and NaNs in the row's own keys, values or query, 0
+// times a masked one, value scales that the halves do not reach (value_exp), or no token to
+// see.  Rare, and not made fast: a wave walks a row's whole context, 45 ms, not 81 us, for one
+// token after 100001 of 32 heads over 8 of 128 (F16).
 template <int FMT, int D>
 __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b, const AttnCall &a,
                                          const KvSeq &s, int seq, int head, int p, const float *q,
                                          float *out) {
   using E = kv_elem<FMT>;
-  const int lane = threadIdx.x & 63;
+  constexpr bool I8 = FMT == NX_KV_INT8;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // what follows from it is not held in registers by the callers' loops
   const E *ck = reinterpret_cast<const E *>(kv.k), *cv = reinterpret_cast<const E *>(kv.v);
-  float m = -INFINITY, l = 0.f, acc[(D + 63) / 64] = {};
+  double m = -INFINITY, l = 0., acc[(D + 63) / 64] = {};
   bool any = false;
   const int end = min(p + 1, s.len);
   for (int j0 = 0; j0 < end; j0 += 64) {
@@ -65,13 +78,13 @@ __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b,
     long group = -1;
     if (j < end && sees(a, p, j)) group = kv_group(kv, b, seq, head, j & ~(kKvGroup - 1));
     const int t = j & (kKvGroup - 1);
-    float x = -INFINITY;
+    double x = -INFINITY;
     if (group >= 0) {
-      x = 0.f;
+      x = 0.;
       const E *k = ck + group * (kKvGroup * D);
-      for (int d = 0; d < D; ++d) x = fmaf((float)k[kv_key_at(FMT, t, d)], q[d], x);
+      const float ks = I8 ? kv.ks[group * kKvGroup + t] : 1.f;
+      for (int d = 0; d < D; ++d) x = fma((double)((float)k[kv_key_at(FMT, t, d)] * ks), (double)q[d], x);
       x *= a.scale;
-      if (FMT == NX_KV_INT8) x *= kv.ks[group * kKvGroup + t];
     }
     const uint64_t seen = __ballot(group >= 0);
     if (!seen) continue;
@@ -80,40 +93,31 @@ __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b,
       l = NAN;
       break;
     }
-    float top = x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    const float m1 = fmaxf(m, top), ref = m1 == -INFINITY ? 0.f : m1;
-    const float pr = group >= 0 ? expf(x - ref) : 0.f;
-    const float keep = m == -INFINITY ? 0.f : expf(m - ref);
+    const double m1 = fmax(m, across_wave(x, [](double u, double v) { return fmax(u, v); }));
+    const double ref = m1 == -INFINITY ? 0. : m1;
+    const float w = group >= 0 ? expf((float)(x - ref)) : 0.f;
+    const double keep = m == -INFINITY ? 0. : (double)expf((float)(m - ref));
     m = m1;
-    float sum = pr;
+    l = l * keep + across_wave((double)w, [](double u, double v) { return u + v; });
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-    l = l * keep + sum;
-    // the 64 keys' sum apart: over long contexts a single chain of additions would
-    // lose sqrt(keys) of its last places
-    float part[(D + 63) / 64] = {};
-    float w = pr;
-    if (FMT == NX_KV_INT8 && group >= 0) w *= kv.vs[group * kKvGroup + t];
+    for (int i = 0; i < (D + 63) / 64; ++i) acc[i] *= keep;
+    const float vs = I8 && group >= 0 ? kv.vs[group * kKvGroup + t] : 1.f;
     for (int u = 0; u < 64; ++u) {
       if (!((seen >> u) & 1)) continue;
-      const float wu = __shfl(w, u, 64);
-      const long gu = __shfl(group, u, 64);
-      const E *v = cv + gu * (kKvGroup * D);
+      const double wu = __shfl(w, u, 64);
+      const float su = I8 ? __shfl(vs, u, 64) : 1.f;
+      const E *v = cv + __shfl(group, u, 64) * (kKvGroup * D);
 #pragma unroll
       for (int i = 0; i < (D + 63) / 64; ++i) {
         const int d = lane + 64 * i;
-        if (d < D) part[i] = fmaf(wu, (float)v[kv_value_at(D, (j0 + u) & (kKvGroup - 1), d)], part[i]);
+        if (d < D) acc[i] = fma(wu, (double)((float)v[kv_value_at(D, (j0 + u) & (kKvGroup - 1), d)] * su), acc[i]);
       }
     }
-#pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i) acc[i] = fmaf(acc[i], keep, part[i]);
   }
 #pragma unroll
   for (int i = 0; i < (D + 63) / 64; ++i) {
     const int d = lane + 64 * i;
-    if (d < D) out[d] = any ? acc[i] / l : 0.f;
+    if (d < D) out[d] = any ? (float)(acc[i] / l) : 0.f;
   }
 }
 
@@ -229,18 +233,23 @@ struct Shift {
   __device__ __forceinline__ float weights(float l) const { return I8 ? ldexp1(l, e) : l * f; }
 };
 
-// A value scale's exponent field: 126 and its log2 rounded up, at least 36, so that no
-// weight without its scale passes 2^(90 + kGrow) either (they are summed too).  A NaN
-// (a token that is not finite) outgrows everything, and counts as a scale of 0: rows that
-// see it end without a sum, and attn_row gives what the formula does.
-constexpr float kExpBias = 126.f, kExpNan = 1e9f;
-__device__ __forceinline__ float scale_field(float s) {
-  return fmaxf((float)(__float_as_uint(s) >> 23), 36.f);
+// A value scale's exponent: its log2 rounded up, + kExpBias.  Scales of 2^-90 to 2^95 count:
+// then no weight without its scale passes 2^(90 + kGrow), the largest of them (which are summed
+// too) lies above 2^-87, where 2^x still has 40 binades below it, and the weights with their
+// scales stay in range.  A scale of 0 counts as one less than the least.  A larger or smaller one,
+// or NaN (a token that is not finite), outgrows everything: rows that see it end without a sum,
+// and attn_row gives what the formula does.
+constexpr uint32_t kExpLeast = 37, kExps = 185;  // exponent fields
+constexpr float kExpBias = 126.f - kExpLeast, kExpOut = 1e37f;
+__device__ __forceinline__ uint32_t scale_field(float s) { return (__float_as_uint(s) >> 23) - kExpLeast; }
+__device__ __forceinline__ float value_exp(float s) {
+  const uint32_t e = scale_field(s);
+  return e < kExps ? (float)e : s == 0.f ? -1.f : kExpOut;
 }
 __device__ __forceinline__ float finite_scale(float s) { return fmaxf(s, 0.f); }
 
 // Scores to weights, in place: w = 2^(s c - m) (INT8: times the values' scales dv(j),
-// of exponent fields de(j)), added to l; where a weight has outgrown the reference of its
+// of exponents de(j)), added to l; where a weight has outgrown the reference of its
 // row, m is set anew and l and acc are scaled.  vis: the scores that the row sees,
 // unless `all` of the wave's rows see all of them; `top` makes a maximum that of the
 // row's lanes.
@@ -886,16 +895,18 @@ __global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn
           if (there && key < s.len && sees(a, p, key)) vis |= 1 << j;
         }
       }
-      float de[8], most_de = 0.f;
+      float de[8];
       if constexpr (I8) {
+        uint32_t most_de = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          de[j] = scale_field(dv[j >> 2][j & 3]);
-          most_de = fmaxf(most_de, de[j]);
+          const uint32_t e = scale_field(dv[j >> 2][j & 3]);
+          most_de = max(most_de, e);
+          de[j] = (float)e;
         }
-        if (__any(most_de >= 255.f))
+        if (__any(most_de >= kExps))
 #pragma unroll
-          for (int j = 0; j < 8; ++j) de[j] = dv[j >> 2][j & 3] == dv[j >> 2][j & 3] ? de[j] : kExpNan;
+          for (int j = 0; j < 8; ++j) de[j] = value_exp(dv[j >> 2][j & 3]);
       }
       float pr[8] = {sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]};
       weigh<I8>(pr, [&](int j) { return finite_scale(dv[j >> 2][j & 3]); }, [&](int j) { return de[j]; }, c, all, vis, ref,
@@ -1152,7 +1163,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
       if (I8 && threadIdx.x < 2 * kKvGroup) {
         (threadIdx.x < kKvGroup ? lds.dk : lds.dv)[buf][threadIdx.x & (kKvGroup - 1)] =
             threadIdx.x < kKvGroup ? rs : finite_scale(rs);
-        if (threadIdx.x >= kKvGroup) lds.de[buf][threadIdx.x - kKvGroup] = rs == rs ? scale_field(rs) : kExpNan;
+        if (threadIdx.x >= kKvGroup) lds.de[buf][threadIdx.x - kKvGroup] = value_exp(rs);
       }
     };
 

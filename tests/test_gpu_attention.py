@@ -192,7 +192,7 @@ def test_value_scales_far_apart(ctx, n, H, length, small, large, order):
 
 
 @pytest.mark.parametrize("n,H,length", INT8_STEPS)
-@pytest.mark.parametrize("large", [1.0, 1e20, 1e30])
+@pytest.mark.parametrize("large", [1.0, 1e20, 1e30, 1e36])
 def test_many_small_weights_beside_a_large_value(ctx, n, H, length, large):
     """INT8: one token's value decides the reference, the others' weights the denominator."""
     rng = np.random.default_rng(27)
@@ -201,6 +201,16 @@ def test_many_small_weights_beside_a_large_value(ctx, n, H, length, large):
     _, v = random_kv(rng, length, 2, 128)
     k[7], v[7] = 0, v[7] * np.float32(large)
     close_int8(ctx, k, v, np.tile(u.astype(np.float32), (n, H, 1)), n, 1.0)
+
+
+@pytest.mark.parametrize("n,H,length", INT8_STEPS)
+@pytest.mark.parametrize("low,high", [(-33, -33), (-36, -28), (31, 31), (36, 37), (-36, 37)])
+def test_values_of_any_size(ctx, n, H, length, low, high):
+    """INT8: values from next to f32's smallest to next to its largest, alone and mixed."""
+    rng = np.random.default_rng(28)
+    k, v = random_kv(rng, length, 2, 128)
+    v *= (10.0 ** rng.integers(low, high + 1, (length, 2, 1))).astype(np.float32)
+    close_int8(ctx, k, v, rng.standard_normal((n, H, 128)).astype(np.float32), n, 128 ** -0.5)
 
 
 @pytest.mark.parametrize("H", [4, 204])
