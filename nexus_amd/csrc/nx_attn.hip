@@ -248,21 +248,21 @@ __device__ __forceinline__ float value_exp(float s) {
 }
 __device__ __forceinline__ float finite_scale(float s) { return fmaxf(s, 0.f); }
 
-// Scores to weights, in place: w = 2^(s c - m) (INT8: times the values' scales dv(j),
+// Scores to weights, in place: w = 2^(s c(j) - m) (INT8: times the values' scales dv(j),
 // of exponents de(j)), added to l; where a weight has outgrown the reference of its
 // row, m is set anew and l and acc are scaled.  vis: the scores that the row sees,
 // unless `all` of the wave's rows see all of them; `top` makes a maximum that of the
 // row's lanes.
-template <bool I8, int N, typename Scale, typename Exp, typename Acc, int DT, typename Top>
-__device__ __forceinline__ void weigh(float (&w)[N], Scale dv, Exp de, float c, bool all, int vis, Ref &ref,
+template <bool I8, int N, typename Coef, typename Scale, typename Exp, typename Acc, int DT, typename Top>
+__device__ __forceinline__ void weigh(float (&w)[N], Coef c, Scale dv, Exp de, bool all, int vis, Ref &ref,
                                       float &l, Acc (&acc)[DT], Top top) {
   float sum = 0.f, most = -INFINITY;
   if (all) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = fmaf(w[j], c, -ref.m);
+    for (int j = 0; j < N; ++j) w[j] = fmaf(w[j], c(j), -ref.m);
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = (vis >> j) & 1 ? fmaf(w[j], c, -ref.m) : -INFINITY;
+    for (int j = 0; j < N; ++j) w[j] = (vis >> j) & 1 ? fmaf(w[j], c(j), -ref.m) : -INFINITY;
   }
 #pragma unroll
   for (int j = 0; j < N; ++j) most = fmaxf(most, I8 ? w[j] + de(j) : w[j]);
@@ -876,9 +876,11 @@ __global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn
           sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, qh[ks], sc[h], 0, 0, 0);
           sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, ql[ks], sc[h], 0, 0, 0);
         }
+      // (INT8: the keys' scales on the row's factor, not on sums that they could take past f32)
+      f32x4 kc[2] = {};
       if constexpr (I8) {
-        sc[0] *= dk[0];
-        sc[1] *= dk[1];
+        kc[0] = dk[0] * c;
+        kc[1] = dk[1] * c;
       }
       load_k(gr1);  // the next group's keys, while this one's weights are made
 
@@ -909,7 +911,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn
           for (int j = 0; j < 8; ++j) de[j] = value_exp(dv[j >> 2][j & 3]);
       }
       float pr[8] = {sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]};
-      weigh<I8>(pr, [&](int j) { return finite_scale(dv[j >> 2][j & 3]); }, [&](int j) { return de[j]; }, c, all, vis, ref,
+      weigh<I8>(pr, [&](int j) { return I8 ? kc[j >> 2][j & 3] : c; },
+                [&](int j) { return finite_scale(dv[j >> 2][j & 3]); }, [&](int j) { return de[j]; }, all, vis, ref,
                 l, acc, max_groups);
       f16x8 ph, pl;
       split2(pr, one, ph, pl);
@@ -1202,9 +1205,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, low(ks), sc, 0, 0, 0);
       }
       // sc[8 s + j]: token first + 16 s + 8 h + j
+      // (INT8: the keys' scales on the row's factor, as in k_attn_split)
+      float kc[16];
       if constexpr (I8) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sc[j] *= lds.dk[buf][16 * (j >> 3) + 8 * h + (j & 7)];
+        for (int j = 0; j < 16; ++j) kc[j] = lds.dk[buf][16 * (j >> 3) + 8 * h + (j & 7)] * c;
       }
       const bool all = first + kKvGroup - 1 <= pmin && first + kKvGroup <= s.len &&
                        (a.window == 0 || pmax - first < a.window || first + kKvGroup <= a.sinks);
@@ -1221,8 +1226,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_tile(KvView kv, 
 #pragma unroll
       for (int j = 0; j < 16; ++j) y[j] = sc[j];
       const int at = 8 * h;  // score j's token is at + j + 8 (j >> 3)
-      weigh<I8>(y, [&](int j) { return lds.dv[buf][at + j + (j & 8)]; },
-                [&](int j) { return lds.de[buf][at + j + (j & 8)]; }, c, all, vis, ref, l, acc, max_halves);
+      weigh<I8>(y, [&](int j) { return I8 ? kc[j] : c; },
+                [&](int j) { return lds.dv[buf][at + j + (j & 8)]; },
+                [&](int j) { return lds.de[buf][at + j + (j & 8)]; }, all, vis, ref, l, acc, max_halves);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         float pr[8];

@@ -161,7 +161,7 @@ def test_value_scales_of_all_sizes(ctx):
         cache.close()
 
 
-def close_int8(ctx, k, v, q, n, scale):
+def close_int8(ctx, k, v, q, n, scale, scores=8.0):
     """INT8 attention of the last n of the tokens k, v against its formula."""
     length, G, D = k.shape
     b = Batch(np.random.default_rng(25), [n], [length], 32)
@@ -169,7 +169,7 @@ def close_int8(ctx, k, v, q, n, scale):
     cache.write(b.whole(), b.kv_len, b.pages, k, v)
     H = q.shape[1]
     ref, bound = attention(b, stored(INT8, k), stored(INT8, v), q, H, np.float32(scale))
-    assert_close(cache.attention(*b.args(), q, H, scale=scale), ref, bound)
+    assert_close(cache.attention(*b.args(), q, H, scale=scale), ref, bound, scores)
     cache.close()
 
 
@@ -211,6 +211,17 @@ def test_values_of_any_size(ctx, n, H, length, low, high):
     k, v = random_kv(rng, length, 2, 128)
     v *= (10.0 ** rng.integers(low, high + 1, (length, 2, 1))).astype(np.float32)
     close_int8(ctx, k, v, rng.standard_normal((n, H, 128)).astype(np.float32), n, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("n,H,length", INT8_STEPS)
+def test_keys_next_to_the_largest(ctx, n, H, length):
+    """INT8: keys of 1.4e35 to 1.9e35 under queries of 2^-112: scores of -13.6 to -18.3."""
+    rng = np.random.default_rng(29)
+    u = rng.choice([-1.0, 1.0], 128)
+    _, v = random_kv(rng, length, 2, 128)
+    k = (-rng.uniform(1.4e35, 1.9e35, (length, 2, 1)) * u).astype(np.float32)
+    q = np.tile((2.0 ** -112 * u).astype(np.float32), (n, H, 1))
+    close_int8(ctx, k, v, q, n, 2.0 ** -8, scores=20)
 
 
 @pytest.mark.parametrize("H", [4, 204])
