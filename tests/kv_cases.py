@@ -106,6 +106,32 @@ def attention(batch, k, v, q, heads, scale, window=0, sinks=0):
     return out, bound
 
 
+def attention_dense(batch, k, v, q, heads, scale, window=0, sinks=0):
+    """attention(), of finite keys and values, all rows of a sequence and head at once."""
+    G, D = k.shape[1:]
+    out = np.zeros((batch.rows, heads, D))
+    bound = np.zeros_like(out)
+    at = 0
+    for s, (n, length) in enumerate(zip(batch.ns, batch.lens)):
+        rows = slice(batch.row_start[s], batch.row_start[s] + n)
+        p, j = np.arange(length - n, length)[:, None], np.arange(length)[None]
+        seen = (j <= p) & ((p - j < window) | (j < sinks) if window else True)
+        count = seen.sum(1)[:, None]
+        for h in range(heads) if n else ():
+            kg, vg = (x[at:at + length, h * G // heads].astype(np.float64) for x in (k, v))
+            qh = q[rows, h].astype(np.float64)
+            x = np.where(seen, scale * (qh @ kg.T), -np.inf)
+            mag = np.where(seen, abs(scale) * (np.abs(qh) @ np.abs(kg).T), 0).max(1, keepdims=True)
+            w = np.exp(x - x.max(1, keepdims=True))
+            total = w.sum(1, keepdims=True)
+            out[rows, h] = w @ vg / total
+            part = 4 * ((2.0 ** -21 + D * 2.0 ** -24) * mag + 2.0 ** -21) + 2 * (count + 64) * 2.0 ** -24 + 2.0 ** -21
+            top = (w * np.abs(vg).max(1)).max(1, keepdims=True)
+            bound[rows, h] = (part * (w @ np.abs(vg)) + count * 2.0 ** -33 * top) / total
+        at += length
+    return out, bound
+
+
 def assert_close(got, ref, bound, scores=8.0):
     """Within the bound per value, and as a whole as near as the roundings' root
     mean square.  For scores up to 8 that is some 2^-21 (two halves of q, eight

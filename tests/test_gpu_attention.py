@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import nexus_amd as nx
-from kv_cases import F16, INT8, Batch, assert_close, attention, random_kv, stored
+from kv_cases import F16, INT8, Batch, assert_close, attention, attention_dense, random_kv, stored
 from moe_cases import DeviceArray, assert_same_bits
 from test_gpu_kv import device_batch, ints
 
@@ -482,6 +482,44 @@ def test_many_sequences(ctx):
     ns = [int(n) for n in rng.integers(0, 3, 600)]
     lens = [n + int(x) for n, x in zip(ns, rng.integers(0, 90, 600))]
     check(ctx, F16, 2, 1, 64, 32, ns, lens)
+
+
+# Steps with more tiles than workgroups, or with more than 64 sequences: workgroups that take
+# equal runs of units, over tiles, heads and sequences.  `heads` key/value heads of narrow width,
+# and of 256 (half as many workgroups).
+RUNS = {
+    # long tiles of one sequence, the workgroup's scan over more than eight of them
+    "prompt": dict(heads=(64, 32), ns=[1040], lens=[1077]),
+    "window": dict(heads=(64, 32), ns=[1040], lens=[1500], window=100, sinks=5),
+    # up to four tiles of a sequence, a wave's plan
+    "prompts": dict(heads=(64, 32), ns=[400, 290, 3, 333], lens=[400, 500, 700, 340]),
+    # 16-row tiles
+    "decode": dict(heads=(8, 8), group=2, ns=[1 + s % 3 for s in range(40)], lens=[9 + 37 * s % 300 for s in range(40)]),
+    # more than 64 sequences, a long one among them, in both kernels
+    "many": dict(heads=(3, 3), group=2, ns=[s % 3 for s in range(70)] + [1300] + [1, 40] * 15,
+                 lens=[2 + 61 * s % 400 for s in range(70)] + [1500] + [333, 90] * 15),
+    "many-window": dict(heads=(3, 3), group=2, ns=[1] * 90 + [1300], lens=[1 + 53 * s % 500 for s in range(90)] + [1300],
+                        window=77, sinks=3),
+}
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("name", RUNS)
+def test_equal_runs(ctx, fmt, D, name):
+    print(f"runs fmt={fmt} D={D} {name}", flush=True)
+    case = dict(group=1, window=0, sinks=0) | RUNS[name]
+    G = case["heads"][D == 256]
+    H, rng = G * case["group"], np.random.default_rng([D, len(name)])
+    b = Batch(rng, case["ns"], case["lens"], 64)
+    cache, k, v = filled(ctx, rng, b, fmt, G, D)
+    q = rng.standard_normal((b.rows, H, D)).astype(np.float32)
+    seen = dict(window=case["window"], sinks=case["sinks"])
+    got = cache.attention(*b.args(), q, H, **seen)
+    ref, bound = attention_dense(b, k, v, q, H, np.float32(D ** -0.5), **seen)
+    assert_close(got, ref, bound)
+    assert_same_bits(cache.attention(*b.args(), q, H, **seen), got)
+    cache.close()
 
 
 def test_refusals(ctx):
