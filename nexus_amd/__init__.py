@@ -558,9 +558,11 @@ class KvCache:
         rs = np.ascontiguousarray(row_start, np.int32)
         ln = np.ascontiguousarray(kv_len, np.int32)
         pg = np.ascontiguousarray(pages, np.int32)
-        pg = pg.reshape(ln.size, -1)
         if rs.size != ln.size + 1:
             raise ValueError(f"{rs.size} row starts for {ln.size} sequences")
+        if pg.ndim > 2 or (pg.ndim == 2 and len(pg) != ln.size):
+            raise ValueError(f"page tables of shape {pg.shape} for {ln.size} sequences")
+        pg = pg.reshape(ln.size, -1)
         return KvBatch(ln.size, rows, pg.shape[1], rs.ctypes.data, ln.ctypes.data,
                        pg.ctypes.data), (rs, ln, pg)
 
