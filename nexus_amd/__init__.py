@@ -562,13 +562,13 @@ class KvCache:
             raise ValueError(f"{rs.size} row starts for {ln.size} sequences")
         if pg.ndim > 2 or (pg.ndim == 2 and len(pg) != ln.size):
             raise ValueError(f"page tables of shape {pg.shape} for {ln.size} sequences")
-        pg = pg.reshape(ln.size, -1)
+        pg = pg.reshape(ln.size, -1 if ln.size else 0)
         return KvBatch(ln.size, rows, pg.shape[1], rs.ctypes.data, ln.ctypes.data,
                        pg.ctypes.data), (rs, ln, pg)
 
     def _rows(self, x, width: int) -> np.ndarray:
         x = _f32(x)
-        if x.size % width:
+        if width <= 0 or x.size % width:
             raise ValueError(f"{x.size} values are no rows of {width}")
         return x.reshape(-1, width)
 
@@ -583,7 +583,7 @@ class KvCache:
 
     def read(self, row_start, kv_len, pages, rows: int | None = None):
         """The keys and values [rows x kv_heads x head_dim] of the sequences' last tokens."""
-        n = int(np.asarray(row_start).ravel()[-1]) if rows is None else rows
+        n = int(np.asarray(row_start).ravel()[-1:].sum()) if rows is None else rows
         k = np.zeros((n, self.kv_heads, self.head_dim), np.float32)
         v = np.zeros_like(k)
         b, _keep = self._host_batch(row_start, kv_len, pages, n)

@@ -244,6 +244,16 @@ def test_more_tokens_than_one_launch_takes(ctx):
     cache.close()
 
 
+def test_steps_without_sequences(ctx):
+    cache = nx.KvCache(ctx, F16, 4, 64, 2, 64)
+    none = np.zeros((0, 128), np.float32)
+    cache.write([0], [], np.zeros((0, 4)), none, none)
+    k, v = cache.read([0], [], [])
+    assert k.shape == v.shape == (0, 2, 64)
+    assert cache.attention([0], [], [], none, 4).shape == (0, 4, 64)
+    cache.close()
+
+
 def test_refusals(ctx):
     def refused(code, f, *a, **kw):
         with pytest.raises(nx.NexusError) as e:
