@@ -4,7 +4,6 @@
 // device knows.
 #pragma once
 
-#include <new>
 #include <type_traits>
 
 #include "nx_device.hpp"
@@ -157,18 +156,6 @@ void with_kernel(const nx_kv *kv, F f) {
 
 template <int FMT>
 using kv_elem = std::conditional_t<FMT == NX_KV_INT8, int8_t, _Float16>;
-
-// A C entry's body: no exception leaves it (what they do on the host allocates).
-template <typename F>
-int guarded(F f) {
-  try {
-    return f();
-  } catch (const std::bad_alloc &) {
-    return NX_ERR_OOM;
-  } catch (...) {
-    return NX_ERR_DEVICE;
-  }
-}
 
 inline int refuse(const Refusal &r) { return r ? fail(r.code, r.why) : NX_OK; }
 

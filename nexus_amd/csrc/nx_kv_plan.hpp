@@ -9,12 +9,28 @@
 #include <cmath>
 #include <cstddef>
 #include <cstdint>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "../../include/nexus_hip.h"
 
 namespace nx {
+
+int fail(int code, const std::string &msg);
+
+// A C entry's body: no exception leaves it (what they do on the host allocates).  The messages
+// are short enough for a string to hold without memory of its own.
+template <typename F>
+int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc &) {
+    return fail(NX_ERR_OOM, "out of memory");
+  } catch (...) {
+    return fail(NX_ERR_DEVICE, "internal error");
+  }
+}
 
 // A page holds, for each kv head, page_tokens / 32 groups of 32 tokens.  A
 // group's keys and values lie in the order in which the matrix cores take them
