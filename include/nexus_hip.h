@@ -284,8 +284,9 @@ int nx_kv_destroy(nx_kv *kv);
  * the others.  *_dev calls cannot refuse what the arrays hold: there, tokens
  * before the first one, behind max_pages pages or on a page that the cache does
  * not have are not written, not attended to and read as zeros, and row ranges are
- * cut to num_tokens.  Sequences that share rows, or that write one token's
- * place, get the values of either. */
+ * cut to num_tokens.  Sequences that write one token's place get the values of
+ * either.  A row_start that decreases (sequences that share rows) touches no memory
+ * but the batch's, but which of its tokens are written or read is not defined. */
 typedef struct nx_kv_batch {
   int num_seqs;
   int num_tokens;           /* rows of the call's buffers */
@@ -331,9 +332,10 @@ int nx_kv_read_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float
  * Rows that the matrix products cannot give are done one by one, by the formula alone: those
  * that see an infinity, a NaN or (NX_KV_INT8) a value scale other than 0 outside 2^-90 .. 2^95,
  * and (NX_KV_F16) those with an infinity or NaN in a place that they do not see but whose 32
- * tokens they read: later tokens of a chunk, tokens beside a window's edge, and what earlier
- * owners of a page left behind a sequence's last token.  That is right but slow (one token
- * after 100001, 32 heads over 8 of 128: 45 ms, not 81 us), so write something finite there.
+ * tokens they read: later tokens of a chunk, tokens beside a window's edge, what earlier
+ * owners of a page left behind a sequence's last token, and the cache's first 32 tokens in
+ * place of a page that it does not have.  That is right but slow (one token after 100001, 32
+ * heads over 8 of 128: 45 ms, not 81 us), so write something finite there.
  * The workspace (some 77 MB) is the context's, allocated with the first cache or
  * call on it and never moved, so a captured call may be replayed while the context
  * lives; calls on one context must not overlap in time (two graphs captured from

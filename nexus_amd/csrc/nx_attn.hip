@@ -1009,9 +1009,10 @@ __global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn
 // of them).  Bound by the wave's own alternation: its scores, then maximum, exponentials and
 // halves (F16 134, INT8 220 vector instructions for 32 matrix ones of a group), then its
 // values; the CU's other workgroup fills the gaps, and the matrix cores are busy 43% of the
-// time at about 2 GHz.  32 heads over 8 of 128, F16: a prompt of 4093 tokens 300-310 us, 440-457
-// TFLOP/s with the halves counted once; 2039 tokens through a window of 4096 274 us, 500.
-// INT8, 32 heads over 4, two chunks of 509 tokens at up to 16127: 460-470 us, 455-465.  Scores
+// time at about 2 GHz.  Over cards, 32 heads over 8 of 128, F16: a prompt of 4093 tokens 297-319
+// us, 430-462 TFLOP/s with the halves counted once; 2039 tokens through a window of 4096
+// 272-291 us, 471-504 (INT8 307, 447).  INT8, 32 heads over 4, two chunks of 509 tokens at up to
+// 16127: 458-480 us, 446-467.  Scores
 // of the next group ahead of this one's weights, with q's lower halves in LDS to make room:
 // 346 us for the prompt, against 314.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -1345,6 +1346,9 @@ constexpr int tile_from(int fmt) { return kTile * (fmt == NX_KV_INT8 ? 3 : 2); }
 // sum up the lengths (1024 rows over 1024 tokens 19 us, not 14; 4096 18, not 32), but for the
 // rows of an eighth of the CUs: 512 over 1024, 16384, 65536 and 131072 tokens take k_attn_split
 // 14, 25, 60 and 113 us (INT8 16, 29, 75, 132) and k_attn_tile 25, 37, 64 and 100 (26, 39, 65, 99).
+// (So those few rows lose 15 to 33% over INT8 contexts of 65536 tokens and more, and F16 ones of
+// 131072 13%: the host knows the table's width, not the lengths, and a step behind a wide table
+// that is short would pay some 5 us for the second kernel.)
 constexpr long kFewScores = 40'000'000;  // rows times keys
 
 static int attn_wgs_log2(const nx_ctx *c) { return std::max(4, 31 - __builtin_clz(c->num_cu * kAttnWgsPerCu)); }

@@ -7,10 +7,13 @@
 // 16-byte runs.
 //
 // Four waves have the keys and four the values, and each side waits for its own rows only
-// (all for one, then all for the other: 46 us against 42 below).  INT8, 4 heads of 128, two
-// sequences with 8191 new tokens each: 84 MB written in 19 us and read in 16, 4.4
-// and 5.4 TB/s; a large copy reaches 4.7.  61 single tokens on 8 heads take 6.7 and 4.5 us,
-// one 3.3 and 3.5: launches and two round trips.
+// (all for one, then all for the other: 46 us against 42 below).  4 heads of 128, two
+// sequences with 8191 new tokens each: INT8 84 MB written in 19 us and read in 15.5, 4.4
+// and 5.5 TB/s; F16 101 MB in 17.8 and 17.1, 5.6 and 5.9 (one after the other, out of the
+// caches in part); a large copy reaches 4.7.  Single tokens on 8 heads are launches and two
+// round trips: F16, one 3.3 us written and 3.6 read, 61 of them 3.9 and 4.4; INT8, one 5.4 and
+// 3.6, 61 of them 6.6 and 4.4.  INT8 writes take 2 to 3 us more: a row's maximum over its
+// lanes, the division, and values that leave as single bytes.
 #include <hip/hip_runtime.h>
 
 #include "nx_kv_dev.hpp"
