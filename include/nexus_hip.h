@@ -249,7 +249,7 @@ int nx_matvec_dev(nx_ctx *ctx, const nx_matrix *m, const float *d_x, size_t x_le
 
 /* ---------------------------------------------------------------- key/value cache */
 /* formats of a cache's values */
-#define NX_KV_F16 0  /* IEEE half, rounded to nearest even */
+#define NX_KV_F16 0  /* IEEE half, rounded to nearest even (from 65520 on: infinite) */
 #define NX_KV_INT8 1 /* 8-bit codes with one f32 scale per token and head (keys and values
                         apart): scale = max |x| / 127 in f32, code = x / scale (the exact
                         quotient) rounded to nearest, ties to even, within +-127; read back as the f32
@@ -324,7 +324,8 @@ int nx_kv_read_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, float
  * floats apart, out rows likewise; neither needs an alignment, and out must not
  * overlap q.  f32 in and out: scores, softmax and sums are held in f32, and the f32 factors of the
  * f16 matrix products are split into two halves (relative error about 1e-6
- * against the same cache in 64 bits).  A row's last bits depend on the batch
+ * against the same cache in 64 bits, 3e-6 for NX_KV_INT8 values far from 1: scales of
+ * 2^-55 and less or 2^55 and more).  A row's last bits depend on the batch
  * that it is in, the width of its table among it (the order of the sums does), not on the
  * run.
  * attention_decode (src/engine/mod.rs:452-500) and

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 import nexus_amd as nx
-from kv_cases import F16, INT8, Batch, assert_close, attention, attention_dense, random_kv, stored
+from kv_cases import F16, INT8, Batch, assert_close, attention, random_kv, stored
+from kv_cases import attention_dense
 from moe_cases import DeviceArray, assert_same_bits
 from test_gpu_kv import device_batch, ints
 
