@@ -52,6 +52,11 @@
  *       InferenceEngine::attention_decode    src/engine/mod.rs:452-500
  *       kernel::grouped_query_attention      src/kernel/mod.rs:40-99
  *       causal, for any new tokens of each sequence; with a window, too
+ *   nx_qk_rope / nx_qk_rope_dev
+ *       kernel::rope_single                  src/kernel/mod.rs:258-271
+ *       for every head and token of a step, behind a norm of the head
+ *   nx_logprobs / nx_logprobs_dev
+ *       no counterpart; beside InferenceEngine::sample_token  src/engine/mod.rs:819
  *   nx_device_count / nx_ctx_* / nx_sync / nx_mem_info
  *       Backend::{is_available, memory_info, synchronize}
  *                                            src/backend/mod.rs:74-96
@@ -348,6 +353,68 @@ int nx_attention(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const f
 int nx_attention_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *d_q,
                      size_t q_stride, int heads, float scale, int window, int sinks, float *d_out,
                      size_t out_stride);
+
+/* ---------------------------------------------------------------- norm and rotation of heads */
+/* which elements of a head's first rotary_dim make pair i of them */
+#define NX_ROPE_HALVES 0 /* i and i + rotary_dim / 2 */
+#define NX_ROPE_PAIRS 1  /* 2 i and 2 i + 1 */
+
+/* How a model norms and rotates its query and key heads.  The struct is host memory, read
+ * during the call; its arrays are device memory for *_dev calls, host memory for the others. */
+typedef struct nx_rope {
+  int head_dim;   /* even, up to 512 */
+  int rotary_dim; /* even, 0 .. head_dim: so many of a head's first elements are rotated */
+  int style;      /* NX_ROPE_HALVES or NX_ROPE_PAIRS */
+  float eps;
+  const float *freq;   /* [rotary_dim / 2] the angle, in radians, of one position: base^(-2 i /
+                          rotary_dim), or as a model with a longer context scales it */
+  const float *q_norm; /* [head_dim] the norm's weights, the same for every query head; null: */
+  const float *k_norm; /* no norm.  And those of the key heads. */
+} nx_rope;
+
+/* Every head x of a step's rows, normed (nx_rms_norm's formula on the head alone),
+ *   y = x / sqrt(sum_i x_i^2 / head_dim + eps) * weight,
+ * and its pairs turned by the angle t = position * freq_i of its row's token,
+ *   (a, b) -> (a cos t - b sin t, a sin t + b cos t);
+ * elements from rotary_dim on keep y.  For rows r < num_tokens: `heads` query heads at
+ * q + r * q_stride and `kv_heads` key heads at k + r * k_stride, to q_out and k_out likewise
+ * (strides in floats).  An output may be its own input, with its stride; any other overlap is
+ * refused.  heads or kv_heads may be 0.  positions[r] may be any number: a sequence that gave
+ * tokens up (nx_kv_evict) keeps the positions that it counts.  f32 in and out, the sum of squares
+ * and the angle in 64 bits: within 2^-20 of the head's largest normed value, at any position.  kernel::rope_single (src/kernel/mod.rs:258-271), and kernel::rms_norm
+ * (src/kernel/mod.rs:199-209) on each head. */
+int nx_qk_rope(nx_ctx *ctx, const nx_rope *rope, const int32_t *positions, int num_tokens, int heads,
+               int kv_heads, const float *q, size_t q_stride, const float *k, size_t k_stride, float *q_out,
+               size_t q_out_stride, float *k_out, size_t k_out_stride);
+int nx_qk_rope_dev(nx_ctx *ctx, const nx_rope *rope, const int32_t *d_positions, int num_tokens, int heads,
+                   int kv_heads, const float *d_q, size_t q_stride, const float *d_k, size_t k_stride,
+                   float *d_q_out, size_t q_out_stride, float *d_k_out, size_t k_out_stride);
+
+/* ---------------------------------------------------------------- log probabilities */
+/* What rows of logits (an output head's nx_matvec) say.  Row r has `vocab` logits x at
+ * logits + r * stride (floats); with l = log sum_j exp(x_j),
+ *   logprobs[r * given + i] = x_t - l     for t = tokens[r * given + i]
+ *   entropy[r]              = -sum_j p_j log p_j,  p_j = exp(x_j - l)
+ *   top_ids, top_logprobs [r * top + i]:  the `top` (up to 64) likeliest tokens, the likeliest
+ *                             first, of equal ones the lower id first, and their log probabilities.
+ * given and top may be 0, and entropy null: not asked for.  A logit of -infinity is a token that
+ * a mask has taken out: its log probability is -infinity and it is no alternative; where there are
+ * fewer than `top` others, id -1 and -infinity fill the row up.  A row in which every token
+ * is taken out has entropy 0.  (A mask of the type's lowest finite value is a logit like any
+ * other.)  A row with a NaN or +infinity has NaNs for entropy and log probabilities, but for
+ * the -infinity of filled-up places; its alternatives are those by value, NaNs left out.  A token
+ * that is not 0 .. vocab - 1 names none: its log probability is 0.  Accuracy: entropy and log
+ * probabilities within 2^-20 (1 + |value| + the spread of the likely logits).  Outputs must
+ * not overlap inputs.  The library's workspace for few long rows (2 MB) is the context's, as the
+ * attention's: a context's first call with fewer than 2048 rows is refused while its stream is
+ * captured, and calls on one context must not overlap in time.  Sampling's softmax over the
+ * logits (src/engine/mod.rs:819), for the tokens that were chosen. */
+int nx_logprobs(nx_ctx *ctx, const float *logits, size_t stride, int num_tokens, int vocab,
+                const int32_t *tokens, int given, float *logprobs, float *entropy, int top,
+                int32_t *top_ids, float *top_logprobs);
+int nx_logprobs_dev(nx_ctx *ctx, const float *d_logits, size_t stride, int num_tokens, int vocab,
+                    const int32_t *d_tokens, int given, float *d_logprobs, float *d_entropy, int top,
+                    int32_t *d_top_ids, float *d_top_logprobs);
 
 /* ---------------------------------------------------------------- GGUF */
 typedef struct nx_gguf nx_gguf;

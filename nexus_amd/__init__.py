@@ -31,6 +31,7 @@ PATH_AUTO, PATH_GEMV, PATH_MFMA_F16, PATH_MFMA_BF16, PATH_MFMA_SPLIT = 0, 1, 2, 
 ROLE_GATE, ROLE_UP, ROLE_DOWN = 0, 1, 2
 EXPERT_SHARED = -1
 KV_F16, KV_INT8 = 0, 1
+ROPE_HALVES, ROPE_PAIRS = 0, 1
 FORMAT_NAMES = {F32: "F32", Q4_0: "Q4_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q2_K: "Q2_K", F16: "F16",
                 BF16: "BF16"}
 BLOCK = {Q4_0: (32, 18), Q8_0: (32, 34), Q4_K: (256, 144), Q2_K: (256, 84), F32: (1, 4),
@@ -53,6 +54,7 @@ EXPORTS = [
     "nx_matrix_load_gguf", "nx_moe_last_routes", "nx_moe_forward_noalloc",
     "nx_kv_create", "nx_kv_info", "nx_kv_destroy", "nx_kv_write", "nx_kv_write_dev",
     "nx_kv_read", "nx_kv_read_dev", "nx_attention", "nx_attention_dev",
+    "nx_qk_rope", "nx_qk_rope_dev", "nx_logprobs", "nx_logprobs_dev",
 ]
 
 _lib = None
@@ -65,6 +67,11 @@ _ip = C.POINTER(C.c_int)
 class _KvBatch(C.Structure):
     _fields_ = [("num_seqs", C.c_int), ("num_tokens", C.c_int), ("max_pages", C.c_int),
                 ("row_start", _vp), ("kv_len", _vp), ("pages", _vp)]
+
+
+class _Rope(C.Structure):
+    _fields_ = [("head_dim", C.c_int), ("rotary_dim", C.c_int), ("style", C.c_int),
+                ("eps", C.c_float), ("freq", _vp), ("q_norm", _vp), ("k_norm", _vp)]
 
 
 class NexusError(RuntimeError):
@@ -172,6 +179,12 @@ def lib():
         "nx_kv_write": (rows, C.c_int), "nx_kv_write_dev": (rows, C.c_int),
         "nx_kv_read": (rows, C.c_int), "nx_kv_read_dev": (rows, C.c_int),
         "nx_attention": (attention, C.c_int), "nx_attention_dev": (attention, C.c_int),
+    })
+    rope = [_vp, C.POINTER(_Rope), _vp, C.c_int, C.c_int, C.c_int] + [_vp, C.c_size_t] * 4
+    logprobs = [_vp, _vp, C.c_size_t, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, C.c_int, _vp, _vp]
+    sig.update({
+        "nx_qk_rope": (rope, C.c_int), "nx_qk_rope_dev": (rope, C.c_int),
+        "nx_logprobs": (logprobs, C.c_int), "nx_logprobs_dev": (logprobs, C.c_int),
     })
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -331,6 +344,67 @@ class Context:
         """nx_rms_norm_dev on device pointers (enqueued on the context's stream)."""
         check(lib().nx_rms_norm_dev(self.h, _vp(x_ptr), x_len, _vp(w_ptr), w_len, eps,
                                     num_tokens, hidden, 1 if exact else 0, _vp(out_ptr)))
+
+    # ----------------------------------------------------------- heads
+    def qk_rope(self, positions, q, k, freq, style: int = ROPE_HALVES, q_norm=None, k_norm=None,
+                eps: float = 1e-6):
+        """Query heads [T x heads x D] and key heads [T x kv_heads x D] (either None: none),
+        normed where weights [D] are given and rotated by their tokens' positions [T] with the
+        angles freq [rotary / 2] of one position."""
+        pos = np.ascontiguousarray(positions, np.int32).ravel()
+        x = [np.zeros((pos.size, 0, 0), np.float32) if a is None else _f32(a) for a in (q, k)]
+        dims = {a.shape[2] for a in x if a.ndim == 3 and a.shape[1]}
+        if any(a.ndim != 3 or len(a) != pos.size for a in x) or len(dims) > 1:
+            raise ValueError(f"heads of shapes {x[0].shape} and {x[1].shape} for {pos.size} positions")
+        D = dims.pop() if dims else 2
+        norms = [None if w is None else _f32(w).ravel() for w in (q_norm, k_norm)]
+        if any(w is not None and w.size != D for w in norms):
+            raise ValueError(f"a norm's weights are not {D}")
+        freq = _f32(freq).ravel()
+        rope = Rope(D, 2 * freq.size, freq.ctypes.data, style,
+                    *(0 if w is None else w.ctypes.data for w in norms), eps=eps)
+        out, args = [np.empty_like(a) for a in x], []
+        for a in x + out:
+            args += [a.ctypes.data, a.shape[1] * a.shape[2]]
+        check(lib().nx_qk_rope(self.h, rope.ref, pos.ctypes.data, pos.size, x[0].shape[1], x[1].shape[1],
+                               *args))
+        return out[0], out[1]
+
+    def qk_rope_dev(self, rope: Rope, positions_ptr: int, num_tokens: int, heads: int, kv_heads: int,
+                    q_ptr: int, q_stride: int, k_ptr: int, k_stride: int, q_out_ptr: int,
+                    q_out_stride: int, k_out_ptr: int, k_out_stride: int):
+        """nx_qk_rope_dev on device pointers (enqueued on the context's stream); an output may be
+        its own input."""
+        check(lib().nx_qk_rope_dev(self.h, rope.ref, positions_ptr, num_tokens, heads, kv_heads, q_ptr,
+                                   q_stride, k_ptr, k_stride, q_out_ptr, q_out_stride, k_out_ptr,
+                                   k_out_stride))
+
+    # ----------------------------------------------------------- log probabilities
+    def logprobs(self, logits, tokens=None, top: int = 0):
+        """Of rows of logits [T x vocab]: the log probabilities [T x n] of tokens [T x n], the
+        entropy [T], and the ids and log probabilities [T x top] of the likeliest tokens."""
+        x = _f32(logits)
+        if x.ndim != 2 or not x.shape[1]:
+            raise ValueError(f"logits of shape {x.shape}")
+        T, V = x.shape
+        ids = np.zeros((T, 0), np.int32) if tokens is None else np.ascontiguousarray(tokens, np.int32)
+        if ids.ndim != 2 or len(ids) != T:
+            raise ValueError(f"tokens of shape {ids.shape} for {T} rows")
+        if top < 0:
+            raise ValueError("negative number of alternatives")
+        lp, ent = np.empty(ids.shape, np.float32), np.empty(T, np.float32)
+        top_ids, top_lp = np.empty((T, top), np.int32), np.empty((T, top), np.float32)
+        check(lib().nx_logprobs(self.h, x.ctypes.data, V, T, V, ids.ctypes.data, ids.shape[1],
+                                lp.ctypes.data, ent.ctypes.data, top, top_ids.ctypes.data,
+                                top_lp.ctypes.data))
+        return lp, ent, top_ids, top_lp
+
+    def logprobs_dev(self, logits_ptr: int, stride: int, num_tokens: int, vocab: int, tokens_ptr: int,
+                     given: int, logprobs_ptr: int, entropy_ptr: int, top: int, top_ids_ptr: int,
+                     top_logprobs_ptr: int):
+        """nx_logprobs_dev on device pointers (enqueued on the context's stream)."""
+        check(lib().nx_logprobs_dev(self.h, logits_ptr, stride, num_tokens, vocab, tokens_ptr, given,
+                                    logprobs_ptr, entropy_ptr, top, top_ids_ptr, top_logprobs_ptr))
 
     def route_topk(self, logits, num_tokens: int, num_experts: int, top_k: int,
                    score_mode: int = SCORE_SOFTMAX):
@@ -510,6 +584,17 @@ class Matrix:
             self.close()
         except Exception:
             pass
+
+
+class Rope:
+    """How a model norms and rotates its heads (nx_rope), by the addresses of f32 arrays: the
+    angles freq [rotary_dim / 2] of one position, and the norms' weights [head_dim] (0: no
+    norm).  The arrays must outlive the descriptor's use."""
+
+    def __init__(self, head_dim: int, rotary_dim: int, freq_ptr: int, style: int = ROPE_HALVES,
+                 q_norm_ptr: int = 0, k_norm_ptr: int = 0, eps: float = 1e-6):
+        self.c = _Rope(head_dim, rotary_dim, style, eps, freq_ptr, q_norm_ptr, k_norm_ptr)
+        self.ref = C.byref(self.c)
 
 
 class KvBatch:

@@ -604,14 +604,6 @@ __device__ __forceinline__ void finish_rows(const KvView &kv, const nx_kv_batch 
   }
 }
 
-// Memory that workgroups of one kernel pass on, on any XCD: each has an L2 of its own,
-// so these stores write through it and these loads go past it (device-scope atomics,
-// relaxed).  A device-wide fence instead writes back everything that the L2 holds:
-// with one per workgroup a decode batch took 442 us, not 233.
-template <typename T>
-__device__ __forceinline__ void store_through(T *p, T v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 __device__ __forceinline__ void store_through(float *p, f32x4 v) {
   const auto w = __builtin_bit_cast(ulong2, v);
   store_through(reinterpret_cast<unsigned long *>(p), w.x);
@@ -629,9 +621,6 @@ __device__ __forceinline__ f32x4 load4(const float *p) {
                     __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)};
   return __builtin_bit_cast(f32x4, w);
 }
-// waits until this wave's stores are where they go
-__device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 constexpr int kTile = 16, kRows = 128;  // rows of a tile of k_attn_split, k_attn_tile
 
 template <int D, int NW>

@@ -1,0 +1,402 @@
+// nx_logprobs.hip — log probabilities, entropy and the likeliest tokens of rows of logits.
+//
+//   l = m + log sum_j e^(x_j - m),   entropy = log S - W / S,  S = sum_j e^(x_j - m),
+//   W = sum_j e^(x_j - m) (x_j - m),
+// with the running maximum m of what was read: one pass over the logits, which memory bounds.
+// Where few rows do not fill the card, several workgroups share a row, and the last of them to
+// end puts their sums together in the order of the parts.
+//
+// The likeliest tokens in the same pass: a wave keeps those that passed a threshold in LDS, as
+// keys (value, then lower id first) that are all distinct.  When the list is full, the `top`
+// largest stay and the least of them is the threshold from then on, so most steps pass nothing
+// and cost one comparison with their maximum.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "nx_device.hpp"
+#include "nx_internal.hpp"
+#include "nx_kv_dev.hpp"
+#include "nx_step_plan.hpp"
+
+namespace nx {
+
+struct LogprobCall {
+  const float *x;
+  size_t stride;
+  const int32_t *tokens;
+  float *logprobs, *entropy, *top_logprobs;
+  int32_t *top_ids;
+  int first;  // the launch's first row
+  int vocab, given, top;
+  RowSplit split;
+  int *done;       // [rows] parts that are written, 0 between calls
+  uint64_t *part;  // [rows][parts] records
+};
+
+constexpr int kLogprobWaves = 4, kLogprobThreads = 64 * kLogprobWaves;
+constexpr int kHeld = 512;               // keys of a wave's list
+constexpr int kAhead = 4;                // steps on their way
+constexpr int kRecord = 2 + kMaxTop;     // of a part: {m, S}, {W, 0}, its keys
+constexpr float kLowest = -3.4028234663852886e38f, kLog2e1 = 1.4426950408889634f;
+
+// orders as the value, then by the lower id; above 0 for anything but NaNs
+__device__ __forceinline__ uint64_t key_of(float x, int id) {
+  const uint32_t b = __float_as_uint(x + 0.f);  // (-0 is 0)
+  return (uint64_t)(b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u)) << 32 | (uint32_t)~id;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t b = (uint32_t)(key >> 32);
+  return __uint_as_float(b ^ ((int)b < 0 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ int id_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+__device__ __forceinline__ int lanes_before(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// Leaves the k largest of a wave's n <= 64 R keys (0: none) in its list, in no order; the
+// largest t that k keys reach, bit by bit.  The least key's value, -infinity where there are
+// not more than k.
+template <int R>
+__device__ __forceinline__ float keep_top(uint64_t *list, int &n, int k) {
+  const int lane = threadIdx.x & 63;
+  if (n <= k) return -INFINITY;
+  wave_handoff();
+  uint64_t key[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) key[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0;
+  uint64_t t = 0;
+  int reach = n;
+  for (int bit = 63; bit >= 0 && reach != k; --bit) {
+    const uint64_t with = t | (uint64_t)1 << bit;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) count += __popcll(__ballot(key[i] >= with));
+    if (count < k) continue;
+    t = with;
+    reach = count;
+  }
+  wave_handoff();
+  int at = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const bool stays = key[i] >= t && key[i] != 0;
+    const uint64_t mask = __ballot(stays);
+    if (stays) list[at + lanes_before(mask)] = key[i];
+    at += __popcll(mask);
+  }
+  wave_handoff();
+  n = at;
+  if (n < k) return -INFINITY;  // (keys of none among them)
+  // the least key's high word: all of the kept reach t, and t's value is at most theirs
+  uint32_t least = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < R; ++i) least = key[i] >= t ? min(least, (uint32_t)(key[i] >> 32)) : least;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
+  return value_of((uint64_t)least << 32);
+}
+
+struct Sums {
+  float m, s, w;
+};
+// w's terms e (x - m), where e is 0 and x - m may be infinite
+__device__ __forceinline__ float far(float d) { return fmaxf(d, -1e4f); }
+__device__ __forceinline__ Sums joined(const Sums &a, const Sums &b) {
+  const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m;
+  const float fa = __builtin_amdgcn_exp2f(da * kLog2e1), fb = __builtin_amdgcn_exp2f(db * kLog2e1);
+  return {m, a.s * fa + b.s * fb, (a.w + far(da) * a.s) * fa + (b.w + far(db) * b.s) * fb};
+}
+__device__ __forceinline__ Sums across(Sums a) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1)
+    a = joined(a, {__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64), __shfl_xor(a.w, d, 64)});
+  return a;
+}
+template <int N>
+__device__ __forceinline__ void add(Sums &a, const float (&x)[N], float most) {
+  const float m = fmaxf(a.m, most), d = a.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e1);
+  a.w = (a.w + far(d) * a.s) * f;
+  a.s *= f;
+  a.m = m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = x[i] - m, e = __builtin_amdgcn_exp2f(y * kLog2e1);
+    a.s += e;
+    a.w = fmaf(e, far(y), a.w);
+  }
+}
+
+// A wave's list of the likeliest so far.
+struct List {
+  uint64_t *keys;
+  int n, top;
+  float least;  // what a logit has to pass
+  // N of each lane, of ids that all come behind those taken so far
+  template <int N, typename Id>
+  __device__ __forceinline__ void take(const float (&x)[N], float most, Id id) {
+    if (!__any(most > least)) return;
+    uint64_t mask[N];
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) count += __popcll(__ballot(x[i] > least));
+    if (n + count > kHeld) least = keep_top<kHeld / 64>(keys, n, top);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      mask[i] = __ballot(x[i] > least);
+      if (x[i] > least) keys[n + lanes_before(mask[i])] = key_of(x[i], id(i));
+      n += __popcll(mask[i]);
+    }
+  }
+};
+
+struct RowLds {
+  uint64_t keys[kLogprobWaves][kHeld];
+  uint64_t best[kLogprobWaves * kMaxTop];
+  Sums sums[kLogprobWaves];
+  bool last;
+};
+
+// the workgroup's sums, in all of its threads, and its top keys (or none) in best[0 .. top)
+__device__ __forceinline__ Sums gather(RowLds &lds, Sums mine, List &list, int top) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  mine = across(mine);
+  if (lane == 0) lds.sums[wave] = mine;
+  if (top > 0) {
+    keep_top<kHeld / 64>(list.keys, list.n, top);
+    wave_handoff();
+    if (lane < top) lds.best[wave * top + lane] = lane < list.n ? list.keys[lane] : 0;
+  }
+  __syncthreads();
+  Sums all = lds.sums[0];
+#pragma unroll
+  for (int i = 1; i < kLogprobWaves; ++i) all = joined(all, lds.sums[i]);
+  if (top > 0 && wave == 0) {
+    int n = kLogprobWaves * top;
+    keep_top<kMaxTop * kLogprobWaves / 64>(lds.best, n, top);
+    if (lane >= n && lane < top) lds.best[lane] = 0;
+  }
+  __syncthreads();
+  return all;
+}
+
+__device__ __forceinline__ void write_row(const LogprobCall &a, size_t row, const Sums &all, RowLds &lds) {
+  const float *x = a.x + row * a.stride, total = logf(all.s);
+  auto logprob = [&](float v) {  // (nothing is likely in a row of masked tokens)
+    return all.s == 0.f || v == -INFINITY ? (all.s == all.s ? -INFINITY : NAN) : v - all.m - total;
+  };
+  if (threadIdx.x == 0 && a.entropy) {
+    const float e = total - all.w / all.s;
+    a.entropy[row] = all.s == 0.f || e < 0.f ? 0.f : e;
+  }
+  for (int i = threadIdx.x; i < a.given; i += kLogprobThreads) {
+    const int id = a.tokens[row * a.given + i];
+    a.logprobs[row * a.given + i] = id >= 0 && id < a.vocab ? logprob(x[id]) : 0.f;
+  }
+  if (a.top == 0 || threadIdx.x >= 64) return;
+  const int lane = threadIdx.x;
+  uint64_t key = lane < a.top ? lds.best[lane] : 0;
+  // the largest first (a bitonic sort of the lanes that have any)
+  for (int size = 2; size < 2 * a.top; size <<= 1)
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      const uint64_t other = __shfl_xor((unsigned long long)key, d, 64);
+      const bool larger = ((lane & d) == 0) == ((lane & size) == 0);
+      key = larger == (key > other) ? key : other;
+    }
+  if (lane < a.top) {
+    a.top_ids[row * a.top + lane] = key ? id_of(key) : -1;
+    a.top_logprobs[row * a.top + lane] = key ? logprob(value_of(key)) : -INFINITY;
+  }
+}
+
+__global__ __launch_bounds__(kLogprobThreads) void k_logprobs(LogprobCall a) {
+  __shared__ RowLds lds;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int parts = a.split.parts, part = blockIdx.x % parts;
+  const size_t row = a.first + blockIdx.x / parts;
+  const float *x = a.x + row * a.stride;
+  // the part's logits [lo, hi): any in front of a 16-byte boundary, whole float4, and a rest
+  const int front = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) / 4 & 3), a.vocab);
+  const int whole = (a.vocab - front) / 4, rest = front + 4 * whole;
+  const int lo = min(part * (a.split.share / 4), whole);
+  const int hi = part + 1 == parts ? whole : min(lo + a.split.share / 4, whole);
+  const float4 *x4 = reinterpret_cast<const float4 *>(x + front);
+
+  Sums sums{kLowest, 0.f, 0.f};
+  List list{lds.keys[wave], 0, a.top, -INFINITY};
+  auto single = [&](int from, int to) {  // a few logits, one of each lane
+    const int i = from + lane;
+    const float v[1] = {i < to ? x[i] : -INFINITY};
+    add(sums, v, v[0]);
+    if (a.top > 0) list.take(v, v[0], [&](int) { return i; });
+  };
+  if (part == 0 && wave == 0 && front > 0) single(0, front);
+  constexpr float4 kNone = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  float4 next[kAhead];
+  auto fetch = [&](int at) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = at + j * kLogprobThreads + (int)threadIdx.x;
+      next[j] = i < hi ? x4[i] : kNone;
+    }
+  };
+  fetch(lo);
+  for (int at = lo; at < hi; at += kAhead * kLogprobThreads) {
+    float v[4 * kAhead], most[kAhead], all = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      v[4 * j] = next[j].x, v[4 * j + 1] = next[j].y, v[4 * j + 2] = next[j].z, v[4 * j + 3] = next[j].w;
+      most[j] = fmaxf(fmaxf(next[j].x, next[j].y), fmaxf(next[j].z, next[j].w));
+      all = fmaxf(all, most[j]);
+    }
+    fetch(at + kAhead * kLogprobThreads);
+    add(sums, v, all);
+    if (a.top > 0 && __any(all > list.least)) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float u[4] = {v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
+        const int id = front + 4 * (at + j * kLogprobThreads + (int)threadIdx.x);
+        list.take(u, most[j], [&](int i) { return id + i; });
+      }
+    }
+  }
+  if (part + 1 == parts && wave == 0 && rest < a.vocab) single(rest, a.vocab);
+  Sums all = gather(lds, sums, list, a.top);
+
+  if (parts > 1) {
+    const size_t local = blockIdx.x / parts;
+    uint64_t *record = a.part + (local * parts + part) * kRecord;
+    auto pack = [](float p, float q) { return (uint64_t)__float_as_uint(q) << 32 | __float_as_uint(p); };
+    if (threadIdx.x == 0) {
+      store_through(record, pack(all.m, all.s));
+      store_through(record + 1, pack(all.w, 0.f));
+    }
+    if ((int)threadIdx.x < a.top) store_through(record + 2 + threadIdx.x, lds.best[threadIdx.x]);
+    stores_done();  // this part, before the count says so
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      lds.last = atomicAdd(&a.done[local], 1) == parts - 1;
+      if (lds.last) a.done[local] = 0;  // for the next call
+    }
+    __syncthreads();
+    if (!lds.last) return;
+    // a part to each lane for the sums; to each wave in turn for its keys
+    sums = {kLowest, 0.f, 0.f};
+    const uint64_t *first = a.part + local * parts * kRecord;
+    if ((int)threadIdx.x < parts) {
+      const uint64_t ms = load_past(first + threadIdx.x * kRecord), w = load_past(first + threadIdx.x * kRecord + 1);
+      sums = {__uint_as_float((uint32_t)ms), __uint_as_float((uint32_t)(ms >> 32)), __uint_as_float((uint32_t)w)};
+    }
+    list.n = 0;
+    list.least = -INFINITY;
+    for (int i0 = wave * 64; i0 < parts * a.top; i0 += kLogprobThreads) {
+      const int i = i0 + lane, p = i / a.top;
+      const uint64_t key = p < parts ? load_past(first + p * kRecord + 2 + (i - p * a.top)) : 0;
+      const uint64_t mask = __ballot(key != 0);
+      if (list.n + 64 > kHeld) keep_top<kHeld / 64>(list.keys, list.n, a.top);
+      if (key) list.keys[list.n + lanes_before(mask)] = key;
+      list.n += __popcll(mask);
+    }
+    all = gather(lds, sums, list, a.top);
+  }
+  write_row(a, row, all, lds);
+}
+
+// Memory of the split rows: of one size for every call, allocated once, never moved.
+static int logprob_workspace(nx_ctx *c, void **out) {
+  constexpr size_t kCounts = kLogprobWgs * sizeof(int);
+  constexpr size_t kBytes = kCounts + (size_t)kLogprobWgs * kRecord * 8;
+  DevBuf &ws = c->ws[WS_LOGPROBS];
+  if (!ws.ptr) {
+    NX_TRY(refuse_capture(c));
+    void *p = nullptr;
+    if (hipMalloc(&p, kBytes) != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(NX_ERR_OOM, "device allocation of " + std::to_string(kBytes) + " bytes failed");
+    }
+    // counts begin at 0, and the workspace is there once they are
+    if (hipMemsetAsync(p, 0, kCounts, c->stream) != hipSuccess || hipStreamSynchronize(c->stream) != hipSuccess) {
+      (void)hipGetLastError();
+      (void)hipFree(p);
+      return fail(NX_ERR_DEVICE, "clearing the workspace of log probabilities failed");
+    }
+    ws = {p, kBytes};
+  }
+  *out = ws.ptr;
+  return NX_OK;
+}
+
+static int logprobs_dev(nx_ctx *c, LogprobCall a, int rows) {
+  a.split = logprob_split(rows, a.vocab);
+  if (a.split.parts > 1) {
+    void *p;
+    NX_TRY(logprob_workspace(c, &p));
+    a.done = static_cast<int *>(p);
+    a.part = reinterpret_cast<uint64_t *>(a.done + kLogprobWgs);
+  }
+  constexpr int kRows = 1 << 22;  // of a launch, which has fewer than 2^32 threads
+  for (a.first = 0; a.first < rows; a.first += kRows) {
+    const int now = std::min(rows - a.first, kRows);
+    NX_TRY(launch(c, "logprobs", [&] {
+      go(c, k_logprobs, dim3(now * a.split.parts), dim3(kLogprobThreads), 0, a);
+    }));
+  }
+  return NX_OK;
+}
+
+static int logprobs(nx_ctx *c, LogprobCall a, int rows, bool host) {
+  if (!c) return fail(NX_ERR_INVALID_ARG, "null context");
+  NX_HIP(hipSetDevice(c->device));
+  NX_TRY(refuse(logprobs_check(a.x, a.stride, rows, a.vocab, a.tokens, a.given, a.logprobs, a.top, a.top_ids,
+                               a.top_logprobs)));
+  if (rows == 0) return NX_OK;
+  if (!host) return logprobs_dev(c, a, rows);
+  const size_t V = a.vocab, T = rows, n = T * a.given, m = T * a.top;
+  void *px, *pt, *po;
+  NX_TRY(ws_get(c, WS_LOGITS, T * V * 4, &px));
+  NX_TRY(ws_get(c, WS_XIN, n * 4, &pt));
+  NX_TRY(ws_get(c, WS_OUT, (n + T + 2 * m) * 4, &po));
+  LogprobCall d = a;
+  d.x = static_cast<const float *>(px);
+  d.stride = V;
+  d.tokens = static_cast<const int32_t *>(pt);
+  d.logprobs = static_cast<float *>(po);
+  d.entropy = d.logprobs + n;
+  d.top_logprobs = d.entropy + T;
+  d.top_ids = reinterpret_cast<int32_t *>(d.top_logprobs + m);
+  NX_HIP(hipMemcpy2DAsync(px, V * 4, a.x, a.stride * 4, V * 4, T, hipMemcpyHostToDevice, c->stream));
+  if (n) NX_HIP(hipMemcpyAsync(pt, a.tokens, n * 4, hipMemcpyHostToDevice, c->stream));
+  NX_TRY(logprobs_dev(c, d, rows));
+  if (n) NX_HIP(hipMemcpyAsync(a.logprobs, d.logprobs, n * 4, hipMemcpyDeviceToHost, c->stream));
+  if (a.entropy) NX_HIP(hipMemcpyAsync(a.entropy, d.entropy, T * 4, hipMemcpyDeviceToHost, c->stream));
+  if (m) {
+    NX_HIP(hipMemcpyAsync(a.top_logprobs, d.top_logprobs, m * 4, hipMemcpyDeviceToHost, c->stream));
+    NX_HIP(hipMemcpyAsync(a.top_ids, d.top_ids, m * 4, hipMemcpyDeviceToHost, c->stream));
+  }
+  NX_HIP(hipStreamSynchronize(c->stream));
+  return NX_OK;
+}
+
+}  // namespace nx
+
+using namespace nx;
+
+extern "C" {
+
+int nx_logprobs(nx_ctx *c, const float *logits, size_t stride, int rows, int vocab, const int32_t *tokens, int given,
+                float *logprobs, float *entropy, int top, int32_t *top_ids, float *top_logprobs) {
+  return guarded([&] {
+    return nx::logprobs(c, {logits, stride, tokens, logprobs, entropy, top_logprobs, top_ids, 0, vocab, given, top}, rows,
+                        true);
+  });
+}
+int nx_logprobs_dev(nx_ctx *c, const float *logits, size_t stride, int rows, int vocab, const int32_t *tokens,
+                    int given, float *logprobs, float *entropy, int top, int32_t *top_ids, float *top_logprobs) {
+  return guarded([&] {
+    return nx::logprobs(c, {logits, stride, tokens, logprobs, entropy, top_logprobs, top_ids, 0, vocab, given, top}, rows,
+                        false);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,106 @@
+// nx_step_plan.hpp — what the calls around a step's cache and attention accept (heads normed
+// and rotated, log probabilities), and how they share their work out.
+//
+// Plain C++ (no HIP): the CPU tests compile this header on its own.
+#pragma once
+
+#include "nx_kv_plan.hpp"
+
+namespace nx {
+
+constexpr int kMaxRopeHead = 512;  // the widest head
+constexpr int kMaxTop = 64;        // alternatives of a row: one for each lane of a wave
+
+// Whether rows of `wa` floats, `sa` apart, share memory with rows of `wb`, `sb` apart.  Rows of
+// one stride may lie in each other's gaps; of two strides, anything between the first and the
+// last counts.
+inline bool rows_overlap(const float *a, size_t sa, size_t wa, const float *b, size_t sb, size_t wb, long rows) {
+  using Wide = unsigned __int128;
+  if (!a || !b || !wa || !wb || rows <= 0) return false;
+  const Wide a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  const Wide a1 = a0 + 4 * ((Wide)(rows - 1) * sa + wa), b1 = b0 + 4 * ((Wide)(rows - 1) * sb + wb);
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (rows == 1 || sa != sb) return true;
+  const Wide pitch = 4 * (Wide)sa, off = b0 >= a0 ? (b0 - a0) % pitch : (pitch - (a0 - b0) % pitch) % pitch;
+  return off < 4 * (Wide)wa || off + 4 * (Wide)wb > pitch;
+}
+
+// The buffers of a rotation's rows.
+struct RopeRows {
+  const float *q, *k;
+  float *q_out, *k_out;
+  size_t q_stride, k_stride, q_out_stride, k_out_stride;
+};
+
+inline Refusal rope_check(const nx_rope *r, const int32_t *positions, int rows, int heads, int kv_heads,
+                          const RopeRows &x) {
+  if (!r) return {NX_ERR_INVALID_ARG, "null rotation"};
+  if (rows < 0 || heads < 0 || kv_heads < 0) return {NX_ERR_INVALID_ARG, "negative rows or heads"};
+  if (r->head_dim <= 0 || r->rotary_dim < 0) return {NX_ERR_INVALID_ARG, "head_dim must be positive"};
+  if (r->style != NX_ROPE_HALVES && r->style != NX_ROPE_PAIRS)
+    return {NX_ERR_INVALID_ARG, "unknown order of pairs " + std::to_string(r->style)};
+  if (r->rotary_dim > r->head_dim)
+    return {NX_ERR_SHAPE, std::to_string(r->rotary_dim) + " rotated elements of heads of " + std::to_string(r->head_dim)};
+  if (r->head_dim % 2 || r->rotary_dim % 2 || r->head_dim > kMaxRopeHead)
+    return {NX_ERR_UNSUPPORTED, "head_dim and rotary_dim are even, up to " + std::to_string(kMaxRopeHead) + ", not " +
+                                    std::to_string(r->head_dim) + " and " + std::to_string(r->rotary_dim)};
+  if (!(r->eps >= 0.f) || !std::isfinite(r->eps)) return {NX_ERR_INVALID_ARG, "eps is negative or not finite"};
+  if (heads > 65536 || kv_heads > 65536) return {NX_ERR_UNSUPPORTED, "more than 65536 heads"};
+  if (rows > (1 << 24)) return {NX_ERR_UNSUPPORTED, "more than 2^24 rows"};
+  if (rows == 0 || heads + kv_heads == 0) return {};
+  if (r->rotary_dim > 0 && (!r->freq || !positions)) return {NX_ERR_INVALID_ARG, "null positions or frequencies"};
+  if ((heads && (!x.q || !x.q_out)) || (kv_heads && (!x.k || !x.k_out))) return {NX_ERR_INVALID_ARG, "null buffer"};
+  for (size_t s : {x.q_stride, x.k_stride, x.q_out_stride, x.k_out_stride})
+    if (s > (size_t)1 << 40) return {NX_ERR_UNSUPPORTED, "row stride above 2^40"};
+  const size_t wq = (size_t)heads * r->head_dim, wk = (size_t)kv_heads * r->head_dim;
+  if (heads) {
+    if (Refusal f = kv_check_rows("query", (long)x.q_stride, (long)wq)) return f;
+    if (Refusal f = kv_check_rows("query output", (long)x.q_out_stride, (long)wq)) return f;
+  }
+  if (kv_heads) {
+    if (Refusal f = kv_check_rows("key", (long)x.k_stride, (long)wk)) return f;
+    if (Refusal f = kv_check_rows("key output", (long)x.k_out_stride, (long)wk)) return f;
+  }
+  const bool same_q = x.q_out == x.q && x.q_out_stride == x.q_stride;
+  const bool same_k = x.k_out == x.k && x.k_out_stride == x.k_stride;
+  if ((!same_q && rows_overlap(x.q, x.q_stride, wq, x.q_out, x.q_out_stride, wq, rows)) ||
+      (!same_k && rows_overlap(x.k, x.k_stride, wk, x.k_out, x.k_out_stride, wk, rows)) ||
+      rows_overlap(x.q, x.q_stride, wq, x.k_out, x.k_out_stride, wk, rows) ||
+      rows_overlap(x.k, x.k_stride, wk, x.q_out, x.q_out_stride, wq, rows) ||
+      rows_overlap(x.q_out, x.q_out_stride, wq, x.k_out, x.k_out_stride, wk, rows))
+    return {NX_ERR_INVALID_ARG, "outputs overlap rows that are not their own"};
+  return {};
+}
+
+inline Refusal logprobs_check(const float *logits, size_t stride, int rows, int vocab, const int32_t *tokens,
+                              int given, const float *logprobs, int top, const int32_t *top_ids,
+                              const float *top_logprobs) {
+  if (rows < 0 || given < 0 || top < 0) return {NX_ERR_INVALID_ARG, "negative rows, tokens or alternatives"};
+  if (vocab <= 0) return {NX_ERR_INVALID_ARG, "the number of logits must be positive"};
+  if (rows > (1 << 24)) return {NX_ERR_UNSUPPORTED, "more than 2^24 rows"};
+  if (vocab > (1 << 30)) return {NX_ERR_UNSUPPORTED, "more than 2^30 logits"};
+  if (top > kMaxTop) return {NX_ERR_UNSUPPORTED, "more than " + std::to_string(kMaxTop) + " alternatives"};
+  if (given > (1 << 20)) return {NX_ERR_UNSUPPORTED, "more than 2^20 tokens of a row"};
+  if (stride > (size_t)1 << 40) return {NX_ERR_UNSUPPORTED, "row stride above 2^40"};
+  if (Refusal f = kv_check_rows("logit", (long)stride, vocab)) return f;
+  if (rows == 0) return {};
+  if (!logits || (given > 0 && (!tokens || !logprobs)) || (top > 0 && (!top_ids || !top_logprobs)))
+    return {NX_ERR_INVALID_ARG, "null buffer"};
+  return {};
+}
+
+// Workgroups that share a row's logits, and the logits of each (a multiple of 4).
+constexpr int kLogprobWgs = 2048;   // as many as fill the card, and no more where rows are split
+constexpr int kLogprobLeast = 1024; // of one, in logits
+constexpr int kLogprobParts = 64;
+struct RowSplit {
+  int parts, share;
+};
+inline RowSplit logprob_split(int rows, int vocab) {
+  const int want = std::max(1, kLogprobWgs / rows), most = (vocab + kLogprobLeast - 1) / kLogprobLeast;
+  const int parts = std::max(1, std::min({want, most, kLogprobParts}));
+  const int share = ((vocab + parts - 1) / parts + 3) / 4 * 4;
+  return {(vocab + share - 1) / share, share};
+}
+
+}  // namespace nx
