@@ -52,6 +52,9 @@
  *       InferenceEngine::attention_decode    src/engine/mod.rs:452-500
  *       kernel::grouped_query_attention      src/kernel/mod.rs:40-99
  *       causal, for any new tokens of each sequence; with a window, too
+ *   nx_kv_evict / nx_kv_evict_dev
+ *       no counterpart; beside KvCache::add, whose cache only grows
+ *                                            src/engine/mod.rs:410-426
  *   nx_qk_rope / nx_qk_rope_dev
  *       kernel::rope_single                  src/kernel/mod.rs:258-271
  *       for every head and token of a step, behind a norm of the head
@@ -353,6 +356,32 @@ int nx_attention(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const f
 int nx_attention_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *d_q,
                      size_t q_stride, int heads, float scale, int window, int sinks, float *d_out,
                      size_t out_stride);
+
+/* Gives up cached tokens: each sequence of the batch keeps its first `sinks` tokens, its last
+ * `recent` ones and, of those between, the heaviest, `keep` in all (a sequence of `keep` tokens or
+ * fewer, all).  They are chosen for every key/value head apart, by the weights at
+ *   mass + (sequence * kv_heads + head) * mass_stride,  one of each token
+ * (nx_attention_mass gathers them; any f32 will do, of equal ones the lower token is kept,
+ * and a NaN counts less than any number, a token behind mass_stride as NaN), and move, in their
+ * order, to the pages to_pages[sequence * to_max_pages + p], as they are stored.  Of the batch,
+ * kv_len, pages, max_pages and num_seqs are read (row_start and num_tokens are not).
+ * Writes kept [num_seqs x kv_heads x keep], the tokens that each head kept, then -1;
+ * new_len[num_seqs], min(kv_len, keep); and, unless new_mass is null, the kept tokens' weights
+ * to new_mass + (sequence * kv_heads + head) * new_mass_stride.  The sequence's old pages stay as
+ * they were: with new_len and to_pages it goes on in the new ones, and they are the caller's
+ * to free.  Every token behind it sees what was kept (nx_attention counts places, so a window
+ * counts the kept tokens); its next tokens take places new_len, new_len + 1, ... and the positions
+ * (nx_qk_rope) that follow its old ones.
+ * The new pages must be none that the batch's sequences use, each named once: host calls refuse
+ * others, *_dev calls cannot (there, what such pages hold afterwards is not defined; entries
+ * that name no page are left out, and tokens on no page move as zeros).  The rest of the last
+ * group of 32 tokens of a new page is cleared.  Needs no workspace. */
+int nx_kv_evict(nx_ctx *ctx, nx_kv *kv, const nx_kv_batch *batch, const int32_t *to_pages, int to_max_pages,
+                int keep, int sinks, int recent, const float *mass, size_t mass_stride, int32_t *kept,
+                int32_t *new_len, float *new_mass, size_t new_mass_stride);
+int nx_kv_evict_dev(nx_ctx *ctx, nx_kv *kv, const nx_kv_batch *batch, const int32_t *d_to_pages,
+                    int to_max_pages, int keep, int sinks, int recent, const float *d_mass, size_t mass_stride,
+                    int32_t *d_kept, int32_t *d_new_len, float *d_new_mass, size_t new_mass_stride);
 
 /* ---------------------------------------------------------------- norm and rotation of heads */
 /* which elements of a head's first rotary_dim make pair i of them */

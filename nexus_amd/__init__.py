@@ -55,6 +55,7 @@ EXPORTS = [
     "nx_kv_create", "nx_kv_info", "nx_kv_destroy", "nx_kv_write", "nx_kv_write_dev",
     "nx_kv_read", "nx_kv_read_dev", "nx_attention", "nx_attention_dev",
     "nx_qk_rope", "nx_qk_rope_dev", "nx_logprobs", "nx_logprobs_dev",
+    "nx_kv_evict", "nx_kv_evict_dev",
 ]
 
 _lib = None
@@ -181,9 +182,11 @@ def lib():
         "nx_attention": (attention, C.c_int), "nx_attention_dev": (attention, C.c_int),
     })
     rope = [_vp, C.POINTER(_Rope), _vp, C.c_int, C.c_int, C.c_int] + [_vp, C.c_size_t] * 4
+    evict = [_vp, _vp, _kvb, _vp] + [C.c_int] * 4 + [_vp, C.c_size_t, _vp, _vp, _vp, C.c_size_t]
     logprobs = [_vp, _vp, C.c_size_t, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, C.c_int, _vp, _vp]
     sig.update({
         "nx_qk_rope": (rope, C.c_int), "nx_qk_rope_dev": (rope, C.c_int),
+        "nx_kv_evict": (evict, C.c_int), "nx_kv_evict_dev": (evict, C.c_int),
         "nx_logprobs": (logprobs, C.c_int), "nx_logprobs_dev": (logprobs, C.c_int),
     })
     for name, (args, res) in sig.items():
@@ -638,6 +641,13 @@ class KvCache:
         check(lib().nx_attention_dev(self.ctx.h, self.h, batch.ref, q_ptr, q_stride, heads, scale,
                                      window, sinks, out_ptr, out_stride))
 
+    def evict_dev(self, batch: KvBatch, to_pages_ptr: int, to_max_pages: int, keep: int, sinks: int,
+                  recent: int, mass_ptr: int, mass_stride: int, kept_ptr: int, new_len_ptr: int,
+                  new_mass_ptr: int = 0, new_mass_stride: int = 0) -> None:
+        check(lib().nx_kv_evict_dev(self.ctx.h, self.h, batch.ref, to_pages_ptr, to_max_pages, keep, sinks,
+                                    recent, mass_ptr, mass_stride, kept_ptr, new_len_ptr, new_mass_ptr,
+                                    new_mass_stride))
+
     # ---- host arrays
     def _host_batch(self, row_start, kv_len, pages, rows: int):
         rs = np.ascontiguousarray(row_start, np.int32)
@@ -686,6 +696,27 @@ class KvCache:
                                  self.head_dim ** -0.5 if scale is None else scale, window, sinks,
                                  out.ctypes.data, q.shape[1]))
         return out
+
+    def evict(self, kv_len, pages, to_pages, keep: int, mass, sinks: int = 0, recent: int = 0):
+        """Keeps the `keep` heaviest tokens of each sequence and head (the first `sinks` and the
+        last `recent` always), by mass [sequences x kv_heads x tokens], on the pages to_pages:
+        the kept tokens [sequences x kv_heads x keep], the new lengths, and the kept weights."""
+        ln = np.ascontiguousarray(kv_len, np.int32)
+        b, _keep = self._host_batch(np.zeros(ln.size + 1), ln, pages, 0)
+        to = np.ascontiguousarray(to_pages, np.int32)
+        m = _f32(mass)
+        if to.ndim != 2 or len(to) != ln.size:
+            raise ValueError(f"new page tables of shape {to.shape} for {ln.size} sequences")
+        if m.ndim != 3 or m.shape[:2] != (ln.size, self.kv_heads):
+            raise ValueError(f"weights of shape {m.shape} for {ln.size} sequences of {self.kv_heads} heads")
+        if keep < 0:
+            raise ValueError("negative number of tokens to keep")
+        kept = np.empty((ln.size, self.kv_heads, keep), np.int32)
+        new_len, new_mass = np.empty(ln.size, np.int32), np.zeros(kept.shape, np.float32)
+        check(lib().nx_kv_evict(self.ctx.h, self.h, b.ref, to.ctypes.data, to.shape[1], keep, sinks, recent,
+                                m.ctypes.data, m.shape[2], kept.ctypes.data, new_len.ctypes.data,
+                                new_mass.ctypes.data, keep))
+        return kept, new_len, new_mass
 
     def close(self):
         if self.h:

@@ -14,8 +14,7 @@
 // sequences go where: tile_from and kFewScores below.
 #include <hip/hip_runtime.h>
 
-#include "nx_kv_dev.hpp"
-#include "nx_split_dev.hpp"
+#include "nx_attn_dev.hpp"
 
 namespace nx {
 
@@ -27,15 +26,11 @@ struct AttnCall {
   float scale;
   int window, sinks;
   bool wide_q, wide_out;  // rows of whole float4 runs
-  uint32_t magic;         // ceil(2^(31 + shift) / group), shift = ceil(log2 group)
+  uint32_t magic;         // by_group's
   int shift;
 };
 
-// row / a.group for 0 <= row < 2^31: magic group - 2^(31 + shift) < 2^shift, so the
-// quotient's excess row (magic group - 2^(31 + shift)) / 2^(31 + shift) is below 1 / group's step
-__device__ __forceinline__ int by_group(const AttnCall &a, int row) {
-  return (int)(__umulhi(2u * (uint32_t)row, a.magic) >> a.shift);
-}
+__device__ __forceinline__ int by_group(const AttnCall &a, int row) { return by_group(row, a.magic, a.shift); }
 
 // whether token p sees token j <= p
 __device__ __forceinline__ bool sees(const AttnCall &a, int p, int j) {
@@ -147,65 +142,10 @@ __device__ __forceinline__ void attn_row(const KvView &kv, const nx_kv_batch &b,
 // sequences through a window of 1024 tokens 18 against 22.  One token after 516: 10.0 us, of
 // which an empty launch is 4.4 and the rest the round trips of the tables, a page number,
 // the keys, the parts and their count.
-constexpr float kLog2e = 1.4426950408889634f;
 // The largest weight of a row (p, or p times the value's scale) is 2^8 or more when the
 // reference m is set; m is set anew, and the sums scaled, when one passes 2^15.  So
 // halves stay in range, and weights down to 2^-18 of the largest keep all their bits.
 constexpr float kHead = 9.f, kGrow = 15.f, kUnset = -1e30f;
-
-// int8 code -> f16 q 2^-9, exact: 0x80 ^ code as the low bits of a subnormal half
-__device__ __forceinline__ f16x8 from_codes(uint32_t lo, uint32_t hi) { return operand8(lo, hi); }
-
-__device__ __forceinline__ float ldexp1(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
-
-// 8 values as two halves each, x = hi + lo to 22 bits.  `one` is 1 that the compiler
-// does not know: x one - hi is then one instruction that reads the packed half.
-__device__ __forceinline__ void split2(const float (&x)[8], float one, f16x8 &h, f16x8 &l) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  f16x2 hi[4], lo[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hi[i] = __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), f16x2);
-    asm("" : "+v"(hi[i]));  // converted once, packed
-    lo[i] = __builtin_convertvector(
-        (f32x2{fmaf(x[2 * i], one, -(float)hi[i][0]), fmaf(x[2 * i + 1], one, -(float)hi[i][1])}), f16x2);
-  }
-  h = f16x8{hi[0][0], hi[0][1], hi[1][0], hi[1][1], hi[2][0], hi[2][1], hi[3][0], hi[3][1]};
-  l = f16x8{lo[0][0], lo[0][1], lo[1][0], lo[1][1], lo[2][0], lo[2][1], lo[3][0], lo[3][1]};
-}
-__device__ __forceinline__ void load8(const float *p, bool wide, float (&x)[8]) {
-  if (wide) {
-    const f32x4 lo = *reinterpret_cast<const f32x4 *>(p), hi = *reinterpret_cast<const f32x4 *>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = lo[i];
-      x[4 + i] = hi[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
-  }
-}
-__device__ __forceinline__ float opaque_one() {
-  float one = 1.f;
-  asm("" : "+s"(one));
-  return one;
-}
-
-// the largest (sum) over the four lane groups, in all of them
-template <typename Op>
-__device__ __forceinline__ float across_groups(float v, Op op) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-__device__ __forceinline__ float max_groups(float v) {
-  return across_groups(v, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float sum_groups(float v) {
-  return across_groups(v, [](float a, float b) { return a + b; });
-}
 
 // A row's running reference: m, and whether none is set yet (m is 0 then).
 struct Ref {
@@ -1004,19 +944,6 @@ __global__ __launch_bounds__(64 * kDecodeWaves<D>, D == 256 ? 1 : 2) void k_attn
 // 16127: 458-480 us, 446-467.  Scores
 // of the next group ahead of this one's weights, with q's lower halves in LDS to make room:
 // 346 us for the prompt, against 314.
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-// the other half of the wave's value
-template <typename Op>
-__device__ __forceinline__ float across_halves(float v, Op op) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-
-__device__ __forceinline__ float max_halves(float v) {
-  return across_halves(v, [](float x, float y) { return fmaxf(x, y); });
-}
-
 template <int FMT, int D>
 struct TileLds {
   // keys [D / 8][32 rows][8], then values [4][D][8], of two groups
@@ -1373,8 +1300,8 @@ int attn_workspace(nx_ctx *c, void **out) {
 static int attention_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, AttnCall a) {
   a.wide_q = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride % 4 == 0;
   a.wide_out = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.out_stride % 4 == 0;
-  a.shift = a.group > 1 ? 32 - __builtin_clz(a.group - 1) : 0;
-  a.magic = (uint32_t)((((uint64_t)1 << (31 + a.shift)) + a.group - 1) / a.group);
+  a.shift = group_shift(a.group);
+  a.magic = group_magic(a.group);
   void *p;
   NX_TRY(attn_workspace(c, &p));
   // Which kernels the batch may need: only the device knows its sequences' rows.  With a row

@@ -252,13 +252,18 @@ int refuse_capture(nx_ctx *c) {
                                   "outside of stream capture");
 }
 
-int kv_check_call(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b) {
+int kv_check_cache(nx_ctx *c, const nx_kv *kv) {
   if (!c) return fail(NX_ERR_INVALID_ARG, "null context");
   NX_HIP(hipSetDevice(c->device));
   if (!kv) return fail(NX_ERR_INVALID_ARG, "null cache");
   if (kv->device != c->device)
     return fail(NX_ERR_INVALID_ARG, "the cache lives on device " + std::to_string(kv->device) +
                                         ", the context on " + std::to_string(c->device));
+  return NX_OK;
+}
+
+int kv_check_call(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b) {
+  NX_TRY(kv_check_cache(c, kv));
   return refuse(kv_check_batch(b, kv->page_tokens));
 }
 

@@ -26,6 +26,8 @@ int attn_workspace(nx_ctx *c, void **out);
 // refuses what allocates and clears memory while the context's stream is captured: the graph
 // would clear it again with every replay, and not before the first
 int refuse_capture(nx_ctx *c);
+// a context, a cache, and both on one device; then the batch's sizes
+int kv_check_cache(nx_ctx *c, const nx_kv *kv);
 int kv_check_call(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b);
 // copies a host batch's arrays to the device; *dev describes them there
 int kv_upload_batch(nx_ctx *c, const nx_kv_batch &b, nx_kv_batch *dev);

@@ -89,6 +89,71 @@ inline Refusal logprobs_check(const float *logits, size_t stride, int rows, int 
   return {};
 }
 
+// The arguments of an eviction besides the cache and the batch.
+struct EvictArgs {
+  const int32_t *to_pages;
+  int to_max_pages, keep, sinks, recent;
+  const float *mass;
+  size_t mass_stride;
+  int32_t *kept, *new_len;
+  float *new_mass;
+  size_t new_mass_stride;
+};
+
+inline Refusal evict_check(const nx_kv_batch *b, int page_tokens, int kv_heads, const EvictArgs &a) {
+  if (!b) return {NX_ERR_INVALID_ARG, "null batch"};
+  if (b->num_seqs < 0 || b->max_pages < 0 || a.to_max_pages < 0) return {NX_ERR_INVALID_ARG, "negative batch size"};
+  if (a.keep <= 0 || a.sinks < 0 || a.recent < 0)
+    return {NX_ERR_INVALID_ARG, "a number of tokens to keep is negative, or none"};
+  if ((int64_t)a.sinks + a.recent > a.keep)
+    return {NX_ERR_SHAPE, std::to_string(a.sinks) + " first and " + std::to_string(a.recent) + " last tokens of " +
+                              std::to_string(a.keep) + " to keep"};
+  if (b->num_seqs == 0) return {};
+  if (!b->kv_len || !b->pages || !a.to_pages) return {NX_ERR_INVALID_ARG, "null batch array"};
+  if (!a.mass || !a.kept || !a.new_len) return {NX_ERR_INVALID_ARG, "null buffer"};
+  if (b->max_pages == 0 || a.to_max_pages == 0) return {NX_ERR_SHAPE, "a batch of sequences without pages"};
+  if ((int64_t)std::max(b->max_pages, a.to_max_pages) * page_tokens > INT32_MAX - 65536 || a.keep > INT32_MAX - 65536)
+    return {NX_ERR_UNSUPPORTED, "sequences of more than 2^31 tokens"};
+  if (b->num_seqs > (1 << 20)) return {NX_ERR_UNSUPPORTED, "more than 2^20 sequences"};
+  if (a.mass_stride == 0) return {NX_ERR_SHAPE, "rows of no weights"};
+  if (a.mass_stride > (size_t)1 << 40 || a.new_mass_stride > (size_t)1 << 40)
+    return {NX_ERR_UNSUPPORTED, "row stride above 2^40"};
+  if (!a.new_mass) return {};
+  if (Refusal f = kv_check_rows("weight", (long)a.new_mass_stride, a.keep)) return f;
+  const size_t width = std::min(a.mass_stride, (size_t)b->max_pages * page_tokens);
+  if (rows_overlap(a.mass, a.mass_stride, width, a.new_mass, a.new_mass_stride, a.keep, (long)b->num_seqs * kv_heads))
+    return {NX_ERR_INVALID_ARG, "the new weights overlap the old ones"};
+  return {};
+}
+
+// What the call on host memory checks besides: lengths and weights, and that the new pages are
+// the cache's, nobody else's of the batch, and named once.
+inline Refusal evict_check_tables(const nx_kv_batch &b, int num_pages, int page_tokens, const EvictArgs &a) {
+  std::vector<int> from, to;
+  for (int s = 0; s < b.num_seqs; ++s) {
+    const int len = b.kv_len[s];
+    const std::string who = "sequence " + std::to_string(s);
+    if (len < 0 || len > (int64_t)b.max_pages * page_tokens) return {NX_ERR_SHAPE, who + " is not as long as its pages"};
+    if ((size_t)len > a.mass_stride) return {NX_ERR_SHAPE, who + " has more tokens than weights"};
+    const int n = std::min(len, a.keep);
+    if (n > (int64_t)a.to_max_pages * page_tokens) return {NX_ERR_SHAPE, who + " keeps more tokens than its new pages hold"};
+    for (int side = 0; side < 2; ++side) {
+      const int32_t *pages = side ? a.to_pages + (size_t)s * a.to_max_pages : b.pages + (size_t)s * b.max_pages;
+      for (int p = 0; p < ((side ? n : len) + page_tokens - 1) / page_tokens; ++p) {
+        if (pages[p] < 0 || pages[p] >= num_pages)
+          return {NX_ERR_INVALID_ARG, "page " + std::to_string(pages[p]) + " of " + who + " is not in the cache"};
+        (side ? to : from).push_back(pages[p]);
+      }
+    }
+  }
+  std::sort(from.begin(), from.end());
+  std::sort(to.begin(), to.end());
+  for (size_t i = 0; i < to.size(); ++i)
+    if ((i && to[i] == to[i - 1]) || std::binary_search(from.begin(), from.end(), to[i]))
+      return {NX_ERR_INVALID_ARG, "new page " + std::to_string(to[i]) + " is in use"};
+  return {};
+}
+
 // Workgroups that share a row's logits, and the logits of each (a multiple of 4).
 constexpr int kLogprobWgs = 2048;   // as many as fill the card, and no more where rows are split
 constexpr int kLogprobLeast = 1024; // of one, in logits

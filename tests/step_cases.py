@@ -86,3 +86,14 @@ def check_logprobs(got, x, tokens, top):
             off = np.where(same, 0, np.abs(g - r))
         b = b + np.where(same, 0, 4 * U * np.abs(r))
         assert (off <= b).all(), (name, float(np.nanmax(off / np.maximum(b, 1e-300))), off.max())
+
+
+def evicted(mass, length, keep, sinks, recent):
+    """The tokens of one head that stay, in their order: by a sort in Python of (weight, lower
+    token), NaN below everything."""
+    if length <= keep:
+        return np.arange(length)
+    middle = range(sinks, length - recent)
+    weight = [(-np.inf, 0) if j >= len(mass) or np.isnan(mass[j]) else (float(mass[j]), 1) for j in range(length)]
+    best = sorted(middle, key=lambda j: (-weight[j][1], -weight[j][0], j))[:keep - sinks - recent]
+    return np.array(sorted(list(range(sinks)) + best + list(range(length - recent, length))), int)
