@@ -52,6 +52,8 @@
  *       InferenceEngine::attention_decode    src/engine/mod.rs:452-500
  *       kernel::grouped_query_attention      src/kernel/mod.rs:40-99
  *       causal, for any new tokens of each sequence; with a window, too
+ *   nx_attention_mass / nx_attention_mass_dev
+ *       the weights of InferenceEngine::attention_decode  src/engine/mod.rs:452-500
  *   nx_kv_evict / nx_kv_evict_dev
  *       no counterpart; beside KvCache::add, whose cache only grows
  *                                            src/engine/mod.rs:410-426
@@ -356,6 +358,28 @@ int nx_attention(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const f
 int nx_attention_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *d_q,
                      size_t q_stride, int heads, float scale, int window, int sinks, float *d_out,
                      size_t out_stride);
+
+/* The weight that the batch's tokens give each cached token of their sequences in nx_attention
+ * (without a window), summed over the tokens and over the heads that share a key/value head:
+ *   mass[s][g][j] = before[s][g][j] + sum_r sum_h p_rh(j),   p_rh = softmax_j(scale q[r][h] . k_j)
+ * over the rows r of sequence s and the heads h of key/value head g, where a row sees the tokens
+ * j <= p up to its own.  Call it where nx_attention is called: q, heads and scale as there, the
+ * step's keys written.  The weights of sequence s and head g begin at (s * kv_heads + g) *
+ * mass_stride, one for each token j < kv_len[s]; tokens of the step itself have no `before`, and
+ * before may be null (nothing was gathered) or mass itself.  What lies behind kv_len or
+ * mass_stride, and the weights of a sequence without rows, stay as they were.
+ * f32, scores and sums as nx_attention's (relative error about 1e-6 of each p; last bits depend
+ * on the batch, not on the run).  A row that sees no token gives nothing, nor does one whose scores are all
+ * -infinity; a row with a NaN or +infinity among the scores that it sees, or scores past
+ * f32's range, gives NaNs to the tokens that it sees and to no others.
+ * At most 2^24 rows times heads in a call.  The workspace (256 MB) is the context's, allocated
+ * with the first call, which is refused while the stream is captured, and never moved; calls on
+ * one context must not overlap in time. */
+int nx_attention_mass(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *q, size_t q_stride,
+                      int heads, float scale, const float *before, float *mass, size_t mass_stride);
+int nx_attention_mass_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *d_q,
+                          size_t q_stride, int heads, float scale, const float *d_before, float *d_mass,
+                          size_t mass_stride);
 
 /* Gives up cached tokens: each sequence of the batch keeps its first `sinks` tokens, its last
  * `recent` ones and, of those between, the heaviest, `keep` in all (a sequence of `keep` tokens or

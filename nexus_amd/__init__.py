@@ -55,7 +55,7 @@ EXPORTS = [
     "nx_kv_create", "nx_kv_info", "nx_kv_destroy", "nx_kv_write", "nx_kv_write_dev",
     "nx_kv_read", "nx_kv_read_dev", "nx_attention", "nx_attention_dev",
     "nx_qk_rope", "nx_qk_rope_dev", "nx_logprobs", "nx_logprobs_dev",
-    "nx_kv_evict", "nx_kv_evict_dev",
+    "nx_attention_mass", "nx_attention_mass_dev", "nx_kv_evict", "nx_kv_evict_dev",
 ]
 
 _lib = None
@@ -182,10 +182,12 @@ def lib():
         "nx_attention": (attention, C.c_int), "nx_attention_dev": (attention, C.c_int),
     })
     rope = [_vp, C.POINTER(_Rope), _vp, C.c_int, C.c_int, C.c_int] + [_vp, C.c_size_t] * 4
+    mass = [_vp, _vp, _kvb, _vp, C.c_size_t, C.c_int, C.c_float, _vp, _vp, C.c_size_t]
     evict = [_vp, _vp, _kvb, _vp] + [C.c_int] * 4 + [_vp, C.c_size_t, _vp, _vp, _vp, C.c_size_t]
     logprobs = [_vp, _vp, C.c_size_t, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, C.c_int, _vp, _vp]
     sig.update({
         "nx_qk_rope": (rope, C.c_int), "nx_qk_rope_dev": (rope, C.c_int),
+        "nx_attention_mass": (mass, C.c_int), "nx_attention_mass_dev": (mass, C.c_int),
         "nx_kv_evict": (evict, C.c_int), "nx_kv_evict_dev": (evict, C.c_int),
         "nx_logprobs": (logprobs, C.c_int), "nx_logprobs_dev": (logprobs, C.c_int),
     })
@@ -641,6 +643,11 @@ class KvCache:
         check(lib().nx_attention_dev(self.ctx.h, self.h, batch.ref, q_ptr, q_stride, heads, scale,
                                      window, sinks, out_ptr, out_stride))
 
+    def attention_mass_dev(self, batch: KvBatch, q_ptr: int, q_stride: int, heads: int, before_ptr: int,
+                           mass_ptr: int, mass_stride: int, scale: float) -> None:
+        check(lib().nx_attention_mass_dev(self.ctx.h, self.h, batch.ref, q_ptr, q_stride, heads, scale,
+                                          before_ptr, mass_ptr, mass_stride))
+
     def evict_dev(self, batch: KvBatch, to_pages_ptr: int, to_max_pages: int, keep: int, sinks: int,
                   recent: int, mass_ptr: int, mass_stride: int, kept_ptr: int, new_len_ptr: int,
                   new_mass_ptr: int = 0, new_mass_stride: int = 0) -> None:
@@ -696,6 +703,24 @@ class KvCache:
                                  self.head_dim ** -0.5 if scale is None else scale, window, sinks,
                                  out.ctypes.data, q.shape[1]))
         return out
+
+    def attention_mass(self, row_start, kv_len, pages, q, heads: int, scale: float | None = None,
+                       before=None) -> np.ndarray:
+        """The weight [sequences x kv_heads x tokens] that q's rows give each cached token, added
+        to `before` (of at least as many tokens, which it is copied from)."""
+        q = self._rows(q, heads * self.head_dim)
+        ln = np.ascontiguousarray(kv_len, np.int32)
+        if before is None:
+            mass = np.zeros((ln.size, self.kv_heads, max(int(ln.max(initial=0)), 1)), np.float32)
+        else:
+            mass = _f32(before).copy()
+            if mass.ndim != 3 or mass.shape[:2] != (ln.size, self.kv_heads):
+                raise ValueError(f"weights of shape {mass.shape} for {ln.size} sequences of {self.kv_heads} heads")
+        b, _keep = self._host_batch(row_start, ln, pages, len(q))
+        check(lib().nx_attention_mass(self.ctx.h, self.h, b.ref, q.ctypes.data, q.shape[1], heads,
+                                      self.head_dim ** -0.5 if scale is None else scale,
+                                      0 if before is None else mass.ctypes.data, mass.ctypes.data, mass.shape[2]))
+        return mass
 
     def evict(self, kv_len, pages, to_pages, keep: int, mass, sinks: int = 0, recent: int = 0):
         """Keeps the `keep` heaviest tokens of each sequence and head (the first `sinks` and the

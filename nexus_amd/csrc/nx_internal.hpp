@@ -171,6 +171,7 @@ enum WsSlot {
   WS_KV_BATCH,   // device copy of a batch's arrays for blocking calls
   WS_ATTN,       // partial results of the attention (one size, never moved)
   WS_LOGPROBS,   // parts of split rows of logits (one size, never moved)
+  WS_MASS,       // scores and statistics of gathered attention weights (one size, never moved)
   WS_COUNT
 };
 static_assert(WS_COUNT <= 32, "workspace slots of a context");

@@ -1,0 +1,792 @@
+// nx_mass.hip — the weight that a step's queries give each cached token:
+//
+//   mass_j = before_j + sum_i p_ij,   p_ij = 2^(x_ij - e_i),   x_ij = log2(e) scale q_i . k_j,
+//   e_i = m_i + log2 sum_j 2^(x_ij - m_i)
+//
+// over the rows i (of a token and a head that shares the key/value head) that see token j.  e_i
+// takes all keys of a row, so the keys are gone through twice:
+//
+// Few rows (k_mass_scores, k_mass_add): the scores of 16 rows against a chunk of the keys are
+// stored beside the chunk's maximum and sum, and read back once all chunks are there: less
+// memory than the keys again.
+// Many rows (k_mass_stats, k_mass_columns): the scores are worked out twice.  First 128 rows are
+// held against the keys that stream by, for e_i; then keys are held against the rows that stream
+// by, so a key's sum stays in its lanes.
+//
+// The scores are nx_attn.hip's: transposed products K Q^T on the f16 matrix cores, q as two
+// halves.  A score is one key's and one row's alone, so nothing that is masked reaches another.
+#include <hip/hip_runtime.h>
+
+#include "nx_attn_dev.hpp"
+#include "nx_step_plan.hpp"
+
+namespace nx {
+
+struct MassCall {
+  const float *q, *before;
+  float *mass;
+  size_t q_stride, mass_stride;
+  int heads, group;  // query heads, and those that share a key/value head
+  float scale;
+  bool wide_q;     // rows of whole float4 runs
+  uint32_t magic;  // by_group's
+  int shift;
+  int rows_above, rows_upto;  // the kernels' sequences: those of so many rows
+};
+
+constexpr float kUnsetMax = -1e30f;
+
+__device__ __forceinline__ int rows_of(const MassCall &a, const KvSeq &q) {
+  const int rows = q.n * a.group;
+  return q.len > 0 && rows > a.rows_above && rows <= a.rows_upto ? rows : 0;
+}
+__device__ __forceinline__ const float *query_of(const MassCall &a, const KvSeq &s, int head, int row, int &tok) {
+  tok = by_group(row, a.magic, a.shift);
+  return a.q + (size_t)(s.row + tok) * a.q_stride;
+}
+
+// -infinity stands for tokens that a row does not see: a score of -infinity is the lowest number
+__device__ __forceinline__ float seen_score(float x) { return x == -INFINITY ? -3.4028234663852886e38f : x; }
+
+// log2 of a row's sum: above everything where it is nothing
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l); }
+
+__device__ __forceinline__ void add_to(const MassCall &a, const KvSeq &s, size_t tile, int j, float sum) {
+  if ((size_t)j >= a.mass_stride) return;
+  const size_t at = tile * a.mass_stride + j;
+  a.mass[at] = (a.before && j < s.first ? a.before[at] : 0.f) + sum;
+}
+
+// ------------------------------------------------------------ few rows
+struct NarrowWork {
+  MassNarrow m;
+  int groups;     // of the page table
+  float *scores;  // [tiles][slots][groups * 32]
+  float2 *stats;  // [tiles][chunks][16] maximum and sum
+};
+
+// 16-row tiles of a sequence
+__device__ __forceinline__ int row_tiles(const MassCall &a, const KvSeq &q) {
+  return (rows_of(a, q) + kMassRows - 1) / kMassRows;
+}
+
+constexpr int kMassWaves = 4, kMassThreads = 64 * kMassWaves;
+
+template <int FMT, int D>
+__global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(KvView kv, nx_kv_batch b, MassCall a,
+                                                                              NarrowWork w) {
+  using E = kv_elem<FMT>;
+  constexpr bool I8 = FMT == NX_KV_INT8;
+  constexpr int KS = D / 32, KL = I8 ? KS : 2 * KS;
+  __shared__ long sums[kMassWaves];
+  __shared__ Place found;
+  __shared__ float2 part[kMassWaves][kMassRows];
+  const int tile = blockIdx.x / w.m.chunks, chunk = blockIdx.x % w.m.chunks;
+  const Place at = find_item<kMassWaves>(
+      kv, b, tile, [&](const KvSeq &q) { return row_tiles(a, q) * kv.heads; }, sums, &found);
+  if (at.s < 0) return;
+  const KvSeq s = at.seq;
+  const int tiles = row_tiles(a, s), head = at.at / tiles, r0 = (at.at - head * tiles) * kMassRows;
+  const int nr = min(kMassRows, rows_of(a, s) - r0);
+  const int begin = chunk * w.m.share, end = min(begin + w.m.share, (s.len + kKvGroup - 1) / kKvGroup);
+  if (begin >= end) return;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+
+  uint4 kf[KL];
+  f32x4 dk[2];  // INT8: scales of the lane's tokens
+  auto group_of = [&](int i) { return kv_group(kv, b, at.s, head, min(i, end - 1) * kKvGroup); };
+  auto load_k = [&](long gr) {  // (pool group 0, masked, for one that is not there)
+    gr = max(gr, 0L);
+    const E *base = reinterpret_cast<const E *>(kv.k) + gr * (kKvGroup * D);
+    if constexpr (I8) {
+      const f32x4 *p = reinterpret_cast<const f32x4 *>(kv.ks + gr * kKvGroup + 8 * g);
+      dk[0] = p[0];
+      dk[1] = p[1];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        kf[ks] = *reinterpret_cast<const uint4 *>(base + ((4 * ks + g) * kKvGroup + 2 * n) * 8);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          kf[2 * ks + h] = *reinterpret_cast<const uint4 *>(
+              base + ((4 * ks + g) * kKvGroup + 16 * (n >> 3) + 8 * h + (n & 7)) * 8);
+    }
+  };
+  long gr = group_of(begin + wave), gr1 = group_of(begin + wave + kMassWaves);
+  load_k(gr);
+
+  // this lane's query (rows behind the tile's last repeat it)
+  int tok;
+  const int row = r0 + min(n, nr - 1);
+  const float *q = query_of(a, s, head, row, tok) + (size_t)(head * a.group + row - tok * a.group) * D + 8 * g;
+  const int p = s.first + tok;
+  const float one = opaque_one();
+  f16x8 qh[KS], ql[KS];
+  float c;
+  {
+    float x[KS][8], mx = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      load8(q + 32 * ks, a.wide_q, x[ks]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
+    }
+    mx = max_groups(mx);
+    // scaled into [2^13, 2^14): both halves keep their bits
+    const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
+    const float up = ldexp1(1.f, 14 - X);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[ks][i] *= up;
+      split2(x[ks], one, qh[ks], ql[ks]);
+    }
+    c = ldexp1(a.scale * kLog2e, X - 14 + (I8 ? 9 : 0));
+  }
+  float *scores = w.scores + ((size_t)tile * w.m.slots + n) * ((size_t)w.groups * kKvGroup);
+  float m = kUnsetMax, l = 0.f;
+  for (int i = begin + wave; i < end; i += kMassWaves) {
+    const int first = i * kKvGroup;
+    const bool there = gr >= 0;
+    f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f16x8 kx;
+        if constexpr (I8)
+          kx = h == 0 ? from_codes(kf[ks].x, kf[ks].y) : from_codes(kf[ks].z, kf[ks].w);
+        else
+          kx = __builtin_bit_cast(f16x8, kf[2 * ks + h]);
+        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, qh[ks], sc[h], 0, 0, 0);
+        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, ql[ks], sc[h], 0, 0, 0);
+      }
+    float x[8], most = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float k = I8 ? dk[j >> 2][j & 3] * c : c;
+      // token first + 8 g + j
+      x[j] = there && first + 8 * g + j <= p ? seen_score(sc[j >> 2][j & 3] * k) : -INFINITY;
+      most = fmaxf(most, x[j]);
+    }
+    gr = gr1;
+    load_k(gr);
+    gr1 = group_of(i + 2 * kMassWaves);
+    l *= __builtin_amdgcn_exp2f(m - most);
+    m = most;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l += __builtin_amdgcn_exp2f(x[j] - m);
+    if (n < nr) {
+      f32x4 *to = reinterpret_cast<f32x4 *>(scores + first + 8 * g);
+      to[0] = f32x4{x[0], x[1], x[2], x[3]};
+      to[1] = f32x4{x[4], x[5], x[6], x[7]};
+    }
+  }
+  const float all = max_groups(m);
+  l = sum_groups(l * __builtin_amdgcn_exp2f(m - all));
+  if (g == 0) part[wave][n] = float2{all, l};
+  __syncthreads();
+  if (threadIdx.x < kMassRows) {
+    float2 o = part[0][threadIdx.x];
+#pragma unroll
+    for (int v = 1; v < kMassWaves; ++v) {
+      const float2 x = part[v][threadIdx.x];
+      const float top = fmaxf(o.x, x.x);
+      o.y = o.y * __builtin_amdgcn_exp2f(o.x - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
+      o.x = top;
+    }
+    w.stats[((size_t)tile * w.m.chunks + chunk) * kMassRows + threadIdx.x] = o;
+  }
+}
+
+// A chunk of the tokens of a sequence and head: their weights, summed over its rows.
+__global__ __launch_bounds__(kMassThreads) void k_mass_add(KvView kv, nx_kv_batch b, MassCall a, NarrowWork w) {
+  __shared__ long before[kMassWaves];
+  __shared__ float2 part[kMassThreads / kMassRows][kMassRows];
+  __shared__ float e[kMassRows];
+  const int unit = blockIdx.x / w.m.chunks, chunk = blockIdx.x % w.m.chunks;
+  const int seq = unit / kv.heads, head = unit % kv.heads;
+  const KvSeq s = kv_seq(b, seq, kv.page_log2);
+  const int tiles = row_tiles(a, s), begin = chunk * w.m.share * kKvGroup, end = min(begin + w.m.share * kKvGroup, s.len);
+  if (tiles == 0 || begin >= end) return;
+  // the sequence's first tile
+  long base = 0;
+  for (int i = threadIdx.x; i < seq; i += kMassThreads) base += row_tiles(a, kv_seq(b, i, kv.page_log2)) * kv.heads;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) base += __shfl_xor(base, d, 64);
+  if ((threadIdx.x & 63) == 0) before[threadIdx.x >> 6] = base;
+  __syncthreads();
+  base = head * tiles;
+#pragma unroll
+  for (int i = 0; i < kMassWaves; ++i) base += before[i];
+  if (base + tiles > w.m.tiles) return;  // (sequences that share rows have more than there is room for)
+
+  const int parts = (s.len + w.m.share * kKvGroup - 1) / (w.m.share * kKvGroup);
+  constexpr int kSub = kMassThreads / kMassRows, kTokens = 64 * kKvGroup / kMassThreads;
+  float sum[kTokens];
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) sum[i] = 0.f;
+  for (int t = 0; t < tiles; ++t) {
+    const int nr = min(kMassRows, rows_of(a, s) - t * kMassRows), r = threadIdx.x % kMassRows, sub = threadIdx.x / kMassRows;
+    float2 o = {kUnsetMax, 0.f};
+    for (int i = sub; i < parts; i += kSub) {
+      const float2 x = w.stats[((size_t)(base + t) * w.m.chunks + i) * kMassRows + r];
+      const float top = fmaxf(o.x, x.x);
+      o.y = o.y * __builtin_amdgcn_exp2f(o.x - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
+      o.x = top;
+    }
+    part[sub][r] = o;
+    __syncthreads();
+    if (threadIdx.x < kMassRows) {
+#pragma unroll
+      for (int i = 1; i < kSub; ++i) {
+        const float2 x = part[i][r];
+        const float top = fmaxf(o.x, x.x);
+        o.y = o.y * __builtin_amdgcn_exp2f(o.x - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
+        o.x = top;
+      }
+      e[r] = log_sum(o.x, o.y);
+    }
+    __syncthreads();
+    const float *scores = w.scores + (size_t)(base + t) * w.m.slots * ((size_t)w.groups * kKvGroup);
+    for (int i = 0; i < nr; ++i, scores += (size_t)w.groups * kKvGroup) {
+      const float ei = e[i];
+#pragma unroll
+      for (int u = 0; u < kTokens; ++u) {
+        const int j = begin + (int)threadIdx.x + u * kMassThreads;
+        const float x = j < end ? scores[j] : -INFINITY;
+        sum[u] += x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - ei);
+      }
+    }
+    __syncthreads();  // e and part are read
+  }
+#pragma unroll
+  for (int u = 0; u < kTokens; ++u) {
+    const int j = begin + (int)threadIdx.x + u * kMassThreads;
+    if (j < end) add_to(a, s, unit, j, sum[u]);
+  }
+}
+
+// ------------------------------------------------------------ many rows
+struct WideWork {
+  MassWide m;
+  int groups;     // of the page table
+  float *e;       // [rows][heads]
+  float *part;    // k_mass_stats: [rows][heads][key_parts] {maximum, sum}; k_mass_columns: [tiles][row_parts][tokens]
+};
+
+__device__ __forceinline__ size_t stat_of(const MassCall &a, const KvSeq &s, int head, int row) {
+  const int tok = by_group(row, a.magic, a.shift);
+  return (size_t)(s.row + tok) * a.heads + head * a.group + (row - tok * a.group);
+}
+
+// 128 rows against a share of the keys: each row's maximum and sum.  As in k_attn_tile, the
+// four waves take a group's keys from LDS, each for 32 rows; a lane holds 16 keys' scores of a row.
+template <int FMT, int D>
+__global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_stats(KvView kv, nx_kv_batch b, MassCall a,
+                                                                             WideWork w) {
+  using E = kv_elem<FMT>;
+  constexpr bool I8 = FMT == NX_KV_INT8;
+  constexpr int KS = D / 16;
+  constexpr int C = kKvGroup * D * (int)sizeof(E) / 16;  // 16-byte chunks of a group's keys
+  constexpr int L = (C + kMassThreads - 1) / kMassThreads;
+  __shared__ f16x8 keys[2][kKvGroup * D / 8];
+  __shared__ float scales[2][kKvGroup];
+  __shared__ long sums[kMassWaves];
+  __shared__ Place found;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+  const float one = opaque_one();
+  for (int u = blockIdx.x;; u += gridDim.x) {
+    __syncthreads();  // the last unit's reads of LDS
+    const int chunk = u % w.m.key_parts;
+    const Place at = find_item<kMassWaves>(
+        kv, b, u / w.m.key_parts,
+        [&](const KvSeq &q) { return (rows_of(a, q) + kMassTile - 1) / kMassTile * kv.heads; }, sums, &found);
+    if (at.s < 0) return;
+    const KvSeq s = at.seq;
+    const int rows = rows_of(a, s), tiles = (rows + kMassTile - 1) / kMassTile;
+    const int head = at.at / tiles, r0 = (at.at - head * tiles) * kMassTile, nr = min(kMassTile, rows - r0);
+    const int row = r0 + min(32 * wave + n, nr - 1), tok = by_group(row, a.magic, a.shift), p = s.first + tok;
+    const int pmin = uniform(s.first + by_group(r0 + min(32 * wave, nr - 1), a.magic, a.shift));
+    const int pmax = uniform(s.first + by_group(r0 + min(32 * wave + 31, nr - 1), a.magic, a.shift));
+    const int last = min(s.first + by_group(r0 + nr - 1, a.magic, a.shift), s.len - 1);
+    const int begin = chunk * w.m.key_share, end = min(begin + w.m.key_share, last < 0 ? 0 : last / kKvGroup + 1);
+    float m = kUnsetMax, l = 0.f;
+    if (begin < end) {
+      f16x8 qh[KS], ql[KS];
+      float c;
+      {
+        const float *q = a.q + (size_t)(s.row + tok) * a.q_stride +
+                         (size_t)(head * a.group + row - tok * a.group) * D + 8 * h;
+        float x[KS][8], mx = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          load8(q + 16 * ks, a.wide_q, x[ks]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
+        }
+        mx = max_halves(mx);
+        const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
+        const float up = ldexp1(1.f, 14 - X);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[ks][i] *= up;
+          split2(x[ks], one, qh[ks], ql[ks]);
+        }
+        c = ldexp1(a.scale * kLog2e, X - 14 + (I8 ? 9 : 0));
+      }
+      // groups on their way: registers, then LDS
+      uint4 rk[L];
+      float rs = 0.f;
+      long gr = kv_group(kv, b, at.s, head, begin * kKvGroup);
+      auto fetch = [&](int i) {
+        const bool there = gr >= 0;
+        const long from = max(gr, 0L);
+        gr = kv_group(kv, b, at.s, head, min(i + 1, end - 1) * kKvGroup);
+        const uint4 *gk = reinterpret_cast<const uint4 *>(kv.k) + from * C;
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+          const int x = threadIdx.x + kMassThreads * j;
+          if (C % kMassThreads == 0 || x < C) rk[j] = gk[x];
+        }
+        if (I8 && threadIdx.x < kKvGroup) rs = kv.ks[from * kKvGroup + threadIdx.x];
+        return there;
+      };
+      auto stage = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+          const int x = threadIdx.x + kMassThreads * j;
+          if (C % kMassThreads != 0 && x >= C) break;
+          if constexpr (I8) {
+            // rows 2 y, 2 y + 1 of a key chunk: tokens t and t + 4
+            const int d8 = x >> 4, t = kv_token(NX_KV_INT8, (x & 15) * 2);
+            keys[buf][d8 * kKvGroup + kv_row(NX_KV_F16, t)] = from_codes(rk[j].x, rk[j].y);
+            keys[buf][d8 * kKvGroup + kv_row(NX_KV_F16, t + 4)] = from_codes(rk[j].z, rk[j].w);
+          } else {
+            keys[buf][x] = __builtin_bit_cast(f16x8, rk[j]);
+          }
+        }
+        if (I8 && threadIdx.x < kKvGroup) scales[buf][threadIdx.x] = rs;
+      };
+      bool there = fetch(begin), there1 = false;
+      stage(begin & 1);
+      if (begin + 1 < end) there1 = fetch(begin + 1);
+      for (int i = begin; i < end; ++i) {
+        const int buf = i & 1, first = i * kKvGroup;
+        __syncthreads();  // group i is in LDS, and no wave reads group i - 1 any more
+        const bool here = there;
+        there = there1;
+        if (i + 1 < end) {
+          stage(buf ^ 1);
+          if (i + 2 < end) there1 = fetch(i + 2);
+        }
+        if (!here || first > pmax) continue;  // nothing that the wave's rows see
+        const f16x8 *k8 = keys[buf] + h * kKvGroup + n;
+        f32x16 sc;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[j] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const f16x8 kx = k8[2 * ks * kKvGroup];
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, qh[ks], sc, 0, 0, 0);
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, ql[ks], sc, 0, 0, 0);
+        }
+        // score j: token first + 16 (j / 8) + 8 h + j % 8
+        float x[16], most = m;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int t = 16 * (j >> 3) + 8 * h + (j & 7);
+          x[j] = sc[j] * (I8 ? scales[buf][t] * c : c);
+        }
+        if (first + kKvGroup - 1 > pmin) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (16 * (j >> 3) + (j & 7) > p - first - 8 * h) x[j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) most = fmaxf(most, x[j]);
+        l *= __builtin_amdgcn_exp2f(m - most);
+        m = most;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) l += __builtin_amdgcn_exp2f(x[j] - m);
+      }
+    }
+    const float all = max_halves(m);
+    l = across_halves(l * __builtin_amdgcn_exp2f(m - all), [](float x, float y) { return x + y; });
+    if (h == 0 && 32 * wave + n < nr) {
+      const size_t o = stat_of(a, s, head, row);
+      if (w.m.key_parts == 1)
+        w.e[o] = log_sum(all, l);
+      else
+        reinterpret_cast<float2 *>(w.part)[o * w.m.key_parts + chunk] = float2{all, l};
+    }
+  }
+}
+
+// e of each row, from its parts
+__global__ __launch_bounds__(kMassThreads) void k_mass_join(nx_kv_batch b, MassCall a, WideWork w, long rows) {
+  for (long r = (long)blockIdx.x * kMassThreads + threadIdx.x; r < rows; r += (long)gridDim.x * kMassThreads) {
+    const float2 *p = reinterpret_cast<const float2 *>(w.part) + r * w.m.key_parts;
+    float2 o = {kUnsetMax, 0.f};
+    for (int i = 0; i < w.m.key_parts; ++i) {
+      const float2 x = p[i];
+      const float top = fmaxf(o.x, x.x);
+      o.y = o.y * __builtin_amdgcn_exp2f(o.x - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
+      o.x = top;
+    }
+    w.e[r] = log_sum(o.x, o.y);
+  }
+}
+
+// groups of keys that a wave holds
+template <int D>
+constexpr int kHeldGroups = D == 256 ? 1 : 2;
+template <int D>
+constexpr int kKeyTile = kMassWaves * kHeldGroups<D>;  // of a workgroup
+
+// In a 32-row tile's accumulator, register j of half h is row 8 (j / 4) + 4 h + j % 4: the token
+// kv_token of h = 0, and so many behind it
+template <int FMT>
+constexpr int kTokenOfHalf = kv_token(FMT, 4);
+
+// the first block of rows that sees a tile of keys, and the sequence's blocks
+__device__ __forceinline__ int first_block(const MassCall &a, const KvSeq &s, int token) {
+  return (int)((long)max(token - s.first, 0) * a.group / kMassBlock);
+}
+
+// A tile of keys against a share of the rows: each wave holds its groups' keys in registers, and
+// blocks of 32 rows go by in LDS, as two halves in operand order.  Score j of a lane is a key's,
+// and the lane's column a row's: sums over rows stay in the lane until the end.
+template <int FMT, int D>
+__global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns(KvView kv, nx_kv_batch b, MassCall a,
+                                                                               WideWork w) {
+  using E = kv_elem<FMT>;
+  constexpr bool I8 = FMT == NX_KV_INT8;
+  constexpr int KS = D / 16, KG = kHeldGroups<D>, C8 = D / 8, Q = (C8 + 7) / 8;
+  __shared__ f16x8 query[2][2][C8 * kMassBlock];  // [buffer][half]
+  __shared__ float coef[2][kMassBlock], lse[2][kMassBlock];
+  __shared__ int token[2][kMassBlock];
+  __shared__ __align__(16) float scales[kMassWaves][KG][2][16];  // INT8: of the keys, as lanes hold their scores
+  __shared__ long sums[kMassWaves];
+  __shared__ Place found;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+  const float one = opaque_one();
+  auto row_parts = [&](const KvSeq &q) {
+    const int blocks = (rows_of(a, q) + kMassBlock - 1) / kMassBlock;
+    return (blocks + w.m.row_share - 1) / w.m.row_share;
+  };
+  auto key_tiles = [&](const KvSeq &q) { return (q.len + kKeyTile<D> * kKvGroup - 1) / (kKeyTile<D> * kKvGroup); };
+  for (int u = blockIdx.x;; u += gridDim.x) {
+    __syncthreads();  // the last unit's reads of LDS
+    const Place at = find_item<kMassWaves>(
+        kv, b, u, [&](const KvSeq &q) { return row_parts(q) * key_tiles(q) * kv.heads; }, sums, &found);
+    if (at.s < 0) return;
+    const KvSeq s = at.seq;
+    const int parts = row_parts(s), tiles = key_tiles(s), rows = rows_of(a, s);
+    const int head = at.at / (parts * tiles), rest = at.at - head * parts * tiles, kt = rest / parts, part = rest - kt * parts;
+    const int k0 = kt * kKeyTile<D> * kKvGroup;
+    const int from = max(part * w.m.row_share, first_block(a, s, k0));
+    const int to = min((part + 1) * w.m.row_share, (rows + kMassBlock - 1) / kMassBlock);
+    if (from >= to) continue;
+
+    // ---- the wave's keys: row n of a group in the cache's order
+    f16x8 kx[KG][KS];
+    bool there[KG];
+#pragma unroll
+    for (int i = 0; i < KG; ++i) {
+      const int first = k0 + (wave * KG + i) * kKvGroup;
+      const long gr = first < s.len ? kv_group(kv, b, at.s, head, first) : -1;
+      there[i] = gr >= 0;
+      const E *base = reinterpret_cast<const E *>(kv.k) + max(gr, 0L) * (kKvGroup * D) + (h * kKvGroup + n) * 8;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        if constexpr (I8) {
+          const uint2 x = *reinterpret_cast<const uint2 *>(base + 2 * j * kKvGroup * 8);
+          kx[i][j] = from_codes(x.x, x.y);
+        } else {
+          kx[i][j] = *reinterpret_cast<const f16x8 *>(base + 2 * j * kKvGroup * 8);
+        }
+      }
+      if constexpr (I8) {
+        if (n < 16) scales[wave][i][h][n] = kv.ks[max(gr, 0L) * kKvGroup + kv_token(FMT, 8 * (n >> 2) + 4 * h + (n & 3))];
+      }
+    }
+    float sum[KG][16];
+#pragma unroll
+    for (int i = 0; i < KG; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
+
+    // ---- blocks of rows on their way: eight threads of a row
+    const int qr = threadIdx.x >> 3, sub = threadIdx.x & 7;
+    float x[Q][8], e = 0.f;
+    auto fetch = [&](int block) {
+      const int row = min(block * kMassBlock + qr, rows - 1), tok = by_group(row, a.magic, a.shift);
+      const float *q = a.q + (size_t)(s.row + tok) * a.q_stride + (size_t)(head * a.group + row - tok * a.group) * D;
+#pragma unroll
+      for (int i = 0; i < Q; ++i)
+        if (C8 % 8 == 0 || sub + 8 * i < C8) load8(q + 8 * (sub + 8 * i), a.wide_q, x[i]);
+      if (sub == 0) e = w.e[stat_of(a, s, head, row)];
+    };
+    auto stage = [&](int block, int buf) {
+      float mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < Q; ++i)
+        if (C8 % 8 == 0 || sub + 8 * i < C8)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(x[i][j]));
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 8));
+      const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
+      const float up = ldexp1(1.f, 14 - X);
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        if (C8 % 8 != 0 && sub + 8 * i >= C8) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] *= up;
+        split2(x[i], one, query[buf][0][(sub + 8 * i) * kMassBlock + qr], query[buf][1][(sub + 8 * i) * kMassBlock + qr]);
+      }
+      if (sub == 0) {
+        const int row = block * kMassBlock + qr;
+        coef[buf][qr] = ldexp1(a.scale * kLog2e, X - 14 + (I8 ? 9 : 0));
+        lse[buf][qr] = e;
+        // (rows behind the last see nothing)
+        token[buf][qr] = row < rows ? s.first + by_group(row, a.magic, a.shift) : -1;
+      }
+    };
+    fetch(from);
+    stage(from, from & 1);
+    if (from + 1 < to) fetch(from + 1);
+    for (int block = from; block < to; ++block) {
+      const int buf = block & 1;
+      __syncthreads();  // the block is in LDS, and no wave reads the one before any more
+      if (block + 1 < to) {
+        stage(block + 1, buf ^ 1);
+        if (block + 2 < to) fetch(block + 2);
+      }
+      const float c = coef[buf][n], ei = lse[buf][n];
+      const int p = token[buf][n];
+      const int pmin = uniform(block * kMassBlock + kMassBlock <= rows ? token[buf][0] : -1);
+      const int pmax = s.first + by_group(min(block * kMassBlock + kMassBlock, rows) - 1, a.magic, a.shift);
+      const f16x8 *qh = query[buf][0] + h * kMassBlock + n, *ql = query[buf][1] + h * kMassBlock + n;
+      const int first = k0 + wave * KG * kKvGroup;
+      if (first > pmax) continue;
+      f32x16 sc[KG];
+#pragma unroll
+      for (int i = 0; i < KG; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[i][j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const f16x8 hi = qh[2 * j * kMassBlock], lo = ql[2 * j * kMassBlock];
+#pragma unroll
+        for (int i = 0; i < KG; ++i) {
+          sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[i][j], hi, sc[i], 0, 0, 0);
+          sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[i][j], lo, sc[i], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < KG; ++i) {
+        const int g0 = first + i * kKvGroup;
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], I8 ? scales[wave][i][h][j] * c : c, -ei));
+        if (g0 + kKvGroup - 1 > pmin) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (kv_token(FMT, 8 * (j >> 2) + (j & 3)) > p - g0 - kTokenOfHalf<FMT> * h) y[j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[i][j] += y[j];
+        __builtin_amdgcn_sched_barrier(0);  // one group's weights at a time: registers
+      }
+    }
+
+    // ---- over the lanes' rows; lane n takes sum n
+    const size_t unit = (size_t)at.s * kv.heads + head;
+#pragma unroll
+    for (int i = 0; i < KG; ++i) {
+      float mine = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float v = sum[i][j];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) v += __shfl_xor(v, d, 32);
+        if (n == j) mine = v;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (n >= 16) continue;
+      const int j = k0 + (wave * KG + i) * kKvGroup + kv_token(FMT, 8 * (n >> 2) + 4 * h + (n & 3));
+      if (j >= s.len) continue;
+      if (!there[i]) mine = 0.f;
+      if (parts == 1)
+        add_to(a, s, unit, j, mine);
+      else
+        w.part[(unit * w.m.row_parts + part) * ((size_t)w.groups * kKvGroup) + j] = mine;
+    }
+  }
+}
+
+// Sums the parts of sequences whose rows were shared out, in their order.
+__global__ __launch_bounds__(kMassThreads) void k_mass_sum(KvView kv, nx_kv_batch b, MassCall a, WideWork w, int key_tile) {
+  __shared__ long sums[kMassWaves];
+  __shared__ Place found;
+  for (int u = blockIdx.x;; u += gridDim.x) {
+    __syncthreads();  // found is read
+    auto parts = [&](const KvSeq &q) {
+      const int blocks = (rows_of(a, q) + kMassBlock - 1) / kMassBlock;
+      return (blocks + w.m.row_share - 1) / w.m.row_share;
+    };
+    const Place at = find_item<kMassWaves>(
+        kv, b, u,
+        [&](const KvSeq &q) { return parts(q) > 1 ? (q.len + kMassThreads - 1) / kMassThreads * kv.heads : 0; }, sums,
+        &found);
+    if (at.s < 0) return;
+    const KvSeq s = at.seq;
+    const int each = (s.len + kMassThreads - 1) / kMassThreads, head = at.at / each;
+    const int j = (at.at - head * each) * kMassThreads + (int)threadIdx.x;
+    if (j >= s.len) continue;
+    const size_t unit = (size_t)at.s * kv.heads + head;
+    float sum = 0.f;
+    for (int i = first_block(a, s, j / (key_tile * kKvGroup) * (key_tile * kKvGroup)) / w.m.row_share; i < parts(s); ++i)
+      sum += w.part[(unit * w.m.row_parts + i) * ((size_t)w.groups * kKvGroup) + j];
+    add_to(a, s, unit, j, sum);
+  }
+}
+
+// The memory of scores and statistics: of one size for every call, allocated once, never moved.
+static int mass_workspace(nx_ctx *c, float **out) {
+  DevBuf &ws = c->ws[WS_MASS];
+  if (!ws.ptr) {
+    NX_TRY(refuse_capture(c));
+    void *p = nullptr;
+    if (hipMalloc(&p, kMassFloats * 4) != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(NX_ERR_OOM, "device allocation of " + std::to_string(kMassFloats * 4) + " bytes failed");
+    }
+    ws = {p, kMassFloats * 4};
+  }
+  *out = static_cast<float *>(ws.ptr);
+  return NX_OK;
+}
+
+// The most rows of a sequence in 16-row tiles, where the batch has longer ones
+constexpr int kMassFew = 16;
+
+static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall a) {
+  a.wide_q = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_stride % 4 == 0;
+  a.shift = group_shift(a.group);
+  a.magic = group_magic(a.group);
+  float *ws;
+  NX_TRY(mass_workspace(c, &ws));
+  const KvView view = view_of(kv);
+  const int groups = all.max_pages * (kv->page_tokens / kKvGroup);
+  // Only the device knows the sequences' rows.  With one or more in each, one has at most
+  // num_tokens - num_seqs + 1; a batch that leaves sequences out for a long one is right on 16-row tiles too.
+  const MassNarrow n = mass_narrow(all.num_seqs, all.num_tokens, a.group, kv->heads, groups);
+  const bool wide = n.seqs == 0 || ((long)all.num_tokens - all.num_seqs + 1) * a.group > kMassFew;
+  a.rows_above = 0;
+  a.rows_upto = n.seqs == 0 ? 0 : wide ? kMassFew : INT32_MAX;
+  for (int s0 = 0; s0 < all.num_seqs && n.seqs > 0; s0 += n.seqs) {
+    nx_kv_batch b = all;
+    b.num_seqs = std::min(n.seqs, all.num_seqs - s0);
+    b.row_start += s0;
+    b.kv_len += s0;
+    b.pages += (size_t)s0 * b.max_pages;
+    MassCall on = a;
+    const size_t skip = (size_t)s0 * kv->heads * a.mass_stride;
+    on.mass += skip;
+    if (on.before) on.before += skip;
+    const NarrowWork w{n, groups, ws, reinterpret_cast<float2 *>(ws + n.tiles * n.slots * groups * kKvGroup)};
+    NX_TRY(launch(c, "mass_scores", [&] {
+      with_kernel(kv, [&](auto fmt, auto D) {
+        go(c, k_mass_scores<fmt(), D()>, dim3((uint32_t)(n.tiles * n.chunks)), dim3(kMassThreads), 0, view, b, on, w);
+      });
+    }));
+    NX_TRY(launch(c, "mass_add", [&] {
+      go(c, k_mass_add, dim3((uint32_t)b.num_seqs * kv->heads * n.chunks), dim3(kMassThreads), 0, view, b, on, w);
+    }));
+  }
+  if (!wide) return NX_OK;
+  a.rows_above = a.rows_upto;
+  a.rows_upto = INT32_MAX;
+  const int key_tile = kv->D == 256 ? kKeyTile<256> : kKeyTile<128>;
+  const MassWide m = mass_wide(all.num_seqs, all.num_tokens, a.heads, kv->heads, groups, key_tile);
+  const WideWork w{m, groups, ws, ws + (kMassFloats - mass_part_floats(all.num_tokens, a.heads))};
+  const long columns = (long)all.num_seqs * kv->heads * m.row_parts * ((groups + key_tile - 1) / key_tile);
+  if (std::max(columns, (long)all.num_seqs * kv->heads * (groups / 8 + 1)) > INT32_MAX)
+    return fail(NX_ERR_UNSUPPORTED, "page tables of more than 2^31 tiles");
+  const dim3 grid(2 * c->num_cu), block(kMassThreads);
+  NX_TRY(launch(c, "mass_stats", [&] {
+    with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_stats<fmt(), D()>, grid, block, 0, view, all, a, w); });
+  }));
+  if (m.key_parts > 1)
+    NX_TRY(launch(c, "mass_join", [&] {
+      go(c, k_mass_join, grid, block, 0, all, a, w, (long)all.num_tokens * a.heads);
+    }));
+  NX_TRY(launch(c, "mass_columns", [&] {
+    with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_columns<fmt(), D()>, grid, block, 0, view, all, a, w); });
+  }));
+  if (m.row_parts == 1) return NX_OK;
+  return launch(c, "mass_sum", [&] { go(c, k_mass_sum, grid, block, 0, view, all, a, w, key_tile); });
+}
+
+static int attention_mass(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const float *q, size_t q_stride, int heads,
+                          float scale, const float *before, float *mass, size_t mass_stride, bool host) {
+  NX_TRY(kv_check_call(c, kv, b));
+  NX_TRY(refuse(attn_check(heads, kv->heads, scale, 0, 0)));
+  if (b->num_seqs == 0 || b->num_tokens == 0) return NX_OK;
+  const size_t width = (size_t)heads * kv->D;
+  NX_TRY(refuse(mass_check(b, kv->heads, heads, q_stride, width, q, before, mass, mass_stride)));
+  MassCall a{q, before, mass, q_stride, mass_stride, heads, heads / kv->heads, scale};
+  if (!host) return mass_dev(c, kv, *b, a);
+  NX_TRY(refuse(kv_check_tables(*b, kv->pages, kv->page_tokens, true, false)));
+  const size_t rows = b->row_start[b->num_seqs], tiles = (size_t)b->num_seqs * kv->heads;
+  if (rows == (size_t)b->row_start[0]) return NX_OK;
+  size_t most = 1;
+  for (int s = 0; s < b->num_seqs; ++s) most = std::max(most, (size_t)b->kv_len[s]);
+  most = std::min(most, mass_stride);
+  nx_kv_batch dev;
+  NX_TRY(kv_upload_batch(c, *b, &dev));
+  void *dq, *dm;
+  NX_TRY(ws_get(c, WS_XIN, rows * width * 4, &dq));
+  NX_TRY(ws_get(c, WS_OUT, tiles * most * 4, &dm));
+  NX_HIP(hipMemcpy2DAsync(dq, width * 4, q, q_stride * 4, width * 4, rows, hipMemcpyHostToDevice, c->stream));
+  if (before)
+    NX_HIP(hipMemcpy2DAsync(dm, most * 4, before, mass_stride * 4, most * 4, tiles, hipMemcpyHostToDevice, c->stream));
+  a.q = static_cast<const float *>(dq);
+  a.q_stride = width;
+  a.mass = static_cast<float *>(dm);
+  a.before = before ? a.mass : nullptr;
+  a.mass_stride = most;
+  dev.num_tokens = (int)rows;
+  NX_TRY(mass_dev(c, kv, dev, a));
+  for (int s = 0; s < b->num_seqs; ++s) {  // (sequences without rows, and what is behind the others, stay the caller's)
+    const size_t len = std::min((size_t)b->kv_len[s], most), at = (size_t)s * kv->heads;
+    if (len && b->row_start[s + 1] > b->row_start[s])
+      NX_HIP(hipMemcpy2DAsync(mass + at * mass_stride, mass_stride * 4, a.mass + at * most, most * 4, len * 4, kv->heads,
+                              hipMemcpyDeviceToHost, c->stream));
+  }
+  NX_HIP(hipStreamSynchronize(c->stream));
+  return NX_OK;
+}
+
+}  // namespace nx
+
+using namespace nx;
+
+extern "C" {
+
+int nx_attention_mass(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const float *q, size_t q_stride, int heads,
+                      float scale, const float *before, float *mass, size_t mass_stride) {
+  return guarded([&] { return attention_mass(c, kv, b, q, q_stride, heads, scale, before, mass, mass_stride, true); });
+}
+int nx_attention_mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const float *q, size_t q_stride, int heads,
+                          float scale, const float *before, float *mass, size_t mass_stride) {
+  return guarded([&] { return attention_mass(c, kv, b, q, q_stride, heads, scale, before, mass, mass_stride, false); });
+}
+
+}  // extern "C"

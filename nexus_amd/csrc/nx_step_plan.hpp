@@ -89,6 +89,70 @@ inline Refusal logprobs_check(const float *logits, size_t stride, int rows, int 
   return {};
 }
 
+// What the calls that gather attention weights check besides attn_check.
+inline Refusal mass_check(const nx_kv_batch *b, int kv_heads, int heads, size_t q_stride, size_t width, const float *q,
+                          const float *before, const float *mass, size_t mass_stride) {
+  if (!q || !mass) return {NX_ERR_INVALID_ARG, "null buffer"};
+  if ((int64_t)b->num_tokens * heads > (1 << 24)) return {NX_ERR_UNSUPPORTED, "more than 2^24 query heads"};
+  if (q_stride > (size_t)1 << 40 || mass_stride > (size_t)1 << 40) return {NX_ERR_UNSUPPORTED, "row stride above 2^40"};
+  if (Refusal f = kv_check_rows("query", (long)q_stride, (long)width)) return f;
+  if (mass_stride == 0) return {NX_ERR_SHAPE, "rows of no weights"};
+  if (before && before != mass &&
+      rows_overlap(before, mass_stride, mass_stride, mass, mass_stride, mass_stride, (long)b->num_seqs * kv_heads))
+    return {NX_ERR_INVALID_ARG, "the weights overlap those before in part"};
+  return {};
+}
+
+// How a batch's gathered weights are worked out (nx_mass.hip).  `groups`: of 32 tokens of the
+// page table; `group`: query heads of a key/value head.
+constexpr int kMassRows = 16, kMassTile = 128, kMassBlock = 32;
+constexpr size_t kMassFloats = (size_t)1 << 26;  // of the workspace
+// tiles of 16 rows whose scores are stored: `seqs` sequences at once
+struct MassNarrow {
+  int seqs;           // 0: not even one fits
+  int share, chunks;  // groups of a chunk, chunks of the table
+  int slots;          // rows of a tile that have room
+  long tiles;         // at most, of `seqs` sequences
+};
+inline MassNarrow mass_narrow(int seqs, int rows, int group, int kv_heads, int groups) {
+  MassNarrow m{};
+  const long want = (long)seqs * kv_heads * groups / 8192;
+  m.share = 4;
+  while (m.share < 64 && m.share < want) m.share *= 2;
+  m.chunks = (groups + m.share - 1) / m.share;
+  const long all = (long)rows * group;
+  m.slots = (int)std::min<long>(kMassRows, all);
+  const size_t tile = (size_t)m.slots * groups * kKvGroup + (size_t)m.chunks * kMassRows * 2;
+  const long most = (long)(kMassFloats / tile), extra = all / kMassRows;
+  // sequences of n rows have at most n group / 16 + 1 tiles of each head
+  const long fit = most / kv_heads - extra;
+  m.seqs = (int)std::max(0L, std::min<long>(seqs, fit));
+  m.tiles = (m.seqs + extra) * kv_heads;
+  return m;
+}
+// tiles of 128 rows against shares of the keys (k_mass_stats), and of keys against shares of the
+// rows (k_mass_columns), whose parts are put together
+struct MassWide {
+  int key_share, key_parts;  // groups; parts of the table
+  int row_share, row_parts;  // blocks of 32 rows; parts of a sequence of all rows
+};
+constexpr size_t mass_part_floats(int rows, int heads) { return kMassFloats - ((size_t)rows * heads + 3) / 4 * 4; }
+inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int groups, int key_tile) {
+  const long group = heads / kv_heads, all = rows * group, room = (long)mass_part_floats(rows, heads);
+  const long tiles = kv_heads * ((all + kMassTile - 1) / kMassTile), blocks = (all + kMassBlock - 1) / kMassBlock;
+  MassWide m{};
+  long parts = std::min({4096 / tiles, (long)groups / 4, room / ((long)rows * heads * 2)});
+  parts = std::max(parts, 1L);
+  m.key_share = (int)((groups + parts - 1) / parts);
+  m.key_parts = (groups + m.key_share - 1) / m.key_share;
+  const long columns = (long)kv_heads * ((groups + key_tile - 1) / key_tile);
+  parts = std::min({2048 / columns, blocks / 4, room / ((long)seqs * kv_heads * groups * kKvGroup)});
+  parts = std::max(parts, 1L);
+  m.row_share = (int)((blocks + parts - 1) / parts);
+  m.row_parts = (int)((blocks + m.row_share - 1) / m.row_share);
+  return m;
+}
+
 // The arguments of an eviction besides the cache and the batch.
 struct EvictArgs {
   const int32_t *to_pages;

@@ -97,3 +97,44 @@ def evicted(mass, length, keep, sinks, recent):
     weight = [(-np.inf, 0) if j >= len(mass) or np.isnan(mass[j]) else (float(mass[j]), 1) for j in range(length)]
     best = sorted(middle, key=lambda j: (-weight[j][1], -weight[j][0], j))[:keep - sinks - recent]
     return np.array(sorted(list(range(sinks)) + best + list(range(length - recent, length))), int)
+
+
+def attention_mass(batch, k, q, heads, scale, before=None, width=None):
+    """mass [seqs x G x width] of keys k [sum(lens) x G x D] that the cache holds, and a bound.
+
+    The bound: a score's terms are each some 2^-21 off and their sum D 2^-24 of the sum of
+    magnitudes, against the row's other scores too, and 2^x 2^-21: e of kv_cases.attention.  The row's
+    log sum adds its N + 64 roundings, its own place and that of the difference to it, 2^-23 of
+    the score's size and log2 N.  Then come as many sums as rows and heads, 2^-24 of the whole each."""
+    G, D = k.shape[1:]
+    width = width or max(max(batch.lens), 1)
+    out = np.zeros((len(batch.ns), G, width)) if before is None else before.astype(np.float64)
+    bound = np.zeros_like(out)
+    at = 0
+    for s, (n, length) in enumerate(zip(batch.ns, batch.lens)):
+        if n:
+            rows = slice(batch.row_start[s], batch.row_start[s] + n)
+            hidden = np.arange(length)[None] > np.arange(length - n, length)[:, None]
+            out[s, :, max(length - n, 0):length] = 0
+            total, off = np.zeros((G, length)), np.zeros((G, length))
+            for h in range(heads):
+                g = h * G // heads
+                ks = k[at:at + length, g].astype(np.float64)
+                qh = q[rows, h].astype(np.float64)
+                with np.errstate(all="ignore"):
+                    x = scale * (qh @ ks.T)
+                    mag = np.where(hidden, 0, abs(scale) * (np.abs(qh) @ np.abs(ks).T)).max(1, keepdims=True)
+                    x = np.where(hidden, -np.inf, x)
+                    top = x.max(1, keepdims=True)
+                    w = np.where(hidden, 0, np.exp(x - np.where(np.isfinite(top), top, 0)))
+                    p = w / w.sum(1, keepdims=True)
+                p = np.where(hidden.all(1)[:, None], 0, p)
+                e = 2 * ((2.0 ** -21 + D * 2.0 ** -24) * mag + 2.0 ** -21)
+                part = 2 * e + (length + 64) * U + 2 * U * (1.5 * mag + np.log2(length + 1))
+                total[g] += p.sum(0)
+                off[g] += (part * p).sum(0)
+            m = min(length, width)
+            out[s, :, :m] += total[:, :m]
+            bound[s, :, :m] = off[:, :m] + (n * heads // G + 8) * U * out[s, :, :m] + 2.0 ** -120
+        at += length
+    return out, bound
