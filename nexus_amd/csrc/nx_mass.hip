@@ -27,7 +27,7 @@ struct MassCall {
   float *mass;
   size_t q_stride, mass_stride;
   int heads, group;  // query heads, and those that share a key/value head
-  float scale;
+  float scale;     // times log2(e)
   bool wide_q;     // rows of whole float4 runs
   uint32_t magic;  // by_group's
   int shift;
@@ -48,8 +48,25 @@ __device__ __forceinline__ const float *query_of(const MassCall &a, const KvSeq 
 // -infinity stands for tokens that a row does not see: a score of -infinity is the lowest number
 __device__ __forceinline__ float seen_score(float x) { return x == -INFINITY ? -3.4028234663852886e38f : x; }
 
+// What a row's scores are multiplied by, with q scale log2(e) scaled into [2^13, 2^14) (both halves
+// keep their bits) by `up`: powers of two.  mx: the largest of |q scale log2(e)|.
+struct RowScale {
+  float up, c;
+  template <bool I8>
+  static __device__ __forceinline__ RowScale of(float mx) {
+    const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
+    return {ldexp1(1.f, 14 - X), ldexp1(1.f, X - 14 + (I8 ? 9 : 0))};
+  }
+};
+
 // log2 of a row's sum: above everything where it is nothing
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l); }
+
+// the sum of two parts of a row
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x);
+  return {top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top)};
+}
 
 __device__ __forceinline__ void add_to(const MassCall &a, const KvSeq &s, size_t tile, int j, float sum) {
   if ((size_t)j >= a.mass_stride) return;
@@ -57,13 +74,43 @@ __device__ __forceinline__ void add_to(const MassCall &a, const KvSeq &s, size_t
   a.mass[at] = (a.before && j < s.first ? a.before[at] : 0.f) + sum;
 }
 
+// Groups of 32 tokens of a sequence and head, looked up in two steps: a page number is on its way
+// while the keys of the groups before it are, and nothing waits for it in between.
+struct Groups {
+  const KvView &kv;
+  const int32_t *pages;
+  int head, end;  // (behind the last one: the last)
+  __device__ __forceinline__ int page(int i) const {
+    int at = min(i, end - 1) * kKvGroup >> kv.page_log2;
+    asm volatile("" : "+v"(at));  // (a number that is known to be alike would be waited for at once)
+    return pages[at];
+  }
+  __device__ __forceinline__ bool there(int page) const { return page >= 0 && page < kv.pages; }
+  // in the pool (group 0, masked, for one that is not there); page: uniform
+  __device__ __forceinline__ long at(int i, int page) const {
+    const int in_page = (min(i, end - 1) * kKvGroup & ((1 << kv.page_log2) - 1)) / kKvGroup;
+    return there(page) ? (((long)page * kv.heads + head) << (kv.page_log2 - 5)) + in_page : 0;
+  }
+};
+__device__ __forceinline__ KvSeq uniform(const KvSeq &s) {
+  return {uniform(s.row), uniform(s.n), uniform(s.first), uniform(s.len)};
+}
+
 // ------------------------------------------------------------ few rows
 struct NarrowWork {
   MassNarrow m;
+  int head0;      // the launch's first key/value head
   int groups;     // of the page table
-  float *scores;  // [tiles][slots][groups * 32]
-  float2 *stats;  // [tiles][chunks][16] maximum and sum
+  // of each sequence's rows, head and 16-row tile: [groups][the tile's rows][32] scores, and a
+  // maximum and sum [the tile's rows][chunks]
+  float *scores;
+  float2 *stats;
 };
+// the first row of a tile, in rows of the whole batch (or 16 of each sequence)
+__device__ __forceinline__ size_t slot_of(const MassCall &a, const NarrowWork &w, const KvSeq &s, int seq, int head, int r0) {
+  if (w.m.one_each) return ((size_t)seq * w.m.heads + (head - w.head0)) * kMassRows;
+  return ((size_t)s.row * w.m.heads + (size_t)(head - w.head0) * s.n) * a.group + r0;
+}
 
 // 16-row tiles of a sequence
 __device__ __forceinline__ int row_tiles(const MassCall &a, const KvSeq &q) {
@@ -81,12 +128,15 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
   __shared__ long sums[kMassWaves];
   __shared__ Place found;
   __shared__ float2 part[kMassWaves][kMassRows];
-  const int tile = blockIdx.x / w.m.chunks, chunk = blockIdx.x % w.m.chunks;
+  // (a chunk of all tiles after the other: late chunks, which few sequences have, on all XCDs)
+  const int tile = blockIdx.x % w.m.tiles, chunk = blockIdx.x / w.m.tiles;
   const Place at = find_item<kMassWaves>(
-      kv, b, tile, [&](const KvSeq &q) { return row_tiles(a, q) * kv.heads; }, sums, &found);
+      kv, b, tile, [&](const KvSeq &q) { return row_tiles(a, q) * w.m.heads; }, sums, &found);
   if (at.s < 0) return;
-  const KvSeq s = at.seq;
-  const int tiles = row_tiles(a, s), head = at.at / tiles, r0 = (at.at - head * tiles) * kMassRows;
+  const KvSeq s = uniform(at.seq);
+  const int seq = uniform(at.s), in_seq = uniform(at.at), tiles = row_tiles(a, s);
+  const int head = w.head0 + in_seq / tiles, r0 = in_seq % tiles * kMassRows;
+  if (head >= kv.heads) return;  // (the last heads may be fewer)
   const int nr = min(kMassRows, rows_of(a, s) - r0);
   const int begin = chunk * w.m.share, end = min(begin + w.m.share, (s.len + kKvGroup - 1) / kKvGroup);
   if (begin >= end) return;
@@ -94,9 +144,10 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
 
   uint4 kf[KL];
   f32x4 dk[2];  // INT8: scales of the lane's tokens
-  auto group_of = [&](int i) { return kv_group(kv, b, at.s, head, min(i, end - 1) * kKvGroup); };
-  auto load_k = [&](long gr) {  // (pool group 0, masked, for one that is not there)
-    gr = max(gr, 0L);
+  const Groups groups{kv, b.pages + (long)seq * b.max_pages, head, end};
+  // read once, past the scores in the L2 (142 + 21 us for the two kernels otherwise, not 138 + 18)
+  auto once = [](const E *p) { return ld_stream16(reinterpret_cast<const uint8_t *>(p)); };
+  auto load_k = [&](long gr) {
     const E *base = reinterpret_cast<const E *>(kv.k) + gr * (kKvGroup * D);
     if constexpr (I8) {
       const f32x4 *p = reinterpret_cast<const f32x4 *>(kv.ks + gr * kKvGroup + 8 * g);
@@ -104,18 +155,18 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
       dk[1] = p[1];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        kf[ks] = *reinterpret_cast<const uint4 *>(base + ((4 * ks + g) * kKvGroup + 2 * n) * 8);
+        kf[ks] = once(base + ((4 * ks + g) * kKvGroup + 2 * n) * 8);
     } else {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          kf[2 * ks + h] = *reinterpret_cast<const uint4 *>(
-              base + ((4 * ks + g) * kKvGroup + 16 * (n >> 3) + 8 * h + (n & 7)) * 8);
+          kf[2 * ks + h] = once(base + ((4 * ks + g) * kKvGroup + 16 * (n >> 3) + 8 * h + (n & 7)) * 8);
     }
   };
-  long gr = group_of(begin + wave), gr1 = group_of(begin + wave + kMassWaves);
-  load_k(gr);
+  int page = groups.page(begin + wave), page1 = groups.page(begin + wave + kMassWaves);
+  page = uniform(page);
+  load_k(groups.at(begin + wave, page));
 
   // this lane's query (rows behind the tile's last repeat it)
   int tok;
@@ -131,25 +182,30 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
     for (int ks = 0; ks < KS; ++ks) {
       load8(q + 32 * ks, a.wide_q, x[ks]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
+      for (int i = 0; i < 8; ++i) {
+        x[ks][i] *= a.scale;
+        mx = fmaxf(mx, fabsf(x[ks][i]));
+      }
     }
-    mx = max_groups(mx);
-    // scaled into [2^13, 2^14): both halves keep their bits
-    const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
-    const float up = ldexp1(1.f, 14 - X);
+    const RowScale by = RowScale::of<I8>(max_groups(mx));
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[ks][i] *= up;
+      for (int i = 0; i < 8; ++i) x[ks][i] *= by.up;
       split2(x[ks], one, qh[ks], ql[ks]);
     }
-    c = ldexp1(a.scale * kLog2e, X - 14 + (I8 ? 9 : 0));
+    c = by.c;
   }
-  float *scores = w.scores + ((size_t)tile * w.m.slots + n) * ((size_t)w.groups * kKvGroup);
+  const size_t slot = slot_of(a, w, s, seq, head, r0);
+  // Lanes without a row store out of range, where nothing is written: a branch around the stores would
+  // make every wait for keys one for the stores before them as well.  (At most 2^28 bytes: kMassFloats.)
+  const __amdgpu_buffer_rsrc_t scores =
+      make_rsrc(w.scores + slot * ((size_t)w.groups * kKvGroup), (uint32_t)nr * w.groups * kKvGroup * 4);
+  const uint32_t mine = n < nr ? (uint32_t)(n * kKvGroup + 8 * g) * 4 : 0x80000000u;
   float m = kUnsetMax, l = 0.f;
   for (int i = begin + wave; i < end; i += kMassWaves) {
     const int first = i * kKvGroup;
-    const bool there = gr >= 0;
+    const bool there = groups.there(page);
     f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
@@ -171,58 +227,41 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
       x[j] = there && first + 8 * g + j <= p ? seen_score(sc[j >> 2][j & 3] * k) : -INFINITY;
       most = fmaxf(most, x[j]);
     }
-    gr = gr1;
-    load_k(gr);
-    gr1 = group_of(i + 2 * kMassWaves);
+    page = uniform(page1);
+    load_k(groups.at(i + kMassWaves, page));
+    page1 = groups.page(i + 2 * kMassWaves);
     l *= __builtin_amdgcn_exp2f(m - most);
     m = most;
 #pragma unroll
     for (int j = 0; j < 8; ++j) l += __builtin_amdgcn_exp2f(x[j] - m);
-    if (n < nr) {
-      f32x4 *to = reinterpret_cast<f32x4 *>(scores + first + 8 * g);
-      to[0] = f32x4{x[0], x[1], x[2], x[3]};
-      to[1] = f32x4{x[4], x[5], x[6], x[7]};
-    }
+#pragma unroll
+    for (int j = 0; j < 8; j += 4)
+      __builtin_amdgcn_raw_buffer_store_b128(
+          __builtin_bit_cast(u32x4_t, f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]}), scores,
+          (int)(mine + (uint32_t)first * nr * 4 + 4 * j), 0, 0);
   }
   const float all = max_groups(m);
   l = sum_groups(l * __builtin_amdgcn_exp2f(m - all));
   if (g == 0) part[wave][n] = float2{all, l};
   __syncthreads();
-  if (threadIdx.x < kMassRows) {
+  if ((int)threadIdx.x < nr) {
     float2 o = part[0][threadIdx.x];
 #pragma unroll
-    for (int v = 1; v < kMassWaves; ++v) {
-      const float2 x = part[v][threadIdx.x];
-      const float top = fmaxf(o.x, x.x);
-      o.y = o.y * __builtin_amdgcn_exp2f(o.x - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
-      o.x = top;
-    }
-    w.stats[((size_t)tile * w.m.chunks + chunk) * kMassRows + threadIdx.x] = o;
+    for (int v = 1; v < kMassWaves; ++v) o = joined(o, part[v][threadIdx.x]);
+    w.stats[(slot + threadIdx.x) * w.m.chunks + chunk] = o;
   }
 }
 
 // A chunk of the tokens of a sequence and head: their weights, summed over its rows.
 __global__ __launch_bounds__(kMassThreads) void k_mass_add(KvView kv, nx_kv_batch b, MassCall a, NarrowWork w) {
-  __shared__ long before[kMassWaves];
   __shared__ float2 part[kMassThreads / kMassRows][kMassRows];
   __shared__ float e[kMassRows];
-  const int unit = blockIdx.x / w.m.chunks, chunk = blockIdx.x % w.m.chunks;
-  const int seq = unit / kv.heads, head = unit % kv.heads;
+  const int units = b.num_seqs * w.m.heads, unit = blockIdx.x % units, chunk = blockIdx.x / units;
+  const int seq = unit / w.m.heads, head = w.head0 + unit % w.m.heads;
+  if (head >= kv.heads) return;
   const KvSeq s = kv_seq(b, seq, kv.page_log2);
   const int tiles = row_tiles(a, s), begin = chunk * w.m.share * kKvGroup, end = min(begin + w.m.share * kKvGroup, s.len);
   if (tiles == 0 || begin >= end) return;
-  // the sequence's first tile
-  long base = 0;
-  for (int i = threadIdx.x; i < seq; i += kMassThreads) base += row_tiles(a, kv_seq(b, i, kv.page_log2)) * kv.heads;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) base += __shfl_xor(base, d, 64);
-  if ((threadIdx.x & 63) == 0) before[threadIdx.x >> 6] = base;
-  __syncthreads();
-  base = head * tiles;
-#pragma unroll
-  for (int i = 0; i < kMassWaves; ++i) base += before[i];
-  if (base + tiles > w.m.tiles) return;  // (sequences that share rows have more than there is room for)
-
   const int parts = (s.len + w.m.share * kKvGroup - 1) / (w.m.share * kKvGroup);
   constexpr int kSub = kMassThreads / kMassRows, kTokens = 64 * kKvGroup / kMassThreads;
   float sum[kTokens];
@@ -231,32 +270,24 @@ __global__ __launch_bounds__(kMassThreads) void k_mass_add(KvView kv, nx_kv_batc
   for (int t = 0; t < tiles; ++t) {
     const int nr = min(kMassRows, rows_of(a, s) - t * kMassRows), r = threadIdx.x % kMassRows, sub = threadIdx.x / kMassRows;
     float2 o = {kUnsetMax, 0.f};
-    for (int i = sub; i < parts; i += kSub) {
-      const float2 x = w.stats[((size_t)(base + t) * w.m.chunks + i) * kMassRows + r];
-      const float top = fmaxf(o.x, x.x);
-      o.y = o.y * __builtin_amdgcn_exp2f(o.x - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
-      o.x = top;
-    }
+    const size_t slot = slot_of(a, w, s, seq, head, t * kMassRows);
+    const float2 *stats = w.stats + (slot + min(r, nr - 1)) * w.m.chunks;
+    for (int i = sub; i < parts; i += kSub) o = joined(o, stats[i]);
     part[sub][r] = o;
     __syncthreads();
     if (threadIdx.x < kMassRows) {
 #pragma unroll
-      for (int i = 1; i < kSub; ++i) {
-        const float2 x = part[i][r];
-        const float top = fmaxf(o.x, x.x);
-        o.y = o.y * __builtin_amdgcn_exp2f(o.x - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
-        o.x = top;
-      }
+      for (int i = 1; i < kSub; ++i) o = joined(o, part[i][r]);
       e[r] = log_sum(o.x, o.y);
     }
     __syncthreads();
-    const float *scores = w.scores + (size_t)(base + t) * w.m.slots * ((size_t)w.groups * kKvGroup);
-    for (int i = 0; i < nr; ++i, scores += (size_t)w.groups * kKvGroup) {
+    const float *scores = w.scores + slot * ((size_t)w.groups * kKvGroup);
+    for (int i = 0; i < nr; ++i) {
       const float ei = e[i];
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) {
         const int j = begin + (int)threadIdx.x + u * kMassThreads;
-        const float x = j < end ? scores[j] : -INFINITY;
+        const float x = j < end ? scores[((size_t)(j / kKvGroup) * nr + i) * kKvGroup + j % kKvGroup] : -INFINITY;
         sum[u] += x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - ei);
       }
     }
@@ -265,13 +296,14 @@ __global__ __launch_bounds__(kMassThreads) void k_mass_add(KvView kv, nx_kv_batc
 #pragma unroll
   for (int u = 0; u < kTokens; ++u) {
     const int j = begin + (int)threadIdx.x + u * kMassThreads;
-    if (j < end) add_to(a, s, unit, j, sum[u]);
+    if (j < end) add_to(a, s, (size_t)seq * kv.heads + head, j, sum[u]);
   }
 }
 
 // ------------------------------------------------------------ many rows
 struct WideWork {
   MassWide m;
+  int *next;      // units that k_mass_stats and k_mass_columns have given out besides a grid's; each clears the other's
   int groups;     // of the page table
   float *e;       // [rows][heads]
   float *part;    // k_mass_stats: [rows][heads][key_parts] {maximum, sum}; k_mass_columns: [tiles][row_parts][tokens]
@@ -282,10 +314,30 @@ __device__ __forceinline__ size_t stat_of(const MassCall &a, const KvSeq &s, int
   return (size_t)(s.row + tok) * a.heads + head * a.group + (row - tok * a.group);
 }
 
+// The units of a batch in the order in which workgroups are free: those of rows that see little
+// are short, and how many there are the host does not know.
+struct Units {
+  int *next, *lds, now, ahead, turn;
+  __device__ __forceinline__ Units(int *next, int *done, int *lds)
+      : next(next), lds(lds), now(blockIdx.x), ahead(0), turn(0) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0;
+  }
+  // takes the next but one while the next is worked on
+  __device__ __forceinline__ void ask() {
+    if (threadIdx.x == 0) ahead = atomicAdd(next, 1) + (int)gridDim.x;
+  }
+  __device__ __forceinline__ void go_on() {
+    turn ^= 1;  // (a wave may still read the last turn's)
+    if (threadIdx.x == 0) lds[turn] = ahead;
+    __syncthreads();  // the last unit's reads of LDS
+    now = uniform(lds[turn]);
+  }
+};
+
 // 128 rows against a share of the keys: each row's maximum and sum.  As in k_attn_tile, the
 // four waves take a group's keys from LDS, each for 32 rows; a lane holds 16 keys' scores of a row.
 template <int FMT, int D>
-__global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_stats(KvView kv, nx_kv_batch b, MassCall a,
+__global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(KvView kv, nx_kv_batch b, MassCall a,
                                                                              WideWork w) {
   using E = kv_elem<FMT>;
   constexpr bool I8 = FMT == NX_KV_INT8;
@@ -298,16 +350,19 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_stats(K
   __shared__ Place found;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
   const float one = opaque_one();
-  for (int u = blockIdx.x;; u += gridDim.x) {
-    __syncthreads();  // the last unit's reads of LDS
-    const int chunk = u % w.m.key_parts;
+  __shared__ int unit[2];
+  for (Units units(w.next, w.next + 1, unit);; units.go_on()) {
+    units.ask();
+    const int u = units.now, chunk = u % w.m.key_parts;
     const Place at = find_item<kMassWaves>(
         kv, b, u / w.m.key_parts,
         [&](const KvSeq &q) { return (rows_of(a, q) + kMassTile - 1) / kMassTile * kv.heads; }, sums, &found);
     if (at.s < 0) return;
-    const KvSeq s = at.seq;
+    const KvSeq s = uniform(at.seq);
+    const int seq = uniform(at.s), in_seq = uniform(at.at);
     const int rows = rows_of(a, s), tiles = (rows + kMassTile - 1) / kMassTile;
-    const int head = at.at / tiles, r0 = (at.at - head * tiles) * kMassTile, nr = min(kMassTile, rows - r0);
+    // (the last rows first: they see most)
+    const int head = in_seq / tiles, r0 = (head * tiles + tiles - 1 - in_seq) * kMassTile, nr = min(kMassTile, rows - r0);
     const int row = r0 + min(32 * wave + n, nr - 1), tok = by_group(row, a.magic, a.shift), p = s.first + tok;
     const int pmin = uniform(s.first + by_group(r0 + min(32 * wave, nr - 1), a.magic, a.shift));
     const int pmax = uniform(s.first + by_group(r0 + min(32 * wave + 31, nr - 1), a.magic, a.shift));
@@ -325,27 +380,30 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_stats(K
         for (int ks = 0; ks < KS; ++ks) {
           load8(q + 16 * ks, a.wide_q, x[ks]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[ks][i]));
+          for (int i = 0; i < 8; ++i) {
+            x[ks][i] *= a.scale;
+            mx = fmaxf(mx, fabsf(x[ks][i]));
+          }
         }
-        mx = max_halves(mx);
-        const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
-        const float up = ldexp1(1.f, 14 - X);
+        const RowScale by = RowScale::of<I8>(max_halves(mx));
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[ks][i] *= up;
+          for (int i = 0; i < 8; ++i) x[ks][i] *= by.up;
           split2(x[ks], one, qh[ks], ql[ks]);
         }
-        c = ldexp1(a.scale * kLog2e, X - 14 + (I8 ? 9 : 0));
+        c = by.c;
       }
       // groups on their way: registers, then LDS
       uint4 rk[L];
       float rs = 0.f;
-      long gr = kv_group(kv, b, at.s, head, begin * kKvGroup);
+      const Groups groups{kv, b.pages + (long)seq * b.max_pages, head, end};
+      int page = groups.page(begin);
       auto fetch = [&](int i) {
-        const bool there = gr >= 0;
-        const long from = max(gr, 0L);
-        gr = kv_group(kv, b, at.s, head, min(i + 1, end - 1) * kKvGroup);
+        page = uniform(page);
+        const bool there = groups.there(page);
+        const long from = groups.at(i, page);
+        page = groups.page(i + 1);
         const uint4 *gk = reinterpret_cast<const uint4 *>(kv.k) + from * C;
 #pragma unroll
         for (int j = 0; j < L; ++j) {
@@ -395,11 +453,11 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_stats(K
           sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, ql[ks], sc, 0, 0, 0);
         }
         // score j: token first + 16 (j / 8) + 8 h + j % 8
-        float x[16], most = m;
+        float x[16], most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int t = 16 * (j >> 3) + 8 * h + (j & 7);
-          x[j] = sc[j] * (I8 ? scales[buf][t] * c : c);
+          x[j] = I8 ? sc[j] * (scales[buf][t] * c) : sc[j];
         }
         if (first + kKvGroup - 1 > pmin) {
 #pragma unroll
@@ -408,10 +466,13 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_stats(K
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) most = fmaxf(most, x[j]);
+        most = fmaxf(m, I8 ? most : most * c);
         l *= __builtin_amdgcn_exp2f(m - most);
         m = most;
+        float more[2] = {0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 16; ++j) l += __builtin_amdgcn_exp2f(x[j] - m);
+        for (int j = 0; j < 16; ++j) more[j & 1] += __builtin_amdgcn_exp2f(I8 ? x[j] - m : fmaf(x[j], c, -m));
+        l += more[0] + more[1];
       }
     }
     const float all = max_halves(m);
@@ -426,19 +487,16 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_stats(K
   }
 }
 
-// e of each row, from its parts
-__global__ __launch_bounds__(kMassThreads) void k_mass_join(nx_kv_batch b, MassCall a, WideWork w, long rows) {
-  for (long r = (long)blockIdx.x * kMassThreads + threadIdx.x; r < rows; r += (long)gridDim.x * kMassThreads) {
-    const float2 *p = reinterpret_cast<const float2 *>(w.part) + r * w.m.key_parts;
-    float2 o = {kUnsetMax, 0.f};
-    for (int i = 0; i < w.m.key_parts; ++i) {
-      const float2 x = p[i];
-      const float top = fmaxf(o.x, x.x);
-      o.y = o.y * __builtin_amdgcn_exp2f(o.x - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
-      o.x = top;
-    }
-    w.e[r] = log_sum(o.x, o.y);
-  }
+// e of each row, from its parts: 16 lanes take them
+__global__ __launch_bounds__(kMassThreads) void k_mass_join(MassCall a, WideWork w, int rows) {
+  const int r = blockIdx.x * (kMassThreads / 16) + threadIdx.x / 16, lane = threadIdx.x & 15;
+  if (r >= rows) return;
+  const float2 *p = reinterpret_cast<const float2 *>(w.part) + (size_t)r * w.m.key_parts;
+  float2 o = {kUnsetMax, 0.f};
+  for (int i = lane; i < w.m.key_parts; i += 16) o = joined(o, p[i]);
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) o = joined(o, float2{__shfl_xor(o.x, d, 16), __shfl_xor(o.y, d, 16)});
+  if (lane == 0) w.e[r] = log_sum(o.x, o.y);
 }
 
 // groups of keys that a wave holds
@@ -479,14 +537,16 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
     return (blocks + w.m.row_share - 1) / w.m.row_share;
   };
   auto key_tiles = [&](const KvSeq &q) { return (q.len + kKeyTile<D> * kKvGroup - 1) / (kKeyTile<D> * kKvGroup); };
-  for (int u = blockIdx.x;; u += gridDim.x) {
-    __syncthreads();  // the last unit's reads of LDS
+  __shared__ int unit[2];
+  for (Units units(w.next + 1, w.next, unit);; units.go_on()) {
+    units.ask();
     const Place at = find_item<kMassWaves>(
-        kv, b, u, [&](const KvSeq &q) { return row_parts(q) * key_tiles(q) * kv.heads; }, sums, &found);
+        kv, b, units.now, [&](const KvSeq &q) { return row_parts(q) * key_tiles(q) * kv.heads; }, sums, &found);
     if (at.s < 0) return;
-    const KvSeq s = at.seq;
+    const KvSeq s = uniform(at.seq);
+    const int seq = uniform(at.s), in_seq = uniform(at.at);
     const int parts = row_parts(s), tiles = key_tiles(s), rows = rows_of(a, s);
-    const int head = at.at / (parts * tiles), rest = at.at - head * parts * tiles, kt = rest / parts, part = rest - kt * parts;
+    const int head = in_seq / (parts * tiles), rest = in_seq - head * parts * tiles, kt = rest / parts, part = rest - kt * parts;
     const int k0 = kt * kKeyTile<D> * kKvGroup;
     const int from = max(part * w.m.row_share, first_block(a, s, k0));
     const int to = min((part + 1) * w.m.row_share, (rows + kMassBlock - 1) / kMassBlock);
@@ -498,7 +558,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
 #pragma unroll
     for (int i = 0; i < KG; ++i) {
       const int first = k0 + (wave * KG + i) * kKvGroup;
-      const long gr = first < s.len ? kv_group(kv, b, at.s, head, first) : -1;
+      const long gr = first < s.len ? kv_group(kv, b, seq, head, first) : -1;
       there[i] = gr >= 0;
       const E *base = reinterpret_cast<const E *>(kv.k) + max(gr, 0L) * (kKvGroup * D) + (h * kKvGroup + n) * 8;
 #pragma unroll
@@ -520,7 +580,9 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
 
-    // ---- blocks of rows on their way: eight threads of a row
+    // ---- blocks of rows on their way: eight threads of a row.  A row's place turns with the
+    // chunk of 8 elements, so that the 16 lanes that write at once hit all banks.
+    auto slot = [](int c8, int row) { return c8 * kMassBlock + (row ^ 2 * (c8 & 7)); };
     const int qr = threadIdx.x >> 3, sub = threadIdx.x & 7;
     float x[Q][8], e = 0.f;
     auto fetch = [&](int block) {
@@ -537,21 +599,24 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
       for (int i = 0; i < Q; ++i)
         if (C8 % 8 == 0 || sub + 8 * i < C8)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(x[i][j]));
+          for (int j = 0; j < 8; ++j) {
+            x[i][j] *= a.scale;
+            mx = fmaxf(mx, fabsf(x[i][j]));
+          }
 #pragma unroll
       for (int d = 1; d < 8; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 8));
-      const int X = mx < INFINITY ? max(__builtin_amdgcn_frexp_expf(mx), -112) : 0;
-      const float up = ldexp1(1.f, 14 - X);
+      const RowScale by = RowScale::of<I8>(mx);
 #pragma unroll
       for (int i = 0; i < Q; ++i) {
         if (C8 % 8 != 0 && sub + 8 * i >= C8) continue;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] *= up;
-        split2(x[i], one, query[buf][0][(sub + 8 * i) * kMassBlock + qr], query[buf][1][(sub + 8 * i) * kMassBlock + qr]);
+        for (int j = 0; j < 8; ++j) x[i][j] *= by.up;
+        const int at = slot(sub + 8 * i, qr);
+        split2(x[i], one, query[buf][0][at], query[buf][1][at]);
       }
       if (sub == 0) {
         const int row = block * kMassBlock + qr;
-        coef[buf][qr] = ldexp1(a.scale * kLog2e, X - 14 + (I8 ? 9 : 0));
+        coef[buf][qr] = by.c;
         lse[buf][qr] = e;
         // (rows behind the last see nothing)
         token[buf][qr] = row < rows ? s.first + by_group(row, a.magic, a.shift) : -1;
@@ -571,7 +636,6 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
       const int p = token[buf][n];
       const int pmin = uniform(block * kMassBlock + kMassBlock <= rows ? token[buf][0] : -1);
       const int pmax = s.first + by_group(min(block * kMassBlock + kMassBlock, rows) - 1, a.magic, a.shift);
-      const f16x8 *qh = query[buf][0] + h * kMassBlock + n, *ql = query[buf][1] + h * kMassBlock + n;
       const int first = k0 + wave * KG * kKvGroup;
       if (first > pmax) continue;
       f32x16 sc[KG];
@@ -581,7 +645,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
         for (int j = 0; j < 16; ++j) sc[i][j] = 0.f;
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
-        const f16x8 hi = qh[2 * j * kMassBlock], lo = ql[2 * j * kMassBlock];
+        const f16x8 hi = query[buf][0][slot(2 * j + h, n)], lo = query[buf][1][slot(2 * j + h, n)];
 #pragma unroll
         for (int i = 0; i < KG; ++i) {
           sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[i][j], hi, sc[i], 0, 0, 0);
@@ -606,7 +670,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
     }
 
     // ---- over the lanes' rows; lane n takes sum n
-    const size_t unit = (size_t)at.s * kv.heads + head;
+    const size_t tile = (size_t)seq * kv.heads + head;
 #pragma unroll
     for (int i = 0; i < KG; ++i) {
       float mine = 0.f;
@@ -623,9 +687,9 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
       if (j >= s.len) continue;
       if (!there[i]) mine = 0.f;
       if (parts == 1)
-        add_to(a, s, unit, j, mine);
+        add_to(a, s, tile, j, mine);
       else
-        w.part[(unit * w.m.row_parts + part) * ((size_t)w.groups * kKvGroup) + j] = mine;
+        w.part[(tile * w.m.row_parts + part) * ((size_t)w.groups * kKvGroup) + j] = mine;
     }
   }
 }
@@ -658,18 +722,28 @@ __global__ __launch_bounds__(kMassThreads) void k_mass_sum(KvView kv, nx_kv_batc
 }
 
 // The memory of scores and statistics: of one size for every call, allocated once, never moved.
-static int mass_workspace(nx_ctx *c, float **out) {
+static int mass_workspace(nx_ctx *c, float **out, int **next) {
+  constexpr size_t kBytes = kMassFloats * 4, kCounts = 256;
   DevBuf &ws = c->ws[WS_MASS];
   if (!ws.ptr) {
     NX_TRY(refuse_capture(c));
     void *p = nullptr;
-    if (hipMalloc(&p, kMassFloats * 4) != hipSuccess) {
+    if (hipMalloc(&p, kBytes + kCounts) != hipSuccess) {
       (void)hipGetLastError();
-      return fail(NX_ERR_OOM, "device allocation of " + std::to_string(kMassFloats * 4) + " bytes failed");
+      return fail(NX_ERR_OOM, "device allocation of " + std::to_string(kBytes + kCounts) + " bytes failed");
     }
-    ws = {p, kMassFloats * 4};
+    // counts begin at 0, and the workspace is there once they are: a call that finds others
+    // would leave units out
+    if (hipMemsetAsync(static_cast<uint8_t *>(p) + kBytes, 0, kCounts, c->stream) != hipSuccess ||
+        hipStreamSynchronize(c->stream) != hipSuccess) {
+      (void)hipGetLastError();
+      (void)hipFree(p);
+      return fail(NX_ERR_DEVICE, "clearing the workspace of gathered weights failed");
+    }
+    ws = {p, kBytes + kCounts};
   }
   *out = static_cast<float *>(ws.ptr);
+  *next = reinterpret_cast<int *>(*out + kMassFloats);
   return NX_OK;
 }
 
@@ -681,33 +755,27 @@ static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall
   a.shift = group_shift(a.group);
   a.magic = group_magic(a.group);
   float *ws;
-  NX_TRY(mass_workspace(c, &ws));
+  int *next;
+  NX_TRY(mass_workspace(c, &ws, &next));
   const KvView view = view_of(kv);
   const int groups = all.max_pages * (kv->page_tokens / kKvGroup);
   // Only the device knows the sequences' rows.  With one or more in each, one has at most
   // num_tokens - num_seqs + 1; a batch that leaves sequences out for a long one is right on 16-row tiles too.
-  const MassNarrow n = mass_narrow(all.num_seqs, all.num_tokens, a.group, kv->heads, groups);
-  const bool wide = n.seqs == 0 || ((long)all.num_tokens - all.num_seqs + 1) * a.group > kMassFew;
+  bool wide = ((long)all.num_tokens - all.num_seqs + 1) * a.group > kMassFew;
+  MassNarrow n = mass_narrow(all.num_seqs, all.num_tokens, a.group, kv->heads, groups, wide);
+  if (n.heads == 0) wide = true;
+  if (wide && all.num_seqs == 1) n.heads = 0;  // (all rows are one sequence's)
   a.rows_above = 0;
-  a.rows_upto = n.seqs == 0 ? 0 : wide ? kMassFew : INT32_MAX;
-  for (int s0 = 0; s0 < all.num_seqs && n.seqs > 0; s0 += n.seqs) {
-    nx_kv_batch b = all;
-    b.num_seqs = std::min(n.seqs, all.num_seqs - s0);
-    b.row_start += s0;
-    b.kv_len += s0;
-    b.pages += (size_t)s0 * b.max_pages;
-    MassCall on = a;
-    const size_t skip = (size_t)s0 * kv->heads * a.mass_stride;
-    on.mass += skip;
-    if (on.before) on.before += skip;
-    const NarrowWork w{n, groups, ws, reinterpret_cast<float2 *>(ws + n.tiles * n.slots * groups * kKvGroup)};
+  a.rows_upto = n.heads == 0 ? 0 : wide ? kMassFew : INT32_MAX;
+  for (int head = 0; head < kv->heads && n.heads > 0; head += n.heads) {
+    const NarrowWork w{n, head, groups, ws, reinterpret_cast<float2 *>(ws + n.slots * groups * kKvGroup)};
     NX_TRY(launch(c, "mass_scores", [&] {
       with_kernel(kv, [&](auto fmt, auto D) {
-        go(c, k_mass_scores<fmt(), D()>, dim3((uint32_t)(n.tiles * n.chunks)), dim3(kMassThreads), 0, view, b, on, w);
+        go(c, k_mass_scores<fmt(), D()>, dim3((uint32_t)n.tiles * n.chunks), dim3(kMassThreads), 0, view, all, a, w);
       });
     }));
     NX_TRY(launch(c, "mass_add", [&] {
-      go(c, k_mass_add, dim3((uint32_t)b.num_seqs * kv->heads * n.chunks), dim3(kMassThreads), 0, view, b, on, w);
+      go(c, k_mass_add, dim3((uint32_t)all.num_seqs * n.heads * n.chunks), dim3(kMassThreads), 0, view, all, a, w);
     }));
   }
   if (!wide) return NX_OK;
@@ -715,17 +783,19 @@ static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall
   a.rows_upto = INT32_MAX;
   const int key_tile = kv->D == 256 ? kKeyTile<256> : kKeyTile<128>;
   const MassWide m = mass_wide(all.num_seqs, all.num_tokens, a.heads, kv->heads, groups, key_tile);
-  const WideWork w{m, groups, ws, ws + (kMassFloats - mass_part_floats(all.num_tokens, a.heads))};
+  const WideWork w{m, next, groups, ws, ws + (kMassFloats - mass_part_floats(all.num_tokens, a.heads))};
   const long columns = (long)all.num_seqs * kv->heads * m.row_parts * ((groups + key_tile - 1) / key_tile);
   if (std::max(columns, (long)all.num_seqs * kv->heads * (groups / 8 + 1)) > INT32_MAX)
     return fail(NX_ERR_UNSUPPORTED, "page tables of more than 2^31 tiles");
   const dim3 grid(2 * c->num_cu), block(kMassThreads);
   NX_TRY(launch(c, "mass_stats", [&] {
+    const dim3 grid((kv->D == 256 ? 1 : 3) * c->num_cu);
     with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_stats<fmt(), D()>, grid, block, 0, view, all, a, w); });
   }));
   if (m.key_parts > 1)
     NX_TRY(launch(c, "mass_join", [&] {
-      go(c, k_mass_join, grid, block, 0, all, a, w, (long)all.num_tokens * a.heads);
+      const int rows = all.num_tokens * a.heads;
+      go(c, k_mass_join, dim3((rows + kMassThreads / 16 - 1) / (kMassThreads / 16)), block, 0, a, w, rows);
     }));
   NX_TRY(launch(c, "mass_columns", [&] {
     with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_columns<fmt(), D()>, grid, block, 0, view, all, a, w); });
@@ -741,7 +811,7 @@ static int attention_mass(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, cons
   if (b->num_seqs == 0 || b->num_tokens == 0) return NX_OK;
   const size_t width = (size_t)heads * kv->D;
   NX_TRY(refuse(mass_check(b, kv->heads, heads, q_stride, width, q, before, mass, mass_stride)));
-  MassCall a{q, before, mass, q_stride, mass_stride, heads, heads / kv->heads, scale};
+  MassCall a{q, before, mass, q_stride, mass_stride, heads, heads / kv->heads, scale * kLog2e};
   if (!host) return mass_dev(c, kv, *b, a);
   NX_TRY(refuse(kv_check_tables(*b, kv->pages, kv->page_tokens, true, false)));
   const size_t rows = b->row_start[b->num_seqs], tiles = (size_t)b->num_seqs * kv->heads;

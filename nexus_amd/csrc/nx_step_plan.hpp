@@ -107,27 +107,29 @@ inline Refusal mass_check(const nx_kv_batch *b, int kv_heads, int heads, size_t 
 // page table; `group`: query heads of a key/value head.
 constexpr int kMassRows = 16, kMassTile = 128, kMassBlock = 32;
 constexpr size_t kMassFloats = (size_t)1 << 26;  // of the workspace
-// tiles of 16 rows whose scores are stored: `seqs` sequences at once
+// tiles of 16 rows whose scores are stored: `heads` key/value heads at once
 struct MassNarrow {
-  int seqs;           // 0: not even one fits
+  int heads;          // 0: not even one fits
   int share, chunks;  // groups of a chunk, chunks of the table
-  int slots;          // rows of a tile that have room
-  long tiles;         // at most, of `seqs` sequences
+  int tiles;          // at most, of `heads` heads
+  bool one_each;      // a sequence has one tile of a head, or none: longer ones are not these kernels'
+  size_t slots;       // rows of `heads` heads that there is room for
 };
-inline MassNarrow mass_narrow(int seqs, int rows, int group, int kv_heads, int groups) {
+inline MassNarrow mass_narrow(int seqs, int rows, int group, int kv_heads, int groups, bool one_each) {
   MassNarrow m{};
-  const long want = (long)seqs * kv_heads * groups / 8192;
+  m.one_each = one_each;
+  const long want = (long)seqs * kv_heads * groups / 4096;
   m.share = 4;
   while (m.share < 64 && m.share < want) m.share *= 2;
   m.chunks = (groups + m.share - 1) / m.share;
-  const long all = (long)rows * group;
-  m.slots = (int)std::min<long>(kMassRows, all);
-  const size_t tile = (size_t)m.slots * groups * kKvGroup + (size_t)m.chunks * kMassRows * 2;
-  const long most = (long)(kMassFloats / tile), extra = all / kMassRows;
-  // sequences of n rows have at most n group / 16 + 1 tiles of each head
-  const long fit = most / kv_heads - extra;
-  m.seqs = (int)std::max(0L, std::min<long>(seqs, fit));
-  m.tiles = (m.seqs + extra) * kv_heads;
+  // (sequences of n rows have at most n group / 16 + 1 tiles of each head)
+  const long all = (long)rows * group, tiles = one_each ? seqs : seqs + all / kMassRows;
+  const size_t slots = one_each ? (size_t)seqs * kMassRows : (size_t)all;
+  // a row's scores, and a maximum and a sum of each chunk; a launch has fewer than 2^32 threads
+  const size_t row = (size_t)groups * kKvGroup + (size_t)m.chunks * 2;
+  m.heads = (int)std::min({(long)kv_heads, (long)(kMassFloats / (slots * row)), (1L << 23) / (tiles * m.chunks)});
+  m.tiles = (int)(tiles * m.heads);
+  m.slots = slots * m.heads;
   return m;
 }
 // tiles of 128 rows against shares of the keys (k_mass_stats), and of keys against shares of the
@@ -141,7 +143,7 @@ inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int group
   const long group = heads / kv_heads, all = rows * group, room = (long)mass_part_floats(rows, heads);
   const long tiles = kv_heads * ((all + kMassTile - 1) / kMassTile), blocks = (all + kMassBlock - 1) / kMassBlock;
   MassWide m{};
-  long parts = std::min({4096 / tiles, (long)groups / 4, room / ((long)rows * heads * 2)});
+  long parts = std::min({4096 / tiles, (long)groups / 16, room / ((long)rows * heads * 2)});
   parts = std::max(parts, 1L);
   m.key_share = (int)((groups + parts - 1) / parts);
   m.key_parts = (groups + m.key_share - 1) / m.key_share;
