@@ -459,7 +459,7 @@ int nx_qk_rope_dev(nx_ctx *ctx, const nx_rope *rope, const int32_t *d_positions,
  * that is not 0 .. vocab - 1 names none: its log probability is 0.  Accuracy: entropy and log
  * probabilities within 2^-20 (1 + |value| + the spread of the likely logits).  Outputs must
  * not overlap inputs.  The library's workspace for few long rows (2 MB) is the context's, as the
- * attention's: a context's first call with fewer than 2048 rows is refused while its stream is
+ * attention's: a context's first call with fewer than 1024 rows is refused while its stream is
  * captured, and calls on one context must not overlap in time.  Sampling's softmax over the
  * logits (src/engine/mod.rs:819), for the tokens that were chosen. */
 int nx_logprobs(nx_ctx *ctx, const float *logits, size_t stride, int num_tokens, int vocab,

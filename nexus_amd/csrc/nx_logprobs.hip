@@ -7,9 +7,9 @@
 // end puts their sums together in the order of the parts.
 //
 // The likeliest tokens in the same pass: a wave keeps those that passed a threshold in LDS, as
-// keys (value, then lower id first) that are all distinct.  When the list is full, the `top`
-// largest stay and the least of them is the threshold from then on, so most steps pass nothing
-// and cost one comparison with their maximum.
+// keys (value, then lower id first) that are all distinct.  The first threshold is what `top` of the
+// lanes' own maxima reach; when the list is full, the `top` largest stay and the least of them is
+// the next, so most steps pass nothing and cost one comparison with their maximum.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -36,47 +36,55 @@ struct LogprobCall {
 
 constexpr int kLogprobWaves = 4, kLogprobThreads = 64 * kLogprobWaves;
 constexpr int kHeld = 512;               // keys of a wave's list
+constexpr int kStep = 64 * 4;            // of a step of its lanes, at most; a few more may come behind the last
 constexpr int kAhead = 4;                // steps on their way
 constexpr int kRecord = 2 + kMaxTop;     // of a part: {m, S}, {W, 0}, its keys
 constexpr float kLowest = -3.4028234663852886e38f, kLog2e1 = 1.4426950408889634f;
 
-// orders as the value, then by the lower id; above 0 for anything but NaNs
-__device__ __forceinline__ uint64_t key_of(float x, int id) {
-  const uint32_t b = __float_as_uint(x + 0.f);  // (-0 is 0)
-  return (uint64_t)(b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u)) << 32 | (uint32_t)~id;
+// orders as the value (-0 is 0); above 0 for anything but NaNs
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u);
 }
-__device__ __forceinline__ float value_of(uint64_t key) {
-  const uint32_t b = (uint32_t)(key >> 32);
-  return __uint_as_float(b ^ ((int)b < 0 ? 0x80000000u : 0xffffffffu));
+__device__ __forceinline__ float value_of(uint32_t order) {
+  return __uint_as_float(order ^ ((int)order < 0 ? 0x80000000u : 0xffffffffu));
 }
+// then by the lower id
+__device__ __forceinline__ uint64_t key_of(float x, int id) { return (uint64_t)order_of(x) << 32 | (uint32_t)~id; }
+__device__ __forceinline__ float value_of(uint64_t key) { return value_of((uint32_t)(key >> 32)); }
 __device__ __forceinline__ int id_of(uint64_t key) { return (int)~(uint32_t)key; }
 
 __device__ __forceinline__ int lanes_before(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// Leaves the k largest of a wave's n <= 64 R keys (0: none) in its list, in no order; the
-// largest t that k keys reach, bit by bit.  The least key's value, -infinity where there are
-// not more than k.
-template <int R>
-__device__ __forceinline__ float keep_top(uint64_t *list, int &n, int k) {
-  const int lane = threadIdx.x & 63;
-  if (n <= k) return -INFINITY;
-  wave_handoff();
-  uint64_t key[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) key[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0;
-  uint64_t t = 0;
-  int reach = n;
-  for (int bit = 63; bit >= 0 && reach != k; --bit) {
-    const uint64_t with = t | (uint64_t)1 << bit;
+// A t that k of the lanes' N keys reach and no more than have to: the largest such t, found bit by
+// bit, or its leading bits, where they tell those k apart (0: there are no others).  Of all, `reach`
+// are not 0, k or more.
+template <int N, typename K>
+__device__ __forceinline__ K kth_of(const K (&key)[N], int k, int reach) {
+  K t = 0;
+  for (int bit = 8 * sizeof(K) - 1; bit >= 0 && reach != k; --bit) {
+    const K with = t | (K)1 << bit;
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < R; ++i) count += __popcll(__ballot(key[i] >= with));
+    for (int i = 0; i < N; ++i) count += __popcll(__ballot(key[i] >= with));
     if (count < k) continue;
     t = with;
     reach = count;
   }
+  return t;
+}
+
+// Leaves the k largest of n <= 64 R keys (0: none) in a list, in no order; all lanes of a wave.
+template <int R>
+__device__ __forceinline__ void keep_some(uint64_t *list, int &n, int k) {
+  const int lane = threadIdx.x & 63;
+  wave_handoff();
+  uint64_t key[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) key[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0;
+  const uint64_t t = kth_of(key, k, n);
   wave_handoff();
   int at = 0;
 #pragma unroll
@@ -88,14 +96,16 @@ __device__ __forceinline__ float keep_top(uint64_t *list, int &n, int k) {
   }
   wave_handoff();
   n = at;
-  if (n < k) return -INFINITY;  // (keys of none among them)
-  // the least key's high word: all of the kept reach t, and t's value is at most theirs
-  uint32_t least = 0xffffffffu;
-#pragma unroll
-  for (int i = 0; i < R; ++i) least = key[i] >= t ? min(least, (uint32_t)(key[i] >> 32)) : least;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
-  return value_of((uint64_t)least << 32);
+}
+// (as many registers as the keys take)
+__device__ __forceinline__ void keep_top(uint64_t *list, int &n, int k) {
+  if (n <= k) return;
+  if (n <= 64)
+    keep_some<1>(list, n, k);
+  else if (n <= 128)
+    keep_some<2>(list, n, k);
+  else
+    keep_some<kHeld / 64>(list, n, k);
 }
 
 struct Sums {
@@ -133,27 +143,44 @@ struct List {
   uint64_t *keys;
   int n, top;
   float least;  // what a logit has to pass
-  // N of each lane, of ids that all come behind those taken so far
+  // Before the list is used: of `most`, the largest of each lane's first logits, `top` reach t, so
+  // the row's own `top` do.
+  __device__ __forceinline__ void begin(float most) {
+    const uint32_t o[1] = {most > -INFINITY ? order_of(most) : 0u};
+    // (a NaN has no order; equal ones may reach t in greater number)
+    const int some = __popcll(__ballot(o[0] != 0));
+    if (some < top) return;
+    const uint32_t t = kth_of(o, top, some);
+    // the next lower value: t itself passes (-0 is none)
+    if (t != 0) least = value_of(t - (t == 0x80000000u ? 2 : 1));
+  }
+  // N of each lane, of ids that all come behind those taken so far, for which there is room
   template <int N, typename Id>
-  __device__ __forceinline__ void take(const float (&x)[N], float most, Id id) {
-    if (!__any(most > least)) return;
-    uint64_t mask[N];
-    int count = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) count += __popcll(__ballot(x[i] > least));
-    if (n + count > kHeld) least = keep_top<kHeld / 64>(keys, n, top);
+  __device__ __forceinline__ void push(const float (&x)[N], Id id) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      mask[i] = __ballot(x[i] > least);
-      if (x[i] > least) keys[n + lanes_before(mask[i])] = key_of(x[i], id(i));
-      n += __popcll(mask[i]);
+      const uint64_t mask = __ballot(x[i] > least);
+      if (!mask) continue;
+      if (x[i] > least) keys[n + lanes_before(mask)] = key_of(x[i], id(i));
+      n += __popcll(mask);
     }
+  }
+  // makes room for a step's
+  __device__ __forceinline__ void shrink() {
+    keep_top(keys, n, top);
+    // the least of those kept: what equals it has a higher id
+    const int lane = threadIdx.x & 63;
+    uint32_t o = lane < n ? (uint32_t)(keys[lane] >> 32) : 0xffffffffu;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) o = min(o, (uint32_t)__shfl_xor((int)o, d, 64));
+    least = value_of(o);
   }
 };
 
 struct RowLds {
   uint64_t keys[kLogprobWaves][kHeld];
-  uint64_t best[kLogprobWaves * kMaxTop];
+  uint64_t best[kHeld];
+  int count[kLogprobWaves];
   Sums sums[kLogprobWaves];
   bool last;
 };
@@ -162,20 +189,28 @@ struct RowLds {
 __device__ __forceinline__ Sums gather(RowLds &lds, Sums mine, List &list, int top) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   mine = across(mine);
-  if (lane == 0) lds.sums[wave] = mine;
-  if (top > 0) {
-    keep_top<kHeld / 64>(list.keys, list.n, top);
-    wave_handoff();
-    if (lane < top) lds.best[wave * top + lane] = lane < list.n ? list.keys[lane] : 0;
+  if (top > 0 && list.n > kHeld / kLogprobWaves) keep_top(list.keys, list.n, top);
+  if (lane == 0) {
+    lds.sums[wave] = mine;
+    lds.count[wave] = list.n;
   }
   __syncthreads();
   Sums all = lds.sums[0];
+  int before = 0, n = 0;
 #pragma unroll
-  for (int i = 1; i < kLogprobWaves; ++i) all = joined(all, lds.sums[i]);
-  if (top > 0 && wave == 0) {
-    int n = kLogprobWaves * top;
-    keep_top<kMaxTop * kLogprobWaves / 64>(lds.best, n, top);
-    if (lane >= n && lane < top) lds.best[lane] = 0;
+  for (int i = 0; i < kLogprobWaves; ++i) {
+    if (i > 0) all = joined(all, lds.sums[i]);
+    before += i < wave ? lds.count[i] : 0;
+    n += lds.count[i];
+  }
+  if (top > 0) {
+    wave_handoff();
+    for (int i = lane; i < list.n; i += 64) lds.best[before + i] = list.keys[i];
+    __syncthreads();
+    if (wave == 0) {
+      keep_top(lds.best, n, top);
+      if (lane >= n && lane < top) lds.best[lane] = 0;
+    }
   }
   __syncthreads();
   return all;
@@ -221,7 +256,8 @@ __global__ __launch_bounds__(kLogprobThreads) void k_logprobs(LogprobCall a) {
   const int whole = (a.vocab - front) / 4, rest = front + 4 * whole;
   const int lo = min(part * (a.split.share / 4), whole);
   const int hi = part + 1 == parts ? whole : min(lo + a.split.share / 4, whole);
-  const float4 *x4 = reinterpret_cast<const float4 *>(x + front);
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  const f32x4 *x4 = reinterpret_cast<const f32x4 *>(x + front);
 
   Sums sums{kLowest, 0.f, 0.f};
   List list{lds.keys[wave], 0, a.top, -INFINITY};
@@ -229,42 +265,50 @@ __global__ __launch_bounds__(kLogprobThreads) void k_logprobs(LogprobCall a) {
     const int i = from + lane;
     const float v[1] = {i < to ? x[i] : -INFINITY};
     add(sums, v, v[0]);
-    if (a.top > 0) list.take(v, v[0], [&](int) { return i; });
+    if (a.top > 0) list.push(v, [&](int) { return i; });
   };
   if (part == 0 && wave == 0 && front > 0) single(0, front);
-  constexpr float4 kNone = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  float4 next[kAhead];
-  auto fetch = [&](int at) {
+  constexpr f32x4 kNone = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  f32x4 next[kAhead];
+  auto fetch = [&](int at) {  // (behind the part: its last ones, which are not looked at)
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int i = at + j * kLogprobThreads + (int)threadIdx.x;
-      next[j] = i < hi ? x4[i] : kNone;
-    }
+    for (int j = 0; j < kAhead; ++j)
+      next[j] = __builtin_nontemporal_load(x4 + min(at + j * kLogprobThreads + (int)threadIdx.x, hi - 1));
   };
-  fetch(lo);
+  if (lo < hi) fetch(lo);
   for (int at = lo; at < hi; at += kAhead * kLogprobThreads) {
-    float v[4 * kAhead], most[kAhead], all = -INFINITY;
+    float v[4 * kAhead], all = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
+      if (at + kAhead * kLogprobThreads > hi && at + j * kLogprobThreads + (int)threadIdx.x >= hi) next[j] = kNone;
       v[4 * j] = next[j].x, v[4 * j + 1] = next[j].y, v[4 * j + 2] = next[j].z, v[4 * j + 3] = next[j].w;
-      most[j] = fmaxf(fmaxf(next[j].x, next[j].y), fmaxf(next[j].z, next[j].w));
-      all = fmaxf(all, most[j]);
+      all = fmaxf(all, fmaxf(fmaxf(next[j].x, next[j].y), fmaxf(next[j].z, next[j].w)));
     }
-    fetch(at + kAhead * kLogprobThreads);
+    if (at + kAhead * kLogprobThreads < hi) fetch(at + kAhead * kLogprobThreads);
     add(sums, v, all);
+    if (a.top > 0 && at == lo) list.begin(all);
     if (a.top > 0 && __any(all > list.least)) {
+      int count = 0;
+#pragma unroll
+      for (int j = 0; j < 4 * kAhead; ++j) count += __popcll(__ballot(v[j] > list.least));
+      const bool fits = list.n + count <= kHeld - 4;
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
+        if (!fits && list.n > kHeld - 4 - kStep) list.shrink();
         const float u[4] = {v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
         const int id = front + 4 * (at + j * kLogprobThreads + (int)threadIdx.x);
-        list.take(u, most[j], [&](int i) { return id + i; });
+        list.push(u, [&](int i) { return id + i; });
       }
     }
   }
   if (part + 1 == parts && wave == 0 && rest < a.vocab) single(rest, a.vocab);
-  Sums all = gather(lds, sums, list, a.top);
-
-  if (parts > 1) {
+  // the workgroup's own; then, in the row's last workgroup, those of all
+  for (bool own = true;; own = false) {
+    const Sums all = gather(lds, sums, list, a.top);
+    if (parts == 1 || !own) {
+      write_row(a, row, all, lds);
+      return;
+    }
     const size_t local = blockIdx.x / parts;
     uint64_t *record = a.part + (local * parts + part) * kRecord;
     auto pack = [](float p, float q) { return (uint64_t)__float_as_uint(q) << 32 | __float_as_uint(p); };
@@ -289,18 +333,15 @@ __global__ __launch_bounds__(kLogprobThreads) void k_logprobs(LogprobCall a) {
       sums = {__uint_as_float((uint32_t)ms), __uint_as_float((uint32_t)(ms >> 32)), __uint_as_float((uint32_t)w)};
     }
     list.n = 0;
-    list.least = -INFINITY;
     for (int i0 = wave * 64; i0 < parts * a.top; i0 += kLogprobThreads) {
       const int i = i0 + lane, p = i / a.top;
       const uint64_t key = p < parts ? load_past(first + p * kRecord + 2 + (i - p * a.top)) : 0;
       const uint64_t mask = __ballot(key != 0);
-      if (list.n + 64 > kHeld) keep_top<kHeld / 64>(list.keys, list.n, a.top);
+      if (list.n + 64 > kHeld) keep_top(list.keys, list.n, a.top);
       if (key) list.keys[list.n + lanes_before(mask)] = key;
       list.n += __popcll(mask);
     }
-    all = gather(lds, sums, list, a.top);
   }
-  write_row(a, row, all, lds);
 }
 
 // Memory of the split rows: of one size for every call, allocated once, never moved.

@@ -221,8 +221,8 @@ inline Refusal evict_check_tables(const nx_kv_batch &b, int num_pages, int page_
 }
 
 // Workgroups that share a row's logits, and the logits of each (a multiple of 4).
-constexpr int kLogprobWgs = 2048;   // as many as fill the card, and no more where rows are split
-constexpr int kLogprobLeast = 1024; // of one, in logits
+constexpr int kLogprobWgs = 1024;   // as many as fill the card, and no more where rows are split
+constexpr int kLogprobLeast = 4096; // of one, in logits
 constexpr int kLogprobParts = 64;
 struct RowSplit {
   int parts, share;
