@@ -105,6 +105,11 @@ __device__ __forceinline__ uint32_t scan64(uint32_t v) {
   return v;
 }
 
+// how many lanes of the mask come before this one
+__device__ __forceinline__ int lanes_before(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
 // Which sequence holds item `item` when sequence s has count(its KvSeq) of them, at
 // most 2^31 in all, and which of its items that is; s = -1 past the last one.  All threads
 // of a workgroup of NW waves; up to 64 sequences each wave finds it by itself.

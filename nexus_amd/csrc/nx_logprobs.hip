@@ -54,10 +54,6 @@ __device__ __forceinline__ uint64_t key_of(float x, int id) { return (uint64_t)o
 __device__ __forceinline__ float value_of(uint64_t key) { return value_of((uint32_t)(key >> 32)); }
 __device__ __forceinline__ int id_of(uint64_t key) { return (int)~(uint32_t)key; }
 
-__device__ __forceinline__ int lanes_before(uint64_t mask) {
-  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-}
-
 // A t that k of the lanes' N keys reach and no more than have to: the largest such t, found bit by
 // bit, or its leading bits, where they tell those k apart (0: there are no others).  Of all, `reach`
 // are not 0, k or more.
