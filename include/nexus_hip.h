@@ -372,7 +372,7 @@ int nx_attention_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, con
  * on the batch, not on the run).  A row that sees no token gives nothing, nor does one whose scores are all
  * -infinity; a row with a NaN or +infinity among the scores that it sees, or scores past
  * f32's range, gives NaNs to the tokens that it sees and to no others.
- * At most 2^24 rows times heads in a call.  The workspace (256 MB) is the context's, allocated
+ * The workspace (256 MB) is the context's, allocated
  * with the first call, which is refused while the stream is captured, and never moved; calls on
  * one context must not overlap in time. */
 int nx_attention_mass(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, const float *q, size_t q_stride,

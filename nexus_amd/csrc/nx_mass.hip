@@ -303,15 +303,29 @@ __global__ __launch_bounds__(kMassThreads) void k_mass_add(KvView kv, nx_kv_batc
 // ------------------------------------------------------------ many rows
 struct WideWork {
   MassWide m;
-  int *next;      // units that k_mass_stats and k_mass_columns have given out besides a grid's; each clears the other's
-  int groups;     // of the page table
-  float *e;       // [rows][heads]
-  float *part;    // k_mass_stats: [rows][heads][key_parts] {maximum, sum}; k_mass_columns: [tiles][row_parts][tokens]
+  int first;       // rows [first, first + m.rows) of the call: as many as the halves have room for
+  int *next;       // units that k_mass_stats and k_mass_columns have given out besides a grid's; each clears the other's
+  int groups;      // of the page table
+  float *e, *coef;  // [rows x heads]: e_i, and what the products with the halves are multiplied by
+  _Float16 *halves;  // [rows x heads][2][D] the queries as k_mass_stats splits them
+  float *part;     // k_mass_stats: [rows x heads][key_parts] {maximum, sum}; k_mass_columns: [tiles][row_parts][tokens]
 };
 
-__device__ __forceinline__ size_t stat_of(const MassCall &a, const KvSeq &s, int head, int row) {
-  const int tok = by_group(row, a.magic, a.shift);
-  return (size_t)(s.row + tok) * a.heads + head * a.group + (row - tok * a.group);
+// a sequence's part in the launch's rows, where it is these kernels' at all
+__device__ __forceinline__ KvSeq part_of(const MassCall &a, const WideWork &w, const KvSeq &q) {
+  const int r0 = max(q.row, w.first), r1 = rows_of(a, q) > 0 ? min(q.row + q.n, w.first + w.m.rows) : 0;
+  return {r0, max(r1 - r0, 0), q.first + (r0 - q.row), q.len};
+}
+// where the launch has the rows of a sequence and head, one behind the other
+__device__ __forceinline__ size_t stat_of(const MassCall &a, const WideWork &w, const KvSeq &s, int head) {
+  return (size_t)(s.row - w.first) * a.heads + (size_t)head * s.n * a.group;
+}
+// adds a launch's sum to what the token has: in the sequence's first one, what it had before the call
+__device__ __forceinline__ void add_more(const MassCall &a, const KvSeq &all, const KvSeq &s, size_t tile, int j, float sum) {
+  if (s.row == all.row)
+    add_to(a, all, tile, j, sum);
+  else if ((size_t)j < a.mass_stride)
+    a.mass[tile * a.mass_stride + j] += sum;
 }
 
 // The units of a batch in the order in which workgroups are free: those of rows that see little
@@ -335,17 +349,19 @@ struct Units {
 };
 
 // 128 rows against a share of the keys: each row's maximum and sum.  As in k_attn_tile, the
-// four waves take a group's keys from LDS, each for 32 rows; a lane holds 16 keys' scores of a row.
+// four waves take a step's keys from LDS, each for 32 rows; a lane holds 16 keys' scores of a row.
+// (Each wave loading its operands itself, without LDS and barriers: 214 us, not 182, for a prompt of
+// 4093: the loads' 64 bytes a clock are what a CU's four matrix cores take in.)
 template <int FMT, int D>
 __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(KvView kv, nx_kv_batch b, MassCall a,
                                                                              WideWork w) {
   using E = kv_elem<FMT>;
   constexpr bool I8 = FMT == NX_KV_INT8;
-  constexpr int KS = D / 16;
+  constexpr int KS = D / 16, GS = D == 256 || I8 ? 1 : 2;  // groups of a step (as registers allow)
   constexpr int C = kKvGroup * D * (int)sizeof(E) / 16;  // 16-byte chunks of a group's keys
   constexpr int L = (C + kMassThreads - 1) / kMassThreads;
-  __shared__ f16x8 keys[2][kKvGroup * D / 8];
-  __shared__ float scales[2][kKvGroup];
+  __shared__ f16x8 keys[2][GS][kKvGroup * D / 8];
+  __shared__ float scales[2][GS][kKvGroup];
   __shared__ long sums[kMassWaves];
   __shared__ Place found;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
@@ -356,11 +372,11 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(K
     const int u = units.now, chunk = u % w.m.key_parts;
     const Place at = find_item<kMassWaves>(
         kv, b, u / w.m.key_parts,
-        [&](const KvSeq &q) { return (rows_of(a, q) + kMassTile - 1) / kMassTile * kv.heads; }, sums, &found);
+        [&](const KvSeq &q) { return (part_of(a, w, q).n * a.group + kMassTile - 1) / kMassTile * kv.heads; }, sums, &found);
     if (at.s < 0) return;
-    const KvSeq s = uniform(at.seq);
+    const KvSeq s = part_of(a, w, uniform(at.seq));
     const int seq = uniform(at.s), in_seq = uniform(at.at);
-    const int rows = rows_of(a, s), tiles = (rows + kMassTile - 1) / kMassTile;
+    const int rows = s.n * a.group, tiles = (rows + kMassTile - 1) / kMassTile;
     // (the last rows first: they see most)
     const int head = in_seq / tiles, r0 = (head * tiles + tiles - 1 - in_seq) * kMassTile, nr = min(kMassTile, rows - r0);
     const int row = r0 + min(32 * wave + n, nr - 1), tok = by_group(row, a.magic, a.shift), p = s.first + tok;
@@ -369,6 +385,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(K
     const int last = min(s.first + by_group(r0 + nr - 1, a.magic, a.shift), s.len - 1);
     const int begin = chunk * w.m.key_share, end = min(begin + w.m.key_share, last < 0 ? 0 : last / kKvGroup + 1);
     float m = kUnsetMax, l = 0.f;
+    const bool mine = 32 * wave + n < nr;  // (rows behind the tile's last repeat it)
     if (begin < end) {
       f16x8 qh[KS], ql[KS];
       float c;
@@ -394,91 +411,119 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(K
         }
         c = by.c;
       }
-      // groups on their way: registers, then LDS
-      uint4 rk[L];
+      if (chunk == 0 && mine) {
+        const size_t o = stat_of(a, w, s, head) + row;
+        f16x8 *to = reinterpret_cast<f16x8 *>(w.halves + o * (2 * D)) + h;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          to[2 * ks] = qh[ks];
+          to[2 * ks + D / 8] = ql[ks];
+        }
+        if (h == 0) w.coef[o] = c;
+      }
+      // steps of GS groups on their way: registers, then LDS
+      uint4 rk[GS][L];
       float rs = 0.f;
       const Groups groups{kv, b.pages + (long)seq * b.max_pages, head, end};
-      int page = groups.page(begin);
-      auto fetch = [&](int i) {
-        page = uniform(page);
-        const bool there = groups.there(page);
-        const long from = groups.at(i, page);
-        page = groups.page(i + 1);
-        const uint4 *gk = reinterpret_cast<const uint4 *>(kv.k) + from * C;
+      int page[GS];
+      bool there[GS], there1[GS] = {};
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-          const int x = threadIdx.x + kMassThreads * j;
-          if (C % kMassThreads == 0 || x < C) rk[j] = gk[x];
+      for (int g = 0; g < GS; ++g) page[g] = groups.page(begin + g);
+      auto fetch = [&](int i, bool (&found)[GS]) {
+#pragma unroll
+        for (int g = 0; g < GS; ++g) {
+          const int now = uniform(page[g]);
+          found[g] = i + g < end && groups.there(now);
+          const long from = groups.at(i + g, now);
+          page[g] = groups.page(i + GS + g);
+          const uint4 *gk = reinterpret_cast<const uint4 *>(kv.k) + from * C;
+#pragma unroll
+          for (int j = 0; j < L; ++j) {
+            const int x = threadIdx.x + kMassThreads * j;
+            if (C % kMassThreads == 0 || x < C) rk[g][j] = gk[x];
+          }
+          if (I8 && (int)threadIdx.x / kKvGroup == g) rs = kv.ks[from * kKvGroup + threadIdx.x % kKvGroup];
         }
-        if (I8 && threadIdx.x < kKvGroup) rs = kv.ks[from * kKvGroup + threadIdx.x];
-        return there;
       };
       auto stage = [&](int buf) {
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-          const int x = threadIdx.x + kMassThreads * j;
-          if (C % kMassThreads != 0 && x >= C) break;
-          if constexpr (I8) {
-            // rows 2 y, 2 y + 1 of a key chunk: tokens t and t + 4
-            const int d8 = x >> 4, t = kv_token(NX_KV_INT8, (x & 15) * 2);
-            keys[buf][d8 * kKvGroup + kv_row(NX_KV_F16, t)] = from_codes(rk[j].x, rk[j].y);
-            keys[buf][d8 * kKvGroup + kv_row(NX_KV_F16, t + 4)] = from_codes(rk[j].z, rk[j].w);
-          } else {
-            keys[buf][x] = __builtin_bit_cast(f16x8, rk[j]);
-          }
-        }
-        if (I8 && threadIdx.x < kKvGroup) scales[buf][threadIdx.x] = rs;
-      };
-      bool there = fetch(begin), there1 = false;
-      stage(begin & 1);
-      if (begin + 1 < end) there1 = fetch(begin + 1);
-      for (int i = begin; i < end; ++i) {
-        const int buf = i & 1, first = i * kKvGroup;
-        __syncthreads();  // group i is in LDS, and no wave reads group i - 1 any more
-        const bool here = there;
-        there = there1;
-        if (i + 1 < end) {
-          stage(buf ^ 1);
-          if (i + 2 < end) there1 = fetch(i + 2);
-        }
-        if (!here || first > pmax) continue;  // nothing that the wave's rows see
-        const f16x8 *k8 = keys[buf] + h * kKvGroup + n;
-        f32x16 sc;
+        for (int g = 0; g < GS; ++g)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sc[j] = 0.f;
+          for (int j = 0; j < L; ++j) {
+            const int x = threadIdx.x + kMassThreads * j;
+            if (C % kMassThreads != 0 && x >= C) continue;
+            if constexpr (I8) {
+              // rows 2 y, 2 y + 1 of a key chunk: tokens t and t + 4
+              const int d8 = x >> 4, t = kv_token(NX_KV_INT8, (x & 15) * 2);
+              keys[buf][g][d8 * kKvGroup + kv_row(NX_KV_F16, t)] = from_codes(rk[g][j].x, rk[g][j].y);
+              keys[buf][g][d8 * kKvGroup + kv_row(NX_KV_F16, t + 4)] = from_codes(rk[g][j].z, rk[g][j].w);
+            } else {
+              keys[buf][g][x] = __builtin_bit_cast(f16x8, rk[g][j]);
+            }
+          }
+        if (I8 && threadIdx.x < GS * kKvGroup) scales[buf][threadIdx.x / kKvGroup][threadIdx.x % kKvGroup] = rs;
+      };
+      fetch(begin, there);
+      stage(0);
+      if (begin + GS < end) fetch(begin + GS, there1);
+      for (int i = begin, buf = 0; i < end; i += GS, buf ^= 1) {
+        __syncthreads();  // the step is in LDS, and no wave reads the one before any more
+        bool here[GS];
+#pragma unroll
+        for (int g = 0; g < GS; ++g) {
+          here[g] = there[g];
+          there[g] = there1[g];
+        }
+        if (i + GS < end) {
+          stage(buf ^ 1);
+          if (i + 2 * GS < end) fetch(i + 2 * GS, there1);
+        }
+        if (i * kKvGroup > pmax) continue;  // nothing that the wave's rows see
+        f32x16 sc[GS];
+#pragma unroll
+        for (int g = 0; g < GS; ++g)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sc[g][j] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const f16x8 kx = k8[2 * ks * kKvGroup];
-          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, qh[ks], sc, 0, 0, 0);
-          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, ql[ks], sc, 0, 0, 0);
-        }
-        // score j: token first + 16 (j / 8) + 8 h + j % 8
-        float x[16], most = -INFINITY;
+          f16x8 kx[GS];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int t = 16 * (j >> 3) + 8 * h + (j & 7);
-          x[j] = I8 ? sc[j] * (scales[buf][t] * c) : sc[j];
+          for (int g = 0; g < GS; ++g) {
+            kx[g] = keys[buf][g][(2 * ks + h) * kKvGroup + n];
+            sc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[g], qh[ks], sc[g], 0, 0, 0);
+          }
+#pragma unroll
+          for (int g = 0; g < GS; ++g) sc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx[g], ql[ks], sc[g], 0, 0, 0);
         }
-        if (first + kKvGroup - 1 > pmin) {
+#pragma unroll
+        for (int g = 0; g < GS; ++g) {
+          const int first = (i + g) * kKvGroup;
+          // score j: token first + 16 (j / 8) + 8 h + j % 8
+          float x[16], most = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (16 * (j >> 3) + (j & 7) > p - first - 8 * h) x[j] = -INFINITY;
+            x[j] = I8 ? sc[g][j] * (scales[buf][g][16 * (j >> 3) + 8 * h + (j & 7)] * c) : sc[g][j];
+          if (!here[g] || first + kKvGroup - 1 > pmin) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (!here[g] || 16 * (j >> 3) + (j & 7) > p - first - 8 * h) x[j] = -INFINITY;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) most = fmaxf(most, x[j]);
+          most = fmaxf(m, I8 ? most : most * c);
+          l *= __builtin_amdgcn_exp2f(m - most);
+          m = most;
+          float more[2] = {0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 16; ++j) more[j & 1] += __builtin_amdgcn_exp2f(I8 ? x[j] - m : fmaf(x[j], c, -m));
+          l += more[0] + more[1];
         }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) most = fmaxf(most, x[j]);
-        most = fmaxf(m, I8 ? most : most * c);
-        l *= __builtin_amdgcn_exp2f(m - most);
-        m = most;
-        float more[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 16; ++j) more[j & 1] += __builtin_amdgcn_exp2f(I8 ? x[j] - m : fmaf(x[j], c, -m));
-        l += more[0] + more[1];
       }
     }
     const float all = max_halves(m);
     l = across_halves(l * __builtin_amdgcn_exp2f(m - all), [](float x, float y) { return x + y; });
-    if (h == 0 && 32 * wave + n < nr) {
-      const size_t o = stat_of(a, s, head, row);
+    if (h == 0 && mine) {
+      const size_t o = stat_of(a, w, s, head) + row;
       if (w.m.key_parts == 1)
         w.e[o] = log_sum(all, l);
       else
@@ -523,7 +568,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
                                                                                WideWork w) {
   using E = kv_elem<FMT>;
   constexpr bool I8 = FMT == NX_KV_INT8;
-  constexpr int KS = D / 16, KG = kHeldGroups<D>, C8 = D / 8, Q = (C8 + 7) / 8;
+  constexpr int KS = D / 16, KG = kHeldGroups<D>, C8 = D / 8, Q = 2 * C8 * kMassBlock / kMassThreads;
   __shared__ f16x8 query[2][2][C8 * kMassBlock];  // [buffer][half]
   __shared__ float coef[2][kMassBlock], lse[2][kMassBlock];
   __shared__ int token[2][kMassBlock];
@@ -531,9 +576,8 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
   __shared__ long sums[kMassWaves];
   __shared__ Place found;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-  const float one = opaque_one();
   auto row_parts = [&](const KvSeq &q) {
-    const int blocks = (rows_of(a, q) + kMassBlock - 1) / kMassBlock;
+    const int blocks = (part_of(a, w, q).n * a.group + kMassBlock - 1) / kMassBlock;
     return (blocks + w.m.row_share - 1) / w.m.row_share;
   };
   auto key_tiles = [&](const KvSeq &q) { return (q.len + kKeyTile<D> * kKvGroup - 1) / (kKeyTile<D> * kKvGroup); };
@@ -543,14 +587,19 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
     const Place at = find_item<kMassWaves>(
         kv, b, units.now, [&](const KvSeq &q) { return row_parts(q) * key_tiles(q) * kv.heads; }, sums, &found);
     if (at.s < 0) return;
-    const KvSeq s = uniform(at.seq);
+    const KvSeq all = uniform(at.seq), s = part_of(a, w, all);
     const int seq = uniform(at.s), in_seq = uniform(at.at);
-    const int parts = row_parts(s), tiles = key_tiles(s), rows = rows_of(a, s);
+    const int parts = row_parts(all), tiles = key_tiles(all), rows = s.n * a.group;
     const int head = in_seq / (parts * tiles), rest = in_seq - head * parts * tiles, kt = rest / parts, part = rest - kt * parts;
     const int k0 = kt * kKeyTile<D> * kKvGroup;
     const int from = max(part * w.m.row_share, first_block(a, s, k0));
     const int to = min((part + 1) * w.m.row_share, (rows + kMassBlock - 1) / kMassBlock);
-    if (from >= to) continue;
+    const size_t tile = (size_t)seq * kv.heads + head;
+    if (from >= to) {  // no row sees the keys: but in a sequence's first launch they have what they had
+      const int j = k0 + (int)threadIdx.x;
+      if (parts == 1 && s.row == all.row && j < min(k0 + kKeyTile<D> * kKvGroup, s.len)) add_to(a, all, tile, j, 0.f);
+      continue;
+    }
 
     // ---- the wave's keys: row n of a group in the cache's order
     f16x8 kx[KG][KS];
@@ -580,46 +629,37 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
 
-    // ---- blocks of rows on their way: eight threads of a row.  A row's place turns with the
-    // chunk of 8 elements, so that the 16 lanes that write at once hit all banks.
+    // ---- blocks of rows on their way: 16-byte chunks of a row's halves by neighbouring threads.  A
+    // row's place turns with the chunk, so that the 16 lanes that write at once hit all banks.
     auto slot = [](int c8, int row) { return c8 * kMassBlock + (row ^ 2 * (c8 & 7)); };
-    const int qr = threadIdx.x >> 3, sub = threadIdx.x & 7;
-    float x[Q][8], e = 0.f;
+    f16x8 x[Q];
+    float e = 0.f, c_next = 0.f;
+    const size_t row0 = stat_of(a, w, s, head);
+    const f16x8 *halves = reinterpret_cast<const f16x8 *>(w.halves + row0 * (2 * D));
     auto fetch = [&](int block) {
-      const int row = min(block * kMassBlock + qr, rows - 1), tok = by_group(row, a.magic, a.shift);
-      const float *q = a.q + (size_t)(s.row + tok) * a.q_stride + (size_t)(head * a.group + row - tok * a.group) * D;
-#pragma unroll
-      for (int i = 0; i < Q; ++i)
-        if (C8 % 8 == 0 || sub + 8 * i < C8) load8(q + 8 * (sub + 8 * i), a.wide_q, x[i]);
-      if (sub == 0) e = w.e[stat_of(a, s, head, row)];
-    };
-    auto stage = [&](int block, int buf) {
-      float mx = 0.f;
-#pragma unroll
-      for (int i = 0; i < Q; ++i)
-        if (C8 % 8 == 0 || sub + 8 * i < C8)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            x[i][j] *= a.scale;
-            mx = fmaxf(mx, fabsf(x[i][j]));
-          }
-#pragma unroll
-      for (int d = 1; d < 8; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 8));
-      const RowScale by = RowScale::of<I8>(mx);
 #pragma unroll
       for (int i = 0; i < Q; ++i) {
-        if (C8 % 8 != 0 && sub + 8 * i >= C8) continue;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] *= by.up;
-        const int at = slot(sub + 8 * i, qr);
-        split2(x[i], one, query[buf][0][at], query[buf][1][at]);
+        const int at = threadIdx.x + kMassThreads * i, r = at / (2 * C8), c8 = at - r * (2 * C8);
+        x[i] = halves[(size_t)min(block * kMassBlock + r, rows - 1) * (2 * C8) + c8];
       }
-      if (sub == 0) {
-        const int row = block * kMassBlock + qr;
-        coef[buf][qr] = by.c;
-        lse[buf][qr] = e;
+      if (threadIdx.x < kMassBlock) {
+        const int row = min(block * kMassBlock + (int)threadIdx.x, rows - 1);
+        e = w.e[row0 + row];
+        c_next = w.coef[row0 + row];
+      }
+    };
+    auto stage = [&](int block, int buf) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        const int at = threadIdx.x + kMassThreads * i, r = at / (2 * C8), c8 = at - r * (2 * C8);
+        query[buf][c8 / C8][slot(c8 % C8, r)] = x[i];
+      }
+      if (threadIdx.x < kMassBlock) {
+        const int row = block * kMassBlock + (int)threadIdx.x;
+        coef[buf][threadIdx.x] = c_next;
+        lse[buf][threadIdx.x] = e;
         // (rows behind the last see nothing)
-        token[buf][qr] = row < rows ? s.first + by_group(row, a.magic, a.shift) : -1;
+        token[buf][threadIdx.x] = row < rows ? s.first + by_group(row, a.magic, a.shift) : -1;
       }
     };
     fetch(from);
@@ -670,7 +710,6 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
     }
 
     // ---- over the lanes' rows; lane n takes sum n
-    const size_t tile = (size_t)seq * kv.heads + head;
 #pragma unroll
     for (int i = 0; i < KG; ++i) {
       float mine = 0.f;
@@ -687,7 +726,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
       if (j >= s.len) continue;
       if (!there[i]) mine = 0.f;
       if (parts == 1)
-        add_to(a, s, tile, j, mine);
+        add_more(a, all, s, tile, j, mine);
       else
         w.part[(tile * w.m.row_parts + part) * ((size_t)w.groups * kKvGroup) + j] = mine;
     }
@@ -701,7 +740,7 @@ __global__ __launch_bounds__(kMassThreads) void k_mass_sum(KvView kv, nx_kv_batc
   for (int u = blockIdx.x;; u += gridDim.x) {
     __syncthreads();  // found is read
     auto parts = [&](const KvSeq &q) {
-      const int blocks = (rows_of(a, q) + kMassBlock - 1) / kMassBlock;
+      const int blocks = (part_of(a, w, q).n * a.group + kMassBlock - 1) / kMassBlock;
       return (blocks + w.m.row_share - 1) / w.m.row_share;
     };
     const Place at = find_item<kMassWaves>(
@@ -709,15 +748,15 @@ __global__ __launch_bounds__(kMassThreads) void k_mass_sum(KvView kv, nx_kv_batc
         [&](const KvSeq &q) { return parts(q) > 1 ? (q.len + kMassThreads - 1) / kMassThreads * kv.heads : 0; }, sums,
         &found);
     if (at.s < 0) return;
-    const KvSeq s = at.seq;
+    const KvSeq s = part_of(a, w, at.seq);
     const int each = (s.len + kMassThreads - 1) / kMassThreads, head = at.at / each;
     const int j = (at.at - head * each) * kMassThreads + (int)threadIdx.x;
     if (j >= s.len) continue;
     const size_t unit = (size_t)at.s * kv.heads + head;
     float sum = 0.f;
-    for (int i = first_block(a, s, j / (key_tile * kKvGroup) * (key_tile * kKvGroup)) / w.m.row_share; i < parts(s); ++i)
+    for (int i = first_block(a, s, j / (key_tile * kKvGroup) * (key_tile * kKvGroup)) / w.m.row_share; i < parts(at.seq); ++i)
       sum += w.part[(unit * w.m.row_parts + i) * ((size_t)w.groups * kKvGroup) + j];
-    add_to(a, s, unit, j, sum);
+    add_more(a, at.seq, s, unit, j, sum);
   }
 }
 
@@ -782,26 +821,31 @@ static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall
   a.rows_above = a.rows_upto;
   a.rows_upto = INT32_MAX;
   const int key_tile = kv->D == 256 ? kKeyTile<256> : kKeyTile<128>;
-  const MassWide m = mass_wide(all.num_seqs, all.num_tokens, a.heads, kv->heads, groups, key_tile);
-  const WideWork w{m, next, groups, ws, ws + (kMassFloats - mass_part_floats(all.num_tokens, a.heads))};
-  const long columns = (long)all.num_seqs * kv->heads * m.row_parts * ((groups + key_tile - 1) / key_tile);
-  if (std::max(columns, (long)all.num_seqs * kv->heads * (groups / 8 + 1)) > INT32_MAX)
+  const MassWide m = mass_wide(all.num_seqs, all.num_tokens, a.heads, kv->heads, groups, key_tile, kv->D);
+  const long tiles = (long)all.num_seqs * kv->heads, columns = tiles * m.row_parts * ((groups + key_tile - 1) / key_tile);
+  if (std::max(columns, tiles * (groups / 8 + 1)) > INT32_MAX)
     return fail(NX_ERR_UNSUPPORTED, "page tables of more than 2^31 tiles");
+  const size_t query = m.query;
+  WideWork w{m, 0, next, groups, ws, ws + query, reinterpret_cast<_Float16 *>(ws + 2 * query),
+             ws + (2 + kv->D) * query};
   const dim3 grid(2 * c->num_cu), block(kMassThreads);
-  NX_TRY(launch(c, "mass_stats", [&] {
-    const dim3 grid((kv->D == 256 ? 1 : 3) * c->num_cu);
-    with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_stats<fmt(), D()>, grid, block, 0, view, all, a, w); });
-  }));
-  if (m.key_parts > 1)
-    NX_TRY(launch(c, "mass_join", [&] {
-      const int rows = all.num_tokens * a.heads;
-      go(c, k_mass_join, dim3((rows + kMassThreads / 16 - 1) / (kMassThreads / 16)), block, 0, a, w, rows);
+  for (; w.first < all.num_tokens; w.first += m.rows) {
+    NX_TRY(launch(c, "mass_stats", [&] {
+      const dim3 grid((kv->D == 256 ? 1 : 3) * c->num_cu);
+      with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_stats<fmt(), D()>, grid, block, 0, view, all, a, w); });
     }));
-  NX_TRY(launch(c, "mass_columns", [&] {
-    with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_columns<fmt(), D()>, grid, block, 0, view, all, a, w); });
-  }));
-  if (m.row_parts == 1) return NX_OK;
-  return launch(c, "mass_sum", [&] { go(c, k_mass_sum, grid, block, 0, view, all, a, w, key_tile); });
+    if (m.key_parts > 1)
+      NX_TRY(launch(c, "mass_join", [&] {
+        const int rows = std::min(m.rows, all.num_tokens - w.first) * a.heads;
+        go(c, k_mass_join, dim3((rows + kMassThreads / 16 - 1) / (kMassThreads / 16)), block, 0, a, w, rows);
+      }));
+    NX_TRY(launch(c, "mass_columns", [&] {
+      with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_columns<fmt(), D()>, grid, block, 0, view, all, a, w); });
+    }));
+    if (m.row_parts > 1)
+      NX_TRY(launch(c, "mass_sum", [&] { go(c, k_mass_sum, grid, block, 0, view, all, a, w, key_tile); }));
+  }
+  return NX_OK;
 }
 
 static int attention_mass(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, const float *q, size_t q_stride, int heads,

@@ -93,7 +93,7 @@ inline Refusal logprobs_check(const float *logits, size_t stride, int rows, int 
 inline Refusal mass_check(const nx_kv_batch *b, int kv_heads, int heads, size_t q_stride, size_t width, const float *q,
                           const float *before, const float *mass, size_t mass_stride) {
   if (!q || !mass) return {NX_ERR_INVALID_ARG, "null buffer"};
-  if ((int64_t)b->num_tokens * heads > (1 << 24)) return {NX_ERR_UNSUPPORTED, "more than 2^24 query heads"};
+  if ((int64_t)b->num_tokens * heads > INT32_MAX) return {NX_ERR_UNSUPPORTED, "more than 2^31 query rows"};
   if (q_stride > (size_t)1 << 40 || mass_stride > (size_t)1 << 40) return {NX_ERR_UNSUPPORTED, "row stride above 2^40"};
   if (Refusal f = kv_check_rows("query", (long)q_stride, (long)width)) return f;
   if (mass_stride == 0) return {NX_ERR_SHAPE, "rows of no weights"};
@@ -107,6 +107,7 @@ inline Refusal mass_check(const nx_kv_batch *b, int kv_heads, int heads, size_t 
 // page table; `group`: query heads of a key/value head.
 constexpr int kMassRows = 16, kMassTile = 128, kMassBlock = 32;
 constexpr size_t kMassFloats = (size_t)1 << 26;  // of the workspace
+constexpr long kMassAtOnce = 3 * 256;            // workgroups that run at once, three on a CU
 // tiles of 16 rows whose scores are stored: `heads` key/value heads at once
 struct MassNarrow {
   int heads;          // 0: not even one fits
@@ -133,22 +134,38 @@ inline MassNarrow mass_narrow(int seqs, int rows, int group, int kv_heads, int g
   return m;
 }
 // tiles of 128 rows against shares of the keys (k_mass_stats), and of keys against shares of the
-// rows (k_mass_columns), whose parts are put together
+// rows (k_mass_columns), whose parts are put together: as many rows at once as there is room for
 struct MassWide {
+  int rows;                  // of a launch
+  size_t query;              // room for rows and heads (whole 16-byte runs)
   int key_share, key_parts;  // groups; parts of the table
   int row_share, row_parts;  // blocks of 32 rows; parts of a sequence of all rows
 };
-constexpr size_t mass_part_floats(int rows, int heads) { return kMassFloats - ((size_t)rows * heads + 3) / 4 * 4; }
-inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int groups, int key_tile) {
-  const long group = heads / kv_heads, all = rows * group, room = (long)mass_part_floats(rows, heads);
-  const long tiles = kv_heads * ((all + kMassTile - 1) / kMassTile), blocks = (all + kMassBlock - 1) / kMassBlock;
+inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int groups, int key_tile, int D) {
   MassWide m{};
-  long parts = std::min({4096 / tiles, (long)groups / 16, room / ((long)rows * heads * 2)});
+  // half of the workspace for the queries' halves, with two numbers of each row; the rest for parts
+  m.rows = (int)std::max(1L, std::min((long)rows, (long)(kMassFloats / 2 / ((size_t)heads * (D + 2)))));
+  const long group = heads / kv_heads, all = m.rows * group;
+  m.query = ((size_t)m.rows * heads + 3) / 4 * 4;
+  const long room = (long)(kMassFloats - m.query * (D + 2));
+  // (sequences that these kernels take, and their tiles, at most)
+  const long wide = std::min<long>(seqs, all / kMassRows + 1), tiles = kv_heads * (all / kMassTile + wide);
+  const long blocks = (all + kMassBlock - 1) / kMassBlock;
+  // Parts that differ in length, a prompt's, are many, so that workgroups end together: 182 us for one of
+  // 4093 tokens in 4096 units, 196 in 2048, 227 in 1024 and in 8192.  Where the context is long against
+  // the rows they are alike, and as many as workgroups run at once: 37 tokens behind 32003, two
+  // sequences, 69 us in 744 units, 76 in 4000.
+  const long units = (long)groups * kKvGroup >= 4L * rows ? kMassAtOnce : 4096;
+  long parts = std::min({units / tiles, (long)groups / 16, room / ((long)m.rows * heads * 2)});
   parts = std::max(parts, 1L);
   m.key_share = (int)((groups + parts - 1) / parts);
   m.key_parts = (groups + m.key_share - 1) / m.key_share;
+  // The same for the rows: not shared out where there are tiles of keys for two rounds of workgroups
+  // (those two sequences: 68 us, and no sum to follow, not 77 and 5), else in 2048 units (the
+  // prompt: 212 us; 256 in 1024, 198 and 5 more to sum up in 4096).
   const long columns = (long)kv_heads * ((groups + key_tile - 1) / key_tile);
-  parts = std::min({2048 / columns, blocks / 4, room / ((long)seqs * kv_heads * groups * kKvGroup)});
+  parts = columns * wide >= kMassAtOnce ? 1 : 2048 / columns;
+  parts = std::min({parts, blocks / 4, room / ((long)seqs * kv_heads * groups * kKvGroup)});
   parts = std::max(parts, 1L);
   m.row_share = (int)((blocks + parts - 1) / parts);
   m.row_parts = (int)((blocks + m.row_share - 1) / m.row_share);

@@ -320,8 +320,8 @@ def test_refusals(ctx):
     assert code(q=0) == code(mass=0) == code(heads=0) == code(scale=np.nan) == nx.NX_ERR_INVALID_ARG
     assert code(before=a.ptr + 4100) == code(before=a.ptr + 4096 - 160) == nx.NX_ERR_INVALID_ARG
     assert code(qs=255) == code(heads=5) == code(ms=0) == nx.NX_ERR_SHAPE
-    d.c.num_tokens = 1 << 23
-    assert code() == nx.NX_ERR_UNSUPPORTED
+    d.c.num_tokens = 1 << 24
+    assert code(heads=256, qs=256 * 64) == nx.NX_ERR_UNSUPPORTED
     q = np.zeros((3, 4, 64), np.float32)
     for kw in (dict(kv_len=[1, 20]), dict(kv_len=[400, 20]), dict(row_start=[0, 2, 4])):
         args = dict(row_start=b.row_start, kv_len=b.kv_len, pages=b.pages)
