@@ -330,3 +330,20 @@ def test_refusals(ctx):
             cache.attention_mass(q=q, heads=4, **args)
         assert e.value.code == nx.NX_ERR_SHAPE
     cache.close()
+
+
+def test_calls_in_slices_of_rows(ctx):
+    """More query rows than the workspace holds at once: the first slice sets what the later ones add
+    to, for sequences that begin in either."""
+    rng = np.random.default_rng(14)
+    heads, G, D = 256, 2, 256  # 508 rows at once
+    for ns, lens in (([600], [640]), ([300, 1, 400], [300, 50, 411])):
+        b = Batch(rng, ns, lens, 64)
+        cache, keys = filled(ctx, rng, b, F16, G, D)
+        q = rng.standard_normal((b.rows, heads, D), dtype=np.float32)
+        before = rng.random((len(ns), G, max(lens)), dtype=np.float32)
+        ref, bound = attention_mass(b, keys, q, heads, D ** -0.5, before)
+        got = on_device(cache, b, q, heads, before)
+        for s, n in enumerate(lens):
+            check(got[s, :, :n], ref[s, :, :n], bound[s, :, :n])
+        cache.close()
