@@ -390,7 +390,7 @@ int nx_attention_mass_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch
  * order, to the pages to_pages[sequence * to_max_pages + p], as they are stored.  Of the batch,
  * kv_len, pages, max_pages and num_seqs are read (row_start and num_tokens are not).
  * Writes kept [num_seqs x kv_heads x keep], the tokens that each head kept, then -1;
- * new_len[num_seqs], min(kv_len, keep); and, unless new_mass is null, the kept tokens' weights
+ * new_len[num_seqs], min(kv_len, keep), which must not overlap kv_len; and, unless new_mass is null, the kept tokens' weights
  * to new_mass + (sequence * kv_heads + head) * new_mass_stride.  The sequence's old pages stay as
  * they were: with new_len and to_pages it goes on in the new ones, and they are the caller's
  * to free.  Every token behind it sees what was kept (nx_attention counts places, so a window

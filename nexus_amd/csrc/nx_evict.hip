@@ -127,7 +127,9 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(KvView kv, nx_k
     const bool over = j < stop && k > t, same = j < stop && k == t;
     const uint64_t o = __ballot(over), e = __ballot(same);
     const int rank = maybe + lanes_before(e);
-    if (over || (same && rank < (int)need)) kept[sure + lanes_before(o) + min(rank, (int)need)] = j;
+    const int at = sure + lanes_before(o) + min(rank, (int)need);
+    // (weights that something else writes meanwhile put nothing behind the row)
+    if ((over || (same && rank < (int)need)) && at < n) kept[at] = j;
     sure += __popcll(o);
     maybe += __popcll(e);
   });

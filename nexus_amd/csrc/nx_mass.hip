@@ -40,10 +40,6 @@ __device__ __forceinline__ int rows_of(const MassCall &a, const KvSeq &q) {
   const int rows = q.n * a.group;
   return q.len > 0 && rows > a.rows_above && rows <= a.rows_upto ? rows : 0;
 }
-__device__ __forceinline__ const float *query_of(const MassCall &a, const KvSeq &s, int head, int row, int &tok) {
-  tok = by_group(row, a.magic, a.shift);
-  return a.q + (size_t)(s.row + tok) * a.q_stride;
-}
 
 // -infinity stands for tokens that a row does not see: a score of -infinity is the lowest number
 __device__ __forceinline__ float seen_score(float x) { return x == -INFINITY ? -3.4028234663852886e38f : x; }
@@ -169,9 +165,8 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
   load_k(groups.at(begin + wave, page));
 
   // this lane's query (rows behind the tile's last repeat it)
-  int tok;
-  const int row = r0 + min(n, nr - 1);
-  const float *q = query_of(a, s, head, row, tok) + (size_t)(head * a.group + row - tok * a.group) * D + 8 * g;
+  const int row = r0 + min(n, nr - 1), tok = by_group(row, a.magic, a.shift);
+  const float *q = a.q + (size_t)(s.row + tok) * a.q_stride + (size_t)(head * a.group + row - tok * a.group) * D + 8 * g;
   const int p = s.first + tok;
   const float one = opaque_one();
   f16x8 qh[KS], ql[KS];
@@ -786,7 +781,12 @@ static int mass_workspace(nx_ctx *c, float **out, int **next) {
   return NX_OK;
 }
 
-// The most rows of a sequence in 16-row tiles, where the batch has longer ones
+// The most rows of a sequence whose scores are stored, where the batch has longer ones: one tile.
+// us for 32 heads over 8 of 128, by stored scores and by scores worked out twice,
+//   sequences, tokens, context   16 x 4, 4096   16 x 8, 4096   2 x 8, 32000   61 x 8, 1024   1 x 8, 2000
+//   F16                              86   98       107   97      165  101       103  104       25   35
+//   INT8                             76  104        97  104      144  105        95  107       25   37
+// (so two tiles of INT8 and of short contexts lose up to 10 us by it)
 constexpr int kMassFew = 16;
 
 static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall a) {

@@ -156,7 +156,7 @@ inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int group
   // the rows they are alike, and as many as workgroups run at once: 37 tokens behind 32003, two
   // sequences, 69 us in 744 units, 76 in 4000.
   const long units = (long)groups * kKvGroup >= 4L * rows ? kMassAtOnce : 4096;
-  long parts = std::min({units / tiles, (long)groups / 16, room / ((long)m.rows * heads * 2)});
+  long parts = std::min({units / tiles, (long)groups / 4, room / ((long)m.rows * heads * 2)});
   parts = std::max(parts, 1L);
   m.key_share = (int)((groups + parts - 1) / parts);
   m.key_parts = (groups + m.key_share - 1) / m.key_share;
@@ -198,6 +198,10 @@ inline Refusal evict_check(const nx_kv_batch *b, int page_tokens, int kv_heads, 
   if ((int64_t)std::max(b->max_pages, a.to_max_pages) * page_tokens > INT32_MAX - 65536 || a.keep > INT32_MAX - 65536)
     return {NX_ERR_UNSUPPORTED, "sequences of more than 2^31 tokens"};
   if (b->num_seqs > (1 << 20)) return {NX_ERR_UNSUPPORTED, "more than 2^20 sequences"};
+  // (every head's part of the call reads the lengths)
+  const uintptr_t len = reinterpret_cast<uintptr_t>(b->kv_len), now = reinterpret_cast<uintptr_t>(a.new_len);
+  const uintptr_t bytes = (uintptr_t)b->num_seqs * 4;
+  if (now < len + bytes && len < now + bytes) return {NX_ERR_INVALID_ARG, "the new lengths overlap the old ones"};
   if (a.mass_stride == 0) return {NX_ERR_SHAPE, "rows of no weights"};
   if (a.mass_stride > (size_t)1 << 40 || a.new_mass_stride > (size_t)1 << 40)
     return {NX_ERR_UNSUPPORTED, "row stride above 2^40"};

@@ -220,7 +220,7 @@ def test_refusals(ctx):
     a = DeviceArray(4096)
 
     def code(S=2, mp=c.b.max_pages, ln=a.ptr, pg=a.ptr, to=a.ptr, tmp=2, keep=40, sinks=1, recent=2, m=a.ptr,
-             ms=200, kept=a.ptr, nl=a.ptr, nm=a.ptr + 4000, nms=40):
+             ms=200, kept=a.ptr, nl=a.ptr + 64, nm=a.ptr + 4000, nms=40):
         with pytest.raises(nx.NexusError) as e:
             c.cache.evict_dev(nx.KvBatch(S, 0, mp, 0, ln, pg), to, tmp, keep, sinks, recent, m, ms, kept, nl, nm, nms)
         return e.value.code
@@ -229,6 +229,7 @@ def test_refusals(ctx):
     assert code(ln=0) == code(pg=0) == code(to=0) == code(m=0) == code(kept=0) == code(nl=0) == nx.NX_ERR_INVALID_ARG
     assert code(sinks=30, recent=11) == code(mp=0) == code(tmp=0) == code(ms=0) == code(nms=39) == nx.NX_ERR_SHAPE
     assert code(nm=a.ptr) == code(nm=a.ptr + 16) == nx.NX_ERR_INVALID_ARG  # new weights over old ones
+    assert code(nl=a.ptr) == code(nl=a.ptr + 4) == nx.NX_ERR_INVALID_ARG  # new lengths over old ones
     # host arrays are looked at
     good = (c.b.kv_len, c.b.pages, c.to)
 

@@ -363,3 +363,50 @@ def test_contexts_on_streams_of_their_own():
             check_logprobs((o["lp"].reshape(T, 1), o["ent"], o["ids"].view(np.int32).reshape(T, 5), o["tlp"].reshape(T, 5)),
                            y, np.arange(T)[:, None], 5)
         cache.close()
+
+
+# ---------------------------------------------------------------- far places
+def test_places_past_32_bits():
+    """Pages whose keys lie beyond 4 GiB, and rows as far apart: the same as near ones."""
+    rng = np.random.default_rng(46)
+    G, D, page, pages = 8, 128, 1024, 2300  # 2 MiB of keys a page
+    with nx.Context(0) as ctx:
+        cache = nx.KvCache(ctx, F16, pages, page, G, D)
+        b = Batch(rng, [3, 40], [1500, 2048], page)
+        b.pages = np.array([[2298, 2199], [2201, 2299]], np.int32)
+        b.num_pages = pages
+        k, v = random_kv(rng, 3548, G, D)
+        cache.write(b.whole(), b.kv_len, b.pages, k, v)
+        q = rng.standard_normal((43, 8, D), dtype=np.float32)
+        ref, bound = attention_mass(b, stored(F16, k), q, 8, 0.1)
+        got = cache.attention_mass(*b.args(), q, 8, scale=0.1)
+        assert (np.abs(got - ref) <= bound).all()
+        to = np.array([[2200], [2297]], np.int32)
+        kept, new_len, _ = cache.evict(b.kv_len, b.pages, to, 700, got, 4, 30)
+        gk, gv = cache.read([0, 700, 1400], new_len, to)
+        at = 0
+        for s, n in enumerate(b.lens):
+            for g in range(G):
+                i = evicted(got[s, g], n, 700, 4, 30)
+                assert np.array_equal(kept[s, g], i)
+                assert_same_bits(gk[700 * s:700 * s + 700, g], stored(F16, k[at + i, g]))
+                assert_same_bits(gv[700 * s:700 * s + 700, g], stored(F16, v[at + i, g]))
+            at += n
+        cache.close()
+        # two rows 4.8 GB apart
+        stride, V = 1_200_000_001, 4000
+        far = DeviceArray(stride + V)
+        x = rng.standard_normal((2, V)).astype(np.float32)
+        for r in range(2):
+            far.upload(x[r], r * stride)
+        ent, ids, tlp = DeviceArray(2), DeviceArray(6), DeviceArray(6)
+        ctx.logprobs_dev(far.ptr, stride, 2, V, 0, 0, 0, ent.ptr, 3, ids.ptr, tlp.ptr)
+        ctx.sync()
+        check_logprobs((np.zeros((2, 0)), ent.download(), ids.download().view(np.int32).reshape(2, 3),
+                        tlp.download().reshape(2, 3)), x, np.zeros((2, 0), int), 3)
+        freq, pos, out = DeviceArray(32), ints([7, 123456]), DeviceArray(2 * V)
+        freq.upload(np.linspace(0.1, 1, 32))
+        ctx.qk_rope_dev(nx.Rope(64, 64, freq.ptr, HALVES), pos.ptr, 2, 8, 0, far.ptr, stride, 0, 0, out.ptr, V, 0, 0)
+        ctx.sync()
+        ref, bound = rope([7, 123456], x[:, :512].reshape(2, 8, 64), np.linspace(0.1, 1, 32).astype(np.float32), HALVES)
+        assert (np.abs(out.download().reshape(2, V)[:, :512].reshape(ref.shape) - ref) <= bound).all()

@@ -139,6 +139,10 @@ def test_refusals(tmp_path):
   is(evict(e) == NX_ERR_INVALID_ARG, "over the old ones");
   e.new_mass = m + 400;
   is(evict(e) == NX_OK, "behind the old ones");
+  for (int off : {-1, 0, 1}) {
+    e = a, e.new_len = len + off;
+    is(evict(e) == NX_ERR_INVALID_ARG, "lengths in place");
+  }
   e = a, e.mass_stride = 99;
   is(evict(e) == NX_OK && tables(e) == NX_ERR_SHAPE, "fewer weights than tokens");
   is(tables(a, 9) == NX_ERR_INVALID_ARG && tables(a, 3) == NX_ERR_INVALID_ARG, "pages");
