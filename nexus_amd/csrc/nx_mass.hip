@@ -300,6 +300,7 @@ struct WideWork {
   MassWide m;
   int first;       // rows [first, first + m.rows) of the call: as many as the halves have room for
   int *next;       // units that k_mass_stats and k_mass_columns have given out besides a grid's; each clears the other's
+  bool stats_once, columns_once;  // no more units than workgroups
   int groups;      // of the page table
   float *e, *coef;  // [rows x heads]: e_i, and what the products with the halves are multiplied by
   _Float16 *halves;  // [rows x heads][2][D] the queries as k_mass_stats splits them
@@ -324,18 +325,25 @@ __device__ __forceinline__ void add_more(const MassCall &a, const KvSeq &all, co
 }
 
 // The units of a batch in the order in which workgroups are free: those of rows that see little
-// are short, and how many there are the host does not know.
+// are short, and how many there are the host does not know.  Where they are not more than workgroups,
+// each has one, and as many workgroups are started: 768 that ask one counter wait for each other
+// (40 tokens of 32 heads over 4 of 128 behind 260: 47 us, not 33).
 struct Units {
   int *next, *lds, now, ahead, turn;
-  __device__ __forceinline__ Units(int *next, int *done, int *lds)
-      : next(next), lds(lds), now(blockIdx.x), ahead(0), turn(0) {
+  bool once;
+  __device__ __forceinline__ Units(int *next, int *done, int *lds, bool once)
+      : next(next), lds(lds), now(blockIdx.x), ahead(0), turn(0), once(once) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0;
   }
   // takes the next but one while the next is worked on
   __device__ __forceinline__ void ask() {
-    if (threadIdx.x == 0) ahead = atomicAdd(next, 1) + (int)gridDim.x;
+    if (!once && threadIdx.x == 0) ahead = atomicAdd(next, 1) + (int)gridDim.x;
   }
   __device__ __forceinline__ void go_on() {
+    if (once) {
+      now = -1;
+      return;
+    }
     turn ^= 1;  // (a wave may still read the last turn's)
     if (threadIdx.x == 0) lds[turn] = ahead;
     __syncthreads();  // the last unit's reads of LDS
@@ -362,7 +370,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(K
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
   const float one = opaque_one();
   __shared__ int unit[2];
-  for (Units units(w.next, w.next + 1, unit);; units.go_on()) {
+  for (Units units(w.next, w.next + 1, unit, w.stats_once); units.now >= 0; units.go_on()) {
     units.ask();
     const int u = units.now, chunk = u % w.m.key_parts;
     const Place at = find_item<kMassWaves>(
@@ -577,7 +585,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
   };
   auto key_tiles = [&](const KvSeq &q) { return (q.len + kKeyTile<D> * kKvGroup - 1) / (kKeyTile<D> * kKvGroup); };
   __shared__ int unit[2];
-  for (Units units(w.next + 1, w.next, unit);; units.go_on()) {
+  for (Units units(w.next + 1, w.next, unit, w.columns_once); units.now >= 0; units.go_on()) {
     units.ask();
     const Place at = find_item<kMassWaves>(
         kv, b, units.now, [&](const KvSeq &q) { return row_parts(q) * key_tiles(q) * kv.heads; }, sums, &found);
@@ -826,12 +834,16 @@ static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall
   if (std::max(columns, tiles * (groups / 8 + 1)) > INT32_MAX)
     return fail(NX_ERR_UNSUPPORTED, "page tables of more than 2^31 tiles");
   const size_t query = m.query;
-  WideWork w{m, 0, next, groups, ws, ws + query, reinterpret_cast<_Float16 *>(ws + 2 * query),
+  WideWork w{m, 0, next, false, false, groups, ws, ws + query, reinterpret_cast<_Float16 *>(ws + 2 * query),
              ws + (2 + kv->D) * query};
-  const dim3 grid(2 * c->num_cu), block(kMassThreads);
+  const dim3 block(kMassThreads);
+  const long at_once = (kv->D == 256 ? 1 : 3) * c->num_cu, stats = std::min(at_once, m.key_units);
+  const long columns_at_once = 2 * c->num_cu;
+  w.stats_once = m.key_units <= at_once;
+  w.columns_once = columns <= columns_at_once;
   for (; w.first < all.num_tokens; w.first += m.rows) {
     NX_TRY(launch(c, "mass_stats", [&] {
-      const dim3 grid((kv->D == 256 ? 1 : 3) * c->num_cu);
+      const dim3 grid((uint32_t)stats);
       with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_stats<fmt(), D()>, grid, block, 0, view, all, a, w); });
     }));
     if (m.key_parts > 1)
@@ -840,10 +852,13 @@ static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall
         go(c, k_mass_join, dim3((rows + kMassThreads / 16 - 1) / (kMassThreads / 16)), block, 0, a, w, rows);
       }));
     NX_TRY(launch(c, "mass_columns", [&] {
+      const dim3 grid((uint32_t)std::min(columns_at_once, columns));
       with_kernel(kv, [&](auto fmt, auto D) { go(c, k_mass_columns<fmt(), D()>, grid, block, 0, view, all, a, w); });
     }));
     if (m.row_parts > 1)
-      NX_TRY(launch(c, "mass_sum", [&] { go(c, k_mass_sum, grid, block, 0, view, all, a, w, key_tile); }));
+      NX_TRY(launch(c, "mass_sum", [&] {
+        go(c, k_mass_sum, dim3(2 * c->num_cu), block, 0, view, all, a, w, key_tile);
+      }));
   }
   return NX_OK;
 }

@@ -139,6 +139,7 @@ struct MassWide {
   int rows;                  // of a launch
   size_t query;              // room for rows and heads (whole 16-byte runs)
   int key_share, key_parts;  // groups; parts of the table
+  long key_units;            // tiles' parts, at most
   int row_share, row_parts;  // blocks of 32 rows; parts of a sequence of all rows
 };
 inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int groups, int key_tile, int D) {
@@ -160,6 +161,8 @@ inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int group
   parts = std::max(parts, 1L);
   m.key_share = (int)((groups + parts - 1) / parts);
   m.key_parts = (groups + m.key_share - 1) / m.key_share;
+  // (where no scores are stored, sequences of one row are these kernels' too)
+  m.key_units = kv_heads * (all / kMassTile + std::min(seqs, m.rows)) * m.key_parts;
   // The same for the rows: not shared out where there are tiles of keys for two rounds of workgroups
   // (those two sequences: 68 us, and no sum to follow, not 77 and 5), else in 2048 units (the
   // prompt: 212 us; 256 in 1024, 198 and 5 more to sum up in 4096).

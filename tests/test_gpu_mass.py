@@ -272,6 +272,13 @@ def test_wide_tables(ctx):
     ref, bound = attention_mass(b, keys, q, 16, 0.125)
     check_sequences(b, on_device(cache, b, q, 16, None), ref, bound)
     cache.close()
+    # single tokens beside longer ones, more sequences than rows / 16
+    b = Batch(rng, [1] * 255 + [40], [3 + s % 50 for s in range(255)] + [60], 32, max_pages=600)
+    cache, keys = filled(ctx, rng, b, F16, 1, 64)
+    q = rng.standard_normal((b.rows, 1, 64), dtype=np.float32)
+    ref, bound = attention_mass(b, keys, q, 1, 0.125)
+    check_sequences(b, on_device(cache, b, q, 1, None), ref, bound)
+    cache.close()
     b = Batch(rng, [1, 2], [1500, 7], 1024, max_pages=5000)
     cache, keys = filled(ctx, rng, b, F16, 1, 64)
     q = rng.standard_normal((3, 16, 64), dtype=np.float32)

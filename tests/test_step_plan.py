@@ -82,6 +82,8 @@ def test_gathered_weights_fit_their_workspace(tmp_path):
               is(w.key_parts == 1 || (long)w.rows * heads * w.key_parts * 2 <= room, "statistics fit");
               is((long)w.key_share * w.key_parts >= groups && (long)w.key_share * (w.key_parts - 1) < groups, "keys");
               is(w.row_parts == 1 || (long)seqs * kv_heads * w.row_parts * groups * 32 <= room, "sums fit");
+              // a sequence's last tile may be short
+              is(w.key_units >= kv_heads * ((long)w.rows * group / 128 + std::min(seqs, w.rows)) * w.key_parts, "units");
               const long blocks = ((long)w.rows * group + 31) / 32;
               is((long)w.row_share * w.row_parts >= blocks && (long)w.row_share * (w.row_parts - 1) < blocks, "rows' parts");
             }
