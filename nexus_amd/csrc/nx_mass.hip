@@ -756,8 +756,11 @@ __global__ __launch_bounds__(kMassThreads) void k_mass_sum(KvView kv, nx_kv_batc
     const int j = (at.at - head * each) * kMassThreads + (int)threadIdx.x;
     if (j >= s.len) continue;
     const size_t unit = (size_t)at.s * kv.heads + head;
+    // (where a slice ends in front of the keys, its last part would reach them by its size: none of it was written)
+    const int seen = first_block(a, s, j / (key_tile * kKvGroup) * (key_tile * kKvGroup));
+    const int to = seen < (s.n * a.group + kMassBlock - 1) / kMassBlock ? parts(at.seq) : 0;
     float sum = 0.f;
-    for (int i = first_block(a, s, j / (key_tile * kKvGroup) * (key_tile * kKvGroup)) / w.m.row_share; i < parts(at.seq); ++i)
+    for (int i = seen / w.m.row_share; i < to; ++i)
       sum += w.part[(unit * w.m.row_parts + i) * ((size_t)w.groups * kKvGroup) + j];
     add_more(a, at.seq, s, unit, j, sum);
   }

@@ -354,3 +354,22 @@ def test_calls_in_slices_of_rows(ctx):
         for s, n in enumerate(lens):
             check(got[s, :, :n], ref[s, :, :n], bound[s, :, :n])
         cache.close()
+
+
+def test_slices_that_end_before_a_tile_of_keys(ctx):
+    """A slice's last rows see nothing of the keys behind them, though its last part would reach them
+    by its size: what an earlier call left there is no part of the sum.
+
+    Scores of nothing: each of a token's 8 rows gives 1 / (p + 1) to the p + 1 tokens that it sees.
+    The bound is attention_mass's with scores of no magnitude."""
+    rng = np.random.default_rng(15)
+    heads, G, D, n, first = 256, 32, 256, 1300, 268  # 508 rows at once, 240 of them the sequence's
+    b = Batch(rng, [n], [n], 64, first_row=first)
+    cache, _ = filled(ctx, rng, b, F16, G, D)
+    q = np.zeros((b.rows, heads, D), np.float32)
+    on_device(cache, b, q, heads, None, row_start=[0, n])  # writes what the second call must not read
+    got = on_device(cache, b, q, heads, None)[0]
+    total = np.cumsum((8.0 / np.arange(1, n + 1))[::-1])[::-1]
+    bound = (4 * 2.0 ** -21 + (n + 64 + 2 * np.log2(n + 1) + 8 * n + 8) * 2.0 ** -24) * total
+    check(got, np.tile(total, (G, 1)), np.tile(bound, (G, 1)))
+    cache.close()
