@@ -324,6 +324,85 @@ __device__ __forceinline__ void add_more(const MassCall &a, const KvSeq &all, co
     a.mass[tile * a.mass_stride + j] += sum;
 }
 
+// the first block of rows that sees a tile of keys
+__device__ __forceinline__ int first_block(const MassCall &a, const KvSeq &s, int token) {
+  return (int)((long)max(token - s.first, 0) * a.group / kMassBlock);
+}
+
+// A sequence's units of k_mass_stats: for each share of the keys the tiles of rows that see any of
+// it (of the first share all tiles), those that see most first, so that the last units are short: 170 us
+// for a prompt of 4093, 178 with the others as units that end at once.  Where each workgroup has a
+// unit or none, the others do no harm, and are not counted out (three prompts of 300
+// behind 400 on 16 heads of 64: 41 us, not 50).
+struct KeyUnits {
+  int tiles, whole;  // of rows; shares that all of them see
+  int first, len, group, tokens;
+  __device__ __forceinline__ KeyUnits(const MassCall &a, const WideWork &w, const KvSeq &s)
+      : tiles((s.n * a.group + kMassTile - 1) / kMassTile), first(s.first), len(s.len), group(a.group),
+        tokens(w.m.key_share * kKvGroup) {
+    whole = w.stats_once ? w.m.key_parts : min(max(min(first, len - 1), 0) / tokens + 1, w.m.key_parts);
+  }
+  // tiles that see a share from `whole` on
+  __device__ __forceinline__ int of(int share) const {
+    const long token = (long)share * tokens;
+    return token < len ? (int)max(tiles - (token - first) * group / kMassTile, 0L) : 0;
+  }
+  __device__ __forceinline__ int all() const {
+    int n = whole * tiles;
+    for (int c = whole, k; tiles > 0 && (k = of(c)) > 0; ++c) n += k;
+    return n;
+  }
+  __device__ __forceinline__ void find(int i, int &tile, int &share) const {
+    int k = tiles;
+    share = min(i / tiles, whole);
+    i -= share * tiles;
+    if (share == whole)
+      for (k = of(share); k > 0 && i >= k; k = of(++share)) i -= k;
+    tile = tiles - 1 - min(i, tiles - 1);
+  }
+};
+// A sequence's units of k_mass_columns: for each part of the rows, the last one first, the tiles of keys that
+// any of its rows see: 193 us for that prompt, 211 with all.  (Where there is one part, all tiles: keys
+// that no row sees have what they had.)
+template <int TOKENS>
+struct RowUnits {
+  const MassCall &a;
+  int parts, tiles, whole;  // parts whose rows see into every tile
+  int first, share, blocks;
+  __device__ __forceinline__ RowUnits(const MassCall &a, const WideWork &w, const KvSeq &s)
+      : a(a), first(s.first), share(w.m.row_share) {
+    blocks = (s.n * a.group + kMassBlock - 1) / kMassBlock;
+    tiles = (s.len + TOKENS - 1) / TOKENS;
+    parts = whole = min(blocks, 1);
+    if (w.m.row_parts == 1) return;
+    parts = (blocks + share - 1) / share;
+    if (parts < 2) return;
+    const int seen = w.columns_once ? 0 : first_block(a, s, (tiles - 1) * TOKENS);
+    whole = seen < blocks ? parts - seen / share : 0;
+  }
+  // tiles that a part sees
+  __device__ __forceinline__ int of(int part) const {
+    const int last = first + by_group((int)(min((part + 1) * share, blocks) * (uint32_t)kMassBlock - 1), a.magic, a.shift);
+    return last < 0 ? 0 : min(last / TOKENS + 1, tiles);
+  }
+  __device__ __forceinline__ int all() const {
+    int n = whole * tiles;
+    for (int p = parts - whole - 1; p >= 0; --p) n += of(p);
+    return n;
+  }
+  __device__ __forceinline__ void find(int i, int &tile, int &part) const {
+    part = 0;
+    tile = i;
+    if (parts == 1) return;
+    const int before = min(i / tiles, whole);
+    i -= before * tiles;
+    part = parts - 1 - before;
+    if (before == whole)
+      for (int k; part > 0 && i >= (k = of(part)); --part) i -= k;
+    tile = min(i, tiles - 1);
+  }
+};
+
 // The units of a batch in the order in which workgroups are free: those of rows that see little
 // are short, and how many there are the host does not know.  Where they are not more than workgroups,
 // each has one, and as many workgroups are started: 768 that ask one counter wait for each other
@@ -372,21 +451,26 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(K
   __shared__ int unit[2];
   for (Units units(w.next, w.next + 1, unit, w.stats_once); units.now >= 0; units.go_on()) {
     units.ask();
-    const int u = units.now, chunk = u % w.m.key_parts;
     const Place at = find_item<kMassWaves>(
-        kv, b, u / w.m.key_parts,
-        [&](const KvSeq &q) { return (part_of(a, w, q).n * a.group + kMassTile - 1) / kMassTile * kv.heads; }, sums, &found);
+        kv, b, units.now, [&](const KvSeq &q) { return KeyUnits(a, w, part_of(a, w, q)).all() * kv.heads; }, sums, &found);
     if (at.s < 0) return;
     const KvSeq s = part_of(a, w, uniform(at.seq));
-    const int seq = uniform(at.s), in_seq = uniform(at.at);
-    const int rows = s.n * a.group, tiles = (rows + kMassTile - 1) / kMassTile;
-    // (the last rows first: they see most)
-    const int head = in_seq / tiles, r0 = (head * tiles + tiles - 1 - in_seq) * kMassTile, nr = min(kMassTile, rows - r0);
+    const int seq = uniform(at.s), in_seq = uniform(at.at), head = in_seq % kv.heads;
+    int tile, chunk;
+    KeyUnits(a, w, s).find(in_seq / kv.heads, tile, chunk);
+    const int rows = s.n * a.group, r0 = tile * kMassTile, nr = min(kMassTile, rows - r0);
     const int row = r0 + min(32 * wave + n, nr - 1), tok = by_group(row, a.magic, a.shift), p = s.first + tok;
     const int pmin = uniform(s.first + by_group(r0 + min(32 * wave, nr - 1), a.magic, a.shift));
     const int pmax = uniform(s.first + by_group(r0 + min(32 * wave + 31, nr - 1), a.magic, a.shift));
     const int last = min(s.first + by_group(r0 + nr - 1, a.magic, a.shift), s.len - 1);
-    const int begin = chunk * w.m.key_share, end = min(begin + w.m.key_share, last < 0 ? 0 : last / kKvGroup + 1);
+    const int seen = last < 0 ? 0 : last / kKvGroup + 1;
+    const int begin = chunk * w.m.key_share, end = min(begin + w.m.key_share, seen);
+    if (chunk == 0) {  // the shares that are not the tile's
+      const int from = max((seen + w.m.key_share - 1) / w.m.key_share, 1), none = w.m.key_parts - from;
+      float2 *part = reinterpret_cast<float2 *>(w.part) + (stat_of(a, w, s, head) + r0) * w.m.key_parts + from;
+      for (int i = threadIdx.x; i < none * nr; i += kMassThreads)
+        part[(size_t)(i / none) * w.m.key_parts + i % none] = float2{kUnsetMax, 0.f};
+    }
     float m = kUnsetMax, l = 0.f;
     const bool mine = 32 * wave + n < nr;  // (rows behind the tile's last repeat it)
     if (begin < end) {
@@ -558,11 +642,6 @@ constexpr int kKeyTile = kMassWaves * kHeldGroups<D>;  // of a workgroup
 template <int FMT>
 constexpr int kTokenOfHalf = kv_token(FMT, 4);
 
-// the first block of rows that sees a tile of keys, and the sequence's blocks
-__device__ __forceinline__ int first_block(const MassCall &a, const KvSeq &s, int token) {
-  return (int)((long)max(token - s.first, 0) * a.group / kMassBlock);
-}
-
 // A tile of keys against a share of the rows: each wave holds its groups' keys in registers, and
 // blocks of 32 rows go by in LDS, as two halves in operand order.  Score j of a lane is a key's,
 // and the lane's column a row's: sums over rows stay in the lane until the end.
@@ -579,22 +658,21 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
   __shared__ long sums[kMassWaves];
   __shared__ Place found;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-  auto row_parts = [&](const KvSeq &q) {
-    const int blocks = (part_of(a, w, q).n * a.group + kMassBlock - 1) / kMassBlock;
-    return (blocks + w.m.row_share - 1) / w.m.row_share;
-  };
-  auto key_tiles = [&](const KvSeq &q) { return (q.len + kKeyTile<D> * kKvGroup - 1) / (kKeyTile<D> * kKvGroup); };
+  constexpr int kTokens = kKeyTile<D> * kKvGroup;
   __shared__ int unit[2];
   for (Units units(w.next + 1, w.next, unit, w.columns_once); units.now >= 0; units.go_on()) {
     units.ask();
     const Place at = find_item<kMassWaves>(
-        kv, b, units.now, [&](const KvSeq &q) { return row_parts(q) * key_tiles(q) * kv.heads; }, sums, &found);
+        kv, b, units.now, [&](const KvSeq &q) { return RowUnits<kTokens>(a, w, part_of(a, w, q)).all() * kv.heads; }, sums,
+        &found);
     if (at.s < 0) return;
     const KvSeq all = uniform(at.seq), s = part_of(a, w, all);
-    const int seq = uniform(at.s), in_seq = uniform(at.at);
-    const int parts = row_parts(all), tiles = key_tiles(all), rows = s.n * a.group;
-    const int head = in_seq / (parts * tiles), rest = in_seq - head * parts * tiles, kt = rest / parts, part = rest - kt * parts;
-    const int k0 = kt * kKeyTile<D> * kKvGroup;
+    const int seq = uniform(at.s), in_seq = uniform(at.at), head = in_seq % kv.heads, rows = s.n * a.group;
+    const RowUnits<kTokens> of(a, w, s);
+    const int parts = of.parts;
+    int kt, part;
+    of.find(in_seq / kv.heads, kt, part);
+    const int k0 = kt * kTokens;
     const int from = max(part * w.m.row_share, first_block(a, s, k0));
     const int to = min((part + 1) * w.m.row_share, (rows + kMassBlock - 1) / kMassBlock);
     const size_t tile = (size_t)seq * kv.heads + head;
@@ -833,7 +911,7 @@ static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall
   a.rows_upto = INT32_MAX;
   const int key_tile = kv->D == 256 ? kKeyTile<256> : kKeyTile<128>;
   const MassWide m = mass_wide(all.num_seqs, all.num_tokens, a.heads, kv->heads, groups, key_tile, kv->D);
-  const long tiles = (long)all.num_seqs * kv->heads, columns = tiles * m.row_parts * ((groups + key_tile - 1) / key_tile);
+  const long tiles = (long)all.num_seqs * kv->heads, columns = m.column_units;
   if (std::max(columns, tiles * (groups / 8 + 1)) > INT32_MAX)
     return fail(NX_ERR_UNSUPPORTED, "page tables of more than 2^31 tiles");
   const size_t query = m.query;

@@ -141,6 +141,7 @@ struct MassWide {
   int key_share, key_parts;  // groups; parts of the table
   long key_units;            // tiles' parts, at most
   int row_share, row_parts;  // blocks of 32 rows; parts of a sequence of all rows
+  long column_units;         // tiles of keys and their parts, at most
 };
 inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int groups, int key_tile, int D) {
   MassWide m{};
@@ -172,6 +173,8 @@ inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int group
   parts = std::max(parts, 1L);
   m.row_share = (int)((blocks + parts - 1) / parts);
   m.row_parts = (int)((blocks + m.row_share - 1) / m.row_share);
+  // (of the sequences' parts each but the last is whole, and so is each of their blocks)
+  m.column_units = columns * std::min((long)seqs * m.row_parts, m.row_parts + 2L * seqs);
   return m;
 }
 

@@ -85,6 +85,12 @@ def test_gathered_weights_fit_their_workspace(tmp_path):
               // a sequence's last tile may be short
               is(w.key_units >= kv_heads * ((long)w.rows * group / 128 + std::min(seqs, w.rows)) * w.key_parts, "units");
               const long blocks = ((long)w.rows * group + 31) / 32;
+              // sequences of one row but for one, and of as many rows each
+              const long most = std::min(seqs, w.rows), each = std::max(1, w.rows / seqs);
+              auto parts = [&](long n) { return ((n * group + 31) / 32 + w.row_share - 1) / w.row_share; };
+              const long tiles = kv_heads * (((long)groups + (D == 256 ? 3 : 7)) / (D == 256 ? 4 : 8));
+              is(w.column_units >= tiles * ((most - 1) * parts(1) + parts(w.rows - most + 1)), "columns of one long");
+              is(w.column_units >= tiles * most * parts(each), "columns of even ones");
               is((long)w.row_share * w.row_parts >= blocks && (long)w.row_share * (w.row_parts - 1) < blocks, "rows' parts");
             }
           }
