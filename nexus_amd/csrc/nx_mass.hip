@@ -247,32 +247,44 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
   }
 }
 
-// A chunk of the tokens of a sequence and head: their weights, summed over its rows.
+// Some of the tokens of a sequence and head: their weights, summed over its rows.
 __global__ __launch_bounds__(kMassThreads) void k_mass_add(KvView kv, nx_kv_batch b, MassCall a, NarrowWork w) {
-  __shared__ float2 part[kMassThreads / kMassRows][kMassRows];
+  __shared__ float2 part[kMassWaves][kMassRows];
   __shared__ float e[kMassRows];
   const int units = b.num_seqs * w.m.heads, unit = blockIdx.x % units, chunk = blockIdx.x / units;
   const int seq = unit / w.m.heads, head = w.head0 + unit % w.m.heads;
   if (head >= kv.heads) return;
   const KvSeq s = kv_seq(b, seq, kv.page_log2);
-  const int tiles = row_tiles(a, s), begin = chunk * w.m.share * kKvGroup, end = min(begin + w.m.share * kKvGroup, s.len);
+  const int tiles = row_tiles(a, s), begin = chunk * w.m.add_share * kKvGroup;
+  const int end = min(begin + w.m.add_share * kKvGroup, s.len), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (tiles == 0 || begin >= end) return;
   const int parts = (s.len + w.m.share * kKvGroup - 1) / (w.m.share * kKvGroup);
-  constexpr int kSub = kMassThreads / kMassRows, kTokens = 64 * kKvGroup / kMassThreads;
+  constexpr int kTokens = 64 * kKvGroup / kMassThreads, kAtOnce = 4;
   float sum[kTokens];
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) sum[i] = 0.f;
   for (int t = 0; t < tiles; ++t) {
-    const int nr = min(kMassRows, rows_of(a, s) - t * kMassRows), r = threadIdx.x % kMassRows, sub = threadIdx.x / kMassRows;
+    // the tile's rows, a power of two of them, for as many threads each as there are
+    const int nr = min(kMassRows, rows_of(a, s) - t * kMassRows), log2r = nr > 1 ? 32 - __builtin_clz(nr - 1) : 0;
+    const int r = threadIdx.x & ((1 << log2r) - 1), subs = kMassThreads >> log2r;
     float2 o = {kUnsetMax, 0.f};
     const size_t slot = slot_of(a, w, s, seq, head, t * kMassRows);
     const float2 *stats = w.stats + (slot + min(r, nr - 1)) * w.m.chunks;
-    for (int i = sub; i < parts; i += kSub) o = joined(o, stats[i]);
-    part[sub][r] = o;
-    __syncthreads();
-    if (threadIdx.x < kMassRows) {
+    for (int i = threadIdx.x >> log2r; i < parts; i += kAtOnce * subs) {
+      float2 x[kAtOnce];
 #pragma unroll
-      for (int i = 1; i < kSub; ++i) o = joined(o, part[i][r]);
+      for (int u = 0; u < kAtOnce; ++u) x[u] = stats[min(i + u * subs, parts - 1)];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (i + u * subs < parts) o = joined(o, x[u]);
+    }
+    for (int d = 1 << log2r; d < 64; d <<= 1) o = joined(o, float2{__shfl_xor(o.x, d, 64), __shfl_xor(o.y, d, 64)});
+    if (lane == r) part[wave][r] = o;
+    __syncthreads();
+    if ((int)threadIdx.x < nr) {
+      o = part[0][r];
+#pragma unroll
+      for (int i = 1; i < kMassWaves; ++i) o = joined(o, part[i][r]);
       e[r] = log_sum(o.x, o.y);
     }
     __syncthreads();
@@ -903,7 +915,7 @@ static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall
       });
     }));
     NX_TRY(launch(c, "mass_add", [&] {
-      go(c, k_mass_add, dim3((uint32_t)all.num_seqs * n.heads * n.chunks), dim3(kMassThreads), 0, view, all, a, w);
+      go(c, k_mass_add, dim3((uint32_t)all.num_seqs * n.heads * n.add_chunks), dim3(kMassThreads), 0, view, all, a, w);
     }));
   }
   if (!wide) return NX_OK;

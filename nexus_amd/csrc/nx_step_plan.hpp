@@ -112,6 +112,7 @@ constexpr long kMassAtOnce = 3 * 256;            // workgroups that run at once,
 struct MassNarrow {
   int heads;          // 0: not even one fits
   int share, chunks;  // groups of a chunk, chunks of the table
+  int add_share, add_chunks;  // and of those that k_mass_add sums, which joins all chunks in each
   int tiles;          // at most, of `heads` heads
   bool one_each;      // a sequence has one tile of a head, or none: longer ones are not these kernels'
   size_t slots;       // rows of `heads` heads that there is room for
@@ -119,7 +120,10 @@ struct MassNarrow {
 inline MassNarrow mass_narrow(int seqs, int rows, int group, int kv_heads, int groups, bool one_each) {
   MassNarrow m{};
   m.one_each = one_each;
-  const long want = (long)seqs * kv_heads * groups / 4096;
+  // 512 chunks of the whole batch, of 4 to 64 groups: a workgroup whose waves have one group each has nothing
+  // on its way, and k_mass_add reads what each chunk leaves (4096 chunks: 100001 tokens of one INT8 sequence
+  // of 4 heads 24 + 17 us for the two kernels, not 16 + 8; 61 sequences of 8191 alike)
+  const long want = (long)seqs * kv_heads * groups / 512;
   m.share = 4;
   while (m.share < 64 && m.share < want) m.share *= 2;
   m.chunks = (groups + m.share - 1) / m.share;
@@ -131,6 +135,9 @@ inline MassNarrow mass_narrow(int seqs, int rows, int group, int kv_heads, int g
   m.heads = (int)std::min({(long)kv_heads, (long)(kMassFloats / (slots * row)), (1L << 23) / (tiles * m.chunks)});
   m.tiles = (int)(tiles * m.heads);
   m.slots = slots * m.heads;
+  m.add_share = m.share;
+  while (m.add_share < 64 && (long)seqs * m.heads * groups / m.add_share > 512) m.add_share *= 2;
+  m.add_chunks = (groups + m.add_share - 1) / m.add_share;
   return m;
 }
 // tiles of 128 rows against shares of the keys (k_mass_stats), and of keys against shares of the
@@ -153,10 +160,10 @@ inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int group
   // (sequences that these kernels take, and their tiles, at most)
   const long wide = std::min<long>(seqs, all / kMassRows + 1), tiles = kv_heads * (all / kMassTile + wide);
   const long blocks = (all + kMassBlock - 1) / kMassBlock;
-  // Parts that differ in length, a prompt's, are many, so that workgroups end together: 182 us for one of
-  // 4093 tokens in 4096 units, 196 in 2048, 227 in 1024 and in 8192.  Where the context is long against
+  // Parts that differ in length, a prompt's, are many, so that workgroups end together: 161 to 164 us for one
+  // of 4093 tokens in 2048 and 4096 units, 173 in 6144, 195 in 12288, where loads of queries add up.  Where the context is long against
   // the rows they are alike, and as many as workgroups run at once: 37 tokens behind 32003, two
-  // sequences, 69 us in 744 units, 76 in 4000.
+  // sequences, 62 us in 744 units, 76 in 4000.
   const long units = (long)groups * kKvGroup >= 4L * rows ? kMassAtOnce : 4096;
   long parts = std::min({units / tiles, (long)groups / 4, room / ((long)m.rows * heads * 2)});
   parts = std::max(parts, 1L);
@@ -165,8 +172,8 @@ inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int group
   // (where no scores are stored, sequences of one row are these kernels' too)
   m.key_units = kv_heads * (all / kMassTile + std::min(seqs, m.rows)) * m.key_parts;
   // The same for the rows: not shared out where there are tiles of keys for two rounds of workgroups
-  // (those two sequences: 68 us, and no sum to follow, not 77 and 5), else in 2048 units (the
-  // prompt: 212 us; 256 in 1024, 198 and 5 more to sum up in 4096).
+  // (those two sequences: 67 us, and no sum to follow, not 77 and 5), else in 2048 units (the
+  // prompt: 190 us and 7 to sum up; 213 and 5 in 1024, 208 and 12 in 4096).
   const long columns = (long)kv_heads * ((groups + key_tile - 1) / key_tile);
   parts = columns * wide >= kMassAtOnce ? 1 : 2048 / columns;
   parts = std::min({parts, blocks / 4, room / ((long)seqs * kv_heads * groups * kKvGroup)});
