@@ -13,6 +13,9 @@
 // held against the keys that stream by, for e_i; then keys are held against the rows that stream
 // by, so a key's sum stays in its lanes.
 //
+// 32 heads over 8 of 128 in F16: one token of 61 sequences of up to 8191 155 us (667 MB), every token of a
+// prompt of 4093 364 to 377 (69 GFLOP, four times that with two halves in two passes).
+//
 // The scores are nx_attn.hip's: transposed products K Q^T on the f16 matrix cores, q as two
 // halves.  A score is one key's and one row's alone, so nothing that is masked reaches another.
 #include <hip/hip_runtime.h>
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
   uint4 kf[KL];
   f32x4 dk[2];  // INT8: scales of the lane's tokens
   const Groups groups{kv, b.pages + (long)seq * b.max_pages, head, end};
-  // read once, past the scores in the L2 (142 + 21 us for the two kernels otherwise, not 138 + 18)
+  // read once, past the scores in the L2 (142 us otherwise, not 138, and 21 for k_mass_add, not 18)
   auto once = [](const E *p) { return ld_stream16(reinterpret_cast<const uint8_t *>(p)); };
   auto load_k = [&](long gr) {
     const E *base = reinterpret_cast<const E *>(kv.k) + gr * (kKvGroup * D);
@@ -247,7 +250,9 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
   }
 }
 
-// Some of the tokens of a sequence and head: their weights, summed over its rows.
+// Some of the tokens of a sequence and head: their weights, summed over its rows.  Every workgroup joins all
+// chunks' maxima and sums by itself, with several loads of each thread on their way (a load at a time, 16
+// threads a row, 128 tokens a workgroup: 52 us for 100001 tokens of one INT8 sequence, not 8).
 __global__ __launch_bounds__(kMassThreads) void k_mass_add(KvView kv, nx_kv_batch b, MassCall a, NarrowWork w) {
   __shared__ float2 part[kMassWaves][kMassRows];
   __shared__ float e[kMassRows];
@@ -444,7 +449,7 @@ struct Units {
 
 // 128 rows against a share of the keys: each row's maximum and sum.  As in k_attn_tile, the
 // four waves take a step's keys from LDS, each for 32 rows; a lane holds 16 keys' scores of a row.
-// (Each wave loading its operands itself, without LDS and barriers: 214 us, not 182, for a prompt of
+// (Each wave loading its operands itself, without LDS and barriers: 214 us where this took 182, for a prompt of
 // 4093: the loads' 64 bytes a clock are what a CU's four matrix cores take in.)
 template <int FMT, int D>
 __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(KvView kv, nx_kv_batch b, MassCall a,
@@ -883,11 +888,11 @@ static int mass_workspace(nx_ctx *c, float **out, int **next) {
 }
 
 // The most rows of a sequence whose scores are stored, where the batch has longer ones: one tile.
-// us for 32 heads over 8 of 128, by stored scores and by scores worked out twice,
-//   sequences, tokens, context   16 x 4, 4096   16 x 8, 4096   2 x 8, 32000   61 x 8, 1024   1 x 8, 2000
-//   F16                              86   98       107   97      165  101       103  104       25   35
-//   INT8                             76  104        97  104      144  105        95  107       25   37
-// (so two tiles of INT8 and of short contexts lose up to 10 us by it)
+// us for 32 heads over 8 of 128, 16 rows of each, by stored scores and by scores worked out twice,
+//   sequences, tokens, context   16 x 4, 4096   2 x 4, 32000   61 x 4, 1024   8 x 4, 512   1 x 4, 2000
+//   F16                              52   87        57   90        49   80       21   24       13   20
+//   INT8                             46   96        49   96        42   89       22   28       13   23
+// (Two tiles would take more of the workspace, which sequences of one row beside a prompt need.)
 constexpr int kMassFew = 16;
 
 static int mass_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &all, MassCall a) {

@@ -69,6 +69,7 @@ def test_gathered_weights_fit_their_workspace(tmp_path):
               if (n.heads == 0) continue;
               is(n.slots * ((size_t)groups * 32 + 2 * (size_t)n.chunks) <= kMassFloats, "scores fit");
               is((long)n.share * n.chunks >= groups && (long)n.share * (n.chunks - 1) < groups && n.share <= 64, "chunks");
+              is((long)n.add_share * n.add_chunks >= groups && n.add_share <= 64 && n.add_chunks <= n.chunks, "sums");
               is((long)n.tiles * n.chunks * 256 < 1L << 32 && (long)seqs * n.heads * n.chunks * 256 < 1L << 32, "launch");
               is(n.slots >= (one ? (size_t)seqs * 16 : (size_t)rows * group) * n.heads, "rows");
               is(n.tiles >= (one ? (long)seqs : (long)rows * group / 16 + (seqs < rows ? seqs : 0)) * n.heads, "tiles");
