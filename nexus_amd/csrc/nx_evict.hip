@@ -171,7 +171,8 @@ __global__ __launch_bounds__(kEvictThreads) void k_evict_move(KvView kv, nx_kv_b
     from[tid] = g;
     in_group[tid] = j & (kKvGroup - 1);
     const int chunk = g >= 0 ? j >> 3 : -1;
-    const uint32_t starts = (uint32_t)__ballot(tid == 0 || chunk != __shfl_up(chunk, 1, 64));
+    const int before = __shfl_up(chunk, 1, 64);  // (all 32 lanes: one that is not there hands nothing over)
+    const uint32_t starts = (uint32_t)__ballot(tid == 0 || chunk != before);
     if (starts >> tid & 1) run[__popc(starts & ((1u << tid) - 1))] = tid;
     if (tid == 0) {
       runs = __popc(starts);
