@@ -95,6 +95,48 @@ __device__ __forceinline__ KvSeq uniform(const KvSeq &s) {
   return {uniform(s.row), uniform(s.n), uniform(s.first), uniform(s.len)};
 }
 
+// ------------------------------------------------------------ scores by the formula alone
+// A query's halves may have signs of their own, or be 0 where the query is not: the products with an
+// infinite key then add up to a NaN where the score is an infinity.  (An infinity that they do add up to is the
+// score.)  So a sum that ends as a NaN, with the products done, is worked out again from q and the keys
+// as they are, in 64 bits: a wave takes the row's tokens, or the key's rows, one for each lane.  What the
+// products go through is left as it is, and a NaN that is the formula's ends at the first token or row that has one.
+template <int FMT, int D>
+__device__ __forceinline__ float score_of(const KvView &kv, long group, int t, const float *q, float scale) {
+  using E = kv_elem<FMT>;
+  typedef E Chunk __attribute__((ext_vector_type(8)));
+  const Chunk *k = reinterpret_cast<const Chunk *>(reinterpret_cast<const E *>(kv.k) + group * (kKvGroup * D)) + kv_row(FMT, t);
+  double sum = 0.;
+#pragma unroll 1
+  for (int c = 0; c < D / 8; ++c) {
+    const Chunk x = k[c * kKvGroup];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fma((double)q[8 * c + i] * scale, (double)(float)x[i], sum);
+  }
+  if constexpr (FMT == NX_KV_INT8) sum *= kv.ks[group * kKvGroup + t];
+  return (float)sum;
+}
+
+// the maximum and sum over a row's tokens [from, to), in all lanes; a sum of NaN where it is the formula's
+template <int FMT, int D>
+__device__ __forceinline__ float2 row_by_formula(const KvView &kv, const nx_kv_batch &b, int seq, int head, const float *q,
+                                              float scale, int from, int to) {
+  const int lane = threadIdx.x & 63;
+  float2 o = {kUnsetMax, 0.f};
+#pragma unroll 1
+  for (int t0 = from; t0 < to; t0 += 64) {
+    const int t = t0 + lane;
+    const long group = t < to ? kv_group(kv, b, seq, head, t & ~(kKvGroup - 1)) : -1;
+    const float x = group >= 0 ? score_of<FMT, D>(kv, group, t & (kKvGroup - 1), q, scale) : -INFINITY;
+    if (__any(!(x < INFINITY))) return {kUnsetMax, NAN};
+    const float most = fmaxf(o.x, x);
+    o = {most, o.y * __builtin_amdgcn_exp2f(o.x - most) + __builtin_amdgcn_exp2f(x - most)};
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) o = joined(o, float2{__shfl_xor(o.x, d, 64), __shfl_xor(o.y, d, 64)});
+  return o;
+}
+
 // ------------------------------------------------------------ few rows
 struct NarrowWork {
   MassNarrow m;
@@ -238,8 +280,32 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_scores(
           __builtin_bit_cast(u32x4_t, f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]}), scores,
           (int)(mine + (uint32_t)first * nr * 4 + 4 * j), 0, 0);
   }
-  const float all = max_groups(m);
+  float all = max_groups(m);
   l = sum_groups(l * __builtin_amdgcn_exp2f(m - all));
+  uint32_t odd = (uint32_t)__ballot(lane < nr && l != l);
+  if (odd) stores_done();  // of the same scores, by other lanes
+  for (; odd; odd &= odd - 1) {  // the wave's scores of a row, two groups at once
+    const int r = __builtin_ctz(odd), now = by_group(r0 + r, a.magic, a.shift);
+    const float *qr = a.q + (size_t)(s.row + now) * a.q_stride + (size_t)(head * a.group + r0 + r - now * a.group) * D;
+    float *to = w.scores + slot * ((size_t)w.groups * kKvGroup);
+    const int t = lane & (kKvGroup - 1);
+    float2 o = {kUnsetMax, 0.f};
+#pragma unroll 1
+    for (int i0 = begin + wave; i0 < end; i0 += 2 * kMassWaves) {
+      const int i = i0 + lane / kKvGroup * kMassWaves, at = i * kKvGroup + t;
+      const long group = i < end && at <= s.first + now && at < s.len ? kv_group(kv, b, seq, head, i * kKvGroup) : -1;
+      const float x = group >= 0 ? seen_score(score_of<FMT, D>(kv, group, t, qr, a.scale)) : -INFINITY;
+      if (i < end) to[((size_t)i * nr + r) * kKvGroup + t] = x;
+      const float most = fmaxf(o.x, x);
+      o = {most, o.y * __builtin_amdgcn_exp2f(o.x - most) + __builtin_amdgcn_exp2f(x - most)};
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) o = joined(o, float2{__shfl_xor(o.x, d, 64), __shfl_xor(o.y, d, 64)});
+    if (n == r) {
+      all = o.x;
+      l = o.y;
+    }
+  }
   if (g == 0) part[wave][n] = float2{all, l};
   __syncthreads();
   if ((int)threadIdx.x < nr) {
@@ -624,8 +690,18 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(K
         }
       }
     }
-    const float all = max_halves(m);
+    float all = max_halves(m);
     l = across_halves(l * __builtin_amdgcn_exp2f(m - all), [](float x, float y) { return x + y; });
+    for (uint32_t odd = (uint32_t)__ballot(mine && l != l); odd; odd &= odd - 1) {
+      const int i = __builtin_ctz(odd), r = r0 + 32 * wave + i, now = by_group(r, a.magic, a.shift);
+      const float *q = a.q + (size_t)(s.row + now) * a.q_stride + (size_t)(head * a.group + r - now * a.group) * D;
+      const float2 o = row_by_formula<FMT, D>(kv, b, seq, head, q, a.scale, begin * kKvGroup,
+                                              min(end * kKvGroup, min(s.first + now + 1, s.len)));
+      if (n == i) {
+        all = o.x;
+        l = o.y;
+      }
+    }
     if (h == 0 && mine) {
       const size_t o = stat_of(a, w, s, head) + row;
       if (w.m.key_parts == 1)
@@ -658,6 +734,46 @@ constexpr int kKeyTile = kMassWaves * kHeldGroups<D>;  // of a workgroup
 // kv_token of h = 0, and so many behind it
 template <int FMT>
 constexpr int kTokenOfHalf = kv_token(FMT, 4);
+
+// The arguments of a kernel as it has them in memory, for what is hardly ever done: kept in registers for that they
+// took others' (k_mass_columns 198 us for a prompt of 4093, not 191).
+struct WideArgs {
+  KvView kv;
+  nx_kv_batch b;
+  MassCall a;
+  WideWork w;
+};
+__device__ __forceinline__ const WideArgs &arguments() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const WideArgs *)p;
+}
+
+// the weight that rows [from, to) give a token, in all lanes: NaN where any that sees it has no log sum
+template <int FMT, int D>
+__device__ __forceinline__ float column_by_formula(const WideArgs &all, const KvSeq &s, int seq, int head, int token,
+                                                 int from, int to) {
+  const KvView kv = all.kv;
+  const nx_kv_batch b = all.b;
+  const MassCall a = all.a;
+  const WideWork w = all.w;
+  const int lane = threadIdx.x & 63;
+  const float *e = w.e + stat_of(a, w, s, head);
+  from = max(from, max(token - s.first, 0) * a.group);
+  for (int r = from + lane; r - lane < to; r += 64)
+    if (__any(r < to && e[min(r, to - 1)] != e[min(r, to - 1)])) return NAN;
+  const long group = kv_group(kv, b, seq, head, token & ~(kKvGroup - 1));
+  float sum = 0.f;
+#pragma unroll 1
+  for (int r = from + lane; r < to; r += 64) {
+    const int now = by_group(r, a.magic, a.shift);
+    const float *q = a.q + (size_t)(s.row + now) * a.q_stride + (size_t)(head * a.group + r - now * a.group) * D;
+    sum += __builtin_amdgcn_exp2f(score_of<FMT, D>(kv, group, token & (kKvGroup - 1), q, a.scale) - e[r]);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+  return sum;
+}
 
 // A tile of keys against a share of the rows: each wave holds its groups' keys in registers, and
 // blocks of 32 rows go by in LDS, as two halves in operand order.  Score j of a lane is a key's,
@@ -819,10 +935,14 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
         if (n == j) mine = v;
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (n >= 16) continue;
-      const int j = k0 + (wave * KG + i) * kKvGroup + kv_token(FMT, 8 * (n >> 2) + 4 * h + (n & 3));
-      if (j >= s.len) continue;
+      const int j = k0 + (wave * KG + i) * kKvGroup + kv_token(FMT, 8 * (n >> 2 & 3) + 4 * h + (n & 3));
       if (!there[i]) mine = 0.f;
+      for (uint64_t odd = __ballot(n < 16 && j < s.len && mine != mine); odd; odd &= odd - 1) {
+        const int l = __builtin_ctzll(odd), t = __builtin_amdgcn_readlane(j, l);
+        const float x = column_by_formula<FMT, D>(arguments(), s, seq, head, t, from * kMassBlock, min(to * kMassBlock, rows));
+        if (lane == l) mine = x;
+      }
+      if (n >= 16 || j >= s.len) continue;
       if (parts == 1)
         add_more(a, all, s, tile, j, mine);
       else

@@ -50,3 +50,140 @@ def test_first_kept_tokens_of_a_group(ctx, fmt):
         assert tuple(got[0][0, g, 32:34]) == (a + 32, b + 32)
     c.check(got, 32, 0)
     c.cache.close()
+
+
+# ---------------------------------------------------------------- gathered weights
+def mass_by_rows(b, keys, q, heads, scale, before=None):
+    """mass [seqs x G x width], a bound, and which tokens get NaNs, of keys and queries that may hold
+    anything: the formula in 64 bits row by row.  A row with a NaN or +infinity among its scores gives
+    NaNs to the tokens that it sees; a score of -infinity is a token of no weight.
+
+    The bound is step_cases.attention_mass's, whose magnitudes are those of finite terms: a score that is
+    an infinity has no rounding."""
+    G, D = keys.shape[1:]
+    width = max(max(b.lens), 1)
+    out = np.zeros((len(b.ns), G, width)) if before is None else before.astype(np.float64)
+    bound, nan, at = np.zeros_like(out), np.zeros(out.shape, bool), 0
+    U = 2.0 ** -24
+    for s, (n, length) in enumerate(zip(b.ns, b.lens)):
+        if n:
+            out[s, :, length - n:length] = 0
+        for i in range(n):
+            p = length - n + i
+            for h in range(heads):
+                g = h * G // heads
+                k = keys[at:at + p + 1, g].astype(np.float64)
+                r = q[b.row_start[s] + i, h].astype(np.float64)
+                with np.errstate(all="ignore"):
+                    terms = scale * (r * k)
+                    x = terms.sum(1)
+                    mag = np.where(np.isfinite(terms), np.abs(terms), 0).sum(1).max()
+                if np.isnan(x).any() or (x == np.inf).any():
+                    nan[s, g, :p + 1] = True
+                    continue
+                if (x == -np.inf).all():
+                    continue
+                w = np.exp(x - x.max())
+                w /= w.sum()
+                e = 2 * ((2.0 ** -21 + D * U) * mag + 2.0 ** -21)
+                out[s, g, :p + 1] += w
+                bound[s, g, :p + 1] += (2 * e + (length + 64) * U + 2 * U * (1.5 * mag + np.log2(length + 1))) * w
+        bound[s] += (n * heads // G + 8) * U * out[s] + 2.0 ** -120
+        at += length
+    return out, bound, nan
+
+
+def mass_of(ctx, b, fmt, k, q, heads, scale, before=None):
+    """What the call gives, and the keys that its cache holds."""
+    cache = nx.KvCache(ctx, fmt, b.num_pages, b.page_tokens, *k.shape[1:])
+    cache.write(b.whole(), b.kv_len, b.pages, k, np.zeros_like(k))
+    got = cache.attention_mass(*b.args(), q, heads, scale=scale, before=before)
+    cache.close()
+    return got, stored(fmt, k)
+
+
+def check_mass(b, got, ref, bound, nan):
+    for s, (n, length) in enumerate(zip(b.ns, b.lens)):
+        if not n:
+            continue
+        g, r, o, bad = (a[s, :, :length] for a in (got, ref, bound, nan))
+        assert np.array_equal(np.isnan(g), bad), (s, np.isnan(g).sum(1), bad.sum(1))
+        off = np.abs(g.astype(np.float64) - r)[~bad]
+        assert (off <= o[~bad]).all(), float((off / o[~bad]).max())
+
+
+SHAPES = [
+    (4, 1, 64, [1], [70]),
+    (8, 2, 128, [3, 1, 0], [133, 40, 9]),
+    (16, 2, 96, [1, 2], [500, 33]),
+    (4, 2, 256, [2], [65]),
+    (8, 2, 64, [40], [100]),          # tiles of many rows
+    (24, 1, 128, [33, 1], [64, 300]),
+    (4, 2, 96, [150], [300]),
+    (4, 4, 256, [70, 2], [90, 80]),
+]
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
+def test_infinite_keys_that_no_row_gives_weight(ctx, heads, G, D, ns, lens, sign):
+    """F16 keys above 65520 are infinities.  Where a query's element has the other sign the score is
+    -infinity: the token has no weight, and the others what they have without it."""
+    rng = np.random.default_rng(31 + D)
+    b = Batch(rng, ns, lens, 32)
+    k, _ = random_kv(rng, sum(lens), G, D)
+    q = rng.standard_normal((b.rows, heads, D), dtype=np.float32)
+    # elements whose halves differ in sign or not, of a short one and of one with no second half, and one
+    # that is next to nothing beside the others
+    q[..., 5] = -sign * np.abs(q[..., 5])
+    q[..., 17] = -sign * np.float32(0.25)
+    q[..., 40] = -sign * np.abs(q[..., 40]) * np.float32(1e-20)
+    for at, d in ((0, 5), (3, 17), (7, 40), (20, 5), (31, 17)):
+        k[at, :, d] = sign * np.float32(1e6)
+    k[25, :, 5], k[25, :, 17], k[26, 0, 40] = sign * np.inf, sign * np.float32(65536), sign * np.inf
+    before = rng.random((len(ns), G, max(lens)), dtype=np.float32) / 50
+    got, keys = mass_of(ctx, b, F16, k, q, heads, D ** -0.5, before)
+    assert np.isinf(keys).any()
+    ref, bound, nan = mass_by_rows(b, keys, q, heads, D ** -0.5, before)
+    assert not nan.any()
+    check_mass(b, got, ref, bound, nan)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
+def test_keys_that_are_not_finite_under_any_query(ctx, fmt, heads, G, D, ns, lens):
+    """Rows with a NaN or +infinity among their scores give NaNs to all tokens that they see, and
+    only to those; the heads beside them, and rows before the token, are as ever."""
+    rng = np.random.default_rng(32 + D)
+    b = Batch(rng, ns, lens, 32)
+    for bad in (np.inf, -np.inf, np.nan):
+        k, _ = random_kv(rng, sum(lens), G, D)
+        q = rng.standard_normal((b.rows, heads, D), dtype=np.float32)
+        end = np.cumsum(lens)
+        for s, n in enumerate(ns):  # among the step's own tokens, and before them
+            k[end[s] - max(n, 1) // 2 - 1, G - 1, 9] = bad
+        k[2, 0, 11] = bad
+        q[0, 0, 11] = 0  # an infinity by nothing
+        got, keys = mass_of(ctx, b, fmt, k, q, heads, 0.1)
+        check_mass(b, got, *mass_by_rows(b, keys, q, heads, 0.1))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
+def test_queries_that_are_not_finite(ctx, fmt, heads, G, D, ns, lens):
+    """A row's own NaN or infinity spoils all tokens that it sees, and no other row's; a row whose
+    scores are all -infinity gives nothing."""
+    rng = np.random.default_rng(33 + D)
+    b = Batch(rng, ns, lens, 32)
+    for bad in (np.inf, -np.inf, np.nan):
+        k, _ = random_kv(rng, sum(lens), G, D)
+        q = rng.standard_normal((b.rows, heads, D), dtype=np.float32)
+        q[b.rows // 2, heads - 1, 3] = bad
+        got, keys = mass_of(ctx, b, fmt, k, q, heads, 0.1)
+        check_mass(b, got, *mass_by_rows(b, keys, q, heads, 0.1))
+    k[..., 3] = np.abs(k[..., 3]) + 1
+    q[b.rows // 2, heads - 1, 3] = -np.inf
+    got, keys = mass_of(ctx, b, fmt, k, q, heads, 0.1)
+    ref = mass_by_rows(b, keys, q, heads, 0.1)
+    assert not ref[2].any()
+    check_mass(b, got, *ref)
