@@ -368,12 +368,13 @@ int nx_attention_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch, con
  * mass_stride, one for each token j < kv_len[s]; tokens of the step itself have no `before`, and
  * before may be null (nothing was gathered) or mass itself.  What lies behind kv_len or
  * mass_stride, and the weights of a sequence without rows, stay as they were.
- * f32, scores and sums as nx_attention's (relative error about 1e-6 of each p; last bits depend
- * on the batch, not on the run).  A row that sees no token gives nothing, nor does one whose scores are all
- * -infinity; a row with a NaN or +infinity among the scores that it sees, or scores past
- * f32's range, gives NaNs to the tokens that it sees and to no others.  Rows and tokens that the
+ * f32, scores and sums as nx_attention's (relative error about 1e-6 of each p for scores of some
+ * tens, and 2^-22 of the scores' size beyond; last bits depend on the batch, not on the run).  A row that sees no token gives nothing, nor does one whose scores are all
+ * -infinity; a row with a NaN or +infinity among the scores that it sees gives NaNs to the
+ * tokens that it sees and to no others.  Scores are held as multiples of log 2: one past f32's range
+ * as such is an infinity.  Rows and tokens that the
  * matrix products give a NaN are done by the formula alone (every token of a prompt of 4093, an
- * infinite F16 key in each head: 3.7 ms, not 0.37).
+ * infinite F16 key in each head: 0.75 ms, not 0.37).
  * The workspace (256 MB) is the context's, allocated
  * with the first call, which is refused while the stream is captured, and never moved; calls on
  * one context must not overlap in time. */

@@ -37,7 +37,8 @@ struct MassCall {
   int rows_above, rows_upto;  // the kernels' sequences: those of so many rows
 };
 
-constexpr float kUnsetMax = -1e30f;
+// a row's maximum before its first score, which any may pass; less than this is only -infinity's stand-in
+constexpr float kUnsetMax = -0x1.fffffcp127f;
 
 __device__ __forceinline__ int rows_of(const MassCall &a, const KvSeq &q) {
   const int rows = q.n * a.group;
@@ -57,6 +58,13 @@ struct RowScale {
     return {ldexp1(1.f, 14 - X), ldexp1(1.f, X - 14 + (I8 ? 9 : 0))};
   }
 };
+
+// x by - less, the product rounded first
+__device__ __forceinline__ float score_less(float x, float by, float less) {
+#pragma clang fp contract(off)
+  const float y = x * by;
+  return y - less;
+}
 
 // log2 of a row's sum: above everything where it is nothing
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l); }
@@ -98,9 +106,8 @@ __device__ __forceinline__ KvSeq uniform(const KvSeq &s) {
 // ------------------------------------------------------------ scores by the formula alone
 // A query's halves may have signs of their own, or be 0 where the query is not: the products with an
 // infinite key then add up to a NaN where the score is an infinity.  (An infinity that they do add up to is the
-// score.)  So a sum that ends as a NaN, with the products done, is worked out again from q and the keys
-// as they are, in 64 bits: a wave takes the row's tokens, or the key's rows, one for each lane.  What the
-// products go through is left as it is, and a NaN that is the formula's ends at the first token or row that has one.
+// score.)  So where a row's or a token's sum ends as a NaN, the scores that are NaNs are worked out again from q and
+// the keys as they are, in 64 bits.  The loops of the products stay as they are.
 template <int FMT, int D>
 __device__ __forceinline__ float score_of(const KvView &kv, long group, int t, const float *q, float scale) {
   using E = kv_elem<FMT>;
@@ -115,26 +122,6 @@ __device__ __forceinline__ float score_of(const KvView &kv, long group, int t, c
   }
   if constexpr (FMT == NX_KV_INT8) sum *= kv.ks[group * kKvGroup + t];
   return (float)sum;
-}
-
-// the maximum and sum over a row's tokens [from, to), in all lanes; a sum of NaN where it is the formula's
-template <int FMT, int D>
-__device__ __forceinline__ float2 row_by_formula(const KvView &kv, const nx_kv_batch &b, int seq, int head, const float *q,
-                                              float scale, int from, int to) {
-  const int lane = threadIdx.x & 63;
-  float2 o = {kUnsetMax, 0.f};
-#pragma unroll 1
-  for (int t0 = from; t0 < to; t0 += 64) {
-    const int t = t0 + lane;
-    const long group = t < to ? kv_group(kv, b, seq, head, t & ~(kKvGroup - 1)) : -1;
-    const float x = group >= 0 ? score_of<FMT, D>(kv, group, t & (kKvGroup - 1), q, scale) : -INFINITY;
-    if (__any(!(x < INFINITY))) return {kUnsetMax, NAN};
-    const float most = fmaxf(o.x, x);
-    o = {most, o.y * __builtin_amdgcn_exp2f(o.x - most) + __builtin_amdgcn_exp2f(x - most)};
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) o = joined(o, float2{__shfl_xor(o.x, d, 64), __shfl_xor(o.y, d, 64)});
-  return o;
 }
 
 // ------------------------------------------------------------ few rows
@@ -389,6 +376,20 @@ struct WideWork {
   _Float16 *halves;  // [rows x heads][2][D] the queries as k_mass_stats splits them
   float *part;     // k_mass_stats: [rows x heads][key_parts] {maximum, sum}; k_mass_columns: [tiles][row_parts][tokens]
 };
+
+// The arguments of a kernel as it has them in memory, for what is hardly ever done: kept in registers for that they
+// took others' (k_mass_columns 198 us for a prompt of 4093, not 191).
+struct WideArgs {
+  KvView kv;
+  nx_kv_batch b;
+  MassCall a;
+  WideWork w;
+};
+__device__ __forceinline__ const WideArgs &arguments() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const WideArgs *)p;
+}
 
 // a sequence's part in the launch's rows, where it is these kernels' at all
 __device__ __forceinline__ KvSeq part_of(const MassCall &a, const WideWork &w, const KvSeq &q) {
@@ -685,23 +686,55 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 3) void k_mass_stats(K
           m = most;
           float more[2] = {0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 16; ++j) more[j & 1] += __builtin_amdgcn_exp2f(I8 ? x[j] - m : fmaf(x[j], c, -m));
+          for (int j = 0; j < 16; ++j) more[j & 1] += __builtin_amdgcn_exp2f(I8 ? score_less(x[j], 1.f, m) : fmaf(x[j], c, -m));
           l += more[0] + more[1];
         }
       }
-    }
-    float all = max_halves(m);
-    l = across_halves(l * __builtin_amdgcn_exp2f(m - all), [](float x, float y) { return x + y; });
-    for (uint32_t odd = (uint32_t)__ballot(mine && l != l); odd; odd &= odd - 1) {
-      const int i = __builtin_ctz(odd), r = r0 + 32 * wave + i, now = by_group(r, a.magic, a.shift);
-      const float *q = a.q + (size_t)(s.row + now) * a.q_stride + (size_t)(head * a.group + r - now * a.group) * D;
-      const float2 o = row_by_formula<FMT, D>(kv, b, seq, head, q, a.scale, begin * kKvGroup,
-                                              min(end * kKvGroup, min(s.first + now + 1, s.len)));
-      if (n == i) {
-        all = o.x;
-        l = o.y;
+      // Once more, with the scores that are NaNs by the formula.  The others are those of k_mass_columns to the last
+      // bit, as the whole row's would not be: far from 0 that is a factor of any size.
+      if (__any(mine && l != l)) {
+        const WideArgs &in = arguments();
+        const float *q = in.a.q + (size_t)(s.row + tok) * in.a.q_stride + (size_t)(head * in.a.group + row - tok * in.a.group) * D;
+        m = kUnsetMax;
+        l = 0.f;
+#pragma unroll 1
+        for (int i = chunk * in.w.m.key_share; i < end; ++i) {
+          const int page = uniform(groups.page(i));
+          if (!groups.there(page)) continue;
+          const long group = groups.at(i, page);
+          const E *base = reinterpret_cast<const E *>(in.kv.k) + group * (kKvGroup * D) + (h * kKvGroup + n) * 8;
+          f32x16 sc;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sc[j] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            f16x8 kx;
+            if constexpr (I8) {
+              const uint2 x = *reinterpret_cast<const uint2 *>(base + 2 * ks * kKvGroup * 8);
+              kx = from_codes(x.x, x.y);
+            } else {
+              kx = *reinterpret_cast<const f16x8 *>(base + 2 * ks * kKvGroup * 8);
+            }
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, qh[ks], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, ql[ks], sc, 0, 0, 0);
+          }
+#pragma unroll 1
+          for (int j = 0; j < 16; ++j) {
+            const int t = kv_token(FMT, 8 * (j >> 2) + 4 * h + (j & 3));
+            float x = sc[0] * (I8 ? in.kv.ks[group * kKvGroup + t] * c : c);
+#pragma unroll
+            for (int next = 1; next < 16; ++next) sc[next - 1] = sc[next];
+            if (i * kKvGroup + t > p) continue;
+            if (x != x && l == l) x = score_of<FMT, D>(in.kv, group, t, q, in.a.scale);
+            const float most = fmaxf(m, x);
+            l = l * __builtin_amdgcn_exp2f(m - most) + __builtin_amdgcn_exp2f(score_less(x, 1.f, most));
+            m = most;
+          }
+        }
       }
     }
+    const float all = max_halves(m);
+    l = across_halves(l * __builtin_amdgcn_exp2f(m - all), [](float x, float y) { return x + y; });
     if (h == 0 && mine) {
       const size_t o = stat_of(a, w, s, head) + row;
       if (w.m.key_parts == 1)
@@ -734,20 +767,6 @@ constexpr int kKeyTile = kMassWaves * kHeldGroups<D>;  // of a workgroup
 // kv_token of h = 0, and so many behind it
 template <int FMT>
 constexpr int kTokenOfHalf = kv_token(FMT, 4);
-
-// The arguments of a kernel as it has them in memory, for what is hardly ever done: kept in registers for that they
-// took others' (k_mass_columns 198 us for a prompt of 4093, not 191).
-struct WideArgs {
-  KvView kv;
-  nx_kv_batch b;
-  MassCall a;
-  WideWork w;
-};
-__device__ __forceinline__ const WideArgs &arguments() {
-  auto p = __builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  return *(const WideArgs *)p;
-}
 
 // the weight that rows [from, to) give a token, in all lanes: NaN where any that sees it has no log sum
 template <int FMT, int D>
@@ -887,6 +906,10 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
         if (block + 2 < to) fetch(block + 2);
       }
       const float c = coef[buf][n], ei = lse[buf][n];
+      // INT8: far from 0 a score is rounded before e is taken off, as k_mass_stats does, where the rounding alone is
+      // a factor of e^(2^-12) and more.  (Without the condition: 70.5 us for the last queries of two prompts, not 69.  F16's
+      // factor is a power of two.)
+      const bool far = I8 && __any(fabsf(ei) > 4096.f);
       const int p = token[buf][n];
       const int pmin = uniform(block * kMassBlock + kMassBlock <= rows ? token[buf][0] : -1);
       const int pmax = s.first + by_group(min(block * kMassBlock + kMassBlock, rows) - 1, a.magic, a.shift);
@@ -910,8 +933,18 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
       for (int i = 0; i < KG; ++i) {
         const int g0 = first + i * kKvGroup;
         float y[16];
+        float by[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], I8 ? scales[wave][i][h][j] * c : c, -ei));
+        for (int j = 0; j < 16; ++j) by[j] = I8 ? scales[wave][i][h][j] * c : c;
+        if (far) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            sc[i][j] *= by[j];
+            by[j] = 1.f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], by[j], -ei));
         if (g0 + kKvGroup - 1 > pmin) {
 #pragma unroll
           for (int j = 0; j < 16; ++j)

@@ -187,3 +187,51 @@ def test_queries_that_are_not_finite(ctx, fmt, heads, G, D, ns, lens):
     ref = mass_by_rows(b, keys, q, heads, 0.1)
     assert not ref[2].any()
     check_mass(b, got, *ref)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("size", [1e29, 3e30, 1e33, 1e37])
+@pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
+def test_scores_far_below_zero(ctx, fmt, heads, G, D, ns, lens, size):
+    """Rows whose scores are all of that size below 0: the highest takes all, and the only token of a
+    row takes it, as with any other scores.
+
+    Tokens differ by a thousandth or more, far above any rounding, so a weight is 0 or 1 and their sums
+    are whole numbers, which f32 holds."""
+    rng = np.random.default_rng(34 + D)
+    b = Batch(rng, ns, lens, 32)
+    # D terms of q k scale / D, q of one size and k of another
+    k_size = 100.0 if fmt == F16 else 1e18
+    k = np.empty((sum(lens), G, D), np.float32)
+    at = 0
+    for n in lens:
+        for g in range(G):
+            k[at:at + n, g] = (k_size * (1 + rng.permutation(n) / 50))[:, None]
+        at += n
+    q = np.full((b.rows, heads, D), -size / k_size * (1 / D), np.float32) * (1 + rng.random((b.rows, heads, 1), dtype=np.float32))
+    got, keys = mass_of(ctx, b, fmt, k, q, heads, 1.0)
+    want, at = np.zeros_like(got), 0
+    for s, (n, length) in enumerate(zip(ns, lens)):
+        for p in range(length - n, length):
+            for g in range(G):
+                want[s, g, keys[at:at + p + 1, g, 0].argmin()] += heads // G
+        at += length
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
+def test_low_scores_beside_infinite_ones(ctx, heads, G, D, ns, lens):
+    """A finite score of any size has weight beside those of -infinity."""
+    rng = np.random.default_rng(35 + D)
+    b = Batch(rng, ns, lens, 32)
+    k = np.full((sum(lens), G, D), np.inf, np.float32)
+    at = 0
+    for n in lens:
+        k[at + n // 3] = 1
+        at += n
+    q = np.full((b.rows, heads, D), -1e32, np.float32)
+    got, _ = mass_of(ctx, b, F16, k, q, heads, 1.0)
+    want = np.zeros_like(got)
+    for s, (n, length) in enumerate(zip(ns, lens)):
+        want[s, :, length // 3] = heads // G * min(n, length - length // 3)
+    assert np.array_equal(got, want)
