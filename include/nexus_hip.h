@@ -460,7 +460,8 @@ int nx_qk_rope_dev(nx_ctx *ctx, const nx_rope *rope, const int32_t *d_positions,
  * other.)  A row with a NaN or +infinity has NaNs for entropy and log probabilities, but for
  * the -infinity of filled-up places; its alternatives are those by value, NaNs left out.  A token
  * that is not 0 .. vocab - 1 names none: its log probability is 0.  Accuracy: entropy and log
- * probabilities within 2^-20 (1 + |value| + the spread of the likely logits).  Outputs must
+ * probabilities within 2^-20 (1 + |value| + spread), whatever the number of logits; the spread is
+ * how far below the largest logit the row's are, on average by their probability.  Outputs must
  * not overlap inputs.  The library's workspace for few long rows (0.5 MB) is the context's, as the
  * attention's: a context's first call with fewer than 1024 rows is refused while its stream is
  * captured, and calls on one context must not overlap in time.  Sampling's softmax over the

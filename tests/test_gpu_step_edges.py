@@ -235,3 +235,56 @@ def test_low_scores_beside_infinite_ones(ctx, heads, G, D, ns, lens):
     for s, (n, length) in enumerate(zip(ns, lens)):
         want[s, :, length // 3] = heads // G * min(n, length - length // 3)
     assert np.array_equal(got, want)
+
+
+# ---------------------------------------------------------------- log probabilities
+def promised(value, spread):
+    """What a log probability or an entropy may be off."""
+    return 2.0 ** -20 * (1 + np.abs(value) + spread)
+
+
+def on_rows(ctx, x, tokens):
+    """logprobs_dev of device rows: the log probabilities of one token each, and the entropy."""
+    T, V = x.shape
+    d = DeviceArray(x.size)
+    d.upload(x)
+    dt, lp, ent = DeviceArray(T), DeviceArray(T), DeviceArray(T)
+    dt.upload(np.asarray(tokens, np.int32).view(np.float32))
+    ctx.logprobs_dev(d.ptr, V, T, V, dt.ptr, 1, lp.ptr, ent.ptr, 0, 0, 0)
+    ctx.sync()
+    return lp.download().astype(np.float64), ent.download().astype(np.float64)
+
+
+@pytest.mark.parametrize("T,V", [(1, 1 << 26), (5, 1 << 23), (513, 262144)])
+def test_flat_rows_of_many_logits(ctx, T, V):
+    """One logit above V - 1 equal ones: every term rounds the same way, so a sum of many of them in
+    f32 would be further off the more there are."""
+    for low in np.linspace(-14, -0.25, 4) if T == 1 else [None]:
+        c = np.float32([low] if T == 1 else np.linspace(-14, -0.25, T))
+        x = np.empty((T, V), np.float32)
+        x[:] = c[:, None]
+        peak = (np.arange(T) * 7919) % V
+        x[np.arange(T), peak] = 0
+        lp, ent = on_rows(ctx, x, (peak + 1) % V)
+        d = c.astype(np.float64)
+        p = np.exp(d)
+        S = 1 + (V - 1) * p
+        want = d - np.log(S)
+        spread = (V - 1) * p / S * -d
+        for name, got, ref in (("logprobs", lp, want), ("entropy", ent, np.log(S) + spread)):
+            off = np.abs(got - ref) / promised(ref, spread)
+            assert (off <= 1).all(), (name, off.max(), c[off.argmax()])
+
+
+@pytest.mark.parametrize("T,V", [(1, 1 << 24), (513, 100003)])
+@pytest.mark.parametrize("rise", [0.75, 40.0])
+def test_rising_rows_of_many_logits(ctx, T, V, rise):
+    """The largest logit so far moves on with every step."""
+    row = np.linspace(-rise, 0, V).astype(np.float32)
+    lp, ent = on_rows(ctx, np.broadcast_to(row, (T, V)), np.arange(T))
+    d = row.astype(np.float64)
+    p = np.exp(d)
+    S, spread = p.sum(), (p * -d).sum() / p.sum()
+    for got, ref in ((lp, d[:T] - np.log(S)), (ent, np.log(S) + spread)):
+        off = np.abs(got - ref) / promised(ref, spread)
+        assert (off <= 1).all(), off.max()
