@@ -463,8 +463,9 @@ int nx_qk_rope_dev(nx_ctx *ctx, const nx_rope *rope, const int32_t *d_positions,
  * probabilities within 2^-20 (1 + |value| + spread), whatever the number of logits; the spread is
  * how far below the largest logit the row's are, on average by their probability.  Outputs must
  * not overlap inputs.  The library's workspace for few long rows (0.5 MB) is the context's, as the
- * attention's: a context's first call with fewer than 1024 rows is refused while its stream is
- * captured, and calls on one context must not overlap in time.  Sampling's softmax over the
+ * attention's.  Calls of up to 512 rows of more than 4096 logits take it, and no others: a context's
+ * first such call allocates it and is refused while its stream is captured, whatever other calls went
+ * before.  Calls on one context must not overlap in time.  Sampling's softmax over the
  * logits (src/engine/mod.rs:819), for the tokens that were chosen. */
 int nx_logprobs(nx_ctx *ctx, const float *logits, size_t stride, int num_tokens, int vocab,
                 const int32_t *tokens, int given, float *logprobs, float *entropy, int top,

@@ -7,6 +7,7 @@ import nexus_amd as nx
 from kv_cases import F16, INT8, Batch, random_kv, stored
 from moe_cases import DeviceArray, assert_same_bits
 from test_gpu_evict import Case
+from test_gpu_step import Hip
 
 pytestmark = pytest.mark.gpu
 FORMATS = [F16, INT8]
@@ -288,3 +289,52 @@ def test_rising_rows_of_many_logits(ctx, T, V, rise):
     for got, ref in ((lp, d[:T] - np.log(S)), (ent, np.log(S) + spread)):
         off = np.abs(got - ref) / promised(ref, spread)
         assert (off <= 1).all(), off.max()
+
+
+def test_workspace_of_few_long_rows_under_capture():
+    """Calls of more or shorter rows do not allocate what few long rows take: the first of those is
+    refused while the stream is captured, the others are not, and after one outside it is taken."""
+    hip = Hip()
+    rng = np.random.default_rng(41)
+    shapes = [(600, 4097), (512, 4096), (512, 4097), (3, 9000)]
+    with nx.Context(0) as ctx:
+        stream = hip.stream()
+        ctx.set_stream(stream.value)
+        x = rng.standard_normal(600 * 4097).astype(np.float32)
+        d, ent = DeviceArray(x.size), DeviceArray(600)
+        d.upload(x)
+
+        def call(T, V):
+            ctx.logprobs_dev(d.ptr, V, T, V, 0, 0, 0, ent.ptr, 0, 0, 0)
+
+        for warm in (False, True):
+            for T, V in shapes[:2] + shapes[2:] * warm:
+                call(T, V)
+            ctx.sync()
+            refused = []
+
+            def calls():
+                for shape in shapes[:2] + shapes[2:] * (not warm):
+                    try:
+                        call(*shape)
+                    except nx.NexusError as e:
+                        refused.append((shape, e.code))
+                if warm:
+                    call(*shapes[3])
+
+            g, graph = hip.graph(stream, calls)
+            assert refused == ([] if warm else [(s, nx.NX_ERR_UNSUPPORTED) for s in shapes[2:]])
+            for _ in range(3):
+                ent.upload(np.zeros(600))
+                hip.hipGraphLaunch(graph, stream)
+                ctx.sync()
+                T, V = shapes[3] if warm else shapes[1]
+                rows = x[:T * V].reshape(T, V).astype(np.float64)
+                p = np.exp(rows - rows.max(1, keepdims=True))
+                p /= p.sum(1, keepdims=True)
+                ref, spread = -(p * np.log(p)).sum(1), (p * (rows.max(1, keepdims=True) - rows)).sum(1)
+                assert (np.abs(ent.download()[:T] - ref) <= promised(ref, spread)).all()
+            hip.hipGraphExecDestroy(graph)
+            hip.hipGraphDestroy(g)
+        ctx.set_stream(None)
+        hip.hipStreamDestroy(stream)
