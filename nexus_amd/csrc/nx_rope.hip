@@ -42,12 +42,18 @@ __device__ __forceinline__ float2 turn_of(int position, float freq) {
   return {fmaf(-lo, s, c), fmaf(lo, c, s)};
 }
 
-// what a head's elements are scaled by, from its lanes' sums (L of them, a power of two)
+// What a head's elements are multiplied by, from its lanes' sums (L of them, a power of two): first by `up`, a
+// power of two that is 1 but where eps is 0 and the head all but is, whose factor f32 does not hold.
+struct NormScale {
+  float up, s;
+};
 template <int L>
-__device__ __forceinline__ float scale_of(double sum, int D, float eps) {
+__device__ __forceinline__ NormScale scale_of(double sum, int D, float eps) {
 #pragma unroll
   for (int d = 1; d < L; d <<= 1) sum += __shfl_xor(sum, d, L);
-  return (float)(1.0 / sqrt(sum / D + (double)eps));
+  const double s = 1.0 / sqrt(sum / D + (double)eps);
+  const bool large = s > 0x1p100;
+  return {large ? 0x1p100f : 1.f, (float)(large ? s * 0x1p-100 : s)};
 }
 
 struct Head {
@@ -103,7 +109,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_wide(RopeCall a, int roun
       double sum = 0.;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = fma((double)e[i], (double)e[i], sum);
-      const float s = scale_of<L>(sum, a.D, a.eps);
+      const NormScale s = scale_of<L>(sum, a.D, a.eps);
       float w[8] = {};
       if (whole) {
         const float4 w0 = *reinterpret_cast<const float4 *>(head.w + at0);
@@ -111,7 +117,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_wide(RopeCall a, int roun
         w[0] = w0.x, w[1] = w0.y, w[2] = w0.z, w[3] = w0.w, w[4] = w1.x, w[5] = w1.y, w[6] = w1.z, w[7] = w1.w;
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = e[i] * s * w[i];
+      for (int i = 0; i < 8; ++i) e[i] = e[i] * s.up * s.s * w[i];
     }
     if (rotated) {
 #pragma unroll
@@ -155,12 +161,13 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_any(RopeCall a, int per_w
       e[j] = 2 * (lane + 64 * j) < a.D ? float2{head.in[at0[j]], head.in[at1[j]]} : float2{0.f, 0.f};
       sum = fma((double)e[j].x, (double)e[j].x, fma((double)e[j].y, (double)e[j].y, sum));
     }
-    const float s = head.w ? scale_of<64>(sum, a.D, a.eps) : 1.f;
+    const NormScale s = head.w ? scale_of<64>(sum, a.D, a.eps) : NormScale{1.f, 1.f};
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) {
       const int p = lane + 64 * j;
       if (2 * p >= a.D) continue;
-      const float x = head.w ? e[j].x * s * head.w[at0[j]] : e[j].x, y = head.w ? e[j].y * s * head.w[at1[j]] : e[j].y;
+      const float x = head.w ? e[j].x * s.up * s.s * head.w[at0[j]] : e[j].x;
+      const float y = head.w ? e[j].y * s.up * s.s * head.w[at1[j]] : e[j].y;
       const bool rotated = 2 * p < a.R;
       head.out[at0[j]] = rotated ? fmaf(x, turn[j].x, -(y * turn[j].y)) : x;
       head.out[at1[j]] = rotated ? fmaf(x, turn[j].y, y * turn[j].x) : y;

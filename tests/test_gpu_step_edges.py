@@ -6,6 +6,7 @@ import pytest
 import nexus_amd as nx
 from kv_cases import F16, INT8, Batch, random_kv, stored
 from moe_cases import DeviceArray, assert_same_bits
+from step_cases import HALVES, PAIRS, rope
 from test_gpu_evict import Case
 from test_gpu_step import Hip
 
@@ -236,6 +237,27 @@ def test_low_scores_beside_infinite_ones(ctx, heads, G, D, ns, lens):
     for s, (n, length) in enumerate(zip(ns, lens)):
         want[s, :, length // 3] = heads // G * min(n, length - length // 3)
     assert np.array_equal(got, want)
+
+
+# ---------------------------------------------------------------- rotation
+@pytest.mark.parametrize("D", [64, 62, 256, 512])
+@pytest.mark.parametrize("eps", [0.0, 1e-45, 1e-30])
+def test_norm_of_heads_next_to_nothing(ctx, D, eps):
+    """Heads of subnormal values, one of them even of the least, with an eps that does not cover them;
+    heads of zeros, whose norm without eps is 0 / 0."""
+    rng = np.random.default_rng(51)
+    x = rng.standard_normal((7, 2, D)).astype(np.float32)
+    for i, size in enumerate((1e-38, 1e-40, 1e-43, 1e-30, 1e-20, 1.0)):
+        x[i] *= np.float32(size)
+    x[2, 1] = 0
+    x[2, 1, D // 2 + 1] = 2.0 ** -149
+    x[6] = 0
+    w, freq = (1 + rng.random(D)).astype(np.float32), np.linspace(1, 0.01, D // 2).astype(np.float32)
+    for style in (HALVES, PAIRS):
+        got, _ = ctx.qk_rope(np.arange(7), x, None, freq, style, w, None, eps)
+        ref, bound = rope(np.arange(7), x, freq, style, w, eps)
+        assert (np.abs(got[:6] - ref[:6]) <= bound[:6]).all()
+        assert np.isnan(got[6]).all() if eps == 0 else not got[6].any()
 
 
 # ---------------------------------------------------------------- log probabilities
