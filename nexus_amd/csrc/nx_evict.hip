@@ -280,7 +280,8 @@ static int evict(nx_ctx *c, nx_kv *kv, const nx_kv_batch *b, const EvictArgs &a,
   NX_HIP(hipMemcpyAsync(len, b->kv_len, S * 4, hipMemcpyHostToDevice, c->stream));
   NX_HIP(hipMemcpyAsync(pages, b->pages, table * 4, hipMemcpyHostToDevice, c->stream));
   NX_HIP(hipMemcpyAsync(to_pages, a.to_pages, to * 4, hipMemcpyHostToDevice, c->stream));
-  NX_HIP(hipMemcpy2DAsync(pm, width * 4, a.mass, a.mass_stride * 4, width * 4, tiles, hipMemcpyHostToDevice, c->stream));
+  NX_TRY(upload_weights(c, static_cast<float *>(pm), width, a.mass, a.mass_stride,
+                        weight_rows(b->num_seqs, kv->heads, [&](int s) { return (size_t)b->kv_len[s]; })));
   NX_TRY(evict_dev(c, kv, on, d));
   NX_HIP(hipMemcpyAsync(a.kept, d.kept, kept * 4, hipMemcpyDeviceToHost, c->stream));
   NX_HIP(hipMemcpyAsync(a.new_len, new_len, S * 4, hipMemcpyDeviceToHost, c->stream));

@@ -179,6 +179,17 @@ void with_kernel(const nx_kv *kv, F f) {
 template <int FMT>
 using kv_elem = std::conditional_t<FMT == NX_KV_INT8, int8_t, _Float16>;
 
+// rows of weights (nx_step_plan.hpp's WeightRows) from the host, `from_stride` apart, to rows of `width`
+template <typename Rows>
+int upload_weights(nx_ctx *c, float *to, size_t width, const float *from, size_t from_stride, const Rows &r) {
+  if (r.rows > 1)
+    NX_HIP(hipMemcpy2DAsync(to, width * 4, from, from_stride * 4, width * 4, r.rows - 1, hipMemcpyHostToDevice, c->stream));
+  if (r.rows > 0)
+    NX_HIP(hipMemcpyAsync(to + (r.rows - 1) * width, from + (r.rows - 1) * from_stride, r.last * 4, hipMemcpyHostToDevice,
+                          c->stream));
+  return NX_OK;
+}
+
 inline int refuse(const Refusal &r) { return r ? fail(r.code, r.why) : NX_OK; }
 
 }  // namespace nx

@@ -1135,8 +1135,11 @@ static int attention_mass(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, cons
   NX_TRY(ws_get(c, WS_XIN, rows * width * 4, &dq));
   NX_TRY(ws_get(c, WS_OUT, tiles * most * 4, &dm));
   NX_HIP(hipMemcpy2DAsync(dq, width * 4, q, q_stride * 4, width * 4, rows, hipMemcpyHostToDevice, c->stream));
-  if (before)
-    NX_HIP(hipMemcpy2DAsync(dm, most * 4, before, mass_stride * 4, most * 4, tiles, hipMemcpyHostToDevice, c->stream));
+  if (before)  // (of sequences that have rows, the tokens before them)
+    NX_TRY(upload_weights(c, static_cast<float *>(dm), most, before, mass_stride, weight_rows(b->num_seqs, kv->heads, [&](int s) {
+                            const int n = b->row_start[s + 1] - b->row_start[s];
+                            return n > 0 ? std::min((size_t)(b->kv_len[s] - n), most) : 0;
+                          })));
   a.q = static_cast<const float *>(dq);
   a.q_stride = width;
   a.mass = static_cast<float *>(dm);

@@ -185,6 +185,19 @@ inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int group
   return m;
 }
 
+// How the rows of weights of a host call are read, need(sequence) of each row of a sequence: `rows` - 1 whole ones of
+// `width`, and of the last sequence that has any its last row's `last` weights, for the caller's memory may
+// end with them.
+struct WeightRows {
+  size_t rows, last;
+};
+template <typename Need>
+WeightRows weight_rows(int seqs, int kv_heads, Need need) {
+  for (int s = seqs - 1; s >= 0; --s)
+    if (const size_t n = need(s)) return {(size_t)(s + 1) * kv_heads, n};
+  return {0, 0};
+}
+
 // The arguments of an eviction besides the cache and the batch.
 struct EvictArgs {
   const int32_t *to_pages;

@@ -54,6 +54,43 @@ def test_first_kept_tokens_of_a_group(ctx, fmt):
     c.cache.close()
 
 
+@pytest.mark.parametrize("lens", [[300, 40], [300, 40, 0], [60, 300]])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_host_weights_that_end_with_the_last_token(ctx, fmt, lens):
+    """Rows of weights as far apart as the longest sequence is long, in memory that ends with the last
+    sequence's last weight: the host calls' results are those of whole rows."""
+    G, heads, D, keep, stride = 2, 4, 64, 37, 311
+    rng = np.random.default_rng(23)
+    c = Case(ctx, rng, fmt, lens, 32, G, D, keep)
+    S, last = len(lens), max(s for s, n in enumerate(lens) if n)
+    end = (last * G + G - 1) * stride + lens[last]
+    rows = np.full((S, G, stride), np.nan, np.float32)
+    rows[:, :, :max(lens)] = c.mass
+    whole = c.cache.evict(c.b.kv_len, c.b.pages, c.to, keep, c.mass, 2, 3)
+    memory = np.full(rows.size + 3 * S * G * keep, 7, np.float32)
+    exact, moved = memory[:end], memory[-S * G * keep:].reshape(S, G, keep)
+    exact[:] = rows.ravel()[:end]
+    L, kept, new_len = nx.lib(), np.zeros((S, G, keep), np.int32), np.zeros(S, np.int32)
+    b, hold = c.cache._host_batch(np.zeros(S + 1), c.b.kv_len, c.b.pages, 0)
+    nx.check(L.nx_kv_evict(ctx.h, c.cache.h, b.ref, c.to.ctypes.data, c.to.shape[1], keep, 2, 3, exact.ctypes.data, stride,
+                           kept.ctypes.data, new_len.ctypes.data, moved.ctypes.data, keep))
+    assert np.array_equal(kept, whole[0]) and np.array_equal(new_len, whole[1])
+    for s in range(S):
+        assert_same_bits(moved[s, :, :new_len[s]], whole[2][s, :, :new_len[s]])
+    # a new token of each sequence that has any
+    starts = np.concatenate([[0], np.cumsum(np.minimum(lens, 1))]).astype(np.int32)
+    q = rng.standard_normal((starts[-1], heads, D), dtype=np.float32)
+    want = c.cache.attention_mass(starts, c.b.kv_len, c.b.pages, q, heads, before=np.nan_to_num(rows, nan=7))
+    b, hold = c.cache._host_batch(starts, c.b.kv_len, c.b.pages, len(q))
+    got = exact.copy()
+    nx.check(L.nx_attention_mass(ctx.h, c.cache.h, b.ref, q.ctypes.data, heads * D, heads, D ** -0.5, got.ctypes.data,
+                                 got.ctypes.data, stride))
+    got = np.append(got, np.full(rows.size - end, 7, np.float32)).reshape(rows.shape)
+    for s, n in enumerate(lens):
+        assert_same_bits(got[s, :, :n], want[s, :, :n])
+    c.cache.close()
+
+
 # ---------------------------------------------------------------- gathered weights
 def mass_by_rows(b, keys, q, heads, scale, before=None):
     """mass [seqs x G x width], a bound, and which tokens get NaNs, of keys and queries that may hold
