@@ -389,7 +389,7 @@ int nx_attention_mass_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch
  * fewer, all).  They are chosen for every key/value head apart, by the weights at
  *   mass + (sequence * kv_heads + head) * mass_stride,  one of each token
  * (nx_attention_mass gathers them; any f32 will do, of equal ones the lower token is kept,
- * and a NaN counts less than any number, a token behind mass_stride as NaN), and move, in their
+ * and a NaN counts less than any number, a token behind mass_stride as NaN; its new weight is 0), and move, in their
  * order, to the pages to_pages[sequence * to_max_pages + p], as they are stored.  Of the batch,
  * kv_len, pages, max_pages and num_seqs are read (row_start and num_tokens are not).
  * Writes kept [num_seqs x kv_heads x keep], the tokens that each head kept, then -1;
@@ -401,7 +401,8 @@ int nx_attention_mass_dev(nx_ctx *ctx, const nx_kv *kv, const nx_kv_batch *batch
  * (nx_qk_rope) that follow its old ones.
  * The new pages must be none that the batch's sequences use, each named once: host calls refuse
  * others, *_dev calls cannot (there, what such pages hold afterwards is not defined; entries
- * that name no page are left out, and tokens on no page move as zeros).  The rest of the last
+ * that name no page are left out, and tokens on no page move as zeros).  New weights must not
+ * overlap the old ones (*_dev calls, which do not know the lengths, take rows of mass_stride for whole ones).  The rest of the last
  * group of 32 tokens of a new page is cleared.  Needs no workspace. */
 int nx_kv_evict(nx_ctx *ctx, nx_kv *kv, const nx_kv_batch *batch, const int32_t *to_pages, int to_max_pages,
                 int keep, int sinks, int recent, const float *mass, size_t mass_stride, int32_t *kept,

@@ -252,10 +252,10 @@ static int evict_dev(nx_ctx *c, const nx_kv *kv, const nx_kv_batch &b, const Evi
 
 static int evict(nx_ctx *c, nx_kv *kv, const nx_kv_batch *b, const EvictArgs &a, bool host) {
   NX_TRY(kv_check_cache(c, kv));
-  NX_TRY(refuse(evict_check(b, kv->page_tokens, kv->heads, a)));
+  NX_TRY(refuse(evict_check(b, kv->page_tokens, kv->heads, a, host)));
   if (b->num_seqs == 0) return NX_OK;
   if (!host) return evict_dev(c, kv, *b, a);
-  NX_TRY(refuse(evict_check_tables(*b, kv->pages, kv->page_tokens, a)));
+  NX_TRY(refuse(evict_check_tables(*b, kv->pages, kv->page_tokens, a, kv->heads)));
   const size_t S = b->num_seqs, tiles = S * kv->heads, table = S * b->max_pages, to = S * a.to_max_pages;
   const size_t kept = tiles * a.keep;
   size_t width = 1;  // weights that are looked at

@@ -1120,10 +1120,11 @@ static int attention_mass(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, cons
   NX_TRY(refuse(attn_check(heads, kv->heads, scale, 0, 0)));
   if (b->num_seqs == 0 || b->num_tokens == 0) return NX_OK;
   const size_t width = (size_t)heads * kv->D;
-  NX_TRY(refuse(mass_check(b, kv->heads, heads, q_stride, width, q, before, mass, mass_stride)));
+  NX_TRY(refuse(mass_check(b, kv->heads, heads, q_stride, width, q, before, mass, mass_stride, host)));
   MassCall a{q, before, mass, q_stride, mass_stride, heads, heads / kv->heads, scale * kLog2e};
   if (!host) return mass_dev(c, kv, *b, a);
   NX_TRY(refuse(kv_check_tables(*b, kv->pages, kv->page_tokens, true, false)));
+  NX_TRY(refuse(mass_check_tables(*b, kv->heads, before, mass, mass_stride)));
   const size_t rows = b->row_start[b->num_seqs], tiles = (size_t)b->num_seqs * kv->heads;
   if (rows == (size_t)b->row_start[0]) return NX_OK;
   size_t most = 1;
@@ -1136,10 +1137,7 @@ static int attention_mass(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, cons
   NX_TRY(ws_get(c, WS_OUT, tiles * most * 4, &dm));
   NX_HIP(hipMemcpy2DAsync(dq, width * 4, q, q_stride * 4, width * 4, rows, hipMemcpyHostToDevice, c->stream));
   if (before)  // (of sequences that have rows, the tokens before them)
-    NX_TRY(upload_weights(c, static_cast<float *>(dm), most, before, mass_stride, weight_rows(b->num_seqs, kv->heads, [&](int s) {
-                            const int n = b->row_start[s + 1] - b->row_start[s];
-                            return n > 0 ? std::min((size_t)(b->kv_len[s] - n), most) : 0;
-                          })));
+    NX_TRY(upload_weights(c, static_cast<float *>(dm), most, before, mass_stride, weight_rows(b->num_seqs, kv->heads, [&](int s) { return mass_read(*b, s, most); })));
   a.q = static_cast<const float *>(dq);
   a.q_stride = width;
   a.mass = static_cast<float *>(dm);

@@ -89,16 +89,59 @@ inline Refusal logprobs_check(const float *logits, size_t stride, int rows, int 
   return {};
 }
 
-// What the calls that gather attention weights check besides attn_check.
+// How the rows of weights of a host call are read, need(sequence) of each row of a sequence: `rows` - 1 whole ones of
+// `width`, and of the last sequence that has any its last row's `last` weights, for the caller's memory may
+// end with them.
+struct WeightRows {
+  size_t rows, last;
+};
+template <typename Need>
+WeightRows weight_rows(int seqs, int kv_heads, Need need) {
+  for (int s = seqs - 1; s >= 0; --s)
+    if (const size_t n = need(s)) return {(size_t)(s + 1) * kv_heads, n};
+  return {0, 0};
+}
+// Whether they, `sa` apart, share memory with others, `sb` apart: between the first weights and the last ones of
+// both, and there as rows of wa and wb.
+inline bool weights_overlap(const float *a, size_t sa, size_t wa, const WeightRows &ra, const float *b, size_t sb, size_t wb,
+                            const WeightRows &rb) {
+  if (!ra.rows || !rb.rows) return false;
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  if (a0 + 4 * ((ra.rows - 1) * sa + ra.last) <= b0 || b0 + 4 * ((rb.rows - 1) * sb + rb.last) <= a0) return false;
+  return rows_overlap(a, sa, wa, b, sb, wb, (long)std::max(ra.rows, rb.rows));
+}
+
+// What the calls that gather attention weights check besides attn_check.  Calls on device memory, whose lengths
+// are not known, take rows of weights for whole ones; `host`: mass_check_tables looks at them.
 inline Refusal mass_check(const nx_kv_batch *b, int kv_heads, int heads, size_t q_stride, size_t width, const float *q,
-                          const float *before, const float *mass, size_t mass_stride) {
+                          const float *before, const float *mass, size_t mass_stride, bool host = false) {
   if (!q || !mass) return {NX_ERR_INVALID_ARG, "null buffer"};
   if ((int64_t)b->num_tokens * heads > INT32_MAX) return {NX_ERR_UNSUPPORTED, "more than 2^31 query rows"};
   if (q_stride > (size_t)1 << 40 || mass_stride > (size_t)1 << 40) return {NX_ERR_UNSUPPORTED, "row stride above 2^40"};
   if (Refusal f = kv_check_rows("query", (long)q_stride, (long)width)) return f;
   if (mass_stride == 0) return {NX_ERR_SHAPE, "rows of no weights"};
-  if (before && before != mass &&
+  if (!host && before && before != mass &&
       rows_overlap(before, mass_stride, mass_stride, mass, mass_stride, mass_stride, (long)b->num_seqs * kv_heads))
+    return {NX_ERR_INVALID_ARG, "the weights overlap those before in part"};
+  return {};
+}
+
+// Of a host batch whose tables were checked: the tokens of a row of weights that are read (those before the
+// step's own) and written.
+inline size_t mass_read(const nx_kv_batch &b, int s, size_t mass_stride) {
+  const int n = b.row_start[s + 1] - b.row_start[s];
+  return n > 0 ? std::min((size_t)(b.kv_len[s] - n), mass_stride) : 0;
+}
+inline size_t mass_written(const nx_kv_batch &b, int s, size_t mass_stride) {
+  return b.row_start[s + 1] > b.row_start[s] ? std::min((size_t)b.kv_len[s], mass_stride) : 0;
+}
+inline Refusal mass_check_tables(const nx_kv_batch &b, int kv_heads, const float *before, const float *mass,
+                                 size_t mass_stride) {
+  if (before && before != mass &&
+      weights_overlap(before, mass_stride, mass_stride,
+                      weight_rows(b.num_seqs, kv_heads, [&](int s) { return mass_read(b, s, mass_stride); }), mass,
+                      mass_stride, mass_stride,
+                      weight_rows(b.num_seqs, kv_heads, [&](int s) { return mass_written(b, s, mass_stride); })))
     return {NX_ERR_INVALID_ARG, "the weights overlap those before in part"};
   return {};
 }
@@ -185,19 +228,6 @@ inline MassWide mass_wide(int seqs, int rows, int heads, int kv_heads, int group
   return m;
 }
 
-// How the rows of weights of a host call are read, need(sequence) of each row of a sequence: `rows` - 1 whole ones of
-// `width`, and of the last sequence that has any its last row's `last` weights, for the caller's memory may
-// end with them.
-struct WeightRows {
-  size_t rows, last;
-};
-template <typename Need>
-WeightRows weight_rows(int seqs, int kv_heads, Need need) {
-  for (int s = seqs - 1; s >= 0; --s)
-    if (const size_t n = need(s)) return {(size_t)(s + 1) * kv_heads, n};
-  return {0, 0};
-}
-
 // The arguments of an eviction besides the cache and the batch.
 struct EvictArgs {
   const int32_t *to_pages;
@@ -209,7 +239,8 @@ struct EvictArgs {
   size_t new_mass_stride;
 };
 
-inline Refusal evict_check(const nx_kv_batch *b, int page_tokens, int kv_heads, const EvictArgs &a) {
+// `host`: evict_check_tables looks at the rows of weights
+inline Refusal evict_check(const nx_kv_batch *b, int page_tokens, int kv_heads, const EvictArgs &a, bool host = false) {
   if (!b) return {NX_ERR_INVALID_ARG, "null batch"};
   if (b->num_seqs < 0 || b->max_pages < 0 || a.to_max_pages < 0) return {NX_ERR_INVALID_ARG, "negative batch size"};
   if (a.keep <= 0 || a.sinks < 0 || a.recent < 0)
@@ -234,14 +265,14 @@ inline Refusal evict_check(const nx_kv_batch *b, int page_tokens, int kv_heads, 
   if (!a.new_mass) return {};
   if (Refusal f = kv_check_rows("weight", (long)a.new_mass_stride, a.keep)) return f;
   const size_t width = std::min(a.mass_stride, (size_t)b->max_pages * page_tokens);
-  if (rows_overlap(a.mass, a.mass_stride, width, a.new_mass, a.new_mass_stride, a.keep, (long)b->num_seqs * kv_heads))
+  if (!host && rows_overlap(a.mass, a.mass_stride, width, a.new_mass, a.new_mass_stride, a.keep, (long)b->num_seqs * kv_heads))
     return {NX_ERR_INVALID_ARG, "the new weights overlap the old ones"};
   return {};
 }
 
-// What the call on host memory checks besides: lengths and weights, and that the new pages are
-// the cache's, nobody else's of the batch, and named once.
-inline Refusal evict_check_tables(const nx_kv_batch &b, int num_pages, int page_tokens, const EvictArgs &a) {
+// What the call on host memory checks besides: lengths and weights (of kv_heads heads), and that the new pages
+// are the cache's, nobody else's of the batch, and named once.
+inline Refusal evict_check_tables(const nx_kv_batch &b, int num_pages, int page_tokens, const EvictArgs &a, int kv_heads = 1) {
   std::vector<int> from, to;
   for (int s = 0; s < b.num_seqs; ++s) {
     const int len = b.kv_len[s];
@@ -259,6 +290,14 @@ inline Refusal evict_check_tables(const nx_kv_batch &b, int num_pages, int page_
       }
     }
   }
+  size_t most = 0;
+  for (int s = 0; s < b.num_seqs; ++s) most = std::max(most, (size_t)b.kv_len[s]);
+  if (a.new_mass && weights_overlap(a.mass, a.mass_stride, most,
+                                    weight_rows(b.num_seqs, kv_heads, [&](int s) { return (size_t)b.kv_len[s]; }),
+                                    a.new_mass, a.new_mass_stride, a.keep, weight_rows(b.num_seqs, kv_heads, [&](int s) {
+                                      return (size_t)std::min(b.kv_len[s], a.keep);
+                                    })))
+    return {NX_ERR_INVALID_ARG, "the new weights overlap the old ones"};
   std::sort(from.begin(), from.end());
   std::sort(to.begin(), to.end());
   for (size_t i = 0; i < to.size(); ++i)

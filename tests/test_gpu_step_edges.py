@@ -58,7 +58,8 @@ def test_first_kept_tokens_of_a_group(ctx, fmt):
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_host_weights_that_end_with_the_last_token(ctx, fmt, lens):
     """Rows of weights as far apart as the longest sequence is long, in memory that ends with the last
-    sequence's last weight: the host calls' results are those of whole rows."""
+    sequence's last weight: the host calls' results are those of whole rows.  What lies behind may be
+    the same call's new weights."""
     G, heads, D, keep, stride = 2, 4, 64, 37, 311
     rng = np.random.default_rng(23)
     c = Case(ctx, rng, fmt, lens, 32, G, D, keep)
@@ -67,8 +68,8 @@ def test_host_weights_that_end_with_the_last_token(ctx, fmt, lens):
     rows = np.full((S, G, stride), np.nan, np.float32)
     rows[:, :, :max(lens)] = c.mass
     whole = c.cache.evict(c.b.kv_len, c.b.pages, c.to, keep, c.mass, 2, 3)
-    memory = np.full(rows.size + 3 * S * G * keep, 7, np.float32)
-    exact, moved = memory[:end], memory[-S * G * keep:].reshape(S, G, keep)
+    memory = np.full(end + S * G * keep, 7, np.float32)
+    exact, moved = memory[:end], memory[end:].reshape(S, G, keep)
     exact[:] = rows.ravel()[:end]
     L, kept, new_len = nx.lib(), np.zeros((S, G, keep), np.int32), np.zeros(S, np.int32)
     b, hold = c.cache._host_batch(np.zeros(S + 1), c.b.kv_len, c.b.pages, 0)
