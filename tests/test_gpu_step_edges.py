@@ -8,6 +8,7 @@ from kv_cases import F16, INT8, Batch, random_kv, stored
 from moe_cases import DeviceArray, assert_same_bits
 from step_cases import HALVES, PAIRS, rope
 from test_gpu_evict import Case
+from test_gpu_kv import device_batch
 from test_gpu_step import Hip
 
 pytestmark = pytest.mark.gpu
@@ -229,6 +230,54 @@ def test_queries_that_are_not_finite(ctx, fmt, heads, G, D, ns, lens):
     check_mass(b, got, *ref)
 
 
+@pytest.mark.parametrize("heads,G,D,n,length,first", [
+    (256, 32, 256, 1300, 1300, 268),  # slices of 508 rows, of which the first has 240
+    (32, 8, 128, 2000, 2000, 0),
+    (32, 4, 128, 37, 20000, 0),       # the keys shared out
+    (32, 4, 128, 1, 20000, 0),
+])
+def test_infinite_keys_of_long_calls(ctx, heads, G, D, n, length, first):
+    """Scores of 0, and -infinity for every 97th token: a row gives each of the others that it sees the
+    same weight, whatever parts and slices it is worked out in.
+
+    The bound is step_cases.attention_mass's with scores of no magnitude."""
+    rng = np.random.default_rng(36)
+    b = Batch(rng, [n], [length], 64, first_row=first)
+    k, _ = random_kv(rng, length, G, D)
+    k[:, :, 3] = 0
+    k[5::97, :, 3] = np.inf
+    q = np.zeros((b.rows, heads, D), np.float32)
+    q[:, :, 3] = -rng.random((b.rows, heads), dtype=np.float32) - np.float32(1e-3)
+    got, _ = mass_of(ctx, b, F16, k, q, heads, 0.1)
+    finite = np.ones(length)
+    finite[5::97] = 0
+    sees = np.cumsum(finite)[length - n:]  # of each row
+    group = heads // G
+    each = np.zeros(length)
+    each[length - n:] = group / sees
+    total = np.cumsum(each[::-1])[::-1] * finite
+    bound = (4 * 2.0 ** -21 + (length + 64 + 2 * np.log2(length + 1) + group * n + 8) * 2.0 ** -24) * total
+    assert (np.abs(got[0] - total) <= bound).all()
+
+
+@pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
+def test_products_past_the_range_under_scores_within(ctx, heads, G, D, ns, lens):
+    """INT8: a key's scale and a query's size whose product f32 does not hold, at elements that do not
+    meet: the score is 0."""
+    rng = np.random.default_rng(37 + D)
+    b = Batch(rng, ns, lens, 32)
+    k = np.zeros((sum(lens), G, D), np.float32)
+    k[..., 0] = rng.standard_normal(k.shape[:2]) * 1e-20
+    k[2::9, :, 0] = 0
+    k[2::9, :, 1] = 3e38
+    q = np.zeros((b.rows, heads, D), np.float32)
+    q[..., 0] = rng.standard_normal(q.shape[:2]) * 1e20
+    got, keys = mass_of(ctx, b, INT8, k, q, heads, 1.0)
+    ref = mass_by_rows(b, keys, q, heads, 1.0)
+    assert not ref[2].any()
+    check_mass(b, got, *ref)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("size", [1e29, 3e30, 1e33, 1e37])
 @pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
@@ -396,5 +445,42 @@ def test_workspace_of_few_long_rows_under_capture():
                 assert (np.abs(ent.download()[:T] - ref) <= promised(ref, spread)).all()
             hip.hipGraphExecDestroy(graph)
             hip.hipGraphDestroy(g)
+        ctx.set_stream(None)
+        hip.hipStreamDestroy(stream)
+
+
+@pytest.mark.parametrize("ns,lens", [([2, 1], [70, 40]), ([60, 1], [300, 40])])
+def test_infinite_keys_in_a_graph(ns, lens):
+    """What is done by the formula is replayed with the rest, whatever eager calls come between."""
+    hip = Hip()
+    rng = np.random.default_rng(38)
+    heads, G, D = 8, 2, 64
+    b = Batch(rng, ns, lens, 32)
+    k, v = random_kv(rng, sum(lens), G, D)
+    k[9, :, 7] = np.inf
+    q = rng.standard_normal((2, b.rows, heads, D), dtype=np.float32)
+    q[..., 7] = -np.abs(q[..., 7])
+    with nx.Context(0) as ctx:
+        cache = nx.KvCache(ctx, F16, b.num_pages, 32, G, D)
+        cache.write(b.whole(), b.kv_len, b.pages, k, v)
+        want = [cache.attention_mass(*b.args(), x, heads) for x in q]
+        assert all(np.isfinite(w).all() for w in want)
+        stream, d, dq = hip.stream(), device_batch(b), DeviceArray(q[0].size)
+        mass = DeviceArray(want[0].size)
+        ctx.sync()
+        ctx.set_stream(stream.value)
+        g, graph = hip.graph(stream, lambda: cache.attention_mass_dev(d, dq.ptr, heads * D, heads, 0, mass.ptr, max(lens),
+                                                                      D ** -0.5))
+        for x, w in zip(q[[0, 1, 0]], [want[0], want[1], want[0]]):
+            dq.upload(x), mass.upload(np.zeros(w.size))
+            hip.hipGraphLaunch(graph, stream)
+            ctx.sync()
+            got = mass.download().reshape(w.shape)
+            for s, n in enumerate(lens):
+                assert_same_bits(got[s, :, :n], w[s, :, :n])
+            cache.attention_mass(*b.args(), q[1], heads)
+        hip.hipGraphExecDestroy(graph)
+        hip.hipGraphDestroy(g)
+        cache.close()
         ctx.set_stream(None)
         hip.hipStreamDestroy(stream)
