@@ -435,8 +435,8 @@ typedef struct nx_rope {
  *   (a, b) -> (a cos t - b sin t, a sin t + b cos t);
  * elements from rotary_dim on keep y.  For rows r < num_tokens: `heads` query heads at
  * q + r * q_stride and `kv_heads` key heads at k + r * k_stride, to q_out and k_out likewise
- * (strides in floats).  An output may be its own input, with its stride; any other overlap is
- * refused.  heads or kv_heads may be 0.  positions[r] may be any number: a sequence that gave
+ * (strides in floats).  An output may be its own input, with its stride; any other overlap of
+ * heads' rows is refused.  heads or kv_heads may be 0.  positions[r] may be any number: a sequence that gave
  * tokens up (nx_kv_evict) keeps the positions that it counts.  f32 in and out, the sum of squares
  * and the angle in 64 bits: within 2^-20 of the head's largest normed value, at any position.  kernel::rope_single (src/kernel/mod.rs:258-271), and kernel::rms_norm
  * (src/kernel/mod.rs:199-209) on each head. */

@@ -14,7 +14,8 @@
 // by, so a key's sum stays in its lanes.
 //
 // 32 heads over 8 of 128 in F16: one token of 61 sequences of up to 8191 155 us (667 MB), every token of a
-// prompt of 4093 364 to 377 (69 GFLOP, four times that with two halves in two passes).
+// prompt of 4093 364 to 377 (69 GFLOP, four times that with two halves in two passes).  Cards differ by 5%:
+// where two figures are compared below, both are of one card.
 //
 // The scores are nx_attn.hip's: transposed products K Q^T on the f16 matrix cores, q as two
 // halves.  A score is one key's and one row's alone, so nothing that is masked reaches another.

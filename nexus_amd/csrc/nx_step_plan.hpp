@@ -1,5 +1,5 @@
 // nx_step_plan.hpp — what the calls around a step's cache and attention accept (heads normed
-// and rotated, log probabilities), and how they share their work out.
+// and rotated, gathered weights, eviction, log probabilities), and how they share their work out.
 //
 // Plain C++ (no HIP): the CPU tests compile this header on its own.
 #pragma once
