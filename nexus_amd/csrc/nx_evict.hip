@@ -5,7 +5,7 @@
 // by counting the weights' leading 11, next 11 and last 10 bits (as keys that order as the values
 // do); then every wave numbers the kept ones of its stretch of tokens, in their order.  What one
 // CU can count bounds it: 16381 tokens of 8 heads 17 us, 5003 of 4 heads of 23 sequences 15, 100000 of
-one head, whose weights are read in every pass, 101.  Weights that are alike count into one bin: 53 and 300.
+// one head, whose weights are read in every pass, 101.  Weights that are alike count into one bin: 53 and 300.
 // k_evict_move, a workgroup of 32 kept tokens of a head: out of their groups' operand order into
 // that of the new group.  4096 tokens of 8 heads in F16 15 us (34 MB), 3001 of 4 heads of 23
 // sequences in INT8 44 us (128 MB, 2.9 TB/s): keys are read in pieces of 8 and 16 bytes, and a
