@@ -908,8 +908,8 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
       }
       const float c = coef[buf][n], ei = lse[buf][n];
       // INT8: far from 0 a score is rounded before e is taken off, as k_mass_stats does, where the rounding alone is
-      // a factor of e^(2^-12) and more.  (Without the condition: 70.5 us for the last queries of two prompts, not 69.  F16's
-      // factor is a power of two.)
+      // a factor of 2^(2^-12) and more.  (Without the condition: 70.5 us for the last queries of two prompts, not
+      // 69.  F16's factor is a power of two.)
       const bool far = I8 && __any(fabsf(ei) > 4096.f);
       const int p = token[buf][n];
       const int pmin = uniform(block * kMassBlock + kMassBlock <= rows ? token[buf][0] : -1);
@@ -1138,7 +1138,8 @@ static int attention_mass(nx_ctx *c, const nx_kv *kv, const nx_kv_batch *b, cons
   NX_TRY(ws_get(c, WS_OUT, tiles * most * 4, &dm));
   NX_HIP(hipMemcpy2DAsync(dq, width * 4, q, q_stride * 4, width * 4, rows, hipMemcpyHostToDevice, c->stream));
   if (before)  // (of sequences that have rows, the tokens before them)
-    NX_TRY(upload_weights(c, static_cast<float *>(dm), most, before, mass_stride, weight_rows(b->num_seqs, kv->heads, [&](int s) { return mass_read(*b, s, most); })));
+    NX_TRY(upload_weights(c, static_cast<float *>(dm), most, before, mass_stride,
+                          weight_rows(b->num_seqs, kv->heads, [&](int s) { return mass_read(*b, s, most); })));
   a.q = static_cast<const float *>(dq);
   a.q_stride = width;
   a.mass = static_cast<float *>(dm);
