@@ -838,6 +838,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
     // ---- the wave's keys: row n of a group in the cache's order
     f16x8 kx[KG][KS];
     bool there[KG];
+    float scale[KG];
 #pragma unroll
     for (int i = 0; i < KG; ++i) {
       const int first = k0 + (wave * KG + i) * kKvGroup;
@@ -853,9 +854,20 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
           kx[i][j] = *reinterpret_cast<const f16x8 *>(base + 2 * j * kKvGroup * 8);
         }
       }
-      if constexpr (I8) {
-        if (n < 16) scales[wave][i][h][n] = kv.ks[max(gr, 0L) * kKvGroup + kv_token(FMT, 8 * (n >> 2) + 4 * h + (n & 3))];
-      }
+      if constexpr (I8) scale[i] = kv.ks[max(gr, 0L) * kKvGroup + kv_token(FMT, 8 * (n >> 2 & 3) + 4 * h + (n & 3))];
+    }
+    // INT8: a score is rounded times its key's scale, and the row's c and e follow in one step: c is a power of two,
+    // so that is the score as k_mass_stats rounds it, times scale and c at once.  (Rounded with e taken off,
+    // scores of 2^24 and more would be a factor of any size off.)  Scales that could pass f32's range so are held lower.
+    float lift = 1.f;
+    if constexpr (I8) {
+      bool large = false;
+#pragma unroll
+      for (int i = 0; i < KG; ++i) large = large || scale[i] >= 0x1p100f;
+      if (__any(large)) lift = 0x1p30f;
+#pragma unroll
+      for (int i = 0; i < KG; ++i)
+        if (n < 16) scales[wave][i][h][n] = scale[i] * (1.f / lift);
     }
     float sum[KG][16];
 #pragma unroll
@@ -906,11 +918,7 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
         stage(block + 1, buf ^ 1);
         if (block + 2 < to) fetch(block + 2);
       }
-      const float c = coef[buf][n], ei = lse[buf][n];
-      // INT8: far from 0 a score is rounded before e is taken off, as k_mass_stats does, where the rounding alone is
-      // a factor of 2^(2^-12) and more.  (Without the condition: 70.5 us for the last queries of two prompts, not
-      // 69.  F16's factor is a power of two.)
-      const bool far = I8 && __any(fabsf(ei) > 4096.f);
+      const float c = coef[buf][n] * lift, ei = lse[buf][n];
       const int p = token[buf][n];
       const int pmin = uniform(block * kMassBlock + kMassBlock <= rows ? token[buf][0] : -1);
       const int pmax = s.first + by_group(min(block * kMassBlock + kMassBlock, rows) - 1, a.magic, a.shift);
@@ -934,18 +942,11 @@ __global__ __launch_bounds__(kMassThreads, D == 256 ? 1 : 2) void k_mass_columns
       for (int i = 0; i < KG; ++i) {
         const int g0 = first + i * kKvGroup;
         float y[16];
-        float by[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) by[j] = I8 ? scales[wave][i][h][j] * c : c;
-        if (far) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            sc[i][j] *= by[j];
-            by[j] = 1.f;
-          }
+        for (int j = 0; j < 16; ++j) {
+          const float x = I8 ? sc[i][j] * scales[wave][i][h][j] : sc[i][j];
+          y[j] = __builtin_amdgcn_exp2f(fmaf(x, c, -ei));
         }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], by[j], -ei));
         if (g0 + kKvGroup - 1 > pmin) {
 #pragma unroll
           for (int j = 0; j < 16; ++j)

@@ -278,6 +278,25 @@ def test_products_past_the_range_under_scores_within(ctx, heads, G, D, ns, lens)
     check_mass(b, got, *ref)
 
 
+@pytest.mark.parametrize("up", [1e36, 1e33, 1e-33])
+@pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
+def test_sizes_that_meet_in_ordinary_scores(ctx, heads, G, D, ns, lens, up):
+    """INT8 keys next to f32's largest under queries next to nothing, and the other way round; tokens of
+    ordinary size among them."""
+    rng = np.random.default_rng(39 + D)
+    b = Batch(rng, ns, lens, 32)
+    k, _ = random_kv(rng, sum(lens), G, D)
+    k *= np.float32(up)
+    k[4::11] *= np.float32(1 / up)
+    q = rng.standard_normal((b.rows, heads, D), dtype=np.float32) * np.float32(1 / up)
+    if up < 1:
+        k[4::11] = 0  # (ordinary keys would leave the range)
+    got, keys = mass_of(ctx, b, INT8, k, q, heads, 0.125)
+    ref = mass_by_rows(b, keys, q, heads, 0.125)
+    assert not ref[2].any()
+    check_mass(b, got, *ref)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("size", [1e29, 3e30, 1e33, 1e37])
 @pytest.mark.parametrize("heads,G,D,ns,lens", SHAPES)
